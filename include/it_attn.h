@@ -73,6 +73,42 @@ int it_attn_prep_f16_q16(float* q, int q_tok_stride, const float* k, const float
                          int sec2, int sec3, int round_mode, uint16_t* q16, int q16_tok_stride, float scale,
                          void* stream);
 
+/* The same pass with the rotation given by the caller, for tokens whose positions are not their cache rows (a
+ * drafted tree, a cache that no longer starts at position 0) and for other rotations than the model's own:
+ *   pos    : device int32 [nt], the position of token t (any int32 value), or NULL for pos0 + t.
+ *   row0   : K and V of token t go to cache row row0 + t.
+ *   n_rot  : rotated dims per head, even, <= hd. layout IT_ROPE_HALVES: dims (i, i + n_rot/2) turn together, n_rot a
+ *            multiple of hd/32; IT_ROPE_PAIRS: dims (2i, 2i + 1).
+ *   freq   : device f32 [n_rot/2], the angle of pair i per position (it_rope_freqs makes the usual ones; 0 leaves a
+ *            pair as it is). The angle pos * freq[i] is exact in f64 before it is reduced.
+ *   mscale : factor of cos and sin (1 but for stretched contexts).
+ * The rest as for it_attn_prep_f16 / it_attn_prep_f32kv (q rewritten in place, the gates left as they are). No
+ * counterpart in the reference, whose positions are pos0 + t and whose rotation is the model's. */
+#define IT_ROPE_HALVES 0
+#define IT_ROPE_PAIRS 1
+int it_attn_prep_pos_f16(float* q, int q_tok_stride, const float* k, const float* v, int kv_tok_stride,
+                         const float* q_norm, const float* k_norm, float eps, uint16_t* kc, uint16_t* vc, int kvd,
+                         const int32_t* pos, int pos0, int row0, int hd, int nh, int nkv, int nt, int n_rot,
+                         const float* freq, float mscale, int layout, int round_mode, void* stream);
+int it_attn_prep_pos_f32kv(float* q, int q_tok_stride, const float* k, const float* v, int kv_tok_stride,
+                           const float* q_norm, const float* k_norm, float eps, float* kc, float* vc, int kvd,
+                           const int32_t* pos, int pos0, int row0, int hd, int nh, int nkv, int nt, int n_rot,
+                           const float* freq, float mscale, int layout, void* stream);
+
+/* The rotation table of the calls above (host function, host buffers): freq[i], i < n_rot/2, and *mscale.
+ *   IT_ROPE_PLAIN  : base^(-2i/n_rot), factor and orig_ctx unused.
+ *   IT_ROPE_LINEAR : the same / factor (positions interpolated).
+ *   IT_ROPE_NTK    : the base times factor^(n_rot/(n_rot-2)), so the slowest pair is stretched by factor and the
+ *                    fastest kept.
+ *   IT_ROPE_YARN   : pairs of more than 32 turns over orig_ctx positions kept, those of less than one stretched by
+ *                    factor, a linear blend between; *mscale = 0.1 ln(factor) + 1.
+ * *mscale is 1 for the others. */
+#define IT_ROPE_PLAIN 0
+#define IT_ROPE_LINEAR 1
+#define IT_ROPE_NTK 2
+#define IT_ROPE_YARN 3
+int it_rope_freqs(int n_rot, float base, int kind, float factor, int orig_ctx, float* freq, float* mscale);
+
 /* Bytes of scratch to give it_attn_f16 for this call geometry: more changes nothing (0: none is used).
  * Less is accepted too, see it_attn_f16. A prompt call (nt >= 16) may use only part of them, or none where
  * one pass is faster, and they do not grow evenly with pos0 (the ranges of keys change): one buffer for many
@@ -416,6 +452,33 @@ int it_gdn_prefill(const float* x, int x_tok_stride, const float* conv_w, int K,
                    const float* beta_raw, const float* alpha_raw, int ba_tok_stride, const float* dt,
                    const float* a, float* state, float* out, int out_tok_stride, int nt, int nv, int nk, int S,
                    float eps, void* scratch, size_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Verification of a drafted token tree. The reference drafts chains (src/mtp.rs:166-204: one draft a step, checked by
+ * a batch of two); with several candidates a step the batch is a tree, and these calls stand where the chain's do:
+ *   it_tree_plan                    once a step: masks and positions from the parents
+ *   it_attn_prep_pos_f16            positions of the nodes; node t in cache row pos0 + t     (it_attn_prep_f16)
+ *   it_attn_tree_f16                attention over the cache and each node's own ancestors   (it_attn_f16)
+ *   it_gdn_tree                     the recurrent layer over the tree                        (it_gdn_decode_fused)
+ *   it_kv_tree_commit_f16, it_gdn_tree_commit   keep the accepted node's path, drop the rest (it_gdn_rollback)
+ * A tree is nt <= IT_TREE_MAX nodes in topological order (a parent before its children). anc: device uint64 [nt], bit j
+ * of anc[t] set for node t itself and its ancestors; 0 makes t a padding node (the output rows are zeros, and no
+ * node may name it an ancestor). Several nodes may follow the last committed token.
+ * ---------------------------------------------------------------------------------------------- */
+#define IT_TREE_MAX 64
+
+/* anc [nt] and, unless NULL, pos [nt] (int32, p0 + depth: p0 is the position of the first node after the last
+ * committed token) from parent: device int32 [nt], -1 for a node that follows the last committed token. A node whose
+ * parent is not in -1 .. t-1 is padding, and so are its descendants (anc 0, pos p0). */
+int it_tree_plan(const int32_t* parent, int nt, int p0, uint64_t* anc, int32_t* pos, void* stream);
+
+/* Keeps the path of node `leaf` in a cache whose rows pos0 + t hold the nodes: row pos0 + i <- row pos0 + path[i], path
+ * the nodes of anc[leaf] in order (in place; the rows after the path keep what they hold). leaf = -1, or a padding
+ * node: nothing is kept and nothing moves. kvd a multiple of 8, kc and vc 16-byte aligned. */
+int it_kv_tree_commit_f16(uint16_t* kc, uint16_t* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,
+                          void* stream);
+int it_kv_tree_commit_f32(float* kc, float* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,
+                          void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Reference-shaped dispatch policy (pure host functions, no device access).

@@ -2,6 +2,8 @@
 // kernel launches. Validation runs before any device work, like the reference's fail-closed
 // checks (src/vk/mod.rs:179-220); runtime errors come back as nonzero codes with a thread-local
 // message instead of the reference's panics.
+#include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <unordered_map>
 #include <utility>
@@ -321,6 +323,111 @@ int it_attn_prep_f32kv(float* q, int qts, const float* k, const float* v, int kt
     return check(it::launch_attn_prep_f32kv(q, qts, k, v, kts, q_norm, k_norm, eps, kc, vc, pos0, row0, hd, nh, nkv, nt,
                                             n_rot, theta_scale, sec, (hipStream_t)stream),
                  who);
+}
+
+int it_rope_freqs(int n_rot, float base, int kind, float factor, int orig_ctx, float* freq, float* mscale) {
+    const char* who = "it_rope_freqs";
+    if (n_rot < 2 || n_rot % 2 != 0 || n_rot > 256) return fail("%s: n_rot %d must be even and in [2, 256]", who, n_rot);
+    if (!(base > 1.0f) || !std::isfinite(base)) return fail("%s: base %g must be above 1", who, base);
+    if (kind < IT_ROPE_PLAIN || kind > IT_ROPE_YARN) return fail("%s: unknown kind %d", who, kind);
+    if (kind != IT_ROPE_PLAIN && (!(factor >= 1.0f) || !std::isfinite(factor)))
+        return fail("%s: factor %g must be at least 1", who, factor);
+    if (kind == IT_ROPE_NTK && n_rot < 4) return fail("%s: the NTK base needs n_rot >= 4", who);
+    if (kind == IT_ROPE_YARN && orig_ctx < 1) return fail("%s: orig_ctx %d must be positive", who, orig_ctx);
+    if (!freq || !mscale) return fail("%s: null output", who);
+    const double n = n_rot, b = kind == IT_ROPE_NTK ? base * std::pow((double)factor, n / (n - 2)) : base;
+    // YaRN: the pairs between `fast` and `slow` turns over the original context blend from kept to stretched
+    const double two_pi = 6.283185307179586476925286766559, fast = 32.0, slow = 1.0;
+    const auto pair_of = [&](double turns) { return n * std::log(orig_ctx / (turns * two_pi)) / (2 * std::log((double)base)); };
+    double lo = 0, hi = 0;
+    if (kind == IT_ROPE_YARN) {
+        lo = std::max(std::floor(pair_of(fast)), 0.0);
+        hi = std::min(std::ceil(pair_of(slow)), n - 1);
+    }
+    for (int i = 0; i < n_rot / 2; ++i) {
+        const double f = std::pow(b, -2.0 * i / n);
+        double r = f;
+        if (kind == IT_ROPE_LINEAR) r = f / factor;
+        if (kind == IT_ROPE_YARN) {
+            const double stretch = std::min(std::max((i - lo) / std::max(hi - lo, 1e-3), 0.0), 1.0);
+            r = f / factor * stretch + f * (1 - stretch);
+        }
+        freq[i] = (float)r;
+    }
+    *mscale = kind == IT_ROPE_YARN ? (float)(0.1 * std::log((double)factor) + 1) : 1.0f;
+    g_err.clear();
+    return 0;
+}
+
+}  // extern "C"
+
+template <class KVT>
+static int attn_prep_pos(const char* who, float* q, int qts, const float* k, const float* v, int kts,
+                         const float* q_norm, const float* k_norm, float eps, KVT* kc, KVT* vc, int kvd,
+                         const int32_t* pos, int pos0, int row0, int hd, int nh, int nkv, int nt, int n_rot,
+                         const float* freq, float mscale, int layout, int round_mode, void* stream) {
+    if (layout != IT_ROPE_HALVES && layout != IT_ROPE_PAIRS) return fail("%s: unknown rope layout %d", who, layout);
+    // the common checks want n_rot in whole lane blocks, which pairs inside a lane do not need
+    const bool pairs = layout == IT_ROPE_PAIRS;
+    if (n_rot < 0 || n_rot > hd || n_rot % 2 != 0) return fail("%s: n_rot %d must be even and in [0, %d]", who, n_rot, hd);
+    if (validate_prep(who, q, qts, k, v, kts, q_norm, k_norm, eps, kc, vc, kvd, row0, hd, nh, nkv, nt, pairs ? 0 : n_rot,
+                      1.0f, 0, 0, 0, 0))
+        return -1;
+    if (n_rot > 0 && !freq) return fail("%s: null freq", who);
+    if (!std::isfinite(mscale)) return fail("%s: mscale %g invalid", who, mscale);
+    if (!pos && (pos0 < 0 || (long)pos0 + nt > INT32_MAX)) return fail("%s: pos0 %d invalid", who, pos0);
+    if (nt == 0) { g_err.clear(); return 0; }
+    return check(it::launch_attn_prep_pos<KVT>(q, qts, k, v, kts, q_norm, k_norm, eps, kc, vc, pos, pos0, row0, hd, nh,
+                                               nkv, nt, n_rot, freq, mscale, pairs, round_mode, (hipStream_t)stream),
+                 who);
+}
+
+extern "C" {
+
+int it_attn_prep_pos_f16(float* q, int qts, const float* k, const float* v, int kts, const float* q_norm,
+                         const float* k_norm, float eps, uint16_t* kc, uint16_t* vc, int kvd, const int32_t* pos,
+                         int pos0, int row0, int hd, int nh, int nkv, int nt, int n_rot, const float* freq,
+                         float mscale, int layout, int round_mode, void* stream) {
+    const char* who = "it_attn_prep_pos_f16";
+    if (round_mode != 0 && round_mode != 1) return fail("%s: round_mode must be 0 (RNE) or 1 (RTZ)", who);
+    return attn_prep_pos(who, q, qts, k, v, kts, q_norm, k_norm, eps, kc, vc, kvd, pos, pos0, row0, hd, nh, nkv, nt,
+                         n_rot, freq, mscale, layout, round_mode, stream);
+}
+
+int it_attn_prep_pos_f32kv(float* q, int qts, const float* k, const float* v, int kts, const float* q_norm,
+                           const float* k_norm, float eps, float* kc, float* vc, int kvd, const int32_t* pos, int pos0,
+                           int row0, int hd, int nh, int nkv, int nt, int n_rot, const float* freq, float mscale,
+                           int layout, void* stream) {
+    return attn_prep_pos("it_attn_prep_pos_f32kv", q, qts, k, v, kts, q_norm, k_norm, eps, kc, vc, kvd, pos, pos0, row0,
+                         hd, nh, nkv, nt, n_rot, freq, mscale, layout, 0, stream);
+}
+
+int it_tree_plan(const int32_t* parent, int nt, int p0, uint64_t* anc, int32_t* pos, void* stream) {
+    const char* who = "it_tree_plan";
+    if (nt < 1 || nt > IT_TREE_MAX) return fail("%s: nt %d must be in [1, %d]", who, nt, IT_TREE_MAX);
+    if (p0 < 0 || p0 > INT32_MAX - IT_TREE_MAX) return fail("%s: p0 %d invalid", who, p0);
+    if (!parent || !anc) return fail("%s: null buffer", who);
+    return check(it::launch_tree_plan(parent, nt, p0, anc, pos, (hipStream_t)stream), who);
+}
+
+static int kv_tree_commit(const char* who, void* kc, void* vc, int kvd, size_t size, int pos0, int nt,
+                          const uint64_t* anc, int leaf, void* stream) {
+    if (nt < 1 || nt > IT_TREE_MAX) return fail("%s: nt %d must be in [1, %d]", who, nt, IT_TREE_MAX);
+    if (leaf < -1 || leaf >= nt) return fail("%s: leaf %d must be in [-1, %d)", who, leaf, nt);
+    if (kvd <= 0 || kvd % 8 != 0) return fail("%s: kvd %d must be a positive multiple of 8", who, kvd);
+    if (pos0 < 0 || (long)pos0 + nt > (1L << 22)) return fail("%s: pos0 %d / nt %d invalid", who, pos0, nt);
+    if (!kc || !vc || !anc) return fail("%s: null buffer", who);
+    if (!aligned16(kc) || !aligned16(vc)) return fail("%s: kc/vc must be 16-byte aligned", who);
+    if (leaf < 0) { g_err.clear(); return 0; }
+    return check(it::launch_kv_tree_commit(kc, vc, (size_t)kvd * size, pos0, anc, leaf, (hipStream_t)stream), who);
+}
+int it_kv_tree_commit_f16(uint16_t* kc, uint16_t* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,
+                          void* stream) {
+    return kv_tree_commit("it_kv_tree_commit_f16", kc, vc, kvd, 2, pos0, nt, anc, leaf, stream);
+}
+int it_kv_tree_commit_f32(float* kc, float* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,
+                          void* stream) {
+    return kv_tree_commit("it_kv_tree_commit_f32", kc, vc, kvd, 4, pos0, nt, anc, leaf, stream);
 }
 
 size_t it_attn_f32kv_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv) {

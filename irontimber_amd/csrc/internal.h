@@ -105,6 +105,17 @@ hipError_t launch_gdn_chunked(const CoT* co, int cts, const float* br, const flo
 // out receives wgs * 256 floats.
 hipError_t launch_mfma_peak(int wgs, int iters, float* out, hipStream_t st);
 
+// Drafted token trees (tree.hip, attn_tree.hip, gdn_tree.hip): anc[t] the 64-bit mask of node t and its ancestors.
+hipError_t launch_tree_plan(const int* parent, int nt, int p0, uint64_t* anc, int* pos, hipStream_t st);
+hipError_t launch_kv_tree_commit(void* kc, void* vc, size_t row_bytes, int pos0, const uint64_t* anc, int leaf,
+                                 hipStream_t st);
+// KVT uint16_t (f16 cache) or float; pos null: token t at pos0 + t
+template <class KVT>
+hipError_t launch_attn_prep_pos(float* q, int qts, const float* k, const float* v, int kts, const float* qw,
+                                const float* kw, float eps, KVT* kc, KVT* vc, const int* pos, int pos0, int row0,
+                                int hd, int nh, int nkv, int nt, int n_rot, const float* freq, float mscale,
+                                bool pairs, int rtz, hipStream_t st);
+
 // conv <- ck_conv (nc floats) and ssm <- ck_ssm (ns floats) in one launch.
 hipError_t launch_gdn_rollback(const float* ck_conv, float* conv, size_t nc, const float* ck_ssm, float* ssm,
                                size_t ns, hipStream_t st);

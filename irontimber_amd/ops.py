@@ -433,3 +433,140 @@ def gdn_rollback(ck_conv: torch.Tensor | None, conv_state: torch.Tensor | None, 
         if t is not None and (c is None or c.numel() != t.numel()):
             raise ValueError("checkpoint and state sizes differ")
     call("it_gdn_rollback", _ptr(ck_conv), _ptr(conv_state), cw, _ptr(ck_ssm), _ptr(ssm), sw, _stream())
+
+
+# ---- verification of a drafted token tree (include/it_attn.h has the whole contract)
+
+ROPE_KINDS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3}
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+TREE_MAX = 64
+
+
+def _call_on(t: torch.Tensor, name: str, *args) -> None:
+    """call(name, *args, stream) with t's device current and its current stream."""
+    dev = t.device.index
+    if dev == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _need_all(dtype: torch.dtype, device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        _need(t, dtype, name)
+        if t.device != device:
+            raise ValueError(f"{name} must be on {device}, like the other tensors")
+
+
+def _need_cache(c: torch.Tensor, name: str, dtypes, device: torch.device, kvd: int, rows: int) -> None:
+    if c.dtype not in dtypes or c.dim() != 2 or not c.is_contiguous() or c.shape[1] != kvd:
+        raise ValueError(f"{name} must be contiguous [rows, {kvd}] of {dtypes[0]}")
+    if c.device != device:
+        raise ValueError(f"{name} must be on {device}, like the other tensors")
+    if c.shape[0] < rows:
+        raise ValueError(f"{name} too short: {c.shape[0]} rows, {rows} needed")
+
+
+_F16 = (torch.float16, torch.int16)
+_F32 = (torch.float32,)
+
+
+def rope_freqs(n_rot: int, base: float = 1e7, kind: str = "plain", factor: float = 1.0, orig_ctx: int = 8192,
+               device="cuda") -> tuple[torch.Tensor, float]:
+    """(freq [n_rot/2] f32 on device, mscale) for attn_prep_pos_*: plain, linear, ntk or yarn scaling of the context
+    by factor (it_rope_freqs)."""
+    if kind not in ROPE_KINDS:
+        raise ValueError(f"kind must be one of {sorted(ROPE_KINDS)}")
+    freq, m = torch.empty(max(n_rot // 2, 1), dtype=torch.float32), ctypes.c_float()
+    call("it_rope_freqs", n_rot, float(base), ROPE_KINDS[kind], float(factor), orig_ctx, freq.data_ptr(),
+         ctypes.addressof(m))
+    return freq.to(device), m.value
+
+
+def _prep_pos(name, kinds, q, k, v, kc, vc, pos, row0, nh, nkv, freq, mscale, layout, q_norm, k_norm, eps, pos0, *more):
+    dev = q.device
+    _need_all(torch.float32, dev, q=q, k=k, v=v, freq=freq)
+    if k.dim() != 2 or k.shape[1] % nkv != 0:
+        raise ValueError("k must be [nt, nkv*hd]")
+    nt, kvd = k.shape
+    hd = kvd // nkv
+    if q.shape != (nt, nh * 2 * hd) or v.shape != k.shape:
+        raise ValueError("q must be [nt, nh*2*hd] and v the shape of k [nt, nkv*hd]")
+    if row0 < 0:
+        raise ValueError("row0 must not be negative")
+    _need_cache(kc, "kc", kinds, dev, kvd, row0 + nt)
+    _need_cache(vc, "vc", kinds, dev, kvd, row0 + nt)
+    if pos is not None:
+        _need_all(torch.int32, dev, pos=pos)
+        if pos.shape != (nt,):
+            raise ValueError("pos must be [nt]")
+    for w, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None:
+            _need_all(torch.float32, dev, **{n: w})
+            if w.numel() != hd:
+                raise ValueError(f"{n} must hold head_dim floats")
+    if layout not in ROPE_LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(ROPE_LAYOUTS)}")
+    _call_on(q, name, q.data_ptr(), q.shape[1], k.data_ptr(), v.data_ptr(), kvd, _ptr(q_norm), _ptr(k_norm), float(eps),
+             kc.data_ptr(), vc.data_ptr(), kvd, _ptr(pos), pos0, row0, hd, nh, nkv, nt, 2 * freq.numel(),
+             freq.data_ptr(), float(mscale), ROPE_LAYOUTS[layout], *more)
+
+
+def attn_prep_pos_f16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor,
+                      pos: torch.Tensor | None, row0: int, nh: int, nkv: int, freq: torch.Tensor, mscale: float = 1.0,
+                      layout: str = "half", q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                      eps: float = 1e-6, round_mode: int = 0, pos0: int = 0) -> None:
+    """attn_prep_f16 at given positions: token t at pos[t] int32 (None: pos0 + t), its K/V to cache row row0 + t, the
+    first 2 * freq.numel() dims of each head turned by pos * freq[i] in pairs (i, i + n/2) ("half") or (2i, 2i + 1)
+    ("interleaved"), cos and sin times mscale (it_attn_prep_pos_f16; freq and mscale from rope_freqs)."""
+    _prep_pos("it_attn_prep_pos_f16", _F16, q, k, v, kc, vc, pos, row0, nh, nkv, freq, mscale, layout, q_norm, k_norm, eps,
+              pos0, round_mode)
+
+
+def attn_prep_pos_f32kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor,
+                        pos: torch.Tensor | None, row0: int, nh: int, nkv: int, freq: torch.Tensor, mscale: float = 1.0,
+                        layout: str = "half", q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                        eps: float = 1e-6, pos0: int = 0) -> None:
+    """attn_prep_pos_f16 for the MTP head's f32 cache (it_attn_prep_pos_f32kv)."""
+    _prep_pos("it_attn_prep_pos_f32kv", _F32, q, k, v, kc, vc, pos, row0, nh, nkv, freq, mscale, layout, q_norm, k_norm, eps,
+              pos0)
+
+
+def _need_anc(anc: torch.Tensor, device: torch.device, nt: int) -> None:
+    _need_all(torch.int64, device, anc=anc)
+    if anc.shape != (nt,):
+        raise ValueError(f"anc must be [{nt}]")
+
+
+def tree_plan(parent: torch.Tensor, p0: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """parent [nt] int32 (-1: follows the last committed token; outside -1 .. t-1: padding) -> (anc [nt] int64, the
+    bits of each node and its ancestors, pos [nt] int32 = p0 + depth) (it_tree_plan)."""
+    _need(parent, torch.int32, "parent")
+    nt = parent.numel()
+    anc = torch.empty(nt, device=parent.device, dtype=torch.int64)
+    pos = torch.empty(nt, device=parent.device, dtype=torch.int32)
+    _call_on(parent, "it_tree_plan", parent.data_ptr(), nt, p0, anc.data_ptr(), pos.data_ptr())
+    return anc, pos
+
+
+def _kv_tree_commit(name, kinds, kc, vc, pos0, nt, anc, leaf):
+    if not kc.is_cuda or kc.dim() != 2:
+        raise ValueError("kc must be a device tensor [rows, kvd]")
+    _need_anc(anc, kc.device, nt)
+    if vc.dtype != kc.dtype:
+        raise ValueError("kc and vc must have one dtype")
+    for c, n in ((kc, "kc"), (vc, "vc")):
+        _need_cache(c, n, kinds, kc.device, kc.shape[1], pos0 + nt)
+    _call_on(kc, name, kc.data_ptr(), vc.data_ptr(), kc.shape[1], pos0, nt, anc.data_ptr(), leaf)
+
+
+def kv_tree_commit_f16(kc: torch.Tensor, vc: torch.Tensor, pos0: int, nt: int, anc: torch.Tensor, leaf: int) -> None:
+    """Moves the cache rows of node leaf's path (rows pos0 + t hold the nodes) to rows pos0, pos0 + 1, ...; leaf -1:
+    nothing (it_kv_tree_commit_f16)."""
+    _kv_tree_commit("it_kv_tree_commit_f16", _F16, kc, vc, pos0, nt, anc, leaf)
+
+
+def kv_tree_commit_f32(kc: torch.Tensor, vc: torch.Tensor, pos0: int, nt: int, anc: torch.Tensor, leaf: int) -> None:
+    """kv_tree_commit_f16 for the MTP head's f32 cache."""
+    _kv_tree_commit("it_kv_tree_commit_f32", _F32, kc, vc, pos0, nt, anc, leaf)
