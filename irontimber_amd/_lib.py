@@ -78,6 +78,9 @@ SIGNATURES = {
                                        c_int, c_int, c_int, P, c_float, c_int, P]),
     "it_rope_freqs": (c_int, [c_int, c_float, c_int, c_float, c_int, P, P]),
     "it_tree_plan": (c_int, [P, c_int, c_int, P, P, P]),
+    "it_attn_tree_scratch_bytes": (c_size_t, [c_int] * 5),
+    "it_attn_tree_f16": (c_int, [P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, P, c_float, P, c_int, P,
+                                 c_size_t, P]),
     "it_kv_tree_commit_f16": (c_int, [P, P, c_int, c_int, c_int, P, c_int, P]),
     "it_kv_tree_commit_f32": (c_int, [P, P, c_int, c_int, c_int, P, c_int, P]),
     "it_prefill_chunks": (ctypes.c_long, [c_size_t, c_size_t, P, P, c_size_t]),

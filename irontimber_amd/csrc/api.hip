@@ -410,6 +410,39 @@ int it_tree_plan(const int32_t* parent, int nt, int p0, uint64_t* anc, int32_t* 
     return check(it::launch_tree_plan(parent, nt, p0, anc, pos, (hipStream_t)stream), who);
 }
 
+// Records of a tree call: the context's pos0 keys in splits of `chunk`.
+static size_t tree_scratch(int pos0, int nt, int nh, int chunk) {
+    return (size_t)nt * nh * it::idx::split_count(pos0, chunk) * PART_WORDS * sizeof(float);
+}
+// Keys per split whose records fit `budget` bytes: the preferred split, else doubled (the rule of the fixed
+// arena, src/vk/mod.rs:714-716). 0: even one record per (node, head) is too much.
+static int plan_attn_tree(int pos0, int nt, int nh, int nkv, size_t budget) {
+    int c = it::attn_tree_chunk(pos0, nt, nh, nkv);
+    while (tree_scratch(pos0, nt, nh, c) > budget && c < pos0) c *= 2;
+    return tree_scratch(pos0, nt, nh, c) <= budget ? c : 0;
+}
+size_t it_attn_tree_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv) {
+    (void)hd;
+    if (nt < 1 || nt > IT_TREE_MAX || pos0 < 0 || nh <= 0 || nkv <= 0 || nh % nkv) return 0;
+    return tree_scratch(pos0, nt, nh, it::attn_tree_chunk(pos0, nt, nh, nkv));
+}
+int it_attn_tree_f16(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0, int hd, int nh,
+                     int nkv, int nt, const uint64_t* anc, float scale, float* out, int ots, void* scratch,
+                     size_t scratch_bytes, void* stream) {
+    const char* who = "it_attn_tree_f16";
+    if (nt < 1 || nt > IT_TREE_MAX) return fail("%s: nt %d must be in [1, %d]", who, nt, IT_TREE_MAX);
+    if (validate_attn(q, qts, kc, vc, kvd, pos0, hd, nh, nkv, nt, out, ots)) return -1;
+    if (!anc) return fail("%s: null anc", who);
+    if (scratch && !aligned16(scratch)) return fail("%s: scratch must be 16-byte aligned", who);
+    const int chunk = plan_attn_tree(pos0, nt, nh, nkv, scratch ? scratch_bytes : 0);
+    if (!chunk)
+        return fail("%s: scratch of %zu bytes cannot hold even one partial record per (node, head) (%zu bytes)", who,
+                    scratch ? scratch_bytes : 0, tree_scratch(pos0, nt, nh, pos0));
+    return check(it::launch_attn_tree(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, anc, scale, out, ots, (float*)scratch, chunk,
+                                      (hipStream_t)stream),
+                 who);
+}
+
 static int kv_tree_commit(const char* who, void* kc, void* vc, int kvd, size_t size, int pos0, int nt,
                           const uint64_t* anc, int leaf, void* stream) {
     if (nt < 1 || nt > IT_TREE_MAX) return fail("%s: nt %d must be in [1, %d]", who, nt, IT_TREE_MAX);

@@ -155,7 +155,10 @@ __device__ __forceinline__ u2 mb_load2(MbRsrc r, int idx) {
 // the scores wait for K only. Decode at ctx 8192: partial kernel 5.95 -> 5.65 us, layer 9.41 ->
 // 9.13 us; with few workgroups (ctx 512, 16 of them) the copy is faster (6.09 against 6.27 us per
 // layer), so the launch takes VR from 64 workgroups up.
-template <int NB, bool MULTI, bool MB = false, bool VR = false, bool CR = false>
+//
+// ALL: every row sees all of the pos0 keys and no others (a drafted tree's nodes and their context), instead
+// of the causal pos0 + t + 1.
+template <int NB, bool MULTI, bool MB = false, bool VR = false, bool CR = false, bool ALL = false>
 __device__ __forceinline__ void decode_partial(const float* __restrict__ q, int qts, const uint16_t* __restrict__ kc,
                                                const uint16_t* __restrict__ vc, int kvd, int pos0, int nh, int nkv,
                                                int nt, float scale, float* __restrict__ part, int chunk, int smax,
@@ -172,7 +175,7 @@ __device__ __forceinline__ void decode_partial(const float* __restrict__ q, int 
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, c = l & 15, g = l >> 4;
     const int tmax = (min(R, r0 + ROWS) - 1) / G;
     const int p0 = s * chunk;
-    const int pend = min(p0 + chunk, pos0 + tmax + 1);
+    const int pend = min(p0 + chunk, ALL ? pos0 : pos0 + tmax + 1);
     if (p0 >= pend) return;   // no row of this group sees these keys; the combine never reads them
     const float sc2 = scale * LOG2E_F;
     const size_t head_off = (size_t)kh * HD;
@@ -210,7 +213,7 @@ __device__ __forceinline__ void decode_partial(const float* __restrict__ q, int 
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int rr = r0 + 8 * b + (c & 7);
-        lim[b] = rr < R ? pos0 + rr / G + 1 : 0;
+        lim[b] = rr < R ? (ALL ? pos0 : pos0 + rr / G + 1) : 0;
         m_run[b] = -INFINITY;
     }
     f4 acc[NB][4], lacc[NB];   // O over this wave's 64 dims, and P times a ones column (row sums)
@@ -413,13 +416,13 @@ __device__ __forceinline__ void decode_partial(const float* __restrict__ q, int 
     }
 }
 
-template <int NB, bool MULTI, bool VR = false, bool CR = false>
+template <int NB, bool MULTI, bool VR = false, bool CR = false, bool ALL = false>
 __global__ __launch_bounds__(256) void attn_decode_kernel(const float* __restrict__ q, int qts,
                                                           const uint16_t* __restrict__ kc,
                                                           const uint16_t* __restrict__ vc, int kvd, int pos0, int nh,
                                                           int nkv, int nt, float scale, float* __restrict__ part,
                                                           int chunk, int smax) {
-    decode_partial<NB, MULTI, false, VR, CR>(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, smax, blockIdx.x, blockIdx.y,
+    decode_partial<NB, MULTI, false, VR, CR, ALL>(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, smax, blockIdx.x, blockIdx.y,
                        blockIdx.z);
 }
 
@@ -878,6 +881,38 @@ hipError_t launch_attn_partials(const float* q, int qts, const uint16_t* kc, con
     }
 #undef IT_DECODE_LAUNCH
 #undef IT_DECODE_LAUNCH2
+    return hipGetLastError();
+}
+
+// 260-word records of all nt tokens over keys 0 .. n-1, in splits of `chunk` keys (n > 0).
+hipError_t launch_attn_all_partials(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int n,
+                                    int nh, int nkv, int nt, float scale, float* part, int chunk, hipStream_t st) {
+    const int R = nt * (nh / nkv), smax = idx::split_count(n, chunk);
+    const bool multi = chunk > TK;
+    // blocks of rows as in launch_attn_partials
+    const int rows = multi ? (R <= 8 ? 8 : R <= 16 ? 16 : R <= 24 ? 24 : 32) : (R <= 16 ? 8 : R <= 32 ? 16 : 32);
+    const dim3 grid(smax, nkv, (R + rows - 1) / rows);
+#define IT_ALL(NB_, M_, VR_)                                                                                       \
+    attn_decode_kernel<NB_, M_, VR_, false, true><<<grid, 256, 0, st>>>(q, qts, kc, vc, kvd, n, nh, nkv, nt, scale, part, \
+                                                                       chunk, smax)
+    const bool vr = !multi && rows == 8 && (long)grid.x * grid.y * grid.z >= 64;
+    switch (rows / 8) {
+        case 1:
+            if (multi) IT_ALL(1, true, false);
+            else if (vr) IT_ALL(1, false, true);
+            else IT_ALL(1, false, false);
+            break;
+        case 2:
+            if (multi) IT_ALL(2, true, false);
+            else IT_ALL(2, false, false);
+            break;
+        case 3: IT_ALL(3, true, false); break;
+        default:
+            if (multi) IT_ALL(4, true, false);
+            else IT_ALL(4, false, false);
+            break;
+    }
+#undef IT_ALL
     return hipGetLastError();
 }
 

@@ -109,6 +109,14 @@ hipError_t launch_mfma_peak(int wgs, int iters, float* out, hipStream_t st);
 hipError_t launch_tree_plan(const int* parent, int nt, int p0, uint64_t* anc, int* pos, hipStream_t st);
 hipError_t launch_kv_tree_commit(void* kc, void* vc, size_t row_bytes, int pos0, const uint64_t* anc, int leaf,
                                  hipStream_t st);
+// part: the 260-word records of the pos0 context keys in splits of chunk keys (attn_tree_chunk's or any other
+// multiple of 64), unused where pos0 is 0
+hipError_t launch_attn_all_partials(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int n,
+                                    int nh, int nkv, int nt, float scale, float* part, int chunk, hipStream_t st);
+int attn_tree_chunk(int pos0, int nt, int nh, int nkv);
+hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0,
+                            int nh, int nkv, int nt, const uint64_t* anc, float scale, float* out, int ots,
+                            float* part, int chunk, hipStream_t st);
 // KVT uint16_t (f16 cache) or float; pos null: token t at pos0 + t
 template <class KVT>
 hipError_t launch_attn_prep_pos(float* q, int qts, const float* k, const float* v, int kts, const float* qw,

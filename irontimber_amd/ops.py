@@ -550,6 +550,42 @@ def tree_plan(parent: torch.Tensor, p0: int) -> tuple[torch.Tensor, torch.Tensor
     return anc, pos
 
 
+def attn_tree_scratch_bytes(pos0: int, nt: int, nh: int, nkv: int, hd: int = 256) -> int:
+    return lib().it_attn_tree_scratch_bytes(pos0, nt, hd, nh, nkv)
+
+
+def attn_tree_f16(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, pos0: int, nh: int, nkv: int, anc: torch.Tensor,
+                  scale: float | None = None, out: torch.Tensor | None = None,
+                  scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """attn_f16 for the nodes of a drafted tree: q [nt, nh*2*hd] f32, nodes in cache rows pos0 + t, anc [nt] int64
+    (tree_plan) -> out [nt, nh*hd] f32; zeros for padding nodes (it_attn_tree_f16)."""
+    dev = q.device
+    _need_all(torch.float32, dev, q=q)
+    if q.dim() != 2 or q.shape[1] % (2 * nh) != 0:
+        raise ValueError("q must be [nt, nh*2*hd]")
+    nt, hd = q.shape[0], q.shape[1] // (2 * nh)
+    kvd = nkv * hd
+    _need_cache(kc, "kc", _F16, dev, kvd, pos0 + nt)
+    _need_cache(vc, "vc", _F16, dev, kvd, pos0 + nt)
+    _need_anc(anc, dev, nt)
+    if scale is None:
+        scale = 1.0 / hd ** 0.5
+    if out is None:
+        out = torch.empty(nt, nh * hd, device=dev, dtype=torch.float32)
+    _need_all(torch.float32, dev, out=out)
+    if out.shape != (nt, nh * hd):
+        raise ValueError("out must be [nt, nh*hd]")
+    if scratch is None:
+        need = attn_tree_scratch_bytes(pos0, nt, nh, nkv, hd)
+        scratch = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    elif scratch.device != dev or not scratch.is_contiguous():
+        raise ValueError(f"scratch must be contiguous, on {dev}")
+    nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    _call_on(q, "it_attn_tree_f16", q.data_ptr(), nh * 2 * hd, kc.data_ptr(), vc.data_ptr(), kvd, pos0, hd, nh, nkv, nt,
+             anc.data_ptr(), float(scale), out.data_ptr(), nh * hd, _ptr(scratch), nbytes)
+    return out
+
+
 def _kv_tree_commit(name, kinds, kc, vc, pos0, nt, anc, leaf):
     if not kc.is_cuda or kc.dim() != 2:
         raise ValueError("kc must be a device tensor [rows, kvd]")

@@ -51,6 +51,30 @@ def test_kv_tree_commit_refusals(kw):
             assert getattr(_lib.lib(), name)(F, F, 512, 9, 5, F, -1, None) == 0     # nothing kept: nothing runs
 
 
+@pytest.mark.parametrize("kw", [dict(q=None), dict(kc=None), dict(vc=None), dict(anc=None), dict(out=None), dict(q=F + 8),
+                                dict(out=F + 4), dict(scratch=F + 8), dict(scratch=None), dict(nbytes=5 * 4 * 1040 - 1),
+                                dict(hd=128), dict(nh=6), dict(kvd=256), dict(nt=0), dict(nt=65), dict(pos0=-1),
+                                dict(pos0=(1 << 22) - 4), dict(qts=4 * 512 - 4), dict(ots=1020), dict(qts=2050)])
+def test_attn_tree_refusals(kw):
+    a = dict(q=F, qts=4 * 512, kc=F, vc=F, kvd=512, pos0=700, hd=256, nh=4, nkv=2, nt=5, anc=F, scale=0.0625, out=F,
+             ots=4 * 256, scratch=F, nbytes=1 << 30)
+    a.update(kw)
+    refused("it_attn_tree_f16", *a.values(), None, text="it_attn")
+
+
+@pytest.mark.parametrize("nh,nkv", [(16, 2), (24, 4), (4, 4), (16, 1)])
+def test_attn_tree_scratch(nh, nkv):
+    """The preferred scratch holds whole records, is never below one per (node, head), and stays below 64 MiB."""
+    f = _lib.lib().it_attn_tree_scratch_bytes
+    for nt in (1, 2, 5, 17, 64):
+        assert f(0, nt, 256, nh, nkv) == 0
+        for pos0 in (1, 63, 64, 65, 1000, 8128, 131072, (1 << 22) - nt):
+            got = f(pos0, nt, 256, nh, nkv)
+            assert got % (nt * nh * 1040) == 0 and nt * nh * 1040 <= got <= 64 << 20
+    for bad in ((100, 0, 256, nh, nkv), (100, 65, 256, nh, nkv), (-1, 3, 256, nh, nkv), (100, 3, 256, nh, 0)):
+        assert f(*bad) == 0
+
+
 def freqs(*args):
     f, m = (ctypes.c_float * max(args[0] // 2, 1))(), ctypes.c_float()
     assert _lib.lib().it_rope_freqs(*args, f, ctypes.byref(m)) == 0, _lib.last_error()

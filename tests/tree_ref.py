@@ -57,3 +57,37 @@ def norm_rotate(x, w, eps, pos, freq, mscale, pairs):
     y[..., b] = x[..., a] * s + x[..., b] * c
     size[..., a] = size[..., b] = (np.abs(x[..., a]) + np.abs(x[..., b])) * abs(mscale)
     return y, size
+
+
+def attn(q, k, v, pos0, nh, nkv, anc, scale):
+    """f64 attention of tree nodes: q [nt, nh, 2*hd], k / v [rows, nkv*hd] (hidden rows are not looked at). Returns out
+    [nt, nh, hd] and a bound of an f32 computation's error from it, element by element."""
+    nt, hd = q.shape[0], q.shape[2] // 2
+    rows = len(k)
+    q = q.astype(np.float64)
+    k, v = (x.reshape(rows, nkv, hd) for x in (k, v))
+    out, tol = np.zeros((nt, nh, hd)), np.zeros((nt, nh, hd))
+    for kh in range(nkv):
+        heads = np.arange(nh // nkv) + kh * (nh // nkv)
+        kp, vp = k[:pos0, kh].astype(np.float64), v[:pos0, kh].astype(np.float64)
+        for t in range(nt):
+            own = [j for j in range(nt) if int(anc[t]) >> j & 1]
+            if not own:
+                continue
+            kk = np.concatenate([kp, k[pos0 + np.array(own), kh].astype(np.float64)])
+            vv = np.concatenate([vp, v[pos0 + np.array(own), kh].astype(np.float64)])
+            qt = q[t, heads, :hd]
+            s = scale * qt @ kk.T
+            p = np.exp(s - s.max(-1, keepdims=True))
+            l = p.sum(-1, keepdims=True)
+            o = p @ vv / l
+            gate = 1 / (1 + np.exp(-q[t, heads, hd:]))
+            # scores: q as two f16 (2^-22), 256 additions of independent roundings (16 steps of 2^-24); weights: two
+            # f16 of the largest weight's size (2^-25 a key) and the exponentials (4 steps); the sums alike 16, the
+            # division, the gate and the products 8
+            size = scale * (np.abs(qt) @ np.abs(kk).T).max(-1, keepdims=True)
+            vmax = np.abs(vv).max(0)
+            rel = 2 * (20 * size + 4) + 32
+            out[t, heads] = o * gate
+            tol[t, heads] = (rel * 2.0 ** -24 + len(kk) * 2.0 ** -25 / l) * vmax * gate
+    return out, tol
