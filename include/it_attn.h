@@ -491,6 +491,28 @@ int it_kv_tree_commit_f16(uint16_t* kc, uint16_t* vc, int kvd, int pos0, int nt,
 int it_kv_tree_commit_f32(float* kc, float* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,
                           void* stream);
 
+/* The recurrent layer over a tree: conv + SiLU over each node's own ancestors (before the first node of a path, the conv
+ * state), q/k L2 norm and the gated delta rule along every path, for all nodes at once, in one launch. For a
+ * chain it computes what it_gdn_decode_fused does for consecutive tokens.
+ *   x, w, K, beta_raw, alpha_raw, dt, a, eps: as for it_gdn_decode_fused (x 16-byte aligned, its stride % 4 == 0)
+ *   conv_state [(K-1)][cd], state [nv][S][S]: the committed states, only read
+ *   anc: bits after t and a node whose own bit is clear (padding: zeros out) are ignored
+ *   out [t*out_tok_stride + h*S + j], as it_gdn_step's
+ *   trace: it_gdn_tree_trace_bytes(...) bytes, 16-byte aligned, one per layer: what it_gdn_tree_commit needs
+ * f32 throughout (the decays of a path are summed in f64). A node's result does not depend on nodes that are not its
+ * ancestors, whatever their inputs hold. */
+size_t it_gdn_tree_trace_bytes(int nt, int nv, int nk, int S);
+int it_gdn_tree(const float* x, int x_tok_stride, const float* w, int K, const float* conv_state,
+                const float* beta_raw, const float* alpha_raw, int ba_tok_stride, const float* dt, const float* a,
+                const float* state, const uint64_t* anc, float* out, int out_tok_stride, int nt, int nv, int nk, int S,
+                float eps, void* trace, size_t trace_bytes, void* stream);
+
+/* conv_state and state <- those after node `leaf` of the it_gdn_tree call that wrote trace (the same x, anc, nt and
+ * head counts; both updated in place). leaf = -1, or a padding node: they stay. Stands where it_gdn_rollback does for a
+ * chain. */
+int it_gdn_tree_commit(const float* x, int x_tok_stride, int K, float* conv_state, float* state, const uint64_t* anc,
+                       int leaf, int nt, int nv, int nk, int S, const void* trace, size_t trace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------------
  * Reference-shaped dispatch policy (pure host functions, no device access).
  * ---------------------------------------------------------------------------------------------- */

@@ -81,6 +81,10 @@ SIGNATURES = {
     "it_attn_tree_scratch_bytes": (c_size_t, [c_int] * 5),
     "it_attn_tree_f16": (c_int, [P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, P, c_float, P, c_int, P,
                                  c_size_t, P]),
+    "it_gdn_tree_trace_bytes": (c_size_t, [c_int] * 4),
+    "it_gdn_tree": (c_int, [P, c_int, P, c_int, P, P, P, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_float,
+                            P, c_size_t, P]),
+    "it_gdn_tree_commit": (c_int, [P, c_int, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_size_t, P]),
     "it_kv_tree_commit_f16": (c_int, [P, P, c_int, c_int, c_int, P, c_int, P]),
     "it_kv_tree_commit_f32": (c_int, [P, P, c_int, c_int, c_int, P, c_int, P]),
     "it_prefill_chunks": (ctypes.c_long, [c_size_t, c_size_t, P, P, c_size_t]),

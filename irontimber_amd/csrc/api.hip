@@ -872,6 +872,52 @@ int it_gdn_decode_fused_ckpt(const float* x, int xts, const float* w, int K, con
                  who);
 }
 
+size_t it_gdn_tree_trace_bytes(int nt, int nv, int nk, int S) {
+    if (nt < 1 || nt > IT_TREE_MAX || nv <= 0 || nk <= 0 || nv % nk != 0 || S != 128) return 0;
+    return it::gdn_tree_trace_bytes(nt, nv, nk);
+}
+
+static int validate_gdn_tree(const char* who, const float* x, int xts, int K, const float* cst, const float* state,
+                             const uint64_t* anc, int nt, int nv, int nk, int S, const void* trace, size_t trace_bytes) {
+    if (S != 128) return fail("%s: state size %d unsupported (128)", who, S);
+    if (nv <= 0 || nk <= 0 || nv % nk != 0) return fail("%s: nv %d / nk %d invalid", who, nv, nk);
+    if (nt < 1 || nt > IT_TREE_MAX) return fail("%s: nt %d must be in [1, %d]", who, nt, IT_TREE_MAX);
+    if (K < 2 || K > 4) return fail("%s: kernel size %d unsupported (2..4)", who, K);
+    if (!x || !cst || !state || !anc || !trace) return fail("%s: null buffer", who);
+    if (!aligned16(x) || !aligned16(cst) || !aligned16(state) || !aligned16(trace))
+        return fail("%s: x / conv state / state / trace must be 16-byte aligned", who);
+    if (xts % 4 != 0 || (nt > 1 && xts < (2 * nk + nv) * S))
+        return fail("%s: token stride %d must be a multiple of 4 and hold a row", who, xts);
+    if (trace_bytes < it::gdn_tree_trace_bytes(nt, nv, nk))
+        return fail("%s: trace of %zu bytes, %zu needed", who, trace_bytes, it::gdn_tree_trace_bytes(nt, nv, nk));
+    return 0;
+}
+
+int it_gdn_tree(const float* x, int xts, const float* w, int K, const float* conv_state, const float* br,
+                const float* ar, int bts, const float* dt, const float* a, const float* state, const uint64_t* anc,
+                float* out, int ots, int nt, int nv, int nk, int S, float eps, void* trace, size_t trace_bytes,
+                void* stream) {
+    const char* who = "it_gdn_tree";
+    if (validate_gdn_tree(who, x, xts, K, conv_state, state, anc, nt, nv, nk, S, trace, trace_bytes)) return -1;
+    if (!w || !br || !ar || !dt || !a || !out) return fail("%s: null buffer", who);
+    if (nt > 1 && (ots < nv * S || bts < nv)) return fail("%s: token strides overlap rows", who);
+    if (!(eps >= 0.0f)) return fail("%s: eps must be >= 0", who);
+    return check(it::launch_gdn_tree(x, xts, w, K, conv_state, br, ar, bts, dt, a, state, anc, out, ots, nt, nv, nk, eps,
+                                     (float*)trace, (hipStream_t)stream),
+                 who);
+}
+
+int it_gdn_tree_commit(const float* x, int xts, int K, float* conv_state, float* state, const uint64_t* anc, int leaf,
+                       int nt, int nv, int nk, int S, const void* trace, size_t trace_bytes, void* stream) {
+    const char* who = "it_gdn_tree_commit";
+    if (validate_gdn_tree(who, x, xts, K, conv_state, state, anc, nt, nv, nk, S, trace, trace_bytes)) return -1;
+    if (leaf < -1 || leaf >= nt) return fail("%s: leaf %d must be in [-1, %d)", who, leaf, nt);
+    if (leaf < 0) { g_err.clear(); return 0; }
+    return check(it::launch_gdn_tree_commit(x, xts, K, conv_state, state, anc, leaf, nt, nv, nk, (const float*)trace,
+                                            (hipStream_t)stream),
+                 who);
+}
+
 int it_gdn_step_ckpt(const float* co, int cts, const float* br, const float* ar, int bts, const float* dt,
                      const float* a, float* state, float* out, int ots, int nt, int nv, int nk, int S, float* ck_state,
                      int ck_after, void* stream) {

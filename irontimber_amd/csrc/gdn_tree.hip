@@ -1,0 +1,382 @@
+// The Gated-DeltaNet layer over a drafted token tree, and the commit of one node's states.
+//
+// The recurrence of cpu.rs:216-232 along every root-to-node path at once. With g_i a node's log decay, G_i
+// its sum over the node's path (ancestors and itself) and S0 the committed state, the path's states unroll as in
+// the chunk form of the delta rule, the causal mask replaced by "is an ancestor of":
+//   A_ij = beta_i (k_i . k_j) e^(G_i - G_j)            j a strict ancestor of i, else 0
+//   (I + A) U = beta (V - e^G (K S0))                    row i: the update u_i that node i adds to the state
+//   out_i = (e^G_i q_i S0 + sum_j (q_i . k_j) e^(G_i - G_j) u_j) / sqrt(S)     j an ancestor of i or i itself
+// Topological order makes A strictly lower triangular. G is summed in f64: far down a strongly decaying path
+// the differences would lose f32's digits. All products are f32 (v_mfma_f32_16x16x4_f32).
+// The commit writes S_i = e^G_i S0 + sum_j e^(G_i - G_j) k_j u_j over i's path from the U, k and G that the layer
+// call leaves in its trace. No counterpart in the reference, which steps one token at a time
+// (src/vk/mod.rs:790-806) and copies checkpoints (1018-1025).
+#include "common.h"
+#include "internal.h"
+
+namespace it {
+
+namespace {
+constexpr int S = 128;        // state size, and channels per head
+constexpr int CW = 16;        // state columns per workgroup
+constexpr int KST = S + 4;    // LDS row of a q or k row (floats)
+constexpr int RST = CW + 4;   // LDS row of a node's CW columns
+
+__device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Node t's mask with later nodes' bits off; 0 for a padding node (its own bit is clear).
+__device__ __forceinline__ uint64_t node_mask(const uint64_t* anc, int t) {
+    const uint64_t m = anc[t] & (~(uint64_t)0 >> (63 - t));
+    return m >> t & 1 ? m : 0;
+}
+
+// The conv input j tokens before node t on its path: an ancestor's row of x, or beyond the path's start a
+// row of the conv state (K - 1 rows, oldest first). m: t's mask, dropped bit by bit as the taps walk up.
+template <int K>
+struct Taps {
+    const float* row[K];   // row[j]: the tap's input row, j tokens back
+    __device__ __forceinline__ Taps(uint64_t m, const float* x, int xts, const float* cst, int cd) {
+        int beyond = K - 2;   // the state's newest row first
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const int a = 63 - (int)__builtin_clzll(m | 1);
+            row[j] = m ? x + (size_t)a * xts : cst + (size_t)(beyond--) * cd;
+            if (m) m &= ~((uint64_t)1 << a);
+        }
+    }
+};
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+}  // namespace
+
+// Workgroup = (V head h, CW = 16 state columns), four waves; NB blocks of 16 nodes. A head's q and k rows are
+// convolved and normalised by each of its eight workgroups (into LDS), so no launch or barrier of the whole
+// GPU stands between the conv and the products. The waves share the products out in 16x16 tasks; the inverses of
+// I + A's diagonal blocks go one to a wave, and then every wave solves for all of U in registers (a few
+// products more than one wave's share, but no exchange) and writes the output rows of its block.
+template <int K, int NB>
+__global__ __launch_bounds__(256) void gdn_tree_kernel(
+    const float* __restrict__ x, int xts, const float* __restrict__ cw, const float* __restrict__ cst,
+    const float* __restrict__ br, const float* __restrict__ ar, int bts, const float* __restrict__ dt,
+    const float* __restrict__ A, const float* __restrict__ state, const uint64_t* __restrict__ anc,
+    float* __restrict__ out, int ots, int nt, int nv, int nk, float eps, float* __restrict__ trace) {
+    constexpr int N = 16 * NB, AST = N + 4;
+    __shared__ __align__(16) float qk[2][N][KST];      // normalised q and k rows, zeros for padding
+    __shared__ __align__(16) float na[N][AST];         // -A
+    __shared__ __align__(16) float pm[N][AST];         // (q_i . k_j) e^(G_i - G_j)
+    __shared__ __align__(16) float tin[NB][16][20];    // inverses of the diagonal blocks of I + A
+    __shared__ float vs[N][RST], rs[N][RST], os[N][RST];   // conv'd V, right-hand sides, e^G q S0
+    __shared__ double gs[N];
+    __shared__ float bs[N];
+    __shared__ uint64_t ms[N];
+    __shared__ int spoilt;                             // a value that is not finite went into the products
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, c = l & 15, g = l >> 4;
+    const int cb = blockIdx.x & 7, h = blockIdx.x >> 3, kh = h % nk, cd = (2 * nk + nv) * S;
+    const float* sb = state + (size_t)h * S * S + cb * CW + c;
+
+    // The state slice as the B operand of the S0 products, in the order of the A operand's 16-byte reads: lane
+    // (c, g) holds column c of rows 16 kk + 4 g + e.
+    float s0[8][4];
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s0[kk][e] = sb[(size_t)(16 * kk + 4 * g + e) * S];
+
+    // ---- masks, gates and path sums, a node a lane of wave 0
+    if (w == 0) {
+        const uint64_t m = l < nt ? node_mask(anc, l) : 0;
+        double G = 0.0;
+        float beta = 0.f;
+        if (m) {
+            beta = sigmoidf_(br[(size_t)l * bts + h]);
+            const float lg = softplusf_(ar[(size_t)l * bts + h] + dt[h]) * A[h];
+            G = lg < -200.f ? -200.0 : (double)lg;   // e^-200 is 0 in f32 already; sums stay finite
+        }
+        const uint64_t above = m & ~((uint64_t)1 << l);
+        int up = above ? 63 - (int)__builtin_clzll(above) : -1;
+#pragma unroll
+        for (int r = 1; r < N; r *= 2) {   // after round r a node's sum covers its nearest 2r nodes
+            const double more = __shfl(G, up < 0 ? l : up);
+            const int next = __shfl(up, up < 0 ? l : up);
+            if (up >= 0) { G += more; up = next; }
+        }
+        if (l < N) { ms[l] = m; gs[l] = G; bs[l] = beta; }
+        if (l == 0) spoilt = 0;
+    }
+    // ---- conv + SiLU + L2 norm of the q and k heads: lanes 0-31 four q channels each, lanes 32-63 k
+    {
+        const int ch = (l < 32 ? kh : nk + kh) * S + 4 * (l & 31);
+        f4 wt[K];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < K; ++i) wt[i][e] = cw[(size_t)(ch + e) * K + i];
+#pragma unroll 4
+        for (int i = 0; i < N / 4; ++i) {
+            const int t = 4 * i + w;
+            f4 y = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t m = t < nt ? node_mask(anc, t) : 0;
+            if (m) {
+                const Taps<K> tap(m, x, xts, cst, cd);
+#pragma unroll
+                for (int j = K - 1; j >= 0; --j) y += ld_f4(tap.row[j] + ch) * wt[K - 1 - j];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = siluf_(y[e]);
+                float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
+                ss += dppc<0xB1>(ss);
+                ss += dppc<0x4E>(ss);
+                ss += dppc<0x141>(ss);
+                ss += dppc<0x140>(ss);
+                ss = sum_xor16(ss);
+                y *= 1.0f / fmaxf(sqrtf(ss), eps);
+            }
+            *(f4*)&qk[l >> 5][t][4 * (l & 31)] = y;
+        }
+    }
+    // ---- conv + SiLU of the workgroup's V columns
+    {
+        const int ch = 2 * nk * S + h * S + cb * CW + (tid & 15);
+        float wt[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) wt[i] = cw[(size_t)ch * K + i];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int t = 16 * b + (tid >> 4);
+            float y = 0.f;
+            const uint64_t m = t < nt ? node_mask(anc, t) : 0;
+            if (m) {
+                const Taps<K> tap(m, x, xts, cst, cd);
+#pragma unroll
+                for (int j = K - 1; j >= 0; --j) y += tap.row[j][ch] * wt[K - 1 - j];
+                y = siluf_(y);
+            }
+            vs[t][tid & 15] = y;
+        }
+    }
+    __syncthreads();
+    // ---- products in 16x16 tasks: {K, Q} S0 of each block, then {K, Q} K^T of each pair of blocks bi >= bj
+    bool bad = false;
+    for (int task = w; task < 2 * NB + NB * (NB + 1); task += 4) {
+        const int which = (task & 1) ^ 1;   // 1 k rows, 0 q rows
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        if (task < 2 * NB) {
+            const int b = task >> 1;
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+                const f4 a = ld_f4(&qk[which][16 * b + c][16 * kk + 4 * g]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc = mfma4(a[e], s0[kk][e], acc);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = 16 * b + 4 * g + i;
+                const float d = acc[i] * expf((float)gs[t]);
+                const float v = which ? bs[t] * (vs[t][c] - d) : d;
+                (which ? rs : os)[t][c] = ms[t] ? v : 0.f;
+                bad |= ms[t] && !finite(v);
+            }
+        } else {
+            int p = (task - 2 * NB) >> 1, bi = 0;   // pair p of the lower triangle, row by row
+            while (p > bi) p -= ++bi;
+            const int bj = p;
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+                const f4 a = ld_f4(&qk[which][16 * bi + c][16 * kk + 4 * g]), b = ld_f4(&qk[1][16 * bj + c][16 * kk + 4 * g]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc = mfma4(a[e], b[e], acc);
+            }
+            const int j = 16 * bj + c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = 16 * bi + 4 * g + i;
+                const bool sees = (ms[t] >> j & 1) && (!which || j != t);
+                float v = acc[i] * expf((float)(gs[t] - gs[j]));
+                if (which) v *= -bs[t];
+                (which ? na : pm)[t][j] = sees ? v : 0.f;
+                bad |= sees && !finite(v);
+            }
+        }
+    }
+    if (bad) spoilt = 1;
+    __syncthreads();
+    const float scale = 1.0f / sqrtf((float)S);
+    float* tu = trace + (size_t)h * S + cb * CW;   // U rows, then k rows, then G
+    const size_t ustride = (size_t)nv * S;
+    if (spoilt) {
+        // The block products would carry a NaN or an infinity of one branch to others as 0 * NaN: the same sums node by
+        // node over the ancestors alone.
+        if (tid < CW) {
+            for (int t = 0; t < nt; ++t) {
+                float u = rs[t][tid], o = os[t][tid];
+                for (int j = 0; j < t; ++j)
+                    if (ms[t] >> j & 1) u += na[t][j] * rs[j][tid];
+                rs[t][tid] = u;
+                for (int j = 0; j <= t; ++j)
+                    if (ms[t] >> j & 1) o += pm[t][j] * rs[j][tid];
+                out[(size_t)t * ots + (size_t)h * S + cb * CW + tid] = o * scale;
+                tu[t * ustride + tid] = u;
+            }
+        }
+    } else {
+        // ---- (I + A_bb)^-1, lane column c, forward substitution on a column of the identity (the four lane
+        // groups alike)
+        if (w < NB) {
+            float z[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float v = i == c ? 1.f : 0.f;
+#pragma unroll
+                for (int j4 = 0; j4 < i; j4 += 4) {
+                    const f4 a = ld_f4(&na[16 * w + i][16 * w + j4]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j4 + j < i) v += a[j] * z[j4 + j];
+                }
+                z[i] = v;
+            }
+            if (g == 0) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) tin[w][i][c] = z[i];
+            }
+        }
+        __syncthreads();
+        // ---- U block by block: u[b] holds rows 4 g + e of column c, both a product's result and, in the order of
+        // the A operand's 16-byte reads, the next one's B operand
+        f4 u[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            f4 r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = rs[16 * b + 4 * g + i][c];
+#pragma unroll
+            for (int j = 0; j < b; ++j) {
+                const f4 a = ld_f4(&na[16 * b + c][16 * j + 4 * g]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r = mfma4(a[e], u[j][e], r);
+            }
+            const f4 a = ld_f4(&tin[b][c][4 * g]);
+            u[b] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[b] = mfma4(a[e], r[e], u[b]);
+        }
+        // ---- output and trace rows of block w
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (b != w) continue;   // (static register indexes)
+            f4 o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = os[16 * b + 4 * g + i][c];
+#pragma unroll
+            for (int j = 0; j <= b; ++j) {
+                const f4 a = ld_f4(&pm[16 * b + c][16 * j + 4 * g]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o = mfma4(a[e], u[j][e], o);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = 16 * b + 4 * g + i;
+                if (t < nt) {
+                    out[(size_t)t * ots + (size_t)h * S + cb * CW + c] = o[i] * scale;
+                    tu[t * ustride + c] = u[b][i];
+                }
+            }
+        }
+    }
+    // ---- the rest of the trace: k rows by the QK head's first V head, a sixteenth of the dims a workgroup; G once a head
+    if (h < nk) {
+        float* tk = trace + (size_t)nt * nv * S + (size_t)h * S + cb * CW;
+        for (int i = tid; i < nt * CW; i += 256)
+            tk[(size_t)(i / CW) * nk * S + i % CW] = qk[1][i / CW][cb * CW + i % CW];
+    }
+    if (cb == 0 && tid < nt) ((double*)(trace + (size_t)nt * (nv + nk) * S))[(size_t)tid * nv + h] = gs[tid];
+}
+
+size_t gdn_tree_trace_bytes(int nt, int nv, int nk) {
+    return (size_t)nt * (nv + nk) * S * sizeof(float) + (size_t)nt * nv * sizeof(double);
+}
+
+hipError_t launch_gdn_tree(const float* x, int xts, const float* cw, int K, const float* cst, const float* br,
+                           const float* ar, int bts, const float* dt, const float* a, const float* state,
+                           const uint64_t* anc, float* out, int ots, int nt, int nv, int nk, float eps, float* trace,
+                           hipStream_t st) {
+#define IT_GDN_TREE(K_, NB_)                                                                                       \
+    gdn_tree_kernel<K_, NB_><<<8 * nv, 256, 0, st>>>(x, xts, cw, cst, br, ar, bts, dt, a, state, anc, out, ots, nt, nv, nk, \
+                                                    eps, trace)
+#define IT_GDN_TREE_K(K_)                    \
+    switch ((nt + 15) / 16) {                \
+        case 1: IT_GDN_TREE(K_, 1); break;   \
+        case 2: IT_GDN_TREE(K_, 2); break;   \
+        case 3: IT_GDN_TREE(K_, 3); break;   \
+        default: IT_GDN_TREE(K_, 4); break;  \
+    }
+    switch (K) {
+        case 2: IT_GDN_TREE_K(2) break;
+        case 3: IT_GDN_TREE_K(3) break;
+        default: IT_GDN_TREE_K(4) break;
+    }
+#undef IT_GDN_TREE_K
+#undef IT_GDN_TREE
+    return hipGetLastError();
+}
+
+// Workgroups 0 .. 8 nv - 1: 16 state rows of a head, thread = (row, 8 columns), the path's rank-one updates on top
+// of the decayed state. The others: 256 channels of the conv state, whose rows are the last K - 1 inputs of
+// {old state, the path's rows of x}; a thread reads its channel's old rows before it writes any.
+__global__ __launch_bounds__(256) void gdn_tree_commit_kernel(const float* __restrict__ x, int xts, int K, float* cst,
+                                                              float* __restrict__ state,
+                                                              const uint64_t* __restrict__ anc, int leaf, int nt,
+                                                              int nv, int nk, const float* __restrict__ trace) {
+    __shared__ float coef[64];
+    __shared__ int node[64];
+    const int tid = threadIdx.x, cd = (2 * nk + nv) * S;
+    const uint64_t m = node_mask(anc, leaf);
+    const int np = (int)__popcll(m);
+    if (np == 0) return;   // a padding node: nothing is kept
+    const bool conv = blockIdx.x >= (unsigned)(8 * nv);
+    const int h = conv ? 0 : blockIdx.x >> 3;
+    const double* G = (const double*)(trace + (size_t)nt * (nv + nk) * S);
+    const double Gl = G[(size_t)leaf * nv + h];
+    if (tid < 64 && (m >> tid & 1)) {
+        const int i = (int)__popcll(m & (((uint64_t)1 << tid) - 1));
+        node[i] = tid;
+        coef[i] = expf((float)(Gl - G[(size_t)tid * nv + h]));
+    }
+    __syncthreads();
+    if (conv) {
+        const int ch = (blockIdx.x - 8 * nv) * 256 + tid;
+        if (ch >= cd) return;
+        float r[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {   // row i of the new state: input i + np of {old rows, path}
+            const int s = i + np;
+            if (i < K - 1) r[i] = s < K - 1 ? cst[(size_t)s * cd + ch] : x[(size_t)node[s - (K - 1)] * xts + ch];
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < K - 1) cst[(size_t)i * cd + ch] = r[i];
+        return;
+    }
+    const int row = (blockIdx.x & 7) * 16 + (tid >> 4), col = (tid & 15) * 8;
+    float* s = state + ((size_t)h * S + row) * S + col;
+    const float* tu = trace + (size_t)h * S + col;
+    const float* tk = trace + (size_t)nt * nv * S + (size_t)(h % nk) * S + row;
+    const float eg = expf((float)Gl);
+    f4 s0 = ld_f4(s) * eg, s1 = ld_f4(s + 4) * eg;
+#pragma unroll 4
+    for (int i = 0; i < np; ++i) {
+        const float* u = tu + (size_t)node[i] * nv * S;
+        const float k = tk[(size_t)node[i] * nk * S] * coef[i];
+        s0 += k * ld_f4(u);
+        s1 += k * ld_f4(u + 4);
+    }
+    *(f4*)s = s0;
+    *(f4*)(s + 4) = s1;
+}
+
+hipError_t launch_gdn_tree_commit(const float* x, int xts, int K, float* cst, float* state, const uint64_t* anc,
+                                  int leaf, int nt, int nv, int nk, const float* trace, hipStream_t st) {
+    const int cd = (2 * nk + nv) * S;
+    gdn_tree_commit_kernel<<<8 * nv + (cd + 255) / 256, 256, 0, st>>>(x, xts, K, cst, state, anc, leaf, nt, nv, nk, trace);
+    return hipGetLastError();
+}
+
+}  // namespace it

@@ -117,6 +117,14 @@ int attn_tree_chunk(int pos0, int nt, int nh, int nkv);
 hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0,
                             int nh, int nkv, int nt, const uint64_t* anc, float scale, float* out, int ots,
                             float* part, int chunk, hipStream_t st);
+// trace: U [nt][nv*S], k [nt][nk*S] (f32), G [nt][nv] (f64), written by launch_gdn_tree, read by the commit
+size_t gdn_tree_trace_bytes(int nt, int nv, int nk);
+hipError_t launch_gdn_tree(const float* x, int xts, const float* cw, int K, const float* cst, const float* br,
+                           const float* ar, int bts, const float* dt, const float* a, const float* state,
+                           const uint64_t* anc, float* out, int ots, int nt, int nv, int nk, float eps, float* trace,
+                           hipStream_t st);
+hipError_t launch_gdn_tree_commit(const float* x, int xts, int K, float* cst, float* state, const uint64_t* anc,
+                                  int leaf, int nt, int nv, int nk, const float* trace, hipStream_t st);
 // KVT uint16_t (f16 cache) or float; pos null: token t at pos0 + t
 template <class KVT>
 hipError_t launch_attn_prep_pos(float* q, int qts, const float* k, const float* v, int kts, const float* qw,

@@ -606,3 +606,51 @@ def kv_tree_commit_f16(kc: torch.Tensor, vc: torch.Tensor, pos0: int, nt: int, a
 def kv_tree_commit_f32(kc: torch.Tensor, vc: torch.Tensor, pos0: int, nt: int, anc: torch.Tensor, leaf: int) -> None:
     """kv_tree_commit_f16 for the MTP head's f32 cache."""
     _kv_tree_commit("it_kv_tree_commit_f32", _F32, kc, vc, pos0, nt, anc, leaf)
+
+
+def gdn_tree_trace(nt: int, nv: int, nk: int, device) -> torch.Tensor:
+    """A buffer for what gdn_tree leaves to gdn_tree_commit: one per layer, for trees of up to nt nodes."""
+    return torch.empty(lib().it_gdn_tree_trace_bytes(nt, nv, nk, 128), device=device, dtype=torch.uint8)
+
+
+def _need_gdn_tree(x, conv_state, state, anc, nv, nk, trace):
+    dev = x.device
+    _need_all(torch.float32, dev, x=x, conv_state=conv_state, state=state)
+    cd = (2 * nk + nv) * 128
+    if x.dim() != 2 or x.shape[1] != cd:
+        raise ValueError(f"x must be [nt, {cd}]")
+    if state.shape != (nv, 128, 128):
+        raise ValueError(f"state must be [{nv}, 128, 128]")
+    if conv_state.dim() != 2 or conv_state.shape[1] != cd:
+        raise ValueError(f"conv_state must be [K-1, {cd}]")
+    _need_anc(anc, dev, x.shape[0])
+    _need_all(torch.uint8, dev, trace=trace)
+
+
+def gdn_tree(x: torch.Tensor, w: torch.Tensor, conv_state: torch.Tensor, beta_raw: torch.Tensor, alpha_raw: torch.Tensor,
+             dt: torch.Tensor, a: torch.Tensor, state: torch.Tensor, anc: torch.Tensor, nv: int, nk: int,
+             trace: torch.Tensor, eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The recurrent layer over a drafted tree in one launch: x [nt, (2nk+nv)*128], w [cd, K], conv_state [K-1, cd] and
+    state [nv, 128, 128] (both only read), beta_raw/alpha_raw [nt, nv], anc [nt] int64 (tree_plan) -> out
+    [nt, nv*128]; trace (gdn_tree_trace) keeps what gdn_tree_commit needs (it_gdn_tree)."""
+    _need_gdn_tree(x, conv_state, state, anc, nv, nk, trace)
+    dev, nt, K = x.device, x.shape[0], conv_state.shape[0] + 1
+    if out is None:
+        out = torch.empty(nt, nv * 128, device=dev, dtype=torch.float32)
+    _need_all(torch.float32, dev, w=w, beta_raw=beta_raw, alpha_raw=alpha_raw, dt=dt, a=a, out=out)
+    if w.shape != (x.shape[1], K) or beta_raw.shape != (nt, nv) or alpha_raw.shape != (nt, nv) or dt.numel() != nv or \
+            a.numel() != nv or out.shape != (nt, nv * 128):
+        raise ValueError("w must be [cd, K], beta_raw / alpha_raw [nt, nv], dt / a [nv] and out [nt, nv*128]")
+    _call_on(x, "it_gdn_tree", x.data_ptr(), x.shape[1], w.data_ptr(), K, conv_state.data_ptr(), beta_raw.data_ptr(),
+             alpha_raw.data_ptr(), nv, dt.data_ptr(), a.data_ptr(), state.data_ptr(), anc.data_ptr(), out.data_ptr(),
+             nv * 128, nt, nv, nk, 128, float(eps), trace.data_ptr(), trace.numel())
+    return out
+
+
+def gdn_tree_commit(x: torch.Tensor, conv_state: torch.Tensor, state: torch.Tensor, anc: torch.Tensor, leaf: int, nv: int,
+                    nk: int, trace: torch.Tensor) -> None:
+    """conv_state and state <- those after node leaf of the gdn_tree call that wrote trace (the same x and anc); leaf -1:
+    they stay (it_gdn_tree_commit)."""
+    _need_gdn_tree(x, conv_state, state, anc, nv, nk, trace)
+    _call_on(x, "it_gdn_tree_commit", x.data_ptr(), x.shape[1], conv_state.shape[0] + 1, conv_state.data_ptr(),
+             state.data_ptr(), anc.data_ptr(), leaf, x.shape[0], nv, nk, 128, trace.data_ptr(), trace.numel())

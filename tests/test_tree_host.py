@@ -75,6 +75,38 @@ def test_attn_tree_scratch(nh, nkv):
         assert f(*bad) == 0
 
 
+@pytest.mark.parametrize("kw", [dict(x=None), dict(conv=None), dict(state=None), dict(anc=None), dict(trace=None),
+                                dict(x=F + 4), dict(conv=F + 4), dict(state=F + 8), dict(trace=F + 8), dict(nt=0),
+                                dict(nt=65), dict(K=1), dict(K=5), dict(S=64), dict(nv=5), dict(nk=0), dict(xts=1020),
+                                dict(xts=1026), dict(nbytes=5 * 6 * 512 + 5 * 4 * 8 - 1)])
+def test_gdn_tree_refusals(kw):
+    a = dict(x=F, xts=1024, w=F, K=4, conv=F, beta=F, alpha=F, bts=4, dt=F, a=F, state=F, anc=F, out=F, ots=512, nt=5, nv=4,
+             nk=2, S=128, eps=1e-6, trace=F, nbytes=5 * 6 * 512 + 5 * 4 * 8)
+    a.update(kw)
+    refused("it_gdn_tree", *a.values(), None, text="it_gdn_tree")
+    commit = ("x", "xts", "K", "conv", "state", "anc", 2, "nt", "nv", "nk", "S", "trace", "nbytes")
+    refused("it_gdn_tree_commit", *(a.get(k, k) for k in commit), None, text="it_gdn_tree_commit")
+
+
+@pytest.mark.parametrize("kw", [dict(w=None), dict(beta=None), dict(alpha=None), dict(dt=None), dict(a=None), dict(out=None),
+                                dict(ots=508), dict(bts=3), dict(eps=math.nan)])
+def test_gdn_tree_layer_refusals(kw):
+    a = dict(x=F, xts=1024, w=F, K=4, conv=F, beta=F, alpha=F, bts=4, dt=F, a=F, state=F, anc=F, out=F, ots=512, nt=5, nv=4,
+             nk=2, S=128, eps=1e-6, trace=F, nbytes=1 << 20)
+    a.update(kw)
+    refused("it_gdn_tree", *a.values(), None, text="it_gdn_tree")
+
+
+def test_gdn_tree_commit_leaf():
+    f = _lib.lib().it_gdn_tree_commit
+    for leaf in (-2, 5):
+        assert f(F, 1024, 4, F, F, F, leaf, 5, 4, 2, 128, F, 1 << 20, None) != 0 and "leaf" in _lib.last_error()
+    assert f(F, 1024, 4, F, F, F, -1, 5, 4, 2, 128, F, 1 << 20, None) == 0     # nothing kept: nothing runs
+    trace = _lib.lib().it_gdn_tree_trace_bytes
+    assert trace(5, 4, 2, 128) == 5 * 6 * 512 + 5 * 4 * 8
+    assert trace(0, 4, 2, 128) == trace(65, 4, 2, 128) == trace(5, 5, 2, 128) == trace(5, 4, 2, 64) == 0
+
+
 def freqs(*args):
     f, m = (ctypes.c_float * max(args[0] // 2, 1))(), ctypes.c_float()
     assert _lib.lib().it_rope_freqs(*args, f, ctypes.byref(m)) == 0, _lib.last_error()

@@ -91,3 +91,48 @@ def attn(q, k, v, pos0, nh, nkv, anc, scale):
             out[t, heads] = o * gate
             tol[t, heads] = (rel * 2.0 ** -24 + len(kk) * 2.0 ** -25 / l) * vmax * gate
     return out, tol
+
+
+def gdn(x, w, conv, beta, alpha, dt, a, state, par, nv, nk, eps):
+    """f64 recurrent layer node by node: out [nt, nv, 128] and a bound of an f32 computation's error, and per node the
+    state and its error bound (scalars per head), and the conv window."""
+    S, nt = 128, len(par)
+    x, w, conv, state = (z.astype(np.float64) for z in (x, w, conv, state))
+    K = w.shape[1]
+    out, tol = np.zeros((nt, nv, S)), np.zeros((nt, nv, S))
+    head = np.arange(nv) % nk
+    states, errs, windows = {-1: state}, {-1: np.zeros(nv)}, {-1: conv}
+    sig = lambda z: 1 / (1 + np.exp(-z))
+    for t in range(nt):
+        if path(par, t) is None:
+            continue
+        p = int(par[t])
+        win = np.concatenate([windows[p], x[t:t + 1]])
+        windows[t] = win[1:]
+        y = (win * w.T).sum(0)
+        size = (np.abs(win) * np.abs(w.T)).sum(0).reshape(-1, S).max(-1)     # of the sums that the conv rounds
+        y = (y * sig(y)).reshape(-1, S)
+        q, k, v = y[:nk], y[nk:2 * nk], y[2 * nk:]
+        norms = [np.maximum(np.linalg.norm(z, axis=-1, keepdims=True), eps) for z in (q, k)]
+        # relative error of a normalised row: conv and SiLU 6 steps of the sums' size, the norm 12
+        rq, rk = (6 * size[i * nk:(i + 1) * nk] * np.sqrt(S) / n[:, 0] + 12 for i, n in enumerate(norms))
+        q, k = (q / norms[0])[head], (k / norms[1])[head]
+        rq, rk = rq[head], rk[head]
+        b = sig(beta[t].astype(np.float64))
+        g = np.log1p(np.exp(alpha[t].astype(np.float64) + dt)) * a.astype(np.float64)
+        d = np.exp(g)
+        s = states[p] * d[:, None, None]
+        u = (v - np.einsum("hij,hi->hj", s, k)) * b[:, None]
+        states[t] = s + k[:, :, None] * u[:, None, :]
+        col = np.linalg.norm(s, axis=1).max(-1)                              # largest column norm of each head
+        # the update's error: v (6 steps of its sums, 8 more), S^T k (k's error, 16 steps of the sum, the decays 12, and
+        # what the state's columns are off by already), beta 6
+        vmax = np.abs(v).max(-1)
+        eu = 2.0 ** -24 * (6 * size[2 * nk:] + 14 * vmax + (rk + 34) * col) + errs[p] * d
+        umax = np.abs(u).max(-1)
+        # a column's error grows by the update's (|k| = 1), k's own error and the decays
+        errs[t] = errs[p] * d + eu + 2.0 ** -24 * (rk * umax + 12 * col + 4 * (col + umax))
+        col = np.linalg.norm(states[t], axis=1).max(-1)
+        out[t] = np.einsum("hij,hi->hj", states[t], q) / np.sqrt(S)
+        tol[t] = ((errs[t] + 2.0 ** -24 * (rq + 20) * col) / np.sqrt(S))[:, None]
+    return out, tol, states, errs, windows
