@@ -11,6 +11,7 @@
 
 #include "common.h"
 #include "internal.h"
+#include "kv_tile.h"
 
 namespace it {
 
@@ -18,6 +19,209 @@ namespace {
 constexpr int HD = 256;
 constexpr int PART = idx::PART;
 constexpr int SPL = 8;   // context records a lane loads per batch
+constexpr int BM = 64, BN = 64;          // rows per workgroup and keys per tile of the row-block form
+constexpr float P_BITS = 7.0f;           // weights up to 2^15 of the reference: see the softmax
+constexpr float LN2_F = 0.6931471805599453f;
+}
+
+// The context's records for many rows (R = nt * nh / nkv rows of a KV head, more than 32): workgroup = 64 rows r = t*G + g
+// of one KV head x one key split, four waves of 32 rows x half of each 64-key tile's keys: wave w takes rows
+// 32 (w & 1) .. +31 and keys 32 (w >> 1) .. +31, with a running maximum, sum and O of its own that are joined at the
+// end. The transposed products of the flash form (S^T = K q^T, O^T += V^T P^T, 32x32x16, one query row a lane
+// pair), twice each: q and P go in as f16 pairs hi + lo, so K and V, exact in f16, meet f32 operands to 2^-22 and the
+// f32 records keep f32's accuracy. A tile takes a wave 64 matrix ops of 32 cycles.
+// Splitting rows and keys between the waves halves what a wave reads from LDS against four waves of 16 rows: 1024
+// cycles of LDS a tile and workgroup beside 2048 of the matrix cores.
+__global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restrict__ q, int qts,
+                                                            const uint16_t* __restrict__ kc,
+                                                            const uint16_t* __restrict__ vc, int kvd, int n, int nh,
+                                                            int nkv, int nt, float scale, float* __restrict__ part,
+                                                            int chunk, int smax, int nrb) {
+    __shared__ __align__(16) _Float16 K0[BN * HD];
+    __shared__ __align__(16) _Float16 K1[BN * HD];
+    __shared__ __align__(16) _Float16 V0[BN * HD];
+    __shared__ __align__(16) _Float16 V1[BN * HD];
+    __shared__ float ms[BM], ls[BM];
+
+    // Row blocks of one (split, KV head) read the same keys: their ids differ by multiples of 8, which puts
+    // them on one XCD and its L2.
+    const int G = nh / nkv, R = nt * G;
+    const int grp = (int)blockIdx.x / (8 * nrb) * 8 + (int)blockIdx.x % 8, rb = (int)blockIdx.x / 8 % nrb;
+    if (grp >= smax * nkv) return;   // whole workgroup (the id count is rounded up to multiples of 8)
+    const int s = grp / nkv, kh = grp % nkv;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, hh = l >> 5, c = l & 31;
+    const int wr = w & 1, wk = w >> 1;
+    const int kb0 = s * chunk, kend = min(kb0 + chunk, n);
+    const size_t head_off = (size_t)kh * HD;
+    int cj[8];   // byte offset of the chunk each lane's tile loads bring, plus the KV head's column
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cj[i] = 2 * (int)head_off + 16 * ((l & 31) ^ swz32(16 * w + 2 * i + (l >> 5)));
+
+    // ---- q: wave w reads rows 16w .. 16w+15 of the block whole, and the operand layout comes out of hi and lo planes
+    // in the second K and V buffers, which the first tile does not use. Rows past R read the last row.
+    h8 qh[16], ql[16];
+    {
+        f4 qx[16];
+        const int r0 = rb * BM + 16 * w;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = min(r0 + i, R - 1);
+            qx[i] = ld_f4(q + uniform_off((size_t)(r / G) * qts + (size_t)(kh * G + r % G) * 2 * HD) + 4 * l);
+        }
+        tile_to_lds32(kc, kvd, kb0, kend, cj, K0, w, l);
+        tile_to_lds32(vc, kvd, kb0, kend, cj, V0, w, l);
+        const float sc = scale * LOG2E;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int row = 16 * w + i;
+            h4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                // The product is kept apart from the conversions: fused with them, the hi that is stored and the hi that
+                // lo is the rest of were rounded by different instructions, differently about once in 2^13 values.
+                float v = qx[i][e] * sc;
+                asm("" : "+v"(v));
+                hi[e] = (_Float16)v;
+                lo[e] = (_Float16)(v - (float)hi[e]);
+            }
+            const int at = row * HD + 8 * ((l >> 1) ^ (row & 31)) + 4 * (l & 1);
+            *(h4*)(K1 + at) = hi;
+            *(h4*)(V1 + at) = lo;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int ks = 0; ks < 16; ++ks) {
+            const int at = (32 * wr + c) * HD + 8 * ((2 * ks + hh) ^ c);
+            qh[ks] = ld_h8(K1 + at);
+            ql[ks] = ld_h8(V1 + at);
+        }
+    }
+    f16v o[8];
+#pragma unroll
+    for (int db = 0; db < 8; ++db) o[db] = f16v{};
+    float m_run = -INFINITY, l_run = 0.f;   // log2 units; l over this lane half's keys
+
+    // LDS offsets of the K operand (row 32 wk + c) and of the V transpose reads (rows 32 wk + 16 ks + 4 hh + vrow and 8
+    // further), as in the flash form
+    int koff[8], voff[4][2];
+#pragma unroll
+    for (int k2 = 0; k2 < 8; ++k2) koff[k2] = (32 * wk + c) * HD + 8 * ((2 * k2 + hh) ^ swz32(c));
+    {
+        const int vrow = (l & 15) >> 2, vcol = 16 * ((l >> 4) & 1) + 4 * (l & 3);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int r = 4 * hh + vrow + 8 * half;
+#pragma unroll
+            for (int par = 0; par < 4; ++par)
+                voff[par][half] = (32 * wk + r) * HD + 8 * ((4 * par + (vcol >> 3)) ^ swz32(r)) + (vcol & 7);
+        }
+    }
+
+    auto tile = [&](int kb, const _Float16* K, const _Float16* V, _Float16* Kn, _Float16* Vn) {
+        IT_WAIT_VMCNT(0);
+        __syncthreads();   // tile kb has landed, and every wave is done with the buffers of the next one
+        tile_to_lds32(kc, kvd, kb + BN, kend, cj, Kn, w, l);   // (past the end: the last row again, unused)
+        tile_to_lds32(vc, kvd, kb + BN, kend, cj, Vn, w, l);
+        f16v sa = f16v{}, sb = f16v{};
+#pragma unroll
+        for (int ks = 0; ks < 16; ++ks) {
+            const h8 k = ld_h8(K + koff[ks & 7] + 128 * (ks >> 3));
+            sa = mfma32x32x16(k, qh[ks], sa);
+            sb = mfma32x32x16(k, ql[ks], sb);
+        }
+        sa += sb;
+        if (kb + BN > kend) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (kb + 32 * wk + 8 * (i >> 2) + 4 * hh + (i & 3) >= kend) sa[i] = -INFINITY;
+        }
+        // Online softmax in log2 units. The weights are 2^(s - m_run) with m_run 7 below the maximum seen when it was last
+        // raised, and it is raised when a row's maximum passes m_run + 15: weights stay below 2^15, inside f16, and the
+        // pair hi + lo resolves 2^-24 of them, 2^-31 of a fresh maximum, so that many small weights still count.
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sa[i]);
+        mx = max_xor32(mx);
+        const bool grow = mx > m_run + 2 * P_BITS + 1;
+        if (__any(grow)) {
+            const float mnew = grow ? mx - P_BITS : m_run;
+            const float alpha = (m_run == -INFINITY) ? 0.0f : __builtin_amdgcn_exp2f(m_run - mnew);
+            l_run *= alpha;
+            // wait states between the last matrix ops' writes of O and scale_acc's reads, as in the flash form
+            asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7");
+#pragma unroll
+            for (int db = 0; db < 8; ++db) scale_acc(o[db], alpha);
+            m_run = mnew;
+        }
+        const float msub = (m_run == -INFINITY) ? 0.0f : m_run;
+        float lsum = 0.f;
+        h8 ph[2], pl[2];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float p = __builtin_amdgcn_exp2f(sa[8 * kk + j] - msub);
+                lsum += p;
+                const _Float16 hi = (_Float16)p;
+                ph[kk][j] = hi;
+                pl[kk][j] = (_Float16)(p - (float)hi);
+            }
+        l_run += lsum;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+                const _Float16* v = V + (16 * ks) * HD + 128 * (db >> 2);
+                const h8 va = cat_h4(lds_tr4(v + voff[db & 3][0]), lds_tr4(v + voff[db & 3][1]));
+                o[db] = mfma32x32x16(va, ph[ks], o[db]);
+                o[db] = mfma32x32x16(va, pl[ks], o[db]);
+            }
+    };
+    for (int kb = kb0; kb < kend; kb += 2 * BN) {
+        tile(kb, K0, V0, K1, V1);
+        if (kb + BN < kend) tile(kb + BN, K1, V1, K0, V0);
+    }
+    // ---- join the two key halves of each row: waves 2 and 3 hand over O, {m, l}; waves 0 and 1 merge into the buffer (O^T
+    // of row c at dims 32 db + 8 i4 + 4 hh .. +3, 16-byte chunks XOR-swizzled by row), then all store whole rows
+    IT_WAIT_VMCNT(0);   // the loads issued past the end land in the buffers
+    __syncthreads();
+    l_run = sum_xor32(l_run);
+    float* os = (float*)(wr ? K1 : K0);
+    if (wk == 1) {
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4)
+                *(f4*)(os + c * HD + 4 * ((8 * db + 2 * i4 + hh) ^ c)) =
+                    f4{o[db][4 * i4], o[db][4 * i4 + 1], o[db][4 * i4 + 2], o[db][4 * i4 + 3]};
+        if (hh == 0) { ms[32 * wr + c] = m_run; ls[32 * wr + c] = l_run; }
+    }
+    __syncthreads();
+    if (wk == 0) {
+        const float m2 = ms[32 * wr + c], l2 = ls[32 * wr + c];
+        const float m = fmaxf(m_run, m2);
+        const float a1 = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m);
+        const float a2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - m);
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                f4* p = (f4*)(os + c * HD + 4 * ((8 * db + 2 * i4 + hh) ^ c));
+                *p = *p * a2 + f4{o[db][4 * i4], o[db][4 * i4 + 1], o[db][4 * i4 + 2], o[db][4 * i4 + 3]} * a1;
+            }
+        if (hh == 0) { ms[32 * wr + c] = m * LN2_F; ls[32 * wr + c] = l_run * a1 + l2 * a2; }
+    }
+    __syncthreads();
+    const float* src = (const float*)(w < 2 ? K0 : K1);
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+        const int row = 16 * w + i, r = rb * BM + row;
+        if (r < R) {
+            float* rec = part + idx::rec((r / G) * nh + kh * G + r % G, s, smax) * PART;
+            *(f4*)(rec + 4 + 4 * l) = *(const f4*)(src + (row & 31) * HD + 4 * (l ^ (row & 31)));
+            if (l == 0) *(f4*)rec = f4{ms[row], ls[row], 0.f, 0.f};
+        }
+    }
 }
 
 // One workgroup per (256 / SL * 4 dims, head, node). Thread = (split lane sg of SL, dim lane of 256 / SL, 4
@@ -131,9 +335,16 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
 }
 
 // Keys per context split.
+//   up to 32 rows a KV head: the decode partials, bound by the cache's bytes and the latency of a split: about two
+//   workgroups a CU;
+//   more: one round of the 64-row workgroups, which fill a CU each.
+constexpr int CUS = 256;   // MI355X compute units
+static bool row_blocks(int nt, int nh, int nkv) { return nt * (nh / nkv) > 32; }
 int attn_tree_chunk(int pos0, int nt, int nh, int nkv) {
-    const long tiles = (pos0 + 63) / 64, groups = (long)nkv * ((nt * (nh / nkv) + 31) / 32);
-    return 64 * (int)std::max(1L, (tiles * groups + 511) / 512);
+    const long tiles = (pos0 + 63) / 64;
+    if (!row_blocks(nt, nh, nkv)) return 64 * (int)std::max(1L, (tiles * nkv + 2 * CUS - 1) / (2 * CUS));
+    const long groups = (long)nkv * ((nt * (nh / nkv) + BM - 1) / BM), splits = std::max(1L, CUS / groups);
+    return 64 * (int)std::max(1L, (tiles + splits - 1) / splits);
 }
 
 hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0,
@@ -142,7 +353,15 @@ hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const u
     int smax = 0;
     if (pos0 > 0) {
         smax = idx::split_count(pos0, chunk);
-        const hipError_t e = launch_attn_all_partials(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, st);
+        hipError_t e;
+        if (row_blocks(nt, nh, nkv)) {
+            const int nrb = (nt * (nh / nkv) + BM - 1) / BM;
+            const unsigned grid = (unsigned)((smax * nkv + 7) / 8 * 8 * nrb);
+            attn_tree_ctx_kernel<<<grid, 256, 0, st>>>(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, smax, nrb);
+            e = hipGetLastError();
+        } else {
+            e = launch_attn_all_partials(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, st);
+        }
         if (e != hipSuccess) return e;
     }
     // few rows: a quarter of the dims a workgroup, 16 split lanes; many: the whole row, 4 split lanes
