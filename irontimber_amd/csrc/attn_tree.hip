@@ -117,30 +117,16 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
         }
     }
 
-    auto tile = [&](int kb, const _Float16* K, const _Float16* V, _Float16* Kn, _Float16* Vn) {
-        IT_WAIT_VMCNT(0);
-        __syncthreads();   // tile kb has landed, and every wave is done with the buffers of the next one
-        tile_to_lds32(kc, kvd, kb + BN, kend, cj, Kn, w, l);   // (past the end: the last row again, unused)
-        tile_to_lds32(vc, kvd, kb + BN, kend, cj, Vn, w, l);
-        f16v sa = f16v{}, sb = f16v{};
-#pragma unroll
-        for (int ks = 0; ks < 16; ++ks) {
-            const h8 k = ld_h8(K + koff[ks & 7] + 128 * (ks >> 3));
-            sa = mfma32x32x16(k, qh[ks], sa);
-            sb = mfma32x32x16(k, ql[ks], sb);
-        }
-        sa += sb;
-        if (kb + BN > kend) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (kb + 32 * wk + 8 * (i >> 2) + 4 * hh + (i & 3) >= kend) sa[i] = -INFINITY;
-        }
-        // Online softmax in log2 units. The weights are 2^(s - m_run) with m_run 7 below the maximum seen when it was last
-        // raised, and it is raised when a row's maximum passes m_run + 15: weights stay below 2^15, inside f16, and the
-        // pair hi + lo resolves 2^-24 of them, 2^-31 of a fresh maximum, so that many small weights still count.
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sa[i]);
+    // Operand reads: K rows as the A operand of k-step ks, V as that of (k-step, dim block) j = 8 ks + db.
+    auto k_op = [&](const _Float16* K, int ks) { return ld_h8(K + koff[ks & 7] + 128 * (ks >> 3)); };
+    auto v_op = [&](const _Float16* V, int j) {
+        const _Float16* v = V + (16 * (j >> 3)) * HD + 128 * ((j & 7) >> 2);
+        return cat_h4(lds_tr4(v + voff[j & 3][0]), lds_tr4(v + voff[j & 3][1]));
+    };
+    // Online softmax in log2 units. The weights are 2^(s - m_run) with m_run 7 below the maximum seen when it was last
+    // raised, and it is raised when a row's maximum passes m_run + 15: weights stay below 2^15, inside f16, and the pair
+    // hi + lo resolves 2^-24 of them, 2^-31 of a fresh maximum, so that many small weights still count.
+    auto raise = [&](float mx) {
         mx = max_xor32(mx);
         const bool grow = mx > m_run + 2 * P_BITS + 1;
         if (__any(grow)) {
@@ -153,34 +139,103 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
             for (int db = 0; db < 8; ++db) scale_acc(o[db], alpha);
             m_run = mnew;
         }
-        const float msub = (m_run == -INFINITY) ? 0.0f : m_run;
-        float lsum = 0.f;
-        h8 ph[2], pl[2];
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float p = __builtin_amdgcn_exp2f(sa[8 * kk + j] - msub);
-                lsum += p;
-                const _Float16 hi = (_Float16)p;
-                ph[kk][j] = hi;
-                pl[kk][j] = (_Float16)(p - (float)hi);
-            }
-        l_run += lsum;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int db = 0; db < 8; ++db) {
-                const _Float16* v = V + (16 * ks) * HD + 128 * (db >> 2);
-                const h8 va = cat_h4(lds_tr4(v + voff[db & 3][0]), lds_tr4(v + voff[db & 3][1]));
-                o[db] = mfma32x32x16(va, ph[ks], o[db]);
-                o[db] = mfma32x32x16(va, pl[ks], o[db]);
-            }
     };
-    for (int kb = kb0; kb < kend; kb += 2 * BN) {
-        tile(kb, K0, V0, K1, V1);
-        if (kb + BN < kend) tile(kb + BN, K1, V1, K0, V0);
+    f16v sc;             // the tile's masked scores
+    h8 ph[2], pl[2];     // its weights, hi and lo
+    auto mask1 = [&](const f16v& sa, int lim, int i, float& mx) {
+        sc[i] = 8 * (i >> 2) + (i & 3) < lim ? sa[i] : -INFINITY;
+        mx = fmaxf(mx, sc[i]);
+    };
+    auto weight1 = [&](float msub, int i) {
+        const float p = __builtin_amdgcn_exp2f(sc[i] - msub);
+        const _Float16 hi = (_Float16)p;
+        l_run += p;
+        ph[i >> 3][i & 7] = hi;
+        pl[i >> 3][i & 7] = (_Float16)(p - (float)hi);
+    };
+#define IT_FENCE __builtin_amdgcn_sched_barrier(0)
+    // One tile and the next one's scores, in 32 steps of two dependent matrix ops (hi, lo). One wave a SIMD issues in order,
+    // so what is to run in the shadow of the matrix ops stands between them: each score step holds one of this tile's 16
+    // exponentials with its conversions and one of the 16 loads of coming tiles, each value step one masked score of the
+    // next tile; operands are read four steps ahead. K runs a tile ahead of V: at the start K of the next tile (Kn) and V
+    // of this one have landed, and K of the one after (into Kf) and V of the next (into Vn) go out.
+    auto tile = [&](int kb, const _Float16* Kn, const _Float16* V, _Float16* Kf, _Float16* Vn) {
+        IT_WAIT_VMCNT(0);
+        __syncthreads();   // landed for every wave, and every wave is done with the buffers written now
+        const TileSrc ks_ = tile_src(kc, kvd, kb + 2 * BN, kend), vs_ = tile_src(vc, kvd, kb + BN, kend);
+        const float msub = (m_run == -INFINITY) ? 0.0f : m_run;
+        const int lim = kend - kb - BN - 32 * wk - 4 * hh;
+        f16v sa = f16v{};
+        h8 k[16], v[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = k_op(Kn, i);
+        IT_FENCE;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i < 12) k[i + 4] = k_op(Kn, i + 4);
+            else v[i - 12] = v_op(V, i - 12);
+            sa = mfma32x32x16(k[i], qh[i], sa);
+            weight1(msub, i);
+            IT_FENCE;
+            sa = mfma32x32x16(k[i], ql[i], sa);
+            if (i < 8) tile_piece32(ks_, cj, Kf, w, l, i);
+            else tile_piece32(vs_, cj, Vn, w, l, i - 8);
+            IT_FENCE;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (j < 12) v[j + 4] = v_op(V, j + 4);
+            o[j & 7] = mfma32x32x16(v[j], ph[j >> 3], o[j & 7]);
+            // (not before the third step: the last score op's result takes that long)
+            if (j >= 2) mask1(sa, lim, j - 2, mx);
+            IT_FENCE;
+            o[j & 7] = mfma32x32x16(v[j], pl[j >> 3], o[j & 7]);
+            IT_FENCE;
+        }
+        mask1(sa, lim, 14, mx);
+        mask1(sa, lim, 15, mx);
+        raise(mx);
+    };
+    // first tile's scores: K0, V0 hold it; its successor's K goes to K1 once q has been read from there
+    {
+        IT_WAIT_VMCNT(0);
+        __syncthreads();
+        if (kb0 + BN < kend) tile_to_lds32(kc, kvd, kb0 + BN, kend, cj, K1, w, l);
+        f16v sa = f16v{};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const h8 k = k_op(K0, i);
+            sa = mfma32x32x16(k, qh[i], sa);
+            sa = mfma32x32x16(k, ql[i], sa);
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mask1(sa, kend - kb0 - 32 * wk - 4 * hh, i, mx);
+        raise(mx);
     }
+    int kb = kb0;
+    for (; kb + 2 * BN < kend; kb += 2 * BN) {   // two tiles whose successors exist
+        tile(kb, K1, V0, K0, V1);
+        tile(kb + BN, K0, V1, K1, V0);
+    }
+    const bool even = kb + BN >= kend;   // the last tile's V is in V0, else one more tile precedes it
+    if (!even) tile(kb, K1, V0, K0, V1);
+    IT_WAIT_VMCNT(0);
+    __syncthreads();
+    {
+        const float msub = (m_run == -INFINITY) ? 0.0f : m_run;
+        const _Float16* V = even ? V0 : V1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) weight1(msub, i);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const h8 v = v_op(V, j);
+            o[j & 7] = mfma32x32x16(v, ph[j >> 3], o[j & 7]);
+            o[j & 7] = mfma32x32x16(v, pl[j >> 3], o[j & 7]);
+        }
+    }
+#undef IT_FENCE
     // ---- join the two key halves of each row: waves 2 and 3 hand over O, {m, l}; waves 0 and 1 merge into the buffer (O^T
     // of row c at dims 32 db + 8 i4 + 4 hh .. +3, 16-byte chunks XOR-swizzled by row), then all store whole rows
     IT_WAIT_VMCNT(0);   // the loads issued past the end land in the buffers

@@ -17,19 +17,27 @@ __device__ __forceinline__ int swz32(int r) { return ((r & 3) << 1) | ((r >> 2) 
 // physical slot. Rows past kend-1 repeat row kend-1 (a tile issued past the end only refetches it).
 // Addresses are a uniform row base plus a 32-bit lane offset, so each instruction needs two VALU
 // ops; the chunk part of the offsets (cj, including the head's column) is computed once.
+struct TileSrc {
+    const char* base;   // the tile's first row, clamped
+    int rmax;           // last row to read, from there
+    unsigned rowb;      // bytes per row
+};
+__device__ __forceinline__ TileSrc tile_src(const uint16_t* __restrict__ src, int kvd, int kb, int kend) {
+    const int ts = min(kb, kend - 1);
+    return {(const char*)(src + (size_t)ts * kvd), kend - 1 - ts, 2u * (unsigned)kvd};
+}
+// load i of the wave's eight
+__device__ __forceinline__ void tile_piece32(const TileSrc& t, const int (&cj)[8], _Float16* lds, int w, int l, int i) {
+    typedef __attribute__((address_space(3))) void lds_void;
+    const int r = 16 * w + 2 * i + (l >> 5);
+    const unsigned off = (unsigned)min(r, t.rmax) * t.rowb + (unsigned)cj[i];
+    __builtin_amdgcn_global_load_lds((const void*)(t.base + off), (lds_void*)(lds + (16 * w + 2 * i) * KV_HD), 16, 0, 0);
+}
 __device__ __forceinline__ void tile_to_lds32(const uint16_t* __restrict__ src, int kvd, int kb, int kend,
                                             const int (&cj)[8], _Float16* lds, int w, int l) {
-    typedef __attribute__((address_space(3))) void lds_void;
-    const int ts = min(kb, kend - 1);                      // first row of the tile, clamped
-    const char* base = (const char*)(src + (size_t)ts * kvd);
-    const int rmax = kend - 1 - ts;                        // >= 0
-    const unsigned rowb = 2u * (unsigned)kvd;
+    const TileSrc t = tile_src(src, kvd, kb, kend);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = 16 * w + 2 * i + (l >> 5);
-        const unsigned off = (unsigned)min(r, rmax) * rowb + (unsigned)cj[i];
-        __builtin_amdgcn_global_load_lds((const void*)(base + off), (lds_void*)(lds + (16 * w + 2 * i) * KV_HD), 16, 0, 0);
-    }
+    for (int i = 0; i < 8; ++i) tile_piece32(t, cj, lds, w, l, i);
 }
 
 // acc *= a for an MFMA accumulator tile held in AGPRs, element by element in place (read to a VGPR,
