@@ -125,47 +125,79 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     };
     // Online softmax in log2 units. The weights are 2^(s - m_run) with m_run 7 below the maximum seen when it was last
     // raised, and it is raised when a row's maximum passes m_run + 15: weights stay below 2^15, inside f16, and the pair
-    // hi + lo resolves 2^-24 of them, 2^-31 of a fresh maximum, so that many small weights still count.
-    auto raise = [&](float mx) {
+    // hi + lo resolves 2^-24 of them, 2^-31 of a fresh maximum, so that many small weights still count. The score products
+    // start from -m_run instead of zero, so they come out as exponents; m_run is 0 while a row has seen no key.
+    f16v minit = f16v{};   // -m_run
+    f16v sc;               // the tile's exponents
+    h8 ph[2], pl[2];       // its weights, hi and lo
+    auto settle = [&](float mx) __attribute__((always_inline)) {   // mx: the largest exponent
         mx = max_xor32(mx);
-        const bool grow = mx > m_run + 2 * P_BITS + 1;
+        const bool grow = mx > 2 * P_BITS + 1 || (m_run == -INFINITY && mx > -INFINITY);
         if (__any(grow)) {
-            const float mnew = grow ? mx - P_BITS : m_run;
-            const float alpha = (m_run == -INFINITY) ? 0.0f : __builtin_amdgcn_exp2f(m_run - mnew);
+            const float up = grow ? mx - P_BITS : 0.0f;
+            const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
+            const float mnew = m_run == -INFINITY ? up : m_run + up;
             l_run *= alpha;
             // wait states between the last matrix ops' writes of O and scale_acc's reads, as in the flash form
             asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7");
 #pragma unroll
             for (int db = 0; db < 8; ++db) scale_acc(o[db], alpha);
-            m_run = mnew;
+            if (grow) m_run = mnew;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[i] -= up;
+                minit[i] = m_run == -INFINITY ? 0.0f : -m_run;
+            }
         }
     };
-    f16v sc;             // the tile's masked scores
-    h8 ph[2], pl[2];     // its weights, hi and lo
-    auto mask1 = [&](const f16v& sa, int lim, int i, float& mx) {
-        sc[i] = 8 * (i >> 2) + (i & 3) < lim ? sa[i] : -INFINITY;
-        mx = fmaxf(mx, sc[i]);
+    // keys at or past kend: exponent -inf; returns the largest of the rest
+    auto mask = [&](int kb) __attribute__((always_inline)) {
+        const int lim = kend - kb - 32 * wk - 4 * hh;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (8 * (i >> 2) + (i & 3) >= lim) sc[i] = -INFINITY;
+            mx = fmaxf(mx, sc[i]);
+        }
+        return mx;
     };
-    auto weight1 = [&](float msub, int i) {
-        const float p = __builtin_amdgcn_exp2f(sc[i] - msub);
-        const _Float16 hi = (_Float16)p;
-        l_run += p;
-        ph[i >> 3][i & 7] = hi;
-        pl[i >> 3][i & 7] = (_Float16)(p - (float)hi);
+    auto weight2 = [&](int i) {   // weights i and i + 1
+        const f2 p = {__builtin_amdgcn_exp2f(sc[i]), __builtin_amdgcn_exp2f(sc[i + 1])};
+        const h2 hi = __builtin_convertvector(p, h2);
+        l_run += p[0];
+        l_run += p[1];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            ph[i >> 3][(i & 7) + e] = hi[e];
+            pl[i >> 3][(i & 7) + e] = (_Float16)__builtin_fmaf((float)hi[e], -1.0f, p[e]);
+        }
+    };
+    // Tile loads in flight: offsets of this lane's rows from the tile's first, clamped anew for the last, partial tiles
+    unsigned offk[8], offv[8];
+    const unsigned rowb = 2u * (unsigned)kvd;
+    auto offsets = [&](unsigned (&off)[8], int kb) __attribute__((always_inline)) {
+        const int rmax = max(kend - 1 - kb, 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) off[i] = (unsigned)min(16 * w + 2 * i + (l >> 5), rmax) * rowb + (unsigned)cj[i];
+    };
+    auto row_base = [&](const uint16_t* src, int kb) { return (const char*)(src + (size_t)min(kb, kend - 1) * kvd); };
+    auto piece = [&](const char* base, const unsigned (&off)[8], _Float16* lds, int i) {
+        typedef __attribute__((address_space(3))) void lds_void;
+        __builtin_amdgcn_global_load_lds((const void*)(base + off[i]), (lds_void*)(lds + (16 * w + 2 * i) * HD), 16, 0, 0);
     };
 #define IT_FENCE __builtin_amdgcn_sched_barrier(0)
     // One tile and the next one's scores, in 32 steps of two dependent matrix ops (hi, lo). One wave a SIMD issues in order,
-    // so what is to run in the shadow of the matrix ops stands between them: each score step holds one of this tile's 16
-    // exponentials with its conversions and one of the 16 loads of coming tiles, each value step one masked score of the
-    // next tile; operands are read four steps ahead. K runs a tile ahead of V: at the start K of the next tile (Kn) and V
-    // of this one have landed, and K of the one after (into Kf) and V of the next (into Vn) go out.
-    auto tile = [&](int kb, const _Float16* Kn, const _Float16* V, _Float16* Kf, _Float16* Vn) {
+    // so what is to run in the shadow of the matrix ops stands between them: the score steps hold this tile's 16
+    // exponentials with their conversions and the 16 loads of coming tiles, the value steps the next tile's maximum;
+    // operands are read four steps ahead. K runs a tile ahead of V: at the start K of the next tile (Kn) and V of this
+    // one have landed, and K of the one after (into Kf) and V of the next (into Vn) go out.
+    auto tile = [&](int kb, const _Float16* Kn, const _Float16* V, _Float16* Kf, _Float16* Vn) __attribute__((always_inline)) {
         IT_WAIT_VMCNT(0);
         __syncthreads();   // landed for every wave, and every wave is done with the buffers written now
-        const TileSrc ks_ = tile_src(kc, kvd, kb + 2 * BN, kend), vs_ = tile_src(vc, kvd, kb + BN, kend);
-        const float msub = (m_run == -INFINITY) ? 0.0f : m_run;
-        const int lim = kend - kb - BN - 32 * wk - 4 * hh;
-        f16v sa = f16v{};
+        if (kb + 3 * BN > kend) offsets(offk, kb + 2 * BN);   // (a tile past the end: its last row again, unused)
+        if (kb + 2 * BN > kend) offsets(offv, kb + BN);
+        const char *kbase = row_base(kc, kb + 2 * BN), *vbase = row_base(vc, kb + BN);
+        f16v sa = minit;
         h8 k[16], v[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) k[i] = k_op(Kn, i);
@@ -175,11 +207,11 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
             if (i < 12) k[i + 4] = k_op(Kn, i + 4);
             else v[i - 12] = v_op(V, i - 12);
             sa = mfma32x32x16(k[i], qh[i], sa);
-            weight1(msub, i);
+            if (i & 1) weight2(i - 1);
             IT_FENCE;
             sa = mfma32x32x16(k[i], ql[i], sa);
-            if (i < 8) tile_piece32(ks_, cj, Kf, w, l, i);
-            else tile_piece32(vs_, cj, Vn, w, l, i - 8);
+            if (i < 8) piece(kbase, offk, Kf, i);
+            else piece(vbase, offv, Vn, i - 8);
             IT_FENCE;
         }
         float mx = -INFINITY;
@@ -187,32 +219,37 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
         for (int j = 0; j < 16; ++j) {
             if (j < 12) v[j + 4] = v_op(V, j + 4);
             o[j & 7] = mfma32x32x16(v[j], ph[j >> 3], o[j & 7]);
-            // (not before the third step: the last score op's result takes that long)
-            if (j >= 2) mask1(sa, lim, j - 2, mx);
+            if (j >= 4 && j < 12) {   // (the last score op's result takes the first steps)
+                sc[2 * j - 8] = sa[2 * j - 8];
+                sc[2 * j - 7] = sa[2 * j - 7];
+                mx = fmaxf(fmaxf(mx, sc[2 * j - 8]), sc[2 * j - 7]);
+            }
             IT_FENCE;
             o[j & 7] = mfma32x32x16(v[j], pl[j >> 3], o[j & 7]);
             IT_FENCE;
         }
-        mask1(sa, lim, 14, mx);
-        mask1(sa, lim, 15, mx);
-        raise(mx);
+        if (kb + 2 * BN > kend) mx = mask(kb + BN);
+        settle(mx);
     };
+    offsets(offk, kb0 + BN);
+    offsets(offv, kb0 + BN);
     // first tile's scores: K0, V0 hold it; its successor's K goes to K1 once q has been read from there
     {
         IT_WAIT_VMCNT(0);
         __syncthreads();
-        if (kb0 + BN < kend) tile_to_lds32(kc, kvd, kb0 + BN, kend, cj, K1, w, l);
-        f16v sa = f16v{};
+        if (kb0 + BN < kend) {
+            const char* kbase = row_base(kc, kb0 + BN);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) piece(kbase, offk, K1, i);
+        }
+        sc = f16v{};
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const h8 k = k_op(K0, i);
-            sa = mfma32x32x16(k, qh[i], sa);
-            sa = mfma32x32x16(k, ql[i], sa);
+            sc = mfma32x32x16(k, qh[i], sc);
+            sc = mfma32x32x16(k, ql[i], sc);
         }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mask1(sa, kend - kb0 - 32 * wk - 4 * hh, i, mx);
-        raise(mx);
+        settle(mask(kb0));
     }
     int kb = kb0;
     for (; kb + 2 * BN < kend; kb += 2 * BN) {   // two tiles whose successors exist
@@ -224,10 +261,9 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     IT_WAIT_VMCNT(0);
     __syncthreads();
     {
-        const float msub = (m_run == -INFINITY) ? 0.0f : m_run;
         const _Float16* V = even ? V0 : V1;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) weight1(msub, i);
+        for (int i = 0; i < 16; i += 2) weight2(i);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const h8 v = v_op(V, j);
