@@ -41,7 +41,8 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     __shared__ __align__(16) _Float16 K1[BN * HD];
     __shared__ __align__(16) _Float16 V0[BN * HD];
     __shared__ __align__(16) _Float16 V1[BN * HD];
-    __shared__ float ms[BM], ls[BM];
+    __shared__ float ms[2][BM], ls[2][BM];   // per key half
+    __shared__ f2 rowml[BM];
 
     // Row blocks of one (split, KV head) read the same keys: their ids differ by multiples of 8, which puts
     // them on one XCD and its L2.
@@ -62,11 +63,17 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     h8 qh[16], ql[16];
     {
         f4 qx[16];
-        const int r0 = rb * BM + 16 * w;
+        const int r0 = min(rb * BM + 16 * w, R - 1);
+        const int t0 = __builtin_amdgcn_readfirstlane(r0 / G);
+        int g0 = r0 - t0 * G;   // the row's head in its group; its floats start at `at`
+        size_t at = uniform_off((size_t)t0 * qts + (size_t)(kh * G + g0) * 2 * HD);
+        const int wrap = qts - G * 2 * HD;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int r = min(r0 + i, R - 1);
-            qx[i] = ld_f4(q + uniform_off((size_t)(r / G) * qts + (size_t)(kh * G + r % G) * 2 * HD) + 4 * l);
+            qx[i] = ld_f4(q + at + 4 * l);
+            const bool more = r0 + i + 1 < R, last = g0 + 1 == G;
+            at += more ? 2 * HD + (last ? wrap : 0) : 0;
+            g0 = !more ? g0 : last ? 0 : g0 + 1;
         }
         tile_to_lds32(kc, kvd, kb0, kend, cj, K0, w, l);
         tile_to_lds32(vc, kvd, kb0, kend, cj, V0, w, l);
@@ -76,17 +83,21 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
             const int row = 16 * w + i;
             h4 hi, lo;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                // The product is kept apart from the conversions: fused with them, the hi that is stored and the hi that
+            for (int e = 0; e < 4; e += 2) {
+                // The products are kept apart from the conversions: fused with them, the hi that is stored and the hi that
                 // lo is the rest of were rounded by different instructions, differently about once in 2^13 values.
-                float v = qx[i][e] * sc;
+                f2 v = {qx[i][e] * sc, qx[i][e + 1] * sc};
                 asm("" : "+v"(v));
-                hi[e] = (_Float16)v;
-                lo[e] = (_Float16)(v - (float)hi[e]);
+                const h2 h = __builtin_convertvector(v, h2);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    hi[e + j] = h[j];
+                    lo[e + j] = (_Float16)__builtin_fmaf((float)h[j], -1.0f, v[j]);
+                }
             }
-            const int at = row * HD + 8 * ((l >> 1) ^ (row & 31)) + 4 * (l & 1);
-            *(h4*)(K1 + at) = hi;
-            *(h4*)(V1 + at) = lo;
+            const int to = row * HD + 8 * ((l >> 1) ^ (row & 31)) + 4 * (l & 1);
+            *(h4*)(K1 + to) = hi;
+            *(h4*)(V1 + to) = lo;
         }
         __syncthreads();
 #pragma unroll
@@ -243,13 +254,25 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
             for (int i = 0; i < 8; ++i) piece(kbase, offk, K1, i);
         }
         sc = f16v{};
+        h8 k[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = k_op(K0, i);
+        IT_FENCE;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const h8 k = k_op(K0, i);
-            sc = mfma32x32x16(k, qh[i], sc);
-            sc = mfma32x32x16(k, ql[i], sc);
+            if (i < 8) k[i + 8] = k_op(K0, i + 8);
+            sc = mfma32x32x16(k[i], qh[i], sc);
+            sc = mfma32x32x16(k[i], ql[i], sc);
+            IT_FENCE;
         }
-        settle(mask(kb0));
+        const float mx = max_xor32(mask(kb0));
+        if (mx > -INFINITY) m_run = mx - P_BITS;   // (O and l are zero: nothing to rescale)
+        const float up = mx > -INFINITY ? m_run : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            sc[i] -= up;
+            minit[i] = -up;
+        }
     }
     int kb = kb0;
     for (; kb + 2 * BN < kend; kb += 2 * BN) {   // two tiles whose successors exist
@@ -272,45 +295,71 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
         }
     }
 #undef IT_FENCE
-    // ---- join the two key halves of each row: waves 2 and 3 hand over O, {m, l}; waves 0 and 1 merge into the buffer (O^T
-    // of row c at dims 32 db + 8 i4 + 4 hh .. +3, 16-byte chunks XOR-swizzled by row), then all store whole rows
+    // ---- join the two key halves of each row: a wave keeps the 128 dims 128 wk .. +127 and hands the others to its
+    // partner (O^T of row c at dims 32 db + 8 i4 + 4 hh .. +3, 16-byte chunks XOR-swizzled by row, in one pair of
+    // buffers), the joined rows go out through the other pair, whole rows a store
     IT_WAIT_VMCNT(0);   // the loads issued past the end land in the buffers
     __syncthreads();
     l_run = sum_xor32(l_run);
-    float* os = (float*)(wr ? K1 : K0);
-    if (wk == 1) {
+    float* give = (float*)(wr ? K1 : K0);
+    const auto chunk_at = [&](int db, int i4) { return c * HD + 4 * ((8 * db + 2 * i4 + hh) ^ c); };
+    const auto part_of = [&](int db, int i4) {
+        return f4{o[db][4 * i4], o[db][4 * i4 + 1], o[db][4 * i4 + 2], o[db][4 * i4 + 3]};
+    };
+    if (wk == 0) {   // (static register indexes)
 #pragma unroll
-        for (int db = 0; db < 8; ++db)
+        for (int db = 4; db < 8; ++db)
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4)
-                *(f4*)(os + c * HD + 4 * ((8 * db + 2 * i4 + hh) ^ c)) =
-                    f4{o[db][4 * i4], o[db][4 * i4 + 1], o[db][4 * i4 + 2], o[db][4 * i4 + 3]};
-        if (hh == 0) { ms[32 * wr + c] = m_run; ls[32 * wr + c] = l_run; }
+            for (int i4 = 0; i4 < 4; ++i4) *(f4*)(give + chunk_at(db, i4)) = part_of(db, i4);
+    } else {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) *(f4*)(give + chunk_at(db, i4)) = part_of(db, i4);
     }
+    if (hh == 0) { ms[wk][32 * wr + c] = m_run; ls[wk][32 * wr + c] = l_run; }
     __syncthreads();
-    if (wk == 0) {
-        const float m2 = ms[32 * wr + c], l2 = ls[32 * wr + c];
-        const float m = fmaxf(m_run, m2);
+    float* joined = (float*)(wr ? V1 : V0);
+    {
+        const float m2 = ms[wk ^ 1][32 * wr + c], l2 = ls[wk ^ 1][32 * wr + c], m = fmaxf(m_run, m2);
         const float a1 = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m);
         const float a2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - m);
+        f4 got[16];   // (all read before any is written: the compiler does not know that the buffers differ)
 #pragma unroll
-        for (int db = 0; db < 8; ++db)
+        for (int i = 0; i < 16; ++i) got[i] = *(const f4*)(give + chunk_at(4 * wk + i / 4, i & 3)) * a2;
+        if (wk == 0) {
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-                f4* p = (f4*)(os + c * HD + 4 * ((8 * db + 2 * i4 + hh) ^ c));
-                *p = *p * a2 + f4{o[db][4 * i4], o[db][4 * i4 + 1], o[db][4 * i4 + 2], o[db][4 * i4 + 3]} * a1;
-            }
-        if (hh == 0) { ms[32 * wr + c] = m * LN2_F; ls[32 * wr + c] = l_run * a1 + l2 * a2; }
+            for (int i = 0; i < 16; ++i) got[i] += part_of(i / 4, i & 3) * a1;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) got[i] += part_of(4 + i / 4, i & 3) * a1;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) *(f4*)(joined + chunk_at(4 * wk + i / 4, i & 3)) = got[i];
+        if (wk == 0 && hh == 0) rowml[32 * wr + c] = f2{m * LN2_F, l_run * a1 + l2 * a2};
     }
     __syncthreads();
-    const float* src = (const float*)(w < 2 ? K0 : K1);
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
-        const int row = 16 * w + i, r = rb * BM + row;
-        if (r < R) {
-            float* rec = part + idx::rec((r / G) * nh + kh * G + r % G, s, smax) * PART;
-            *(f4*)(rec + 4 + 4 * l) = *(const f4*)(src + (row & 31) * HD + 4 * (l ^ (row & 31)));
-            if (l == 0) *(f4*)rec = f4{ms[row], ls[row], 0.f, 0.f};
+    {
+        const float* src = (const float*)(w < 2 ? V0 : V1);
+        const int r0 = rb * BM + 16 * w;
+        int tq = __builtin_amdgcn_readfirstlane(r0 / G), gq = r0 - tq * G;
+#pragma unroll
+        for (int i0 = 0; i0 < 16; i0 += 8) {
+            f4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = 16 * w + i0 + i;
+                v[i] = *(const f4*)(src + (row & 31) * HD + 4 * (l ^ (row & 31)));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (r0 + i0 + i < R) {
+                    float* rec = part + idx::rec(tq * nh + kh * G + gq, s, smax) * PART;
+                    *(f4*)(rec + 4 + 4 * l) = v[i];
+                    if (l == 0) *(f4*)rec = f4{rowml[16 * w + i0 + i][0], rowml[16 * w + i0 + i][1], 0.f, 0.f};
+                }
+                if (++gq == G) { gq = 0; ++tq; }
+            }
         }
     }
 }
@@ -334,14 +383,28 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     const int dq = blockIdx.x, h = blockIdx.y, t = blockIdx.z, tid = threadIdx.x, w = tid >> 6, l = tid & 63;
     const int sg = tid / DLN, dl = tid % DLN, d0 = DW * dq + 4 * dl;
     float* dst = out + (size_t)t * ots + (size_t)h * HD + d0;
+    // What does not hang on the mask goes out first: the first batch of the context's records, q and the gate. Slots
+    // past the last record reload it and count nothing.
+    const float* base = part + idx::rec(t * nh + h, 0, smax) * PART;
+    f2 hv[SPL];
+    f4 ov[SPL];
+    auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < SPL; ++j) {
+            const float* rec = base + (size_t)min(s0 + sg + SL * j, smax - 1) * PART;
+            hv[j] = *(const f2*)rec;
+            ov[j] = ld_f4(rec + 4 + d0);
+        }
+    };
+    if (smax > 0) load(0);
+    const float* qrow = q + (size_t)t * qts + (size_t)h * 2 * HD;
+    const f4 qv = ld_f4(qrow + 4 * l), gt = ld_f4(qrow + HD + d0);
     const uint64_t mask = anc[t] & (~(uint64_t)0 >> (64 - nt));
     const int np = (int)__popcll(mask);
     if (np == 0) {   // a padding node
         if (sg == 0) *(f4*)dst = f4{0.f, 0.f, 0.f, 0.f};
         return;
     }
-    const float* qrow = q + (size_t)t * qts + (size_t)h * 2 * HD;
-    const f4 qv = ld_f4(qrow + 4 * l), gt = ld_f4(qrow + HD + d0);
     if (tid < 64 && (mask >> tid & 1)) node[__popcll(mask & (((uint64_t)1 << tid) - 1))] = tid;
     __syncthreads();
     // ---- the path: this lane's V pieces go out first, then the scores, a key a wave
@@ -349,7 +412,7 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     h4 pv[NK];
 #pragma unroll
     for (int j = 0; j < NK; ++j)
-        pv[j] = *(const h4*)(vc + (size_t)(pos0 + node[min(sg + SL * j, np - 1)]) * kvd + head + d0);
+        if (SL * j < np) pv[j] = *(const h4*)(vc + (size_t)(pos0 + node[min(sg + SL * j, np - 1)]) * kvd + head + d0);
     for (int j0 = w; j0 < np; j0 += 16) {
         h4 kv[4];
 #pragma unroll
@@ -364,9 +427,7 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     }
     __syncthreads();
     // ---- the path's own softmax (no reference below the type's range, so that keys of score -inf weigh 0)
-    float M = score[0];
-    for (int j = 1; j < np; ++j) M = fmaxf(M, score[j]);
-    M = fmaxf(M, -FLT_MAX);
+    float M = wave_max(l < np ? score[l] : -FLT_MAX);
     float den = 0.f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -379,16 +440,8 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
         }
     }
     // ---- the context's records
-    const float* base = part + idx::rec(t * nh + h, 0, smax) * PART;
     for (int s0 = 0; s0 < smax; s0 += SL * SPL) {
-        f2 hv[SPL];
-        f4 ov[SPL];
-#pragma unroll
-        for (int j = 0; j < SPL; ++j) {   // slots past the last record reload it and count nothing
-            const float* rec = base + (size_t)min(s0 + sg + SL * j, smax - 1) * PART;
-            hv[j] = *(const f2*)rec;
-            ov[j] = ld_f4(rec + 4 + d0);
-        }
+        if (s0) load(s0);
         float mloc = M;
 #pragma unroll
         for (int j = 0; j < SPL; ++j) mloc = fmaxf(mloc, hv[j][0]);
