@@ -22,7 +22,15 @@ constexpr int SPL = 8;   // context records a lane loads per batch
 constexpr int BM = 64, BN = 64;          // rows per workgroup and keys per tile of the row-block form
 constexpr float P_BITS = 7.0f;           // weights up to 2^15 of the reference: see the softmax
 constexpr float LN2_F = 0.6931471805599453f;
+
+// v = hi + lo to 2^-22 with hi, lo f16: hi by the packed conversion (toward zero), and the rest v - hi, exact in f32, rounded
+// to f16 by the fused form of multiply, add and conversion (neg1 is -1 in a register: with the constant the compiler
+// makes a subtraction and converts back and forth).
+__device__ __forceinline__ void split2(f2 v, float neg1, h2& hi, h2& lo) {
+    hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(v[0], v[1]));
+    lo = h2{(_Float16)__builtin_fmaf((float)hi[0], neg1, v[0]), (_Float16)__builtin_fmaf((float)hi[1], neg1, v[1])};
 }
+}  // namespace
 
 // The context's records for many rows (R = nt * nh / nkv rows of a KV head, more than 32): workgroup = 64 rows r = t*G + g
 // of one KV head x one key split, four waves of 32 rows x half of each 64-key tile's keys: wave w takes rows
@@ -54,6 +62,8 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     const int wr = w & 1, wk = w >> 1;
     const int kb0 = s * chunk, kend = min(kb0 + chunk, n);
     const size_t head_off = (size_t)kh * HD;
+    float neg1 = -1.0f;
+    asm("" : "+v"(neg1));
     int cj[8];   // byte offset of the chunk each lane's tile loads bring, plus the KV head's column
 #pragma unroll
     for (int i = 0; i < 8; ++i) cj[i] = 2 * (int)head_off + 16 * ((l & 31) ^ swz32(16 * w + 2 * i + (l >> 5)));
@@ -81,20 +91,10 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int row = 16 * w + i;
-            h4 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-                // The products are kept apart from the conversions: fused with them, the hi that is stored and the hi that
-                // lo is the rest of were rounded by different instructions, differently about once in 2^13 values.
-                f2 v = {qx[i][e] * sc, qx[i][e + 1] * sc};
-                asm("" : "+v"(v));
-                const h2 h = __builtin_convertvector(v, h2);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    hi[e + j] = h[j];
-                    lo[e + j] = (_Float16)__builtin_fmaf((float)h[j], -1.0f, v[j]);
-                }
-            }
+            h2 h0, h1, l0, l1;
+            split2(f2{qx[i][0] * sc, qx[i][1] * sc}, neg1, h0, l0);
+            split2(f2{qx[i][2] * sc, qx[i][3] * sc}, neg1, h1, l1);
+            const h4 hi = {h0[0], h0[1], h1[0], h1[1]}, lo = {l0[0], l0[1], l1[0], l1[1]};
             const int to = row * HD + 8 * ((l >> 1) ^ (row & 31)) + 4 * (l & 1);
             *(h4*)(K1 + to) = hi;
             *(h4*)(V1 + to) = lo;
@@ -174,13 +174,14 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     };
     auto weight2 = [&](int i) {   // weights i and i + 1
         const f2 p = {__builtin_amdgcn_exp2f(sc[i]), __builtin_amdgcn_exp2f(sc[i + 1])};
-        const h2 hi = __builtin_convertvector(p, h2);
+        h2 hi, lo;
+        split2(p, neg1, hi, lo);
         l_run += p[0];
         l_run += p[1];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             ph[i >> 3][(i & 7) + e] = hi[e];
-            pl[i >> 3][(i & 7) + e] = (_Float16)__builtin_fmaf((float)hi[e], -1.0f, p[e]);
+            pl[i >> 3][(i & 7) + e] = lo[e];
         }
     };
     // Tile loads in flight: offsets of this lane's rows from the tile's first, clamped anew for the last, partial tiles
