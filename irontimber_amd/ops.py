@@ -442,30 +442,34 @@ ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 TREE_MAX = 64
 
 
-def _call_on(t: torch.Tensor, name: str, *args) -> None:
-    """call(name, *args, stream) with t's device current and its current stream."""
-    dev = t.device.index
+def _call_on(dev: int, name: str, *args) -> None:
+    """call(name, *args, stream) with device dev current and its current stream (asked for as a number: the stream
+    object of torch.cuda.current_stream takes 1 us to make, a third of a short launch)."""
     if dev == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _need_all(dtype: torch.dtype, device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        _need(t, dtype, name)
-        if t.device != device:
-            raise ValueError(f"{name} must be on {device}, like the other tensors")
+def _need_all(dtype: torch.dtype, dev: int, tensors, names: str) -> None:
+    """Every tensor contiguous, of dtype and on device dev; names in the tensors' order, for the message. One pass over
+    cheap queries: these checks are most of what a short call costs the host."""
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != dev or dev < 0 or not t.is_contiguous():
+            name = names.split()[[u is t for u in tensors].index(True)]
+            _need(t, dtype, name)
+            raise ValueError(f"{name} must be on the same device as the other tensors")
 
 
-def _need_cache(c: torch.Tensor, name: str, dtypes, device: torch.device, kvd: int, rows: int) -> None:
-    if c.dtype not in dtypes or c.dim() != 2 or not c.is_contiguous() or c.shape[1] != kvd:
-        raise ValueError(f"{name} must be contiguous [rows, {kvd}] of {dtypes[0]}")
-    if c.device != device:
-        raise ValueError(f"{name} must be on {device}, like the other tensors")
-    if c.shape[0] < rows:
-        raise ValueError(f"{name} too short: {c.shape[0]} rows, {rows} needed")
+def _need_caches(dtypes, dev: int, kvd: int, rows: int, kc: torch.Tensor, vc: torch.Tensor) -> None:
+    for c in (kc, vc):
+        if c.dtype not in dtypes or not c.is_contiguous() or c.dim() != 2 or c.shape[1] != kvd:
+            raise ValueError(f"kc and vc must be contiguous [rows, {kvd}] of {dtypes[0]}")
+        if c.get_device() != dev or dev < 0:
+            raise ValueError("kc and vc must be device tensors, on the same device as the other tensors")
+        if c.shape[0] < rows:
+            raise ValueError(f"cache too short: {c.shape[0]} rows, {rows} needed")
 
 
 _F16 = (torch.float16, torch.int16)
@@ -485,8 +489,9 @@ def rope_freqs(n_rot: int, base: float = 1e7, kind: str = "plain", factor: float
 
 
 def _prep_pos(name, kinds, q, k, v, kc, vc, pos, row0, nh, nkv, freq, mscale, layout, q_norm, k_norm, eps, pos0, *more):
-    dev = q.device
-    _need_all(torch.float32, dev, q=q, k=k, v=v, freq=freq)
+    dev = q.get_device()
+    _need_all(torch.float32, dev, [t for t in (q, k, v, freq, q_norm, k_norm) if t is not None],
+              "q k v freq " + ("q_norm " if q_norm is not None else "") + "k_norm")
     if k.dim() != 2 or k.shape[1] % nkv != 0:
         raise ValueError("k must be [nt, nkv*hd]")
     nt, kvd = k.shape
@@ -495,22 +500,18 @@ def _prep_pos(name, kinds, q, k, v, kc, vc, pos, row0, nh, nkv, freq, mscale, la
         raise ValueError("q must be [nt, nh*2*hd] and v the shape of k [nt, nkv*hd]")
     if row0 < 0:
         raise ValueError("row0 must not be negative")
-    _need_cache(kc, "kc", kinds, dev, kvd, row0 + nt)
-    _need_cache(vc, "vc", kinds, dev, kvd, row0 + nt)
+    _need_caches(kinds, dev, kvd, row0 + nt, kc, vc)
     if pos is not None:
-        _need_all(torch.int32, dev, pos=pos)
+        _need_all(torch.int32, dev, (pos,), "pos")
         if pos.shape != (nt,):
             raise ValueError("pos must be [nt]")
-    for w, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None:
-            _need_all(torch.float32, dev, **{n: w})
-            if w.numel() != hd:
-                raise ValueError(f"{n} must hold head_dim floats")
+    if (q_norm is not None and q_norm.numel() != hd) or (k_norm is not None and k_norm.numel() != hd):
+        raise ValueError("q_norm and k_norm must hold head_dim floats")
     if layout not in ROPE_LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(ROPE_LAYOUTS)}")
-    _call_on(q, name, q.data_ptr(), q.shape[1], k.data_ptr(), v.data_ptr(), kvd, _ptr(q_norm), _ptr(k_norm), float(eps),
+    _call_on(dev, name, q.data_ptr(), nh * 2 * hd, k.data_ptr(), v.data_ptr(), kvd, _ptr(q_norm), _ptr(k_norm), eps,
              kc.data_ptr(), vc.data_ptr(), kvd, _ptr(pos), pos0, row0, hd, nh, nkv, nt, 2 * freq.numel(),
-             freq.data_ptr(), float(mscale), ROPE_LAYOUTS[layout], *more)
+             freq.data_ptr(), mscale, ROPE_LAYOUTS[layout], *more)
 
 
 def attn_prep_pos_f16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor,
@@ -533,8 +534,8 @@ def attn_prep_pos_f32kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc: t
               pos0)
 
 
-def _need_anc(anc: torch.Tensor, device: torch.device, nt: int) -> None:
-    _need_all(torch.int64, device, anc=anc)
+def _need_anc(anc: torch.Tensor, dev: int, nt: int) -> None:
+    _need_all(torch.int64, dev, (anc,), "anc")
     if anc.shape != (nt,):
         raise ValueError(f"anc must be [{nt}]")
 
@@ -546,7 +547,7 @@ def tree_plan(parent: torch.Tensor, p0: int) -> tuple[torch.Tensor, torch.Tensor
     nt = parent.numel()
     anc = torch.empty(nt, device=parent.device, dtype=torch.int64)
     pos = torch.empty(nt, device=parent.device, dtype=torch.int32)
-    _call_on(parent, "it_tree_plan", parent.data_ptr(), nt, p0, anc.data_ptr(), pos.data_ptr())
+    _call_on(parent.get_device(), "it_tree_plan", parent.data_ptr(), nt, p0, anc.data_ptr(), pos.data_ptr())
     return anc, pos
 
 
@@ -559,42 +560,41 @@ def attn_tree_f16(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, pos0: int
                   scratch: torch.Tensor | None = None) -> torch.Tensor:
     """attn_f16 for the nodes of a drafted tree: q [nt, nh*2*hd] f32, nodes in cache rows pos0 + t, anc [nt] int64
     (tree_plan) -> out [nt, nh*hd] f32; zeros for padding nodes (it_attn_tree_f16)."""
-    dev = q.device
-    _need_all(torch.float32, dev, q=q)
+    dev = q.get_device()
     if q.dim() != 2 or q.shape[1] % (2 * nh) != 0:
         raise ValueError("q must be [nt, nh*2*hd]")
     nt, hd = q.shape[0], q.shape[1] // (2 * nh)
     kvd = nkv * hd
-    _need_cache(kc, "kc", _F16, dev, kvd, pos0 + nt)
-    _need_cache(vc, "vc", _F16, dev, kvd, pos0 + nt)
+    if out is None:
+        out = torch.empty(nt, nh * hd, device=q.device, dtype=torch.float32)
+    _need_all(torch.float32, dev, (q, out), "q out")
+    if out.shape != (nt, nh * hd):
+        raise ValueError("out must be [nt, nh*hd]")
+    _need_caches(_F16, dev, kvd, pos0 + nt, kc, vc)
     _need_anc(anc, dev, nt)
     if scale is None:
         scale = 1.0 / hd ** 0.5
-    if out is None:
-        out = torch.empty(nt, nh * hd, device=dev, dtype=torch.float32)
-    _need_all(torch.float32, dev, out=out)
-    if out.shape != (nt, nh * hd):
-        raise ValueError("out must be [nt, nh*hd]")
     if scratch is None:
         need = attn_tree_scratch_bytes(pos0, nt, nh, nkv, hd)
-        scratch = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-    elif scratch.device != dev or not scratch.is_contiguous():
-        raise ValueError(f"scratch must be contiguous, on {dev}")
+        scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+    elif scratch.get_device() != dev or not scratch.is_contiguous():
+        raise ValueError("scratch must be contiguous, on the same device as the other tensors")
     nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    _call_on(q, "it_attn_tree_f16", q.data_ptr(), nh * 2 * hd, kc.data_ptr(), vc.data_ptr(), kvd, pos0, hd, nh, nkv, nt,
-             anc.data_ptr(), float(scale), out.data_ptr(), nh * hd, _ptr(scratch), nbytes)
+    _call_on(dev, "it_attn_tree_f16", q.data_ptr(), nh * 2 * hd, kc.data_ptr(), vc.data_ptr(), kvd, pos0, hd, nh, nkv, nt,
+             anc.data_ptr(), scale, out.data_ptr(), nh * hd, _ptr(scratch), nbytes)
     return out
 
 
 def _kv_tree_commit(name, kinds, kc, vc, pos0, nt, anc, leaf):
-    if not kc.is_cuda or kc.dim() != 2:
+    dev = kc.get_device()
+    if dev < 0 or kc.dim() != 2:
         raise ValueError("kc must be a device tensor [rows, kvd]")
-    _need_anc(anc, kc.device, nt)
-    if vc.dtype != kc.dtype:
+    if vc.dtype is not kc.dtype:
         raise ValueError("kc and vc must have one dtype")
-    for c, n in ((kc, "kc"), (vc, "vc")):
-        _need_cache(c, n, kinds, kc.device, kc.shape[1], pos0 + nt)
-    _call_on(kc, name, kc.data_ptr(), vc.data_ptr(), kc.shape[1], pos0, nt, anc.data_ptr(), leaf)
+    kvd = kc.shape[1]
+    _need_caches(kinds, dev, kvd, pos0 + nt, kc, vc)
+    _need_anc(anc, dev, nt)
+    _call_on(dev, name, kc.data_ptr(), vc.data_ptr(), kvd, pos0, nt, anc.data_ptr(), leaf)
 
 
 def kv_tree_commit_f16(kc: torch.Tensor, vc: torch.Tensor, pos0: int, nt: int, anc: torch.Tensor, leaf: int) -> None:
@@ -613,37 +613,27 @@ def gdn_tree_trace(nt: int, nv: int, nk: int, device) -> torch.Tensor:
     return torch.empty(lib().it_gdn_tree_trace_bytes(nt, nv, nk, 128), device=device, dtype=torch.uint8)
 
 
-def _need_gdn_tree(x, conv_state, state, anc, nv, nk, trace):
-    dev = x.device
-    _need_all(torch.float32, dev, x=x, conv_state=conv_state, state=state)
-    cd = (2 * nk + nv) * 128
-    if x.dim() != 2 or x.shape[1] != cd:
-        raise ValueError(f"x must be [nt, {cd}]")
-    if state.shape != (nv, 128, 128):
-        raise ValueError(f"state must be [{nv}, 128, 128]")
-    if conv_state.dim() != 2 or conv_state.shape[1] != cd:
-        raise ValueError(f"conv_state must be [K-1, {cd}]")
-    _need_anc(anc, dev, x.shape[0])
-    _need_all(torch.uint8, dev, trace=trace)
-
-
 def gdn_tree(x: torch.Tensor, w: torch.Tensor, conv_state: torch.Tensor, beta_raw: torch.Tensor, alpha_raw: torch.Tensor,
              dt: torch.Tensor, a: torch.Tensor, state: torch.Tensor, anc: torch.Tensor, nv: int, nk: int,
              trace: torch.Tensor, eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor:
     """The recurrent layer over a drafted tree in one launch: x [nt, (2nk+nv)*128], w [cd, K], conv_state [K-1, cd] and
     state [nv, 128, 128] (both only read), beta_raw/alpha_raw [nt, nv], anc [nt] int64 (tree_plan) -> out
     [nt, nv*128]; trace (gdn_tree_trace) keeps what gdn_tree_commit needs (it_gdn_tree)."""
-    _need_gdn_tree(x, conv_state, state, anc, nv, nk, trace)
-    dev, nt, K = x.device, x.shape[0], conv_state.shape[0] + 1
+    dev, (nt, cd), K = x.get_device(), x.shape, conv_state.shape[0] + 1
     if out is None:
-        out = torch.empty(nt, nv * 128, device=dev, dtype=torch.float32)
-    _need_all(torch.float32, dev, w=w, beta_raw=beta_raw, alpha_raw=alpha_raw, dt=dt, a=a, out=out)
-    if w.shape != (x.shape[1], K) or beta_raw.shape != (nt, nv) or alpha_raw.shape != (nt, nv) or dt.numel() != nv or \
+        out = torch.empty(nt, nv * 128, device=x.device, dtype=torch.float32)
+    _need_all(torch.float32, dev, (x, conv_state, state, w, beta_raw, alpha_raw, dt, a, out),
+              "x conv_state state w beta_raw alpha_raw dt a out")
+    if cd != (2 * nk + nv) * 128 or conv_state.shape != (K - 1, cd) or state.shape != (nv, 128, 128):
+        raise ValueError("x must be [nt, (2nk+nv)*128], conv_state [K-1, (2nk+nv)*128] and state [nv, 128, 128]")
+    if w.shape != (cd, K) or beta_raw.shape != (nt, nv) or alpha_raw.shape != (nt, nv) or dt.numel() != nv or \
             a.numel() != nv or out.shape != (nt, nv * 128):
         raise ValueError("w must be [cd, K], beta_raw / alpha_raw [nt, nv], dt / a [nv] and out [nt, nv*128]")
-    _call_on(x, "it_gdn_tree", x.data_ptr(), x.shape[1], w.data_ptr(), K, conv_state.data_ptr(), beta_raw.data_ptr(),
+    _need_anc(anc, dev, nt)
+    _need_all(torch.uint8, dev, (trace,), "trace")
+    _call_on(dev, "it_gdn_tree", x.data_ptr(), cd, w.data_ptr(), K, conv_state.data_ptr(), beta_raw.data_ptr(),
              alpha_raw.data_ptr(), nv, dt.data_ptr(), a.data_ptr(), state.data_ptr(), anc.data_ptr(), out.data_ptr(),
-             nv * 128, nt, nv, nk, 128, float(eps), trace.data_ptr(), trace.numel())
+             nv * 128, nt, nv, nk, 128, eps, trace.data_ptr(), trace.numel())
     return out
 
 
@@ -651,6 +641,11 @@ def gdn_tree_commit(x: torch.Tensor, conv_state: torch.Tensor, state: torch.Tens
                     nk: int, trace: torch.Tensor) -> None:
     """conv_state and state <- those after node leaf of the gdn_tree call that wrote trace (the same x and anc); leaf -1:
     they stay (it_gdn_tree_commit)."""
-    _need_gdn_tree(x, conv_state, state, anc, nv, nk, trace)
-    _call_on(x, "it_gdn_tree_commit", x.data_ptr(), x.shape[1], conv_state.shape[0] + 1, conv_state.data_ptr(),
-             state.data_ptr(), anc.data_ptr(), leaf, x.shape[0], nv, nk, 128, trace.data_ptr(), trace.numel())
+    dev, (nt, cd), K = x.get_device(), x.shape, conv_state.shape[0] + 1
+    _need_all(torch.float32, dev, (x, conv_state, state), "x conv_state state")
+    if cd != (2 * nk + nv) * 128 or conv_state.shape != (K - 1, cd) or state.shape != (nv, 128, 128):
+        raise ValueError("x must be [nt, (2nk+nv)*128], conv_state [K-1, (2nk+nv)*128] and state [nv, 128, 128]")
+    _need_anc(anc, dev, nt)
+    _need_all(torch.uint8, dev, (trace,), "trace")
+    _call_on(dev, "it_gdn_tree_commit", x.data_ptr(), cd, K, conv_state.data_ptr(), state.data_ptr(), anc.data_ptr(), leaf,
+             nt, nv, nk, 128, trace.data_ptr(), trace.numel())
