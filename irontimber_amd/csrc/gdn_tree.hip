@@ -7,7 +7,7 @@
 //   (I + A) U = beta (V - e^G (K S0))                    row i: the update u_i that node i adds to the state
 //   out_i = (e^G_i q_i S0 + sum_j (q_i . k_j) e^(G_i - G_j) u_j) / sqrt(S)     j an ancestor of i or i itself
 // Topological order makes A strictly lower triangular. G is summed in f64: far down a strongly decaying path
-// the differences would lose f32's digits. All products are f32 (v_mfma_f32_16x16x4_f32).
+// the differences would lose f32's digits.
 // The commit writes S_i = e^G_i S0 + sum_j e^(G_i - G_j) k_j u_j over i's path from the U, k and G that the layer
 // call leaves in its trace. No counterpart in the reference, which steps one token at a time
 // (src/vk/mod.rs:790-806) and copies checkpoints (1018-1025).
@@ -19,7 +19,8 @@ namespace it {
 namespace {
 constexpr int S = 128;        // state size, and channels per head
 constexpr int CW = 16;        // state columns per workgroup
-constexpr int KST = S + 4;    // LDS row of a q or k row (floats)
+constexpr int KST = S + 4;    // LDS row of a state column (floats)
+constexpr int HST = S + 8;    // LDS row of a q or k row (halves)
 constexpr int RST = CW + 4;   // LDS row of a node's CW columns
 
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -30,65 +31,154 @@ __device__ __forceinline__ uint64_t node_mask(const uint64_t* anc, int t) {
     return m >> t & 1 ? m : 0;
 }
 
-// The conv input j tokens before node t on its path: an ancestor's row of x, or beyond the path's start a
-// row of the conv state (K - 1 rows, oldest first). m: t's mask, dropped bit by bit as the taps walk up.
+// The addresses of the K conv inputs of a node, j tokens back: its ancestors' rows of x, and beyond the path's start
+// rows of the conv state (K - 1 rows, the newest last). m: the node's mask, taken bit by bit from the top. Held as
+// integers so that a lane can hand them to its wave.
 template <int K>
-struct Taps {
-    const float* row[K];   // row[j]: the tap's input row, j tokens back
-    __device__ __forceinline__ Taps(uint64_t m, const float* x, int xts, const float* cst, int cd) {
-        int beyond = K - 2;   // the state's newest row first
+__device__ __forceinline__ void taps(uint64_t m, const float* x, int xts, const float* cst, int cd, uint64_t (&row)[K]) {
+    int beyond = K - 2;
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const int a = 63 - (int)__builtin_clzll(m | 1);
-            row[j] = m ? x + (size_t)a * xts : cst + (size_t)(beyond--) * cd;
-            if (m) m &= ~((uint64_t)1 << a);
-        }
+    for (int j = 0; j < K; ++j) {
+        const int a = 63 - (int)__builtin_clzll(m | 1);
+        row[j] = (uint64_t)(uintptr_t)(m ? x + (size_t)a * xts : cst + (size_t)max(beyond, 0) * cd);
+        if (!m) --beyond;
+        m &= ~((uint64_t)1 << a);
     }
-};
+}
+typedef __attribute__((address_space(1))) const float gfloat;
+typedef __attribute__((address_space(1))) const f4 gf4;
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
+           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32;
+}
+__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__shfl((int)(uint32_t)v, lane) | (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane) << 32;
+}
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 }  // namespace
 
-// Workgroup = (V head h, CW = 16 state columns), four waves; NB blocks of 16 nodes. A head's q and k rows are
+// Workgroup = (V head h, CW = 16 state columns), NW waves; NB blocks of 16 nodes. A head's q and k rows are
 // convolved and normalised by each of its eight workgroups (into LDS), so no launch or barrier of the whole
-// GPU stands between the conv and the products. The waves share the products out in 16x16 tasks; the inverses of
-// I + A's diagonal blocks go one to a wave, and then every wave solves for all of U in registers (a few
-// products more than one wave's share, but no exchange) and writes the output rows of its block.
-template <int K, int NB>
-__global__ __launch_bounds__(256) void gdn_tree_kernel(
+// GPU stands between the conv and the products. The normalised rows, at most 1, are kept as f16 pairs hi + lo
+// (2^-22): q K^T and K K^T take three f16 matrix ops of 16 cycles for 32 dims (hi hi, hi lo, lo hi) where f32 ones
+// would take eight of 32; the products with the state, which has no bound, are f32 on hi + lo. The waves share the
+// products out in 16x16 tasks; the inverses of I + A's diagonal blocks go one to a wave, and then each of the first
+// NB waves solves for all of U in registers (a few products more than its share, but no exchange) and writes the
+// output rows of its block.
+// NW: four waves for one block (three nodes: two workgroups a CU and little to share out), eight for more: with one
+// workgroup a CU they hide each other's loads.
+template <int K, int NB, int NW>
+__global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     const float* __restrict__ x, int xts, const float* __restrict__ cw, const float* __restrict__ cst,
     const float* __restrict__ br, const float* __restrict__ ar, int bts, const float* __restrict__ dt,
     const float* __restrict__ A, const float* __restrict__ state, const uint64_t* __restrict__ anc,
     float* __restrict__ out, int ots, int nt, int nv, int nk, float eps, float* __restrict__ trace) {
     constexpr int N = 16 * NB, AST = N + 4;
-    __shared__ __align__(16) float qk[2][N][KST];      // normalised q and k rows, zeros for padding
-    __shared__ __align__(16) float na[N][AST];         // -A
-    __shared__ __align__(16) float pm[N][AST];         // (q_i . k_j) e^(G_i - G_j)
-    __shared__ __align__(16) float tin[NB][16][20];    // inverses of the diagonal blocks of I + A
-    __shared__ float vs[N][RST], rs[N][RST], os[N][RST];   // conv'd V, right-hand sides, e^G q S0
+    __shared__ __align__(16) _Float16 qk[2][2][N][HST];   // [q, k][hi, lo] rows, zeros for padding
+    __shared__ __align__(16) float s0t[CW][KST];          // the state slice, column by column
+    __shared__ __align__(16) float na[N][AST];            // -A
+    __shared__ __align__(16) float pm[N][AST];            // (q_i . k_j) e^(G_i - G_j)
+    __shared__ __align__(16) float tin[NB][16][20];       // inverses of the diagonal blocks of I + A
+    __shared__ float vs[N][RST], rs[N][RST], os[N][RST];  // conv'd V, right-hand sides, e^G q S0
     __shared__ double gs[N];
     __shared__ float bs[N];
     __shared__ uint64_t ms[N];
-    __shared__ int spoilt;                             // a value that is not finite went into the products
+    __shared__ int spoilt;                                // a value that is not finite went into the products
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, c = l & 15, g = l >> 4;
     const int cb = blockIdx.x & 7, h = blockIdx.x >> 3, kh = h % nk, cd = (2 * nk + nv) * S;
-    const float* sb = state + (size_t)h * S * S + cb * CW + c;
 
-    // The state slice as the B operand of the S0 products, in the order of the A operand's 16-byte reads: lane
-    // (c, g) holds column c of rows 16 kk + 4 g + e.
-    float s0[8][4];
+    // ---- everything that hangs on no other load: the masks (a node a lane, in every wave), the state slice, conv
+    // weights, gates
+    const uint64_t m = l < nt ? node_mask(anc, l) : 0;
+    constexpr int SL = S * CW / 4 / (64 * NW);   // 16-byte pieces of the slice per thread
+    f4 sl[SL];
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk)
+    for (int i = 0; i < SL; ++i) {
+        const int p = tid + 64 * NW * i;
+        sl[i] = ld_f4(state + ((size_t)h * S + (p >> 2)) * S + cb * CW + 4 * (p & 3));
+    }
+    const int ch = (l < 32 ? kh : nk + kh) * S + 4 * (l & 31);         // lanes 0-31 four q channels each, 32-63 k
+    const int chv = 2 * nk * S + h * S + cb * CW + (tid & 15);         // V channel
+    f4 wt[K];
+    float wv[K];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s0[kk][e] = sb[(size_t)(16 * kk + 4 * g + e) * S];
+    for (int i = 0; i < K; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wt[i][e] = cw[(size_t)(ch + e) * K + i];
+        wv[i] = cw[(size_t)chv * K + i];
+    }
+    float brv = 0.f, arv = 0.f;
+    if (w == NW - 1 && l < nt) {
+        brv = br[(size_t)l * bts + h];
+        arv = ar[(size_t)l * bts + h] + dt[h];
+    }
+    uint64_t row[K];   // lane = node
+    taps<K>(m, x, xts, cst, cd, row);
 
-    // ---- masks, gates and path sums, a node a lane of wave 0
-    if (w == 0) {
-        const uint64_t m = l < nt ? node_mask(anc, l) : 0;
+    // ---- conv + SiLU + L2 norm of the q and k heads, three or four nodes at a time (padding nodes read the conv state)
+    constexpr int PER = N / NW, BATCH = PER % 4 == 0 ? 4 : 3;
+    static_assert(PER % BATCH == 0 && PER * NW == N, "every node once, none past the LDS rows");
+#pragma unroll
+    for (int i0 = 0; i0 < PER; i0 += BATCH) {
+        f4 in[BATCH][K];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+            for (int j = 0; j < K; ++j) in[i][j] = *(gf4*)((gfloat*)lane_u64(row[j], w + NW * (i0 + i)) + ch);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int t = w + NW * (i0 + i);
+            f4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = K - 1; j >= 0; --j) y += in[i][j] * wt[K - 1 - j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = silu_hw(y[e]);
+            float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
+            ss += dppc<0xB1>(ss);
+            ss += dppc<0x4E>(ss);
+            ss += dppc<0x141>(ss);
+            ss += dppc<0x140>(ss);
+            ss = sum_xor16(ss);
+            const float f = 1.0f / fmaxf(sqrtf(ss), eps);
+            const bool live = lane_u64(m, t) != 0;
+            h4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v = live ? y[e] * f : 0.f;
+                asm("" : "+v"(v));   // (rounded once: fused into the conversions, hi and lo would not belong together)
+                hi[e] = (_Float16)v;
+                lo[e] = (_Float16)(v - (float)hi[e]);
+            }
+            *(h4*)&qk[l >> 5][0][t][4 * (l & 31)] = hi;
+            *(h4*)&qk[l >> 5][1][t][4 * (l & 31)] = lo;
+        }
+    }
+    // ---- conv + SiLU of the workgroup's V columns: 16 lanes a node
+    constexpr int VN = (N + 4 * NW - 1) / (4 * NW);
+    {
+        float in[VN][K];
+#pragma unroll
+        for (int b = 0; b < VN; ++b) {
+            const int t = 4 * NW * b + (tid >> 4);
+#pragma unroll
+            for (int j = 0; j < K; ++j) in[b][j] = ((gfloat*)shfl_u64(row[j], min(t, N - 1)))[chv];
+        }
+#pragma unroll
+        for (int b = 0; b < VN; ++b) {
+            const int t = 4 * NW * b + (tid >> 4);
+            float y = 0.f;
+#pragma unroll
+            for (int j = K - 1; j >= 0; --j) y += in[b][j] * wv[K - 1 - j];
+            if (t < N) vs[t][tid & 15] = silu_hw(y);
+        }
+    }
+    // ---- gates and path sums, a node a lane of the last wave
+    if (w == NW - 1) {
         double G = 0.0;
         float beta = 0.f;
         if (m) {
-            beta = sigmoidf_(br[(size_t)l * bts + h]);
-            const float lg = softplusf_(ar[(size_t)l * bts + h] + dt[h]) * A[h];
+            beta = sigmoidf_(brv);
+            const float lg = softplusf_(arv) * A[h];
             G = lg < -200.f ? -200.0 : (double)lg;   // e^-200 is 0 in f32 already; sums stay finite
         }
         const uint64_t above = m & ~((uint64_t)1 << l);
@@ -102,69 +192,27 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(
         if (l < N) { ms[l] = m; gs[l] = G; bs[l] = beta; }
         if (l == 0) spoilt = 0;
     }
-    // ---- conv + SiLU + L2 norm of the q and k heads: lanes 0-31 four q channels each, lanes 32-63 k
-    {
-        const int ch = (l < 32 ? kh : nk + kh) * S + 4 * (l & 31);
-        f4 wt[K];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+    for (int i = 0; i < SL; ++i) {
+        const int p = tid + 64 * NW * i;
 #pragma unroll
-            for (int i = 0; i < K; ++i) wt[i][e] = cw[(size_t)(ch + e) * K + i];
-#pragma unroll 4
-        for (int i = 0; i < N / 4; ++i) {
-            const int t = 4 * i + w;
-            f4 y = {0.f, 0.f, 0.f, 0.f};
-            const uint64_t m = t < nt ? node_mask(anc, t) : 0;
-            if (m) {
-                const Taps<K> tap(m, x, xts, cst, cd);
-#pragma unroll
-                for (int j = K - 1; j >= 0; --j) y += ld_f4(tap.row[j] + ch) * wt[K - 1 - j];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = siluf_(y[e]);
-                float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
-                ss += dppc<0xB1>(ss);
-                ss += dppc<0x4E>(ss);
-                ss += dppc<0x141>(ss);
-                ss += dppc<0x140>(ss);
-                ss = sum_xor16(ss);
-                y *= 1.0f / fmaxf(sqrtf(ss), eps);
-            }
-            *(f4*)&qk[l >> 5][t][4 * (l & 31)] = y;
-        }
-    }
-    // ---- conv + SiLU of the workgroup's V columns
-    {
-        const int ch = 2 * nk * S + h * S + cb * CW + (tid & 15);
-        float wt[K];
-#pragma unroll
-        for (int i = 0; i < K; ++i) wt[i] = cw[(size_t)ch * K + i];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int t = 16 * b + (tid >> 4);
-            float y = 0.f;
-            const uint64_t m = t < nt ? node_mask(anc, t) : 0;
-            if (m) {
-                const Taps<K> tap(m, x, xts, cst, cd);
-#pragma unroll
-                for (int j = K - 1; j >= 0; --j) y += tap.row[j][ch] * wt[K - 1 - j];
-                y = siluf_(y);
-            }
-            vs[t][tid & 15] = y;
-        }
+        for (int e = 0; e < 4; ++e) s0t[4 * (p & 3) + e][p >> 2] = sl[i][e];
     }
     __syncthreads();
     // ---- products in 16x16 tasks: {K, Q} S0 of each block, then {K, Q} K^T of each pair of blocks bi >= bj
     bool bad = false;
-    for (int task = w; task < 2 * NB + NB * (NB + 1); task += 4) {
+    for (int task = w; task < 2 * NB + NB * (NB + 1); task += NW) {
         const int which = (task & 1) ^ 1;   // 1 k rows, 0 q rows
-        f4 acc = {0.f, 0.f, 0.f, 0.f};
         if (task < 2 * NB) {
             const int b = task >> 1;
+            f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
-                const f4 a = ld_f4(&qk[which][16 * b + c][16 * kk + 4 * g]);
+                const h4 hi = *(const h4*)&qk[which][0][16 * b + c][16 * kk + 4 * g];
+                const h4 lo = *(const h4*)&qk[which][1][16 * b + c][16 * kk + 4 * g];
+                const f4 sv = ld_f4(&s0t[c][16 * kk + 4 * g]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc = mfma4(a[e], s0[kk][e], acc);
+                for (int e = 0; e < 4; ++e) acc = mfma4((float)hi[e] + (float)lo[e], sv[e], acc);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -178,12 +226,16 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(
             int p = (task - 2 * NB) >> 1, bi = 0;   // pair p of the lower triangle, row by row
             while (p > bi) p -= ++bi;
             const int bj = p;
+            f4 acc = {0.f, 0.f, 0.f, 0.f}, small = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-                const f4 a = ld_f4(&qk[which][16 * bi + c][16 * kk + 4 * g]), b = ld_f4(&qk[1][16 * bj + c][16 * kk + 4 * g]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc = mfma4(a[e], b[e], acc);
+            for (int ks = 0; ks < 4; ++ks) {
+                const h8 ah = ld_h8(&qk[which][0][16 * bi + c][32 * ks + 8 * g]), al = ld_h8(&qk[which][1][16 * bi + c][32 * ks + 8 * g]);
+                const h8 bh = ld_h8(&qk[1][0][16 * bj + c][32 * ks + 8 * g]), bl = ld_h8(&qk[1][1][16 * bj + c][32 * ks + 8 * g]);
+                acc = mfma16x16x32(ah, bh, acc);
+                small = mfma16x16x32(ah, bl, small);
+                small = mfma16x16x32(al, bh, small);
             }
+            acc += small;
             const int j = 16 * bj + c;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -217,66 +269,67 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(
             }
         }
     } else {
-        // ---- (I + A_bb)^-1, lane column c, forward substitution on a column of the identity (the four lane
-        // groups alike)
+        // ---- (I + A_bb)^-1, lane column c: a column of the identity, each row's value taken to the rows below as soon as
+        // it is known (the four lane groups alike)
         if (w < NB) {
+            f4 a[16][4];
             float z[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                float v = i == c ? 1.f : 0.f;
+                z[i] = i == c ? 1.f : 0.f;
 #pragma unroll
-                for (int j4 = 0; j4 < i; j4 += 4) {
-                    const f4 a = ld_f4(&na[16 * w + i][16 * w + j4]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j4 + j < i) v += a[j] * z[j4 + j];
-                }
-                z[i] = v;
+                for (int j = 0; j < (i + 3) / 4; ++j) a[i][j] = ld_f4(&na[16 * w + i][16 * w + 4 * j]);
             }
+#pragma unroll
+            for (int j = 0; j < 15; ++j)
+#pragma unroll
+                for (int i = j + 1; i < 16; ++i) z[i] += a[i][j / 4][j % 4] * z[j];
             if (g == 0) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) tin[w][i][c] = z[i];
             }
         }
         __syncthreads();
-        // ---- U block by block: u[b] holds rows 4 g + e of column c, both a product's result and, in the order of
-        // the A operand's 16-byte reads, the next one's B operand
-        f4 u[NB];
+        if (w < NB) {
+            // ---- U block by block: u[b] holds rows 4 g + e of column c, both a product's result and, in the order of
+            // the A operand's 16-byte reads, the next one's B operand
+            f4 u[NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            f4 r;
+            for (int b = 0; b < NB; ++b) {
+                f4 r;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = rs[16 * b + 4 * g + i][c];
+                for (int i = 0; i < 4; ++i) r[i] = rs[16 * b + 4 * g + i][c];
 #pragma unroll
-            for (int j = 0; j < b; ++j) {
-                const f4 a = ld_f4(&na[16 * b + c][16 * j + 4 * g]);
+                for (int j = 0; j < b; ++j) {
+                    const f4 a = ld_f4(&na[16 * b + c][16 * j + 4 * g]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r = mfma4(a[e], u[j][e], r);
+                    for (int e = 0; e < 4; ++e) r = mfma4(a[e], u[j][e], r);
+                }
+                const f4 a = ld_f4(&tin[b][c][4 * g]);
+                u[b] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[b] = mfma4(a[e], r[e], u[b]);
             }
-            const f4 a = ld_f4(&tin[b][c][4 * g]);
-            u[b] = f4{0.f, 0.f, 0.f, 0.f};
+            // ---- output and trace rows of block w
 #pragma unroll
-            for (int e = 0; e < 4; ++e) u[b] = mfma4(a[e], r[e], u[b]);
-        }
-        // ---- output and trace rows of block w
+            for (int b = 0; b < NB; ++b) {
+                if (b != w) continue;   // (static register indexes)
+                f4 o;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (b != w) continue;   // (static register indexes)
-            f4 o;
+                for (int i = 0; i < 4; ++i) o[i] = os[16 * b + 4 * g + i][c];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = os[16 * b + 4 * g + i][c];
+                for (int j = 0; j <= b; ++j) {
+                    const f4 a = ld_f4(&pm[16 * b + c][16 * j + 4 * g]);
 #pragma unroll
-            for (int j = 0; j <= b; ++j) {
-                const f4 a = ld_f4(&pm[16 * b + c][16 * j + 4 * g]);
+                    for (int e = 0; e < 4; ++e) o = mfma4(a[e], u[j][e], o);
+                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o = mfma4(a[e], u[j][e], o);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = 16 * b + 4 * g + i;
-                if (t < nt) {
-                    out[(size_t)t * ots + (size_t)h * S + cb * CW + c] = o[i] * scale;
-                    tu[t * ustride + c] = u[b][i];
+                for (int i = 0; i < 4; ++i) {
+                    const int t = 16 * b + 4 * g + i;
+                    if (t < nt) {
+                        out[(size_t)t * ots + (size_t)h * S + cb * CW + c] = o[i] * scale;
+                        tu[t * ustride + c] = u[b][i];
+                    }
                 }
             }
         }
@@ -284,8 +337,10 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(
     // ---- the rest of the trace: k rows by the QK head's first V head, a sixteenth of the dims a workgroup; G once a head
     if (h < nk) {
         float* tk = trace + (size_t)nt * nv * S + (size_t)h * S + cb * CW;
-        for (int i = tid; i < nt * CW; i += 256)
-            tk[(size_t)(i / CW) * nk * S + i % CW] = qk[1][i / CW][cb * CW + i % CW];
+        for (int i = tid; i < nt * CW; i += 64 * NW) {
+            const int t = i / CW, d = cb * CW + i % CW;
+            tk[(size_t)t * nk * S + i % CW] = (float)qk[1][0][t][d] + (float)qk[1][1][t][d];
+        }
     }
     if (cb == 0 && tid < nt) ((double*)(trace + (size_t)nt * (nv + nk) * S))[(size_t)tid * nv + h] = gs[tid];
 }
@@ -299,7 +354,7 @@ hipError_t launch_gdn_tree(const float* x, int xts, const float* cw, int K, cons
                            const uint64_t* anc, float* out, int ots, int nt, int nv, int nk, float eps, float* trace,
                            hipStream_t st) {
 #define IT_GDN_TREE(K_, NB_)                                                                                       \
-    gdn_tree_kernel<K_, NB_><<<8 * nv, 256, 0, st>>>(x, xts, cw, cst, br, ar, bts, dt, a, state, anc, out, ots, nt, nv, nk, \
+    gdn_tree_kernel<K_, NB_, (NB_ > 1 ? 8 : 4)><<<8 * nv, NB_ > 1 ? 512 : 256, 0, st>>>(x, xts, cw, cst, br, ar, bts, dt, a, state, anc, out, ots, nt, nv, nk, \
                                                     eps, trace)
 #define IT_GDN_TREE_K(K_)                    \
     switch ((nt + 15) / 16) {                \
