@@ -22,6 +22,7 @@ constexpr int CW = 16;        // state columns per workgroup
 constexpr int KST = S + 4;    // LDS row of a state column (floats)
 constexpr int HST = S + 8;    // LDS row of a q or k row (halves)
 constexpr int RST = CW + 4;   // LDS row of a node's CW columns
+constexpr double LOG2E_D = 1.4426950408889634074;
 
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
@@ -31,16 +32,16 @@ __device__ __forceinline__ uint64_t node_mask(const uint64_t* anc, int t) {
     return m >> t & 1 ? m : 0;
 }
 
-// The addresses of the K conv inputs of a node, j tokens back: its ancestors' rows of x, and beyond the path's start
-// rows of the conv state (K - 1 rows, the newest last). m: the node's mask, taken bit by bit from the top. Held as
-// integers so that a lane can hand them to its wave.
+// The addresses of a node's conv inputs 1 .. K-1 tokens back: its ancestors' rows of x, and beyond the path's start
+// rows of the conv state (K - 1 rows, the newest last). m: the mask of its strict ancestors, taken bit by bit from the
+// top. Held as integers so that a lane can hand them to its wave.
 template <int K>
-__device__ __forceinline__ void taps(uint64_t m, const float* x, int xts, const float* cst, int cd, uint64_t (&row)[K]) {
+__device__ __forceinline__ void taps(uint64_t m, const float* x, int xts, const float* cst, int cd, uint64_t (&row)[K - 1]) {
     int beyond = K - 2;
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
+    for (int j = 0; j < K - 1; ++j) {
         const int a = 63 - (int)__builtin_clzll(m | 1);
-        row[j] = (uint64_t)(uintptr_t)(m ? x + (size_t)a * xts : cst + (size_t)max(beyond, 0) * cd);
+        row[j] = (uint64_t)(uintptr_t)(m ? x + (size_t)a * xts : cst + (size_t)beyond * cd);
         if (!m) --beyond;
         m &= ~((uint64_t)1 << a);
     }
@@ -80,16 +81,39 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     __shared__ __align__(16) float pm[N][AST];            // (q_i . k_j) e^(G_i - G_j)
     __shared__ __align__(16) float tin[NB][16][20];       // inverses of the diagonal blocks of I + A
     __shared__ float vs[N][RST], rs[N][RST], os[N][RST];  // conv'd V, right-hand sides, e^G q S0
-    __shared__ double gs[N];
+    __shared__ double gs[N];                              // G in log2 units
     __shared__ float bs[N];
     __shared__ uint64_t ms[N];
     __shared__ int spoilt;                                // a value that is not finite went into the products
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, c = l & 15, g = l >> 4;
     const int cb = blockIdx.x & 7, h = blockIdx.x >> 3, kh = h % nk, cd = (2 * nk + nv) * S;
 
-    // ---- everything that hangs on no other load: the masks (a node a lane, in every wave), the state slice, conv
+    // ---- everything that hangs on no other load: the masks (a node a lane, in every wave), the wave's own rows of x
+    // (a node's own input, whatever its path, and on its way the ancestors' rows into the caches), the state slice, conv
     // weights, gates
     const uint64_t m = l < nt ? node_mask(anc, l) : 0;
+    constexpr int PER = N / NW, BATCH = PER % 4 == 0 ? 4 : 3, VN = (N + 4 * NW - 1) / (4 * NW);
+    static_assert(PER % BATCH == 0 && PER * NW == N, "every node once, none past the LDS rows");
+    const int ch = (l < 32 ? kh : nk + kh) * S + 4 * (l & 31);         // lanes 0-31 four q channels each, 32-63 k
+    const int chv = 2 * nk * S + h * S + cb * CW + (tid & 15);         // V channel; 16 lanes a node
+    f4 own[PER], wt[K];
+    float ownv[VN], wv[K];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) own[i] = ld_f4(x + uniform_off((size_t)min(w + NW * i, nt - 1) * xts) + ch);
+#pragma unroll
+    for (int b = 0; b < VN; ++b) ownv[b] = x[(size_t)min(4 * NW * b + (tid >> 4), nt - 1) * xts + chv];
+    float brv = 0.f, arv = 0.f, av = 0.f;
+    if (w == NW - 1 && l < nt) {
+        brv = br[(size_t)l * bts + h];
+        arv = ar[(size_t)l * bts + h] + dt[h];
+        av = A[h];
+    }
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wt[i][e] = cw[(size_t)(ch + e) * K + i];
+        wv[i] = cw[(size_t)chv * K + i];
+    }
     constexpr int SL = S * CW / 4 / (64 * NW);   // 16-byte pieces of the slice per thread
     f4 sl[SL];
 #pragma unroll
@@ -97,40 +121,45 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
         const int p = tid + 64 * NW * i;
         sl[i] = ld_f4(state + ((size_t)h * S + (p >> 2)) * S + cb * CW + 4 * (p & 3));
     }
-    const int ch = (l < 32 ? kh : nk + kh) * S + 4 * (l & 31);         // lanes 0-31 four q channels each, 32-63 k
-    const int chv = 2 * nk * S + h * S + cb * CW + (tid & 15);         // V channel
-    f4 wt[K];
-    float wv[K];
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) wt[i][e] = cw[(size_t)(ch + e) * K + i];
-        wv[i] = cw[(size_t)chv * K + i];
-    }
-    float brv = 0.f, arv = 0.f;
-    if (w == NW - 1 && l < nt) {
-        brv = br[(size_t)l * bts + h];
-        arv = ar[(size_t)l * bts + h] + dt[h];
-    }
-    uint64_t row[K];   // lane = node
-    taps<K>(m, x, xts, cst, cd, row);
+    const uint64_t above = m & ~((uint64_t)1 << l);   // strict ancestors
+    uint64_t row[K - 1];   // lane = node
+    taps<K>(above, x, xts, cst, cd, row);
+    bool bad = false;
 
     // ---- conv + SiLU + L2 norm of the q and k heads, three or four nodes at a time (padding nodes read the conv state)
-    constexpr int PER = N / NW, BATCH = PER % 4 == 0 ? 4 : 3;
-    static_assert(PER % BATCH == 0 && PER * NW == N, "every node once, none past the LDS rows");
 #pragma unroll
     for (int i0 = 0; i0 < PER; i0 += BATCH) {
-        f4 in[BATCH][K];
+        f4 in[BATCH][K - 1];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i)
 #pragma unroll
-            for (int j = 0; j < K; ++j) in[i][j] = *(gf4*)((gfloat*)lane_u64(row[j], w + NW * (i0 + i)) + ch);
+            for (int j = 0; j < K - 1; ++j) in[i][j] = *(gf4*)((gfloat*)lane_u64(row[j], w + NW * (i0 + i)) + ch);
+        if (i0 == 0 && w == NW - 1) {
+            // gates and path sums, a node a lane of the last wave, while its loads are out
+            double G = 0.0;
+            float beta = 0.f;
+            if (m) {
+                beta = sigmoidf_(brv);
+                const float lg = softplusf_(arv) * av;
+                G = lg < -200.f ? -200.0 : (double)lg;   // e^-200 is 0 in f32 already; sums stay finite
+            }
+            int up = above ? 63 - (int)__builtin_clzll(above) : -1;
+#pragma unroll
+            for (int r = 1; r < N; r *= 2) {   // after round r a node's sum covers its nearest 2r nodes
+                const double more = __shfl(G, up < 0 ? l : up);
+                const int next = __shfl(up, up < 0 ? l : up);
+                if (up >= 0) { G += more; up = next; }
+            }
+            if (l < N) { ms[l] = m; gs[l] = G * LOG2E_D; bs[l] = beta; }
+            if (l == 0) spoilt = 0;
+        }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const int t = w + NW * (i0 + i);
-            f4 y = {0.f, 0.f, 0.f, 0.f};
+            f4 y = in[i][K - 2] * wt[0];
 #pragma unroll
-            for (int j = K - 1; j >= 0; --j) y += in[i][j] * wt[K - 1 - j];
+            for (int j = K - 3; j >= 0; --j) y += in[i][j] * wt[K - 2 - j];
+            y += own[i0 + i] * wt[K - 1];
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = silu_hw(y[e]);
             float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
@@ -141,6 +170,7 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             ss = sum_xor16(ss);
             const float f = 1.0f / fmaxf(sqrtf(ss), eps);
             const bool live = lane_u64(m, t) != 0;
+            bad |= live && !finite(ss);
             h4 hi, lo;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -153,44 +183,22 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             *(h4*)&qk[l >> 5][1][t][4 * (l & 31)] = lo;
         }
     }
-    // ---- conv + SiLU of the workgroup's V columns: 16 lanes a node
-    constexpr int VN = (N + 4 * NW - 1) / (4 * NW);
+    // ---- conv + SiLU of the workgroup's V columns
     {
-        float in[VN][K];
+        float in[VN][K - 1];
+#pragma unroll
+        for (int b = 0; b < VN; ++b)
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j)
+                in[b][j] = ((gfloat*)shfl_u64(row[j], min(4 * NW * b + (tid >> 4), N - 1)))[chv];
 #pragma unroll
         for (int b = 0; b < VN; ++b) {
             const int t = 4 * NW * b + (tid >> 4);
+            float y = ownv[b] * wv[K - 1];
 #pragma unroll
-            for (int j = 0; j < K; ++j) in[b][j] = ((gfloat*)shfl_u64(row[j], min(t, N - 1)))[chv];
-        }
-#pragma unroll
-        for (int b = 0; b < VN; ++b) {
-            const int t = 4 * NW * b + (tid >> 4);
-            float y = 0.f;
-#pragma unroll
-            for (int j = K - 1; j >= 0; --j) y += in[b][j] * wv[K - 1 - j];
+            for (int j = 0; j < K - 1; ++j) y += in[b][j] * wv[K - 2 - j];
             if (t < N) vs[t][tid & 15] = silu_hw(y);
         }
-    }
-    // ---- gates and path sums, a node a lane of the last wave
-    if (w == NW - 1) {
-        double G = 0.0;
-        float beta = 0.f;
-        if (m) {
-            beta = sigmoidf_(brv);
-            const float lg = softplusf_(arv) * A[h];
-            G = lg < -200.f ? -200.0 : (double)lg;   // e^-200 is 0 in f32 already; sums stay finite
-        }
-        const uint64_t above = m & ~((uint64_t)1 << l);
-        int up = above ? 63 - (int)__builtin_clzll(above) : -1;
-#pragma unroll
-        for (int r = 1; r < N; r *= 2) {   // after round r a node's sum covers its nearest 2r nodes
-            const double more = __shfl(G, up < 0 ? l : up);
-            const int next = __shfl(up, up < 0 ? l : up);
-            if (up >= 0) { G += more; up = next; }
-        }
-        if (l < N) { ms[l] = m; gs[l] = G; bs[l] = beta; }
-        if (l == 0) spoilt = 0;
     }
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
@@ -200,24 +208,23 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     }
     __syncthreads();
     // ---- products in 16x16 tasks: {K, Q} S0 of each block, then {K, Q} K^T of each pair of blocks bi >= bj
-    bool bad = false;
     for (int task = w; task < 2 * NB + NB * (NB + 1); task += NW) {
         const int which = (task & 1) ^ 1;   // 1 k rows, 0 q rows
         if (task < 2 * NB) {
             const int b = task >> 1;
-            f4 acc = {0.f, 0.f, 0.f, 0.f};
+            f4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // (two chains: a dependent f32 op waits longer than it takes)
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
                 const h4 hi = *(const h4*)&qk[which][0][16 * b + c][16 * kk + 4 * g];
                 const h4 lo = *(const h4*)&qk[which][1][16 * b + c][16 * kk + 4 * g];
                 const f4 sv = ld_f4(&s0t[c][16 * kk + 4 * g]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc = mfma4((float)hi[e] + (float)lo[e], sv[e], acc);
+                for (int e = 0; e < 4; ++e) acc[e & 1] = mfma4((float)hi[e] + (float)lo[e], sv[e], acc[e & 1]);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = 16 * b + 4 * g + i;
-                const float d = acc[i] * expf((float)gs[t]);
+                const float d = (acc[0][i] + acc[1][i]) * __builtin_amdgcn_exp2f((float)gs[t]);
                 const float v = which ? bs[t] * (vs[t][c] - d) : d;
                 (which ? rs : os)[t][c] = ms[t] ? v : 0.f;
                 bad |= ms[t] && !finite(v);
@@ -236,15 +243,15 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
                 small = mfma16x16x32(al, bh, small);
             }
             acc += small;
+            // (finite where the rows are, which the conv has looked at, and the decays, which the S0 products will)
             const int j = 16 * bj + c;
+            const double gj = gs[j];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = 16 * bi + 4 * g + i;
-                const bool sees = (ms[t] >> j & 1) && (!which || j != t);
-                float v = acc[i] * expf((float)(gs[t] - gs[j]));
-                if (which) v *= -bs[t];
-                (which ? na : pm)[t][j] = sees ? v : 0.f;
-                bad |= sees && !finite(v);
+                const int seen = ((const uint16_t*)&ms[t])[bj] >> c & 1;
+                const float v = acc[i] * __builtin_amdgcn_exp2f((float)(gs[t] - gj)) * (which ? -bs[t] : 1.0f);
+                (which ? na : pm)[t][j] = seen && (!which || j != t) ? v : 0.f;
             }
         }
     }
@@ -342,7 +349,7 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             tk[(size_t)t * nk * S + i % CW] = (float)qk[1][0][t][d] + (float)qk[1][1][t][d];
         }
     }
-    if (cb == 0 && tid < nt) ((double*)(trace + (size_t)nt * (nv + nk) * S))[(size_t)tid * nv + h] = gs[tid];
+    if (cb == 0 && tid < nt) ((double*)(trace + (size_t)nt * (nv + nk) * S))[(size_t)tid * nv + h] = gs[tid];   // in log2 units
 }
 
 size_t gdn_tree_trace_bytes(int nt, int nv, int nk) {
@@ -393,7 +400,7 @@ __global__ __launch_bounds__(256) void gdn_tree_commit_kernel(const float* __res
     if (tid < 64 && (m >> tid & 1)) {
         const int i = (int)__popcll(m & (((uint64_t)1 << tid) - 1));
         node[i] = tid;
-        coef[i] = expf((float)(Gl - G[(size_t)tid * nv + h]));
+        coef[i] = __builtin_amdgcn_exp2f((float)(Gl - G[(size_t)tid * nv + h]));
     }
     __syncthreads();
     if (conv) {
@@ -414,7 +421,7 @@ __global__ __launch_bounds__(256) void gdn_tree_commit_kernel(const float* __res
     float* s = state + ((size_t)h * S + row) * S + col;
     const float* tu = trace + (size_t)h * S + col;
     const float* tk = trace + (size_t)nt * nv * S + (size_t)(h % nk) * S + row;
-    const float eg = expf((float)Gl);
+    const float eg = __builtin_amdgcn_exp2f((float)Gl);
     f4 s0 = ld_f4(s) * eg, s1 = ld_f4(s + 4) * eg;
 #pragma unroll 4
     for (int i = 0; i < np; ++i) {
