@@ -22,14 +22,6 @@ constexpr int SPL = 8;   // context records a lane loads per batch
 constexpr int BM = 64, BN = 64;          // rows per workgroup and keys per tile of the row-block form
 constexpr float P_BITS = 7.0f;           // weights up to 2^15 of the reference: see the softmax
 constexpr float LN2_F = 0.6931471805599453f;
-
-// v = hi + lo to 2^-22 with hi, lo f16: hi by the packed conversion (toward zero), and the rest v - hi, exact in f32, rounded
-// to f16 by the fused form of multiply, add and conversion (neg1 is -1 in a register: with the constant the compiler
-// makes a subtraction and converts back and forth).
-__device__ __forceinline__ void split2(f2 v, float neg1, h2& hi, h2& lo) {
-    hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(v[0], v[1]));
-    lo = h2{(_Float16)__builtin_fmaf((float)hi[0], neg1, v[0]), (_Float16)__builtin_fmaf((float)hi[1], neg1, v[1])};
-}
 }  // namespace
 
 // The context's records for many rows (R = nt * nh / nkv rows of a KV head, more than 32): workgroup = 64 rows r = t*G + g
@@ -62,8 +54,7 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     const int wr = w & 1, wk = w >> 1;
     const int kb0 = s * chunk, kend = min(kb0 + chunk, n);
     const size_t head_off = (size_t)kh * HD;
-    float neg1 = -1.0f;
-    asm("" : "+v"(neg1));
+    const float neg1 = in_register(-1.0f);
     int cj[8];   // byte offset of the chunk each lane's tile loads bring, plus the KV head's column
 #pragma unroll
     for (int i = 0; i < 8; ++i) cj[i] = 2 * (int)head_off + 16 * ((l & 31) ^ swz32(16 * w + 2 * i + (l >> 5)));

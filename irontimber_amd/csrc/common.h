@@ -74,6 +74,19 @@ __device__ __forceinline__ h8 to_h8(f4 x0, f4 x1) {
     return r;
 }
 
+// A constant that the compiler has to take from a register, where knowing its value would cost the fused form below.
+__device__ __forceinline__ float in_register(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+// v = hi + lo to 2^-22 with hi, lo f16: hi by the packed conversion (toward zero), and the rest v - hi, exact in f32, rounded
+// to f16 by the fused form of multiply, add and conversion (neg1: in_register(-1.0f); with the plain constant the
+// compiler makes a subtraction and converts back and forth).
+__device__ __forceinline__ void split2(f2 v, float neg1, h2& hi, h2& lo) {
+    hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(v[0], v[1]));
+    lo = h2{(_Float16)__builtin_fmaf((float)hi[0], neg1, v[0]), (_Float16)__builtin_fmaf((float)hi[1], neg1, v[1])};
+}
+
 // Wave-wide max / sum of a float: DPP within 16-lane rows (xor 1, xor 2 by quad_perm, then the
 // half-row and row mirrors), then the four row results through readlane. Every lane returns the
 // full result; no LDS round trip.

@@ -96,18 +96,19 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     static_assert(PER % BATCH == 0 && PER * NW == N, "every node once, none past the LDS rows");
     const int ch = (l < 32 ? kh : nk + kh) * S + 4 * (l & 31);         // lanes 0-31 four q channels each, 32-63 k
     const int chv = 2 * nk * S + h * S + cb * CW + (tid & 15);         // V channel; 16 lanes a node
+    float brv = 0.f, arv = 0.f, dtv = 0.f, av = 0.f;   // gates: a node a lane of the last wave
+    if (w == NW - 1 && l < nt) {
+        brv = br[(size_t)l * bts + h];
+        arv = ar[(size_t)l * bts + h];
+        dtv = dt[h];
+        av = A[h];
+    }
     f4 own[PER], wt[K];
     float ownv[VN], wv[K];
 #pragma unroll
     for (int i = 0; i < PER; ++i) own[i] = ld_f4(x + uniform_off((size_t)min(w + NW * i, nt - 1) * xts) + ch);
 #pragma unroll
     for (int b = 0; b < VN; ++b) ownv[b] = x[(size_t)min(4 * NW * b + (tid >> 4), nt - 1) * xts + chv];
-    float brv = 0.f, arv = 0.f, av = 0.f;
-    if (w == NW - 1 && l < nt) {
-        brv = br[(size_t)l * bts + h];
-        arv = ar[(size_t)l * bts + h] + dt[h];
-        av = A[h];
-    }
 #pragma unroll
     for (int i = 0; i < K; ++i) {
 #pragma unroll
@@ -125,6 +126,7 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     uint64_t row[K - 1];   // lane = node
     taps<K>(above, x, xts, cst, cd, row);
     bool bad = false;
+    const float neg1 = in_register(-1.0f), ieps = eps > 0.f ? 1.0f / eps : INFINITY;
 
     // ---- conv + SiLU + L2 norm of the q and k heads, three or four nodes at a time (padding nodes read the conv state)
 #pragma unroll
@@ -139,15 +141,15 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             double G = 0.0;
             float beta = 0.f;
             if (m) {
-                beta = sigmoidf_(brv);
-                const float lg = softplusf_(arv) * av;
+                beta = sigmoid_hw(brv);
+                const float lg = softplus_hw(arv + dtv) * av;
                 G = lg < -200.f ? -200.0 : (double)lg;   // e^-200 is 0 in f32 already; sums stay finite
             }
             int up = above ? 63 - (int)__builtin_clzll(above) : -1;
-#pragma unroll
-            for (int r = 1; r < N; r *= 2) {   // after round r a node's sum covers its nearest 2r nodes
-                const double more = __shfl(G, up < 0 ? l : up);
-                const int next = __shfl(up, up < 0 ? l : up);
+            while (__any(up >= 0)) {   // each round a node's sum covers twice as many nodes of its path
+                const int a = up < 0 ? l : up;
+                const double more = __builtin_bit_cast(double, shfl_u64(__builtin_bit_cast(uint64_t, G), a));
+                const int next = __shfl(up, a);
                 if (up >= 0) { G += more; up = next; }
             }
             if (l < N) { ms[l] = m; gs[l] = G * LOG2E_D; bs[l] = beta; }
@@ -168,19 +170,16 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             ss += dppc<0x141>(ss);
             ss += dppc<0x140>(ss);
             ss = sum_xor16(ss);
-            const float f = 1.0f / fmaxf(sqrtf(ss), eps);
+            const float f = fminf(__builtin_amdgcn_rsqf(ss), ieps);   // 1 / max(|y|, eps)
             const bool live = lane_u64(m, t) != 0;
             bad |= live && !finite(ss);
-            h4 hi, lo;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float v = live ? y[e] * f : 0.f;
-                asm("" : "+v"(v));   // (rounded once: fused into the conversions, hi and lo would not belong together)
-                hi[e] = (_Float16)v;
-                lo[e] = (_Float16)(v - (float)hi[e]);
-            }
-            *(h4*)&qk[l >> 5][0][t][4 * (l & 31)] = hi;
-            *(h4*)&qk[l >> 5][1][t][4 * (l & 31)] = lo;
+            for (int e = 0; e < 4; ++e) y[e] = live ? y[e] * f : 0.f;
+            h2 h0, h1, l0, l1;
+            split2(f2{y[0], y[1]}, neg1, h0, l0);
+            split2(f2{y[2], y[3]}, neg1, h1, l1);
+            *(h4*)&qk[l >> 5][0][t][4 * (l & 31)] = h4{h0[0], h0[1], h1[0], h1[1]};
+            *(h4*)&qk[l >> 5][1][t][4 * (l & 31)] = h4{l0[0], l0[1], l1[0], l1[1]};
         }
     }
     // ---- conv + SiLU of the workgroup's V columns
@@ -207,20 +206,32 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
         for (int e = 0; e < 4; ++e) s0t[4 * (p & 3) + e][p >> 2] = sl[i][e];
     }
     __syncthreads();
+    const float one = in_register(1.0f);   // (hi + lo is then one fused instruction, not two conversions and a sum)
     // ---- products in 16x16 tasks: {K, Q} S0 of each block, then {K, Q} K^T of each pair of blocks bi >= bj
     for (int task = w; task < 2 * NB + NB * (NB + 1); task += NW) {
         const int which = (task & 1) ^ 1;   // 1 k rows, 0 q rows
         if (task < 2 * NB) {
             const int b = task >> 1;
-            f4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // (two chains: a dependent f32 op waits longer than it takes)
+            // operands first, then the products in two chains: a dependent f32 op waits longer than it takes
+            f4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            h4 hi[8], lo[8];
+            f4 av[8], sv[8];
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
-                const h4 hi = *(const h4*)&qk[which][0][16 * b + c][16 * kk + 4 * g];
-                const h4 lo = *(const h4*)&qk[which][1][16 * b + c][16 * kk + 4 * g];
-                const f4 sv = ld_f4(&s0t[c][16 * kk + 4 * g]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e & 1] = mfma4((float)hi[e] + (float)lo[e], sv[e], acc[e & 1]);
+                hi[kk] = *(const h4*)&qk[which][0][16 * b + c][16 * kk + 4 * g];
+                lo[kk] = *(const h4*)&qk[which][1][16 * b + c][16 * kk + 4 * g];
+                sv[kk] = ld_f4(&s0t[c][16 * kk + 4 * g]);
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) av[kk][e] = __builtin_fmaf((float)hi[kk][e], one, (float)lo[kk][e]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e & 1] = mfma4(av[kk][e], sv[kk][e], acc[e & 1]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = 16 * b + 4 * g + i;
@@ -234,13 +245,20 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             while (p > bi) p -= ++bi;
             const int bj = p;
             f4 acc = {0.f, 0.f, 0.f, 0.f}, small = {0.f, 0.f, 0.f, 0.f};
+            h8 ah[4], al[4], bh[4], bl[4];
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                const h8 ah = ld_h8(&qk[which][0][16 * bi + c][32 * ks + 8 * g]), al = ld_h8(&qk[which][1][16 * bi + c][32 * ks + 8 * g]);
-                const h8 bh = ld_h8(&qk[1][0][16 * bj + c][32 * ks + 8 * g]), bl = ld_h8(&qk[1][1][16 * bj + c][32 * ks + 8 * g]);
-                acc = mfma16x16x32(ah, bh, acc);
-                small = mfma16x16x32(ah, bl, small);
-                small = mfma16x16x32(al, bh, small);
+                ah[ks] = ld_h8(&qk[which][0][16 * bi + c][32 * ks + 8 * g]);
+                al[ks] = ld_h8(&qk[which][1][16 * bi + c][32 * ks + 8 * g]);
+                bh[ks] = ld_h8(&qk[1][0][16 * bj + c][32 * ks + 8 * g]);
+                bl[ks] = ld_h8(&qk[1][1][16 * bj + c][32 * ks + 8 * g]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                acc = mfma16x16x32(ah[ks], bh[ks], acc);
+                small = mfma16x16x32(ah[ks], bl[ks], small);
+                small = mfma16x16x32(al[ks], bh[ks], small);
             }
             acc += small;
             // (finite where the rows are, which the conv has looked at, and the decays, which the S0 products will)
