@@ -19,8 +19,7 @@ namespace it {
 namespace {
 constexpr int S = 128;        // state size, and channels per head
 constexpr int CW = 16;        // state columns per workgroup
-constexpr int KST = S + 4;    // LDS row of a state column (floats)
-constexpr int HST = S + 8;    // LDS row of a q or k row (halves)
+constexpr int HST = S + 8;    // LDS row of a q or k row or a state column (halves)
 constexpr int RST = CW + 4;   // LDS row of a node's CW columns
 constexpr double LOG2E_D = 1.4426950408889634074;
 
@@ -60,12 +59,12 @@ __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466
 
 // Workgroup = (V head h, CW = 16 state columns), NW waves; NB blocks of 16 nodes. A head's q and k rows are
 // convolved and normalised by each of its eight workgroups (into LDS), so no launch or barrier of the whole
-// GPU stands between the conv and the products. The normalised rows, at most 1, are kept as f16 pairs hi + lo
-// (2^-22): q K^T and K K^T take three f16 matrix ops of 16 cycles for 32 dims (hi hi, hi lo, lo hi) where f32 ones
-// would take eight of 32; the products with the state, which has no bound, are f32 on hi + lo. The waves share the
-// products out in 16x16 tasks; the inverses of I + A's diagonal blocks go one to a wave, and then each of the first
-// NB waves solves for all of U in registers (a few products more than its share, but no exchange) and writes the
-// output rows of its block.
+// GPU stands between the conv and the products. The normalised
+// rows, at most 1, and the state's columns, scaled, are kept as f16 pairs hi + lo (2^-22), and their products take three
+// f16 matrix ops of 16 cycles for 32 dims (hi hi, hi lo, lo hi) where f32 ones would take eight of 32. The waves share
+// the products out by blocks of rows; the inverses of I + A's diagonal blocks go one to a wave, and then each of the first
+// NB waves solves for all of U in registers with f32 products (a few more than its share, but no exchange) and writes
+// the output rows of its block.
 // NW: four waves for one block (three nodes: two workgroups a CU and little to share out), eight for more: with one
 // workgroup a CU they hide each other's loads.
 template <int K, int NB, int NW>
@@ -76,7 +75,9 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     float* __restrict__ out, int ots, int nt, int nv, int nk, float eps, float* __restrict__ trace) {
     constexpr int N = 16 * NB, AST = N + 4;
     __shared__ __align__(16) _Float16 qk[2][2][N][HST];   // [q, k][hi, lo] rows, zeros for padding
-    __shared__ __align__(16) float s0t[CW][KST];          // the state slice, column by column
+    __shared__ __align__(16) _Float16 sp[2][CW][HST];     // [hi, lo] the state slice, column by column, scaled
+    __shared__ __align__(16) float mxs[NW][CW];           // column maxima of the waves' rows
+    __shared__ float inv[CW];                             // what a column was divided by
     __shared__ __align__(16) float na[N][AST];            // -A
     __shared__ __align__(16) float pm[N][AST];            // (q_i . k_j) e^(G_i - G_j)
     __shared__ __align__(16) float tin[NB][16][20];       // inverses of the diagonal blocks of I + A
@@ -96,13 +97,9 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     static_assert(PER % BATCH == 0 && PER * NW == N, "every node once, none past the LDS rows");
     const int ch = (l < 32 ? kh : nk + kh) * S + 4 * (l & 31);         // lanes 0-31 four q channels each, 32-63 k
     const int chv = 2 * nk * S + h * S + cb * CW + (tid & 15);         // V channel; 16 lanes a node
-    float brv = 0.f, arv = 0.f, dtv = 0.f, av = 0.f;   // gates: a node a lane of the last wave
-    if (w == NW - 1 && l < nt) {
-        brv = br[(size_t)l * bts + h];
-        arv = ar[(size_t)l * bts + h];
-        dtv = dt[h];
-        av = A[h];
-    }
+    // gates, a node a lane (by every wave, used by the last: under a branch the loads would be waited for at its end)
+    const size_t gate = (size_t)min(l, nt - 1) * bts + h;
+    const float brv = br[gate], arv = ar[gate], dtv = dt[h], av = A[h];
     f4 own[PER], wt[K];
     float ownv[VN], wv[K];
 #pragma unroll
@@ -182,6 +179,21 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             *(h4*)&qk[l >> 5][1][t][4 * (l & 31)] = h4{l0[0], l0[1], l1[0], l1[1]};
         }
     }
+    // ---- column maxima of the slice: over the thread's pieces, the lanes of its column quad, the waves
+    {
+        f4 mx = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < SL; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fabsf(sl[i][e]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            mx[e] = fmaxf(mx[e], dppc<0x124>(mx[e]));   // row_ror:4
+            mx[e] = fmaxf(mx[e], dppc<0x128>(mx[e]));   // row_ror:8
+            mx[e] = max_xor32(max_xor16(mx[e]));
+        }
+        if (l < 4) *(f4*)&mxs[w][4 * l] = mx;
+    }
     // ---- conv + SiLU of the workgroup's V columns
     {
         float in[VN][K - 1];
@@ -199,77 +211,104 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             if (t < N) vs[t][tid & 15] = silu_hw(y);
         }
     }
+    __syncthreads();
+    // ---- the slice as f16 pairs: each column times the power of two that takes its largest value to 2^13 .. 2^14, so that
+    // the pairs hold every value to 2^-22 of itself or 2^-39 of the column's largest
+    {
+        f4 mx = ld_f4(&mxs[0][4 * (tid & 3)]);
 #pragma unroll
-    for (int i = 0; i < SL; ++i) {
-        const int p = tid + 64 * NW * i;
+        for (int i = 1; i < NW; ++i) {
+            const f4 o = ld_f4(&mxs[i][4 * (tid & 3)]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s0t[4 * (p & 3) + e][p >> 2] = sl[i][e];
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], o[e]);
+        }
+        int ex[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ex[e] = mx[e] > 0.f ? 14 - __builtin_amdgcn_frexp_expf(mx[e]) : 0;
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const int r = (tid + 64 * NW * i) >> 2;
+            f4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(sl[i][e], ex[e]);
+            h2 hi[2], lo[2];
+            split2(f2{v[0], v[1]}, neg1, hi[0], lo[0]);
+            split2(f2{v[2], v[3]}, neg1, hi[1], lo[1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sp[0][4 * (tid & 3) + e][r] = hi[e >> 1][e & 1];
+                sp[1][4 * (tid & 3) + e][r] = lo[e >> 1][e & 1];
+            }
+        }
+        if (tid < 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) inv[4 * tid + e] = __builtin_amdgcn_ldexpf(1.0f, -ex[e]);
+        }
     }
     __syncthreads();
-    const float one = in_register(1.0f);   // (hi + lo is then one fused instruction, not two conversions and a sum)
-    // ---- products in 16x16 tasks: {K, Q} S0 of each block, then {K, Q} K^T of each pair of blocks bi >= bj
-    for (int task = w; task < 2 * NB + NB * (NB + 1); task += NW) {
-        const int which = (task & 1) ^ 1;   // 1 k rows, 0 q rows
-        if (task < 2 * NB) {
-            const int b = task >> 1;
-            // operands first, then the products in two chains: a dependent f32 op waits longer than it takes
-            f4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-            h4 hi[8], lo[8];
-            f4 av[8], sv[8];
+    // ---- products: {K, Q} S0 of each block, {K, Q} K^T of each pair of blocks bi >= bj
+    // A wave takes one block of k or q rows through its products, the rows' operands read once: with the state's columns, and
+    // with the k rows of every block up to its own. Where there are waves enough, two share them: one the state's.
+    constexpr bool SHARE = NW >= 4 * NB;
+    const int combo = SHARE ? w >> 1 : w;
+    if (combo < 2 * NB) {
+        const int which = (combo & 1) ^ 1, bi = combo >> 1;   // 1 k rows, 0 q rows
+        h8 ah[4], al[4];
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-                hi[kk] = *(const h4*)&qk[which][0][16 * b + c][16 * kk + 4 * g];
-                lo[kk] = *(const h4*)&qk[which][1][16 * b + c][16 * kk + 4 * g];
-                sv[kk] = ld_f4(&s0t[c][16 * kk + 4 * g]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int ks = 0; ks < 4; ++ks) {
+            ah[ks] = ld_h8(&qk[which][0][16 * bi + c][32 * ks + 8 * g]);
+            al[ks] = ld_h8(&qk[which][1][16 * bi + c][32 * ks + 8 * g]);
+        }
+        uint64_t mt[4];
+        double gt[4];
+        float bt[4];
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) av[kk][e] = __builtin_fmaf((float)hi[kk][e], one, (float)lo[kk][e]);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e & 1] = mfma4(av[kk][e], sv[kk][e], acc[e & 1]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = 16 * b + 4 * g + i;
-                const float d = (acc[0][i] + acc[1][i]) * __builtin_amdgcn_exp2f((float)gs[t]);
-                const float v = which ? bs[t] * (vs[t][c] - d) : d;
-                (which ? rs : os)[t][c] = ms[t] ? v : 0.f;
-                bad |= ms[t] && !finite(v);
-            }
-        } else {
-            int p = (task - 2 * NB) >> 1, bi = 0;   // pair p of the lower triangle, row by row
-            while (p > bi) p -= ++bi;
-            const int bj = p;
-            f4 acc = {0.f, 0.f, 0.f, 0.f}, small = {0.f, 0.f, 0.f, 0.f};
-            h8 ah[4], al[4], bh[4], bl[4];
+        for (int i = 0; i < 4; ++i) {
+            mt[i] = ms[16 * bi + 4 * g + i];
+            gt[i] = gs[16 * bi + 4 * g + i];
+            bt[i] = which ? -bs[16 * bi + 4 * g + i] : 1.0f;
+        }
+        auto product = [&](const _Float16* bhp, const _Float16* blp) __attribute__((always_inline)) {
+            h8 bh[4], bl[4];
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                ah[ks] = ld_h8(&qk[which][0][16 * bi + c][32 * ks + 8 * g]);
-                al[ks] = ld_h8(&qk[which][1][16 * bi + c][32 * ks + 8 * g]);
-                bh[ks] = ld_h8(&qk[1][0][16 * bj + c][32 * ks + 8 * g]);
-                bl[ks] = ld_h8(&qk[1][1][16 * bj + c][32 * ks + 8 * g]);
+                bh[ks] = ld_h8(bhp + 32 * ks);
+                bl[ks] = ld_h8(blp + 32 * ks);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);   // (all operands out before the first product waits for one)
+            f4 acc = {0.f, 0.f, 0.f, 0.f}, small = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 acc = mfma16x16x32(ah[ks], bh[ks], acc);
                 small = mfma16x16x32(ah[ks], bl[ks], small);
                 small = mfma16x16x32(al[ks], bh[ks], small);
             }
-            acc += small;
-            // (finite where the rows are, which the conv has looked at, and the decays, which the S0 products will)
-            const int j = 16 * bj + c;
-            const double gj = gs[j];
+            return acc + small;
+        };
+        if (!SHARE || !(w & 1)) {
+            const f4 acc = product(&sp[0][c][8 * g], &sp[1][c][8 * g]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = 16 * bi + 4 * g + i;
-                const int seen = ((const uint16_t*)&ms[t])[bj] >> c & 1;
-                const float v = acc[i] * __builtin_amdgcn_exp2f((float)(gs[t] - gj)) * (which ? -bs[t] : 1.0f);
-                (which ? na : pm)[t][j] = seen && (!which || j != t) ? v : 0.f;
+                const float d = acc[i] * inv[c] * __builtin_amdgcn_exp2f((float)gt[i]);
+                const float v = which ? bt[i] * (d - vs[t][c]) : d;
+                (which ? rs : os)[t][c] = mt[i] ? v : 0.f;
+                bad |= mt[i] && !finite(v);
+            }
+        }
+        if (!SHARE || (w & 1)) {
+            // (finite where the rows are, which the conv has looked at, and the decays, which the state's products do)
+            for (int bj = 0; bj <= bi; ++bj) {
+                const int j = 16 * bj + c;
+                const f4 acc = product(&qk[1][0][j][8 * g], &qk[1][1][j][8 * g]);
+                const double gj = gs[j];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = 16 * bi + 4 * g + i;
+                    const bool seen = (uint32_t)(mt[i] >> (16 * bj)) >> c & 1;
+                    const float v = acc[i] * __builtin_amdgcn_exp2f((float)(gt[i] - gj)) * bt[i];
+                    (which ? na : pm)[t][j] = seen && (!which || j != t) ? v : 0.f;
+                }
             }
         }
     }
