@@ -24,7 +24,7 @@ constexpr float P_BITS = 7.0f;           // weights up to 2^15 of the reference:
 constexpr float LN2_F = 0.6931471805599453f;
 }  // namespace
 
-// The context's records for many rows (R = nt * nh / nkv rows of a KV head, more than 32): workgroup = 64 rows r = t*G + g
+// The context's records for many rows or long contexts (plan(), below): workgroup = 64 rows r = t*G + g
 // of one KV head x one key split, four waves of 32 rows x half of each 64-key tile's keys: wave w takes rows
 // 32 (w & 1) .. +31 and keys 32 (w >> 1) .. +31, with a running maximum, sum and O of its own that are joined at the
 // end. The transposed products of the flash form (S^T = K q^T, O^T += V^T P^T, 32x32x16, one query row a lane
@@ -470,18 +470,24 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     }
 }
 
-// Keys per context split.
-//   up to 32 rows a KV head: the decode partials, bound by the cache's bytes and the latency of a split: about two
-//   workgroups a CU;
-//   more: one round of the 64-row workgroups, which fill a CU each.
+// The context's form and keys per split, with R = nt * nh / nkv rows a KV head. The decode partials take up to 32 rows a
+// workgroup, one 64-key tile each while that is one round of the CUs, else the tiles of a split one after the other; their
+// time goes as the 8-row blocks of a workgroup times its tiles. The 64-row workgroups cost 4 us more at their ends,
+// share a tile among twice the rows and stream the next ones while they compute. Whole calls, partials / 64 rows,
+// us, 16/2 heads: 1 node 16384 keys 13.7 / 17.4, 65536 30.5 / 34.9, 131072 55.9 / 57.1; 2 nodes 16384 15.6 / 18.8,
+// 131072 63.9 / 57.3; 3 nodes 16384 17.9 / 20.0, 65536 38.6 / 37.7; 8 nodes (two workgroups of 32 rows a tile) 3000
+// 15.7 / 17.9, 5000 22.6 / 22.1; 64 nodes 200 16.2 / 18.5, 600 24.5 / 21.5; 24/4 heads, 5 nodes 5000 19.5 / 19.5,
+// 8128 21.1 / 20.2.
 constexpr int CUS = 256;   // MI355X compute units
-static bool row_blocks(int nt, int nh, int nkv) { return nt * (nh / nkv) > 32; }
-int attn_tree_chunk(int pos0, int nt, int nh, int nkv) {
-    const long tiles = (pos0 + 63) / 64;
-    if (!row_blocks(nt, nh, nkv)) return 64 * (int)std::max(1L, (tiles * nkv + 2 * CUS - 1) / (2 * CUS));
-    const long groups = (long)nkv * ((nt * (nh / nkv) + BM - 1) / BM), splits = std::max(1L, CUS / groups);
-    return 64 * (int)std::max(1L, (tiles + splits - 1) / splits);
+struct TreePlan { bool blocks; int chunk; };
+static TreePlan plan(int pos0, int nt, int nh, int nkv) {
+    const long tiles = (pos0 + 63) / 64, R = (long)nt * (nh / nkv);
+    const long per_cu = (tiles * nkv * ((R + 31) / 32) + CUS - 1) / CUS;   // tiles a CU, workgroups of up to 32 rows
+    if (R <= 32 ? (R + 7) / 8 * per_cu <= 8 : per_cu <= 1) return {false, 64 * (int)std::max(1L, per_cu)};
+    const long groups = nkv * ((R + BM - 1) / BM), splits = std::max(1L, CUS / groups);   // one round of workgroups
+    return {true, 64 * (int)((tiles + splits - 1) / splits)};
 }
+int attn_tree_chunk(int pos0, int nt, int nh, int nkv) { return plan(pos0, nt, nh, nkv).chunk; }
 
 hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0,
                             int nh, int nkv, int nt, const uint64_t* anc, float scale, float* out, int ots,
@@ -490,7 +496,7 @@ hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const u
     if (pos0 > 0) {
         smax = idx::split_count(pos0, chunk);
         hipError_t e;
-        if (row_blocks(nt, nh, nkv)) {
+        if (plan(pos0, nt, nh, nkv).blocks) {
             const int nrb = (nt * (nh / nkv) + BM - 1) / BM;
             const unsigned grid = (unsigned)((smax * nkv + 7) / 8 * 8 * nrb);
             attn_tree_ctx_kernel<<<grid, 256, 0, st>>>(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, smax, nrb);
@@ -500,8 +506,10 @@ hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const u
         }
         if (e != hipSuccess) return e;
     }
-    // few rows: a quarter of the dims a workgroup, 16 split lanes; many: the whole row, 4 split lanes
-    if (nt * nh < 512)
+    // A quarter of the dims and 16 split lanes a workgroup where a few rows have many records (1 node, 16/2 heads, 8128 keys
+    // in 127 splits: 10.5 us the call against 14.2), else whole rows and 4 split lanes (26 nodes at 600 keys 14.2 against
+    // 19.0, from the path's keys that every workgroup of a row scores).
+    if (smax > 32 && nt * nh <= 192)
         attn_tree_merge_kernel<16><<<dim3(4, nh, nt), 256, 0, st>>>(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, anc, scale,
                                                                   part, smax, out, ots);
     else

@@ -47,6 +47,7 @@ __device__ __forceinline__ void taps(uint64_t m, const float* x, int xts, const 
 }
 typedef __attribute__((address_space(1))) const float gfloat;
 typedef __attribute__((address_space(1))) const f4 gf4;
+typedef __attribute__((address_space(1))) const char gchar;
 __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
            (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32;
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
 #pragma unroll
         for (int i = 0; i < BATCH; ++i)
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j) in[i][j] = *(gf4*)((gfloat*)lane_u64(row[j], w + NW * (i0 + i)) + ch);
+            for (int j = 0; j < K - 1; ++j) in[i][j] = *(gf4*)((gchar*)lane_u64(row[j], w + NW * (i0 + i)) + 4u * (unsigned)ch);
         if (i0 == 0 && w == NW - 1) {
             // gates and path sums, a node a lane of the last wave, while its loads are out
             double G = 0.0;
