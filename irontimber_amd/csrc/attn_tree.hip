@@ -375,7 +375,7 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     const int dq = blockIdx.x, h = blockIdx.y, t = blockIdx.z, tid = threadIdx.x, w = tid >> 6, l = tid & 63;
     const int sg = tid / DLN, dl = tid % DLN, d0 = DW * dq + 4 * dl;
     float* dst = out + (size_t)t * ots + (size_t)h * HD + d0;
-    // What does not hang on the mask goes out first: the first batch of the context's records, q and the gate. Slots
+    // What does not hang on the mask goes out first: the first batch of the context's records, q and the gate. Lanes
     // past the last record reload it and count nothing.
     const float* base = part + idx::rec(t * nh + h, 0, smax) * PART;
     f2 hv[SPL];
@@ -383,12 +383,16 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     auto load = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < SPL; ++j) {
-            const float* rec = base + (size_t)min(s0 + sg + SL * j, smax - 1) * PART;
-            hv[j] = *(const f2*)rec;
-            ov[j] = ld_f4(rec + 4 + d0);
+            hv[j] = f2{-INFINITY, 0.f};
+            ov[j] = f4{0.f, 0.f, 0.f, 0.f};
+            if (s0 + SL * j < smax) {   // (the same for every lane)
+                const float* rec = base + (size_t)min(s0 + sg + SL * j, smax - 1) * PART;
+                hv[j] = *(const f2*)rec;
+                ov[j] = ld_f4(rec + 4 + d0);
+            }
         }
     };
-    if (smax > 0) load(0);
+    load(0);
     const float* qrow = q + (size_t)t * qts + (size_t)h * 2 * HD;
     const f4 qv = ld_f4(qrow + 4 * l), gt = ld_f4(qrow + HD + d0);
     const uint64_t mask = anc[t] & (~(uint64_t)0 >> (64 - nt));
@@ -417,9 +421,18 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
             if (l == 0 && j0 + 4 * j < np) score[j0 + 4 * j] = s * scale;
         }
     }
+    auto batch_max = [&]() {
+        float m = hv[0][0];
+#pragma unroll
+        for (int j = 1; j < SPL; ++j) m = fmaxf(m, hv[j][0]);
+        return m;
+    };
+    if (dl == 0) red_m[sg] = batch_max();
     __syncthreads();
-    // ---- the path's own softmax (no reference below the type's range, so that keys of score -inf weigh 0)
+    // ---- the path and the first batch of records (no reference below the type's range, so that keys of score -inf weigh 0)
     float M = wave_max(l < np ? score[l] : -FLT_MAX);
+#pragma unroll
+    for (int j = 0; j < SL; ++j) M = fmaxf(M, red_m[j]);
     float den = 0.f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -431,30 +444,31 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
             for (int i = 0; i < 4; ++i) o[i] += e * (float)pv[j][i];
         }
     }
-    // ---- the context's records
-    for (int s0 = 0; s0 < smax; s0 += SL * SPL) {
-        if (s0) load(s0);
-        float mloc = M;
-#pragma unroll
-        for (int j = 0; j < SPL; ++j) mloc = fmaxf(mloc, hv[j][0]);
-        if (dl == 0) red_m[sg] = mloc;
-        __syncthreads();
-        float Mn = red_m[0];
-#pragma unroll
-        for (int j = 1; j < SL; ++j) Mn = fmaxf(Mn, red_m[j]);
-        __syncthreads();
-        const float r = __expf(M - Mn);
-        den *= r;
-        o *= r;
+    auto add_batch = [&](int s0) {
 #pragma unroll
         for (int j = 0; j < SPL; ++j) {
             if (s0 + sg + SL * j < smax) {
-                const float wgt = __expf(hv[j][0] - Mn);
+                const float wgt = __expf(hv[j][0] - M);
                 den += hv[j][1] * wgt;
                 o += ov[j] * wgt;
             }
         }
+    };
+    add_batch(0);
+    // ---- the other records
+    for (int s0 = SL * SPL; s0 < smax; s0 += SL * SPL) {
+        load(s0);
+        __syncthreads();   // every lane has read the last batch's maxima
+        if (dl == 0) red_m[sg] = batch_max();
+        __syncthreads();
+        float Mn = M;
+#pragma unroll
+        for (int j = 0; j < SL; ++j) Mn = fmaxf(Mn, red_m[j]);
+        const float r = __expf(M - Mn);
+        den *= r;
+        o *= r;
         M = Mn;
+        add_batch(s0);
     }
     red_o[sg][dl] = o;
     if (dl == 0) red_d[sg] = den;
