@@ -472,16 +472,25 @@ int it_gdn_prefill(const float* x, int x_tok_stride, const float* conv_w, int K,
  * parent is not in -1 .. t-1 is padding, and so are its descendants (anc 0, pos p0). */
 int it_tree_plan(const int32_t* parent, int nt, int p0, uint64_t* anc, int32_t* pos, void* stream);
 
-/* it_attn_f16 for the nodes of a tree: node t's query row sees cache rows 0 .. pos0-1 and the rows pos0 + j of the
- * nodes j whose bit is set in anc[t] (any of the nt bits; higher ones are ignored). Rows that a node does not see are
- * not read for it, whatever they hold. A padding node's output row is zeros. pos0 may be 0. Other arguments and the
- * result as for it_attn_f16 (f32 accumulation, q and the probabilities carried as f16 pairs: about 2e-6 relative).
+/* it_attn_f16 for nodes of a tree: query row t sees cache rows 0 .. pos0-1 and the rows pos0 + j of the nodes j < rows whose
+ * bit is set in anc[t] (higher bits are ignored). Verification asks for all nodes at once, nt = rows; drafting level by
+ * level asks for the newest ones, with anc pointing at their masks and rows counting all nodes so far. Rows that a node
+ * does not see are not read for it, whatever they hold. A row without any bit is zeros. pos0 may be 0. Other arguments
+ * and the result as for it_attn_f16 (f32 accumulation, q and the probabilities carried as f16 pairs: about 2e-6
+ * relative). rows in 1 .. IT_TREE_MAX; nt as well.
  * scratch: the context's records; it_attn_tree_scratch_bytes(...) bytes give the library's split, with fewer the
- * splits get longer, and nt * nh * 1040 bytes are always enough (0 for pos0 = 0). */
+ * splits get longer, and nt * nh * 1040 bytes are always enough (0 for pos0 = 0). Calls that overlap need one each. */
 size_t it_attn_tree_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv);
 int it_attn_tree_f16(const float* q, int q_tok_stride, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0, int hd,
-                     int nh, int nkv, int nt, const uint64_t* anc, float scale, float* out, int out_tok_stride,
+                     int nh, int nkv, int nt, int rows, const uint64_t* anc, float scale, float* out, int out_tok_stride,
                      void* scratch, size_t scratch_bytes, void* stream);
+
+/* The same over the MTP head's f32 cache (at most 16 q heads per KV head), f32 throughout: for drafting a tree with the
+ * head. Stands where it_attn_f32kv does for a chain. */
+size_t it_attn_tree_f32kv_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv);
+int it_attn_tree_f32kv(const float* q, int q_tok_stride, const float* kc, const float* vc, int kvd, int pos0, int hd,
+                       int nh, int nkv, int nt, int rows, const uint64_t* anc, float scale, float* out, int out_tok_stride,
+                       void* scratch, size_t scratch_bytes, void* stream);
 
 /* Keeps the path of node `leaf` in a cache whose rows pos0 + t hold the nodes: row pos0 + i <- row pos0 + path[i], path
  * the nodes of anc[leaf] in order (in place; the rows after the path keep what they hold). leaf = -1, or a padding

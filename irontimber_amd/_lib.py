@@ -79,8 +79,11 @@ SIGNATURES = {
     "it_rope_freqs": (c_int, [c_int, c_float, c_int, c_float, c_int, P, P]),
     "it_tree_plan": (c_int, [P, c_int, c_int, P, P, P]),
     "it_attn_tree_scratch_bytes": (c_size_t, [c_int] * 5),
-    "it_attn_tree_f16": (c_int, [P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, P, c_float, P, c_int, P,
+    "it_attn_tree_f16": (c_int, [P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, c_float, P, c_int, P,
                                  c_size_t, P]),
+    "it_attn_tree_f32kv_scratch_bytes": (c_size_t, [c_int] * 5),
+    "it_attn_tree_f32kv": (c_int, [P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, c_float, P, c_int,
+                                   P, c_size_t, P]),
     "it_gdn_tree_trace_bytes": (c_size_t, [c_int] * 4),
     "it_gdn_tree": (c_int, [P, c_int, P, c_int, P, P, P, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_float,
                             P, c_size_t, P]),

@@ -133,14 +133,11 @@ struct F32kvPlan { int chunk; size_t bytes; };
 // of 4 tiles); 320 / 384 / 512 keys gave 81 / 91 / 114 us (2 rounds of 5 / 6 / 8 tiles), all with four waves
 // a workgroup; with eight, 576 keys (one round of 9 tiles) take 59.6 against 68.5 us.
 constexpr int F32KV_CUS = 256;   // MI355X compute units
-int f32kv_pref_chunk(int pos0, int nt, int nh, int nkv) {
-    const int G = nh / nkv;
-    if ((long)nt * G <= 32) return auto_chunk(pos0, nt, nh, nkv, false);
-    const long total = (long)pos0 + nt;
-    const long blocks = ((long)nt * G + 31) / 32;   // 32-row blocks of the multi-block kernel
+int f32kv_rounds_chunk(long total, int nt, int nh, int nkv) {   // over `total` keys
+    const long blocks = ((long)nt * (nh / nkv) + 31) / 32;   // 32-row blocks of the multi-block kernel
     int best = 64;
     long best_cost = -1;
-    for (long c = 64;; c += 64) {
+    for (long c = 64; best_cost < 0 || c / 64 + 1 <= best_cost; c += 64) {   // (one round of longer splits costs more)
         const long wgs = (total + c - 1) / c * nkv * blocks;
         const long cost = (wgs + F32KV_CUS - 1) / F32KV_CUS * (c / 64 + 1);
         if (best_cost < 0 || cost <= best_cost) {
@@ -150,6 +147,10 @@ int f32kv_pref_chunk(int pos0, int nt, int nh, int nkv) {
         if (c >= total) break;
     }
     return best;
+}
+int f32kv_pref_chunk(int pos0, int nt, int nh, int nkv) {
+    if ((long)nt * (nh / nkv) <= 32) return auto_chunk(pos0, nt, nh, nkv, false);
+    return f32kv_rounds_chunk((long)pos0 + nt, nt, nh, nkv);
 }
 F32kvPlan plan_f32kv(int pos0, int nt, int nh, int nkv, size_t budget) {
     const long total = (long)pos0 + nt;
@@ -414,32 +415,72 @@ int it_tree_plan(const int32_t* parent, int nt, int p0, uint64_t* anc, int32_t* 
 static size_t tree_scratch(int pos0, int nt, int nh, int chunk) {
     return (size_t)nt * nh * it::idx::split_count(pos0, chunk) * PART_WORDS * sizeof(float);
 }
-// Keys per split whose records fit `budget` bytes: the preferred split, else doubled (the rule of the fixed
-// arena, src/vk/mod.rs:714-716). 0: even one record per (node, head) is too much.
-static int plan_attn_tree(int pos0, int nt, int nh, int nkv, size_t budget) {
-    int c = it::attn_tree_chunk(pos0, nt, nh, nkv);
+// Keys per split of a tree call: the preferred split `c` where its records fit `budget` bytes, else doubled (the rule of
+// the fixed arena, src/vk/mod.rs:714-716). 0: even one record per (node, head) is too much.
+static int fit_tree(int pos0, int nt, int nh, int c, size_t budget) {
     while (tree_scratch(pos0, nt, nh, c) > budget && c < pos0) c *= 2;
     return tree_scratch(pos0, nt, nh, c) <= budget ? c : 0;
 }
+static int tree_pref_chunk(bool f32kv, int pos0, int nt, int nh, int nkv) {
+    return f32kv ? f32kv_rounds_chunk(pos0, nt, nh, nkv) : it::attn_tree_chunk(pos0, nt, nh, nkv);
+}
+static size_t tree_scratch_bytes(bool f32kv, int pos0, int nt, int nh, int nkv) {
+    if (nt < 1 || nt > IT_TREE_MAX || pos0 < 0 || nh <= 0 || nkv <= 0 || nh % nkv) return 0;
+    return tree_scratch(pos0, nt, nh, tree_pref_chunk(f32kv, pos0, nt, nh, nkv));
+}
 size_t it_attn_tree_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv) {
     (void)hd;
-    if (nt < 1 || nt > IT_TREE_MAX || pos0 < 0 || nh <= 0 || nkv <= 0 || nh % nkv) return 0;
-    return tree_scratch(pos0, nt, nh, it::attn_tree_chunk(pos0, nt, nh, nkv));
+    return tree_scratch_bytes(false, pos0, nt, nh, nkv);
+}
+size_t it_attn_tree_f32kv_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv) {
+    (void)hd;
+    return tree_scratch_bytes(true, pos0, nt, nh, nkv);
+}
+// The checks of both tree attentions; on success *chunk holds the keys per split.
+static int validate_attn_tree(const char* who, const float* q, int qts, const void* kc, const void* vc, bool f32kv, int kvd,
+                              int pos0, int hd, int nh, int nkv, int nt, int nr, const uint64_t* anc, const float* out,
+                              int ots, const void* scratch, size_t scratch_bytes, int* chunk) {
+    if (hd != HD) return fail("%s: head_dim %d unsupported (256)", who, hd);
+    if (nt < 1 || nt > IT_TREE_MAX) return fail("%s: nt %d must be in [1, %d]", who, nt, IT_TREE_MAX);
+    if (nr < 1 || nr > IT_TREE_MAX) return fail("%s: rows %d must be in [1, %d]", who, nr, IT_TREE_MAX);
+    if (nh <= 0 || nkv <= 0 || nh % nkv != 0) return fail("%s: n_head %d / n_head_kv %d invalid", who, nh, nkv);
+    if (f32kv && nh / nkv > 16) return fail("%s: at most 16 q heads per KV head, not %d", who, nh / nkv);
+    if (kvd != nkv * hd) return fail("%s: kvd %d != n_head_kv*head_dim %d", who, kvd, nkv * hd);
+    if (pos0 < 0 || (long)pos0 + nr > (1L << 22)) return fail("%s: pos0 %d / rows %d invalid", who, pos0, nr);
+    if (!q || !kc || !vc || !anc || !out) return fail("%s: null buffer", who);
+    if (!aligned16(q) || !aligned16(kc) || !aligned16(vc) || !aligned16(out) || (scratch && !aligned16(scratch)))
+        return fail("%s: q/kc/vc/out/scratch must be 16-byte aligned", who);
+    if (qts % 4 != 0 || ots % 4 != 0) return fail("%s: token strides must be multiples of 4", who);
+    if (nt > 1 && (qts < 2 * nh * hd || ots < nh * hd)) return fail("%s: token strides overlap rows", who);
+    const size_t budget = scratch ? scratch_bytes : 0;
+    *chunk = fit_tree(pos0, nt, nh, tree_pref_chunk(f32kv, pos0, nt, nh, nkv), budget);
+    if (!*chunk)
+        return fail("%s: scratch of %zu bytes cannot hold even one partial record per (node, head) (%zu bytes)", who, budget,
+                    tree_scratch(pos0, nt, nh, pos0));
+    return 0;
 }
 int it_attn_tree_f16(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0, int hd, int nh,
-                     int nkv, int nt, const uint64_t* anc, float scale, float* out, int ots, void* scratch,
+                     int nkv, int nt, int rows, const uint64_t* anc, float scale, float* out, int ots, void* scratch,
                      size_t scratch_bytes, void* stream) {
     const char* who = "it_attn_tree_f16";
-    if (nt < 1 || nt > IT_TREE_MAX) return fail("%s: nt %d must be in [1, %d]", who, nt, IT_TREE_MAX);
-    if (validate_attn(q, qts, kc, vc, kvd, pos0, hd, nh, nkv, nt, out, ots)) return -1;
-    if (!anc) return fail("%s: null anc", who);
-    if (scratch && !aligned16(scratch)) return fail("%s: scratch must be 16-byte aligned", who);
-    const int chunk = plan_attn_tree(pos0, nt, nh, nkv, scratch ? scratch_bytes : 0);
-    if (!chunk)
-        return fail("%s: scratch of %zu bytes cannot hold even one partial record per (node, head) (%zu bytes)", who,
-                    scratch ? scratch_bytes : 0, tree_scratch(pos0, nt, nh, pos0));
-    return check(it::launch_attn_tree(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, anc, scale, out, ots, (float*)scratch, chunk,
-                                      (hipStream_t)stream),
+    int chunk = 0;
+    if (validate_attn_tree(who, q, qts, kc, vc, false, kvd, pos0, hd, nh, nkv, nt, rows, anc, out, ots, scratch, scratch_bytes,
+                           &chunk))
+        return -1;
+    return check(it::launch_attn_tree(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, rows, anc, scale, out, ots, (float*)scratch,
+                                      chunk, (hipStream_t)stream),
+                 who);
+}
+int it_attn_tree_f32kv(const float* q, int qts, const float* kc, const float* vc, int kvd, int pos0, int hd, int nh,
+                       int nkv, int nt, int rows, const uint64_t* anc, float scale, float* out, int ots, void* scratch,
+                       size_t scratch_bytes, void* stream) {
+    const char* who = "it_attn_tree_f32kv";
+    int chunk = 0;
+    if (validate_attn_tree(who, q, qts, kc, vc, true, kvd, pos0, hd, nh, nkv, nt, rows, anc, out, ots, scratch, scratch_bytes,
+                           &chunk))
+        return -1;
+    return check(it::launch_attn_tree_f32kv(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, rows, anc, scale, out, ots,
+                                            (float*)scratch, chunk, (hipStream_t)stream),
                  who);
 }
 

@@ -62,7 +62,8 @@ constexpr int F32KV_ROW = F32KV_HD + 4;                 // padded LDS row (float
 // src/vk/mod.rs:740).
 // CR: the same values in the piece layout of common.h (decode and short verify calls whose merge is
 // the wave merge).
-template <int RB, bool DIRECT, bool CR = false>
+// ALL: every row sees all of the pos0 keys and no others (a drafted tree's nodes and their context).
+template <int RB, bool DIRECT, bool CR = false, bool ALL = false>
 __global__ __launch_bounds__(256 * RB) void attn_f32kv_kernel(const float* __restrict__ q, int qts,
                                                          const float* __restrict__ kc, const float* __restrict__ vc,
                                                          int kvd, int pos0, int nh, int nkv, int nt, int tpw,
@@ -82,9 +83,9 @@ __global__ __launch_bounds__(256 * RB) void attn_f32kv_kernel(const float* __res
     const int ntg = min(tpw, nt - t0);
     const int rows = ntg * G;
     const int kb0 = s * chunk;
-    const int kend = min(kb0 + chunk, pos0 + t0 + ntg);   // keys the group's last token sees
+    const int kend = min(kb0 + chunk, ALL ? pos0 : pos0 + t0 + ntg);   // keys the group's last token sees
     if (kb0 >= kend) return;   // whole workgroup: no token of the group sees this split
-    const int total = pos0 + nt;
+    const int total = ALL ? pos0 : pos0 + nt;
     const float* Kw = Ks + 16 * w * F32KV_ROW;            // the key group's 16 K rows
 
     // The wave's share of tile kt: rows 16w + SR * rb + i, lane l bringing dims 4l .. 4l+3. K rows
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(256 * RB) void attn_f32kv_kernel(const float* __res
     const int r = 16 * rb + lr;          // this lane's query row in the workgroup
     const bool rv = r < rows;
     const int tq = t0 + (rv ? r / G : 0), hq = kh * G + (rv ? r % G : 0);
-    const int nvis = pos0 + tq + 1;      // keys visible to this row
+    const int nvis = ALL ? pos0 : pos0 + tq + 1;   // keys visible to this row
     f4 qv[16];
     {
         const float* qp = q + (size_t)tq * qts + (size_t)hq * 2 * F32KV_HD + 4 * lg;
@@ -257,6 +258,23 @@ hipError_t launch_attn_f32kv(const float* q, int qts, const float* kc, const flo
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || direct) return e;
     return launch_attn_combine(q, qts, part, pos0, nh, nt, chunk, out, ots, st, pieces);
+}
+
+// 260-word records of all nt tokens over keys 0 .. n-1, in splits of `chunk` keys (n > 0).
+hipError_t launch_attn_f32kv_all_partials(const float* q, int qts, const float* kc, const float* vc, int kvd, int n,
+                                          int nh, int nkv, int nt, float scale, float* part, int chunk,
+                                          hipStream_t st) {
+    const int G = nh / nkv, smax = idx::split_count(n, chunk);
+    const float qs = scale * 1.44269504088896340736f;
+    const int rb = nt * G > 16 ? 2 : 1, tpw = 16 * rb / G;
+    const dim3 grid((unsigned)smax, (unsigned)nkv, (unsigned)((nt + tpw - 1) / tpw));
+    if (rb == 2)
+        attn_f32kv_kernel<2, false, false, true><<<grid, 512, 0, st>>>(q, qts, kc, vc, kvd, n, nh, nkv, nt, tpw, qs, part,
+                                                                       chunk, smax, nullptr, 0);
+    else
+        attn_f32kv_kernel<1, false, false, true><<<grid, 256, 0, st>>>(q, qts, kc, vc, kvd, n, nh, nkv, nt, tpw, qs, part,
+                                                                       chunk, smax, nullptr, 0);
+    return hipGetLastError();
 }
 
 }  // namespace it

@@ -356,16 +356,22 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     }
 }
 
-// One workgroup per (256 / SL * 4 dims, head, node). Thread = (split lane sg of SL, dim lane of 256 / SL, 4
+// Four cache values
+template <class KVT> struct Kv4 { typedef h4 T; };
+template <> struct Kv4<float> { typedef f4 T; };
+
+// One workgroup per (256 / SL * 4 dims, head, node); nr: the tree's rows in the cache. Thread = (split lane sg of SL, dim lane of 256 / SL, 4
 // dims each): split lane sg takes the context's records sg, sg + SL, ... and the path's keys likewise.
-template <int SL>
+// KVT: the cache's values, uint16_t (f16) or float.
+template <int SL, class KVT>
 __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __restrict__ q, int qts,
-                                                              const uint16_t* __restrict__ kc,
-                                                              const uint16_t* __restrict__ vc, int kvd, int pos0,
-                                                              int nh, int nkv, int nt,
+                                                              const KVT* __restrict__ kc,
+                                                              const KVT* __restrict__ vc, int kvd, int pos0,
+                                                              int nh, int nkv, int nr,
                                                               const uint64_t* __restrict__ anc, float scale,
                                                               const float* __restrict__ part, int smax,
                                                               float* __restrict__ out, int ots) {
+    typedef typename Kv4<KVT>::T V4;
     constexpr int DLN = 256 / SL, DW = 4 * DLN;   // dim lanes, dims per workgroup
     constexpr int NK = 64 / SL;                   // path keys per split lane
     __shared__ int node[64];                      // the path's nodes in order
@@ -395,7 +401,7 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     load(0);
     const float* qrow = q + (size_t)t * qts + (size_t)h * 2 * HD;
     const f4 qv = ld_f4(qrow + 4 * l), gt = ld_f4(qrow + HD + d0);
-    const uint64_t mask = anc[t] & (~(uint64_t)0 >> (64 - nt));
+    const uint64_t mask = anc[t] & (~(uint64_t)0 >> (64 - nr));
     const int np = (int)__popcll(mask);
     if (np == 0) {   // a padding node
         if (sg == 0) *(f4*)dst = f4{0.f, 0.f, 0.f, 0.f};
@@ -405,15 +411,15 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     __syncthreads();
     // ---- the path: this lane's V pieces go out first, then the scores, a key a wave
     const size_t head = (size_t)(h / (nh / nkv)) * HD;
-    h4 pv[NK];
+    V4 pv[NK];
 #pragma unroll
     for (int j = 0; j < NK; ++j)
-        if (SL * j < np) pv[j] = *(const h4*)(vc + (size_t)(pos0 + node[min(sg + SL * j, np - 1)]) * kvd + head + d0);
+        if (SL * j < np) pv[j] = *(const V4*)(vc + (size_t)(pos0 + node[min(sg + SL * j, np - 1)]) * kvd + head + d0);
     for (int j0 = w; j0 < np; j0 += 16) {
-        h4 kv[4];
+        V4 kv[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            kv[j] = *(const h4*)(kc + (size_t)(pos0 + node[min(j0 + 4 * j, np - 1)]) * kvd + head + 4 * l);
+            kv[j] = *(const V4*)(kc + (size_t)(pos0 + node[min(j0 + 4 * j, np - 1)]) * kvd + head + 4 * l);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float s = wave_sum((qv[0] * (float)kv[j][0] + qv[1] * (float)kv[j][1]) +
@@ -503,8 +509,24 @@ static TreePlan plan(int pos0, int nt, int nh, int nkv) {
 }
 int attn_tree_chunk(int pos0, int nt, int nh, int nkv) { return plan(pos0, nt, nh, nkv).chunk; }
 
+template <class KVT>
+static hipError_t launch_merge(const float* q, int qts, const KVT* kc, const KVT* vc, int kvd, int pos0, int nh, int nkv,
+                               int nt, int nr, const uint64_t* anc, float scale, float* out, int ots, const float* part,
+                               int smax, hipStream_t st) {
+    // A quarter of the dims and 16 split lanes a workgroup where a few rows have many records (1 node, 16/2 heads, 8128 keys
+    // in 127 splits: 10.5 us the call against 14.2), else whole rows and 4 split lanes (26 nodes at 600 keys 14.2 against
+    // 19.0, from the path's keys that every workgroup of a row scores).
+    if (smax > 32 && nt * nh <= 192)
+        attn_tree_merge_kernel<16, KVT><<<dim3(4, nh, nt), 256, 0, st>>>(q, qts, kc, vc, kvd, pos0, nh, nkv, nr, anc, scale,
+                                                                       part, smax, out, ots);
+    else
+        attn_tree_merge_kernel<4, KVT><<<dim3(1, nh, nt), 256, 0, st>>>(q, qts, kc, vc, kvd, pos0, nh, nkv, nr, anc, scale,
+                                                                      part, smax, out, ots);
+    return hipGetLastError();
+}
+
 hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0,
-                            int nh, int nkv, int nt, const uint64_t* anc, float scale, float* out, int ots,
+                            int nh, int nkv, int nt, int nr, const uint64_t* anc, float scale, float* out, int ots,
                             float* part, int chunk, hipStream_t st) {
     int smax = 0;
     if (pos0 > 0) {
@@ -520,16 +542,20 @@ hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const u
         }
         if (e != hipSuccess) return e;
     }
-    // A quarter of the dims and 16 split lanes a workgroup where a few rows have many records (1 node, 16/2 heads, 8128 keys
-    // in 127 splits: 10.5 us the call against 14.2), else whole rows and 4 split lanes (26 nodes at 600 keys 14.2 against
-    // 19.0, from the path's keys that every workgroup of a row scores).
-    if (smax > 32 && nt * nh <= 192)
-        attn_tree_merge_kernel<16><<<dim3(4, nh, nt), 256, 0, st>>>(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, anc, scale,
-                                                                  part, smax, out, ots);
-    else
-        attn_tree_merge_kernel<4><<<dim3(1, nh, nt), 256, 0, st>>>(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, anc, scale,
-                                                                 part, smax, out, ots);
-    return hipGetLastError();
+    return launch_merge(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, nr, anc, scale, out, ots, part, smax, st);
+}
+
+hipError_t launch_attn_tree_f32kv(const float* q, int qts, const float* kc, const float* vc, int kvd, int pos0,
+                                  int nh, int nkv, int nt, int nr, const uint64_t* anc, float scale, float* out, int ots,
+                                  float* part, int chunk, hipStream_t st) {
+    int smax = 0;
+    if (pos0 > 0) {
+        smax = idx::split_count(pos0, chunk);
+        const hipError_t e =
+            launch_attn_f32kv_all_partials(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, st);
+        if (e != hipSuccess) return e;
+    }
+    return launch_merge(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, nr, anc, scale, out, ots, part, smax, st);
 }
 
 }  // namespace it

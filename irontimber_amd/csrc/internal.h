@@ -114,9 +114,16 @@ hipError_t launch_kv_tree_commit(void* kc, void* vc, size_t row_bytes, int pos0,
 hipError_t launch_attn_all_partials(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int n,
                                     int nh, int nkv, int nt, float scale, float* part, int chunk, hipStream_t st);
 int attn_tree_chunk(int pos0, int nt, int nh, int nkv);
+hipError_t launch_attn_f32kv_all_partials(const float* q, int qts, const float* kc, const float* vc, int kvd, int n,
+                                          int nh, int nkv, int nt, float scale, float* part, int chunk,
+                                          hipStream_t st);
+// nr: the tree's rows in the cache, which the masks' bits stand for
 hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int pos0,
-                            int nh, int nkv, int nt, const uint64_t* anc, float scale, float* out, int ots,
+                            int nh, int nkv, int nt, int nr, const uint64_t* anc, float scale, float* out, int ots,
                             float* part, int chunk, hipStream_t st);
+hipError_t launch_attn_tree_f32kv(const float* q, int qts, const float* kc, const float* vc, int kvd, int pos0,
+                                  int nh, int nkv, int nt, int nr, const uint64_t* anc, float scale, float* out, int ots,
+                                  float* part, int chunk, hipStream_t st);
 // trace: U [nt][nv*S], k [nt][nk*S] (f32), G [nt][nv] (f64), written by launch_gdn_tree, read by the commit
 size_t gdn_tree_trace_bytes(int nt, int nv, int nk);
 hipError_t launch_gdn_tree(const float* x, int xts, const float* cw, int K, const float* cst, const float* br,

@@ -555,34 +555,54 @@ def attn_tree_scratch_bytes(pos0: int, nt: int, nh: int, nkv: int, hd: int = 256
     return lib().it_attn_tree_scratch_bytes(pos0, nt, hd, nh, nkv)
 
 
-def attn_tree_f16(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, pos0: int, nh: int, nkv: int, anc: torch.Tensor,
-                  scale: float | None = None, out: torch.Tensor | None = None,
-                  scratch: torch.Tensor | None = None) -> torch.Tensor:
-    """attn_f16 for the nodes of a drafted tree: q [nt, nh*2*hd] f32, nodes in cache rows pos0 + t, anc [nt] int64
-    (tree_plan) -> out [nt, nh*hd] f32; zeros for padding nodes (it_attn_tree_f16)."""
+def attn_tree_f32kv_scratch_bytes(pos0: int, nt: int, nh: int, nkv: int, hd: int = 256) -> int:
+    return lib().it_attn_tree_f32kv_scratch_bytes(pos0, nt, hd, nh, nkv)
+
+
+def _attn_tree(name, kinds, scratch_bytes, q, kc, vc, pos0, nh, nkv, anc, scale, out, scratch, rows):
     dev = q.get_device()
     if q.dim() != 2 or q.shape[1] % (2 * nh) != 0:
         raise ValueError("q must be [nt, nh*2*hd]")
     nt, hd = q.shape[0], q.shape[1] // (2 * nh)
     kvd = nkv * hd
+    if rows is None:
+        rows = nt
     if out is None:
         out = torch.empty(nt, nh * hd, device=q.device, dtype=torch.float32)
     _need_all(torch.float32, dev, (q, out), "q out")
     if out.shape != (nt, nh * hd):
         raise ValueError("out must be [nt, nh*hd]")
-    _need_caches(_F16, dev, kvd, pos0 + nt, kc, vc)
+    _need_caches(kinds, dev, kvd, pos0 + rows, kc, vc)
     _need_anc(anc, dev, nt)
     if scale is None:
         scale = 1.0 / hd ** 0.5
     if scratch is None:
-        need = attn_tree_scratch_bytes(pos0, nt, nh, nkv, hd)
+        need = scratch_bytes(pos0, nt, nh, nkv, hd)
         scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
     elif scratch.get_device() != dev or not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous, on the same device as the other tensors")
     nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    _call_on(dev, "it_attn_tree_f16", q.data_ptr(), nh * 2 * hd, kc.data_ptr(), vc.data_ptr(), kvd, pos0, hd, nh, nkv, nt,
+    _call_on(dev, name, q.data_ptr(), nh * 2 * hd, kc.data_ptr(), vc.data_ptr(), kvd, pos0, hd, nh, nkv, nt, rows,
              anc.data_ptr(), scale, out.data_ptr(), nh * hd, _ptr(scratch), nbytes)
     return out
+
+
+def attn_tree_f16(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, pos0: int, nh: int, nkv: int, anc: torch.Tensor,
+                  scale: float | None = None, out: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
+                  rows: int | None = None) -> torch.Tensor:
+    """attn_f16 for nodes of a drafted tree: q [nt, nh*2*hd] f32, the tree's `rows` nodes (None: nt, all of them) in cache
+    rows pos0 + j, anc [nt] int64 (tree_plan) the nodes that each query sees -> out [nt, nh*hd] f32; zeros for padding
+    nodes (it_attn_tree_f16)."""
+    return _attn_tree("it_attn_tree_f16", _F16, attn_tree_scratch_bytes, q, kc, vc, pos0, nh, nkv, anc, scale, out, scratch,
+                      rows)
+
+
+def attn_tree_f32kv(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, pos0: int, nh: int, nkv: int, anc: torch.Tensor,
+                    scale: float | None = None, out: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
+                    rows: int | None = None) -> torch.Tensor:
+    """attn_tree_f16 over the MTP head's f32 cache (it_attn_tree_f32kv)."""
+    return _attn_tree("it_attn_tree_f32kv", _F32, attn_tree_f32kv_scratch_bytes, q, kc, vc, pos0, nh, nkv, anc, scale, out,
+                      scratch, rows)
 
 
 def _kv_tree_commit(name, kinds, kc, vc, pos0, nt, anc, leaf):

@@ -144,10 +144,51 @@ def test_strides_and_streams(dev):
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     _lib.call("it_attn_tree_f16", args[0].data_ptr(), qts, args[1].data_ptr(), args[2].data_ptr(), 512, pos0, 256, nh, nkv,
-              nt, args[3].data_ptr(), 1 / 16, out.data_ptr(), ots, scr.data_ptr(), scr.numel(), s.cuda_stream)
+              nt, nt, args[3].data_ptr(), 1 / 16, out.data_ptr(), ots, scr.data_ptr(), scr.numel(), s.cuda_stream)
     got = host(out)
     assert (got[:, nh * 256:] == 7.0).all()
     assert (np.abs(got[:, :nh * 256].reshape(nt, nh, 256) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+def test_levels_of_a_draft(dev, kv):
+    """The nodes of each depth asked for on their own, with the rows drafted so far, get what all nodes at once get."""
+    nt, pos0, nh, nkv = 20, 90, 16, 2
+    q, k, v = inputs(19, nt, pos0, nh, nkv)
+    if kv == "f32":
+        k, v = k.astype(np.float32), v.astype(np.float32)
+    par = ref.parents("random", nt, 19)
+    par[12:] = np.sort(par[12:])
+    anc = ref.masks(par)
+    call = ops.attn_tree_f16 if kv == "f16" else ops.attn_tree_f32kv
+    qd, kd, vd = dev_f32(q.reshape(nt, -1), dev), torch.from_numpy(k).to(dev), torch.from_numpy(v).to(dev)
+    ad = torch.from_numpy(anc).to(dev)
+    want, tol = ref.attn(q, k, v, pos0, nh, nkv, anc, 1 / 16)
+    for a, b in ((0, 1), (1, 5), (5, 12), (12, 20)):
+        # what lies behind the rows drafted so far is not there yet
+        got = host(call(qd[a:b], kd[:pos0 + b], vd[:pos0 + b], pos0, nh, nkv, ad[a:b], rows=b)).reshape(b - a, nh, 256)
+        assert (np.abs(got - want[a:b]) <= tol[a:b]).all()
+
+
+@pytest.mark.parametrize("nh,nkv", [(16, 2), (24, 4), (4, 4), (16, 1)])
+@pytest.mark.parametrize("nt,pos0,shape", [(1, 0, "chain"), (1, 1, "chain"), (2, 63, "forest"), (3, 64, "star"), (5, 65, "star"),
+                                           (13, 500, "padded"), (33, 333, "random"), (64, 1000, "padded"),
+                                           (64, 2049, "chain")])
+def test_f32_cache(dev, nh, nkv, nt, pos0, shape):
+    announce(f"attn_tree_f32kv nt={nt} pos0={pos0} {nh}/{nkv} {shape}")
+    r = np.random.default_rng(nt + pos0)
+    f = lambda *s: r.standard_normal(s).astype(np.float32)
+    q, k, v = f(nt, nh, 512), f(pos0 + nt, nkv * 256), f(pos0 + nt, nkv * 256)
+    anc = ref.masks(ref.parents(shape, nt, nt))
+    want, tol = ref.attn(q, k, v, pos0, nh, nkv, anc, 1 / 16)
+    k[pos0:][anc == 0], v[pos0:][anc == 0] = np.nan, np.nan     # a padding node's rows are not looked at
+    args = (dev_f32(q.reshape(nt, -1), dev), dev_f32(k, dev), dev_f32(v, dev), pos0, nh, nkv, torch.from_numpy(anc).to(dev))
+    full = ops.attn_tree_f32kv_scratch_bytes(pos0, nt, nh, nkv)
+    for nbytes in {full, nt * nh * 1040 if pos0 else 0}:
+        out = torch.full((nt, nh * 256), float("nan"), device=dev)
+        ops.attn_tree_f32kv(*args, out=out, scratch=torch.empty(nbytes, device=dev, dtype=torch.uint8))
+        got = host(out).reshape(nt, nh, 256)
+        assert (np.abs(got - want) <= tol).all() and (got[anc == 0] == 0).all()
 
 
 def test_offsets_past_32_bits(dev):

@@ -53,26 +53,33 @@ def test_kv_tree_commit_refusals(kw):
 
 @pytest.mark.parametrize("kw", [dict(q=None), dict(kc=None), dict(vc=None), dict(anc=None), dict(out=None), dict(q=F + 8),
                                 dict(out=F + 4), dict(scratch=F + 8), dict(scratch=None), dict(nbytes=5 * 4 * 1040 - 1),
-                                dict(hd=128), dict(nh=6), dict(kvd=256), dict(nt=0), dict(nt=65), dict(pos0=-1),
-                                dict(pos0=(1 << 22) - 4), dict(qts=4 * 512 - 4), dict(ots=1020), dict(qts=2050)])
-def test_attn_tree_refusals(kw):
-    a = dict(q=F, qts=4 * 512, kc=F, vc=F, kvd=512, pos0=700, hd=256, nh=4, nkv=2, nt=5, anc=F, scale=0.0625, out=F,
+                                dict(hd=128), dict(nh=5), dict(kvd=256), dict(nt=0), dict(nt=65), dict(pos0=-1),
+                                dict(rows=0), dict(rows=65), dict(pos0=(1 << 22) - 4), dict(qts=4 * 512 - 4),
+                                dict(ots=1020), dict(qts=2050)])
+@pytest.mark.parametrize("name", ["it_attn_tree_f16", "it_attn_tree_f32kv"])
+def test_attn_tree_refusals(name, kw):
+    a = dict(q=F, qts=4 * 512, kc=F, vc=F, kvd=512, pos0=700, hd=256, nh=4, nkv=2, nt=5, rows=5, anc=F, scale=0.0625, out=F,
              ots=4 * 256, scratch=F, nbytes=1 << 30)
     a.update(kw)
-    refused("it_attn_tree_f16", *a.values(), None, text="it_attn")
+    refused(name, *a.values(), None, text=name)
+
+
+def test_attn_tree_f32kv_refuses_wide_groups():
+    refused("it_attn_tree_f32kv", F, 17 * 512, F, F, 256, 700, 256, 17, 1, 5, 5, F, 0.0625, F, 17 * 256, F, 1 << 30, None,
+            text="16 q heads")
 
 
 @pytest.mark.parametrize("nh,nkv", [(16, 2), (24, 4), (4, 4), (16, 1)])
 def test_attn_tree_scratch(nh, nkv):
-    """The preferred scratch holds whole records, is never below one per (node, head), and stays below 64 MiB."""
-    f = _lib.lib().it_attn_tree_scratch_bytes
-    for nt in (1, 2, 5, 17, 64):
-        assert f(0, nt, 256, nh, nkv) == 0
-        for pos0 in (1, 63, 64, 65, 1000, 8128, 131072, (1 << 22) - nt):
-            got = f(pos0, nt, 256, nh, nkv)
-            assert got % (nt * nh * 1040) == 0 and nt * nh * 1040 <= got <= 64 << 20
-    for bad in ((100, 0, 256, nh, nkv), (100, 65, 256, nh, nkv), (-1, 3, 256, nh, nkv), (100, 3, 256, nh, 0)):
-        assert f(*bad) == 0
+    """The preferred scratch holds whole records, is never below one per (node, head), and stays below 128 MiB."""
+    for f in (_lib.lib().it_attn_tree_scratch_bytes, _lib.lib().it_attn_tree_f32kv_scratch_bytes):
+        for nt in (1, 2, 5, 17, 64):
+            assert f(0, nt, 256, nh, nkv) == 0
+            for pos0 in (1, 63, 64, 65, 1000, 8128, 131072, (1 << 22) - nt):
+                got = f(pos0, nt, 256, nh, nkv)
+                assert got % (nt * nh * 1040) == 0 and nt * nh * 1040 <= got <= 128 << 20
+        for bad in ((100, 0, 256, nh, nkv), (100, 65, 256, nh, nkv), (-1, 3, 256, nh, nkv), (100, 3, 256, nh, 0)):
+            assert f(*bad) == 0
 
 
 @pytest.mark.parametrize("kw", [dict(x=None), dict(conv=None), dict(state=None), dict(anc=None), dict(trace=None),
