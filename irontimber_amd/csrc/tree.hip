@@ -42,7 +42,8 @@ __global__ __launch_bounds__(256) void kv_tree_commit_kernel(u4* kc, u4* vc, int
                                                              const uint64_t* __restrict__ anc, int leaf) {
     __shared__ int path[64];
     const int tid = threadIdx.x, i = tid >> 2, c = 4 * blockIdx.x + (tid & 3);
-    const uint64_t m = anc[leaf] & (~(uint64_t)0 >> (63 - leaf));
+    uint64_t m = anc[leaf] & (~(uint64_t)0 >> (63 - leaf));
+    if (!(m >> leaf & 1)) m = 0;   // a padding node, as the recurrent layer's commit takes it
     if (tid < 64 && (m >> tid & 1)) path[__popcll(m & (((uint64_t)1 << tid) - 1))] = tid;
     __syncthreads();
     u4* cache = (blockIdx.y ? vc : kc) + (size_t)pos0 * pieces + c;

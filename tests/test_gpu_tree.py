@@ -155,3 +155,15 @@ def test_kv_tree_commit(dev, kv, kvd, shape, nt):
             for i, t in enumerate(kept):
                 want[pos0 + i] = old[pos0 + t]
             assert np.array_equal(got, want), f"leaf {leaf}"
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+def test_kv_tree_commit_keeps_nothing_of_a_padding_node(dev, kv):
+    """A node whose own bit is clear is padding whatever else its mask holds, as it is to the recurrent layer's commit."""
+    r = np.random.default_rng(9)
+    dt = np.float16 if kv == "f16" else np.float32
+    k, v = (r.standard_normal((9, 512)).astype(dt) for _ in range(2))
+    anc = torch.tensor([1, 2, 0b10, 0b1000], dtype=torch.int64, device=dev)   # node 2: its ancestor's bit alone
+    kd, vd = torch.from_numpy(k).to(dev), torch.from_numpy(v).to(dev)
+    (ops.kv_tree_commit_f16 if kv == "f16" else ops.kv_tree_commit_f32)(kd, vd, 5, 4, anc, 2)
+    assert np.array_equal(host(kd), k) and np.array_equal(host(vd), v)
