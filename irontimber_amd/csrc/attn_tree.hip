@@ -360,8 +360,8 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
 template <class KVT> struct Kv4 { typedef h4 T; };
 template <> struct Kv4<float> { typedef f4 T; };
 
-// One workgroup per (256 / SL * 4 dims, head, node); nr: the tree's rows in the cache. Thread = (split lane sg of SL, dim lane of 256 / SL, 4
-// dims each): split lane sg takes the context's records sg, sg + SL, ... and the path's keys likewise.
+// One workgroup per (256 / SL * 4 dims, head, node); nr: the tree's rows in the cache. Thread = (split lane sg of SL, dim lane
+// of 256 / SL, 4 dims each): split lane sg takes the context's records sg, sg + SL, ... and the path's keys likewise.
 // KVT: the cache's values, uint16_t (f16) or float.
 template <int SL, class KVT>
 __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __restrict__ q, int qts,
@@ -490,22 +490,36 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
     }
 }
 
-// The context's form and keys per split, with R = nt * nh / nkv rows a KV head. The decode partials take up to 32 rows a
-// workgroup, one 64-key tile each while that is one round of the CUs, else the tiles of a split one after the other; their
-// time goes as the 8-row blocks of a workgroup times its tiles. The 64-row workgroups cost 4 us more at their ends,
-// share a tile among twice the rows and stream the next ones while they compute. Whole calls, partials / 64 rows,
-// us, 16/2 heads: 1 node 16384 keys 13.7 / 17.4, 65536 30.5 / 34.9, 131072 55.9 / 57.1; 2 nodes 16384 15.6 / 18.8,
-// 131072 63.9 / 57.3; 3 nodes 16384 17.9 / 20.0, 65536 38.6 / 37.7; 8 nodes (two workgroups of 32 rows a tile) 3000
-// 15.7 / 17.9, 5000 22.6 / 22.1; 64 nodes 200 16.2 / 18.5, 600 24.5 / 21.5; 24/4 heads, 5 nodes 5000 19.5 / 19.5,
-// 8128 21.1 / 20.2.
+// The context's form and keys per split, with R = nt * nh / nkv rows a KV head. The decode partials take 8 or 16 rows a
+// workgroup: 8 where one 64-key tile each is at most one round of the CUs, else 16 (8 if there are no more), with as many
+// tiles one after the other as make one round. A workgroup of 16 rows takes 8.5 us and 2.1 a tile of a whole call; those of 64
+// rows take 19 and 0.8 to 1.6, share a tile among four times the rows and stream the next ones while they compute. So
+// up to 5 tiles a workgroup go to the partials. Up to 16 rows both forms read each key once, and the partials stay ahead as
+// long as the call is not at the bytes (12 tiles, 16 with 8 rows).
+// Whole calls in us, 16/2 heads, 8 rows / 16: 5 nodes at 600 keys 8.8 / 9.7 (32 rows: 12.1), 8 at 1000 9.5 / 10.2, 12 at 1000
+// 11.2 / 10.2, 4 at 3000 13.5 / 11.3. 16 rows / 64: 4 nodes 8155 keys (2 tiles) 14.4 / 20.9, 20443 (5) 21.1 / 21.6, 24539
+// (6) 23.4 / 22.8; 8 nodes 4059 (2) 13.6 / 20.2, 8155 (4) 18.3 / 23.5, 10203 (5) 20.6 / 21.7, 12251 (6) 22.8 / 22.0; 64
+// nodes 731 (3) 16.4 / 21.6, 1499 (6) 23.0 / 23.2, 2011 (8) 27.6 / 25.8; 2 nodes 65499 (8) 35.7 / 36.0, 131035 (16) 60.0 /
+// 59.9; 8 rows / 64, 1 node 32731 (4) 18.5 / 22.2, 131035 (16) 52.4 / 58.8.
+// Where the tiles do not divide evenly (3 or more a workgroup for one round, though one tile each is two rounds), two
+// workgroups share a CU instead: 26 nodes at 1200 keys 14.7 us, in splits of three tiles 16.1.
 constexpr int CUS = 256;   // MI355X compute units
-struct TreePlan { bool blocks; int chunk; };
+struct TreePlan { int rows, chunk; };   // rows: 8 or 16 (decode partials), or 64
 static TreePlan plan(int pos0, int nt, int nh, int nkv) {
     const long tiles = (pos0 + 63) / 64, R = (long)nt * (nh / nkv);
-    const long per_cu = (tiles * nkv * ((R + 31) / 32) + CUS - 1) / CUS;   // tiles a CU, workgroups of up to 32 rows
-    if (R <= 32 ? (R + 7) / 8 * per_cu <= 8 : per_cu <= 1) return {false, 64 * (int)std::max(1L, per_cu)};
-    const long groups = nkv * ((R + BM - 1) / BM), splits = std::max(1L, CUS / groups);   // one round of workgroups
-    return {true, 64 * (int)((tiles + splits - 1) / splits)};
+    const auto groups = [&](long rows) { return nkv * ((R + rows - 1) / rows); };
+    const auto one_round = [&](long g) {   // tiles a split
+        const long splits = std::max(1L, CUS / g);
+        return (tiles + splits - 1) / splits;
+    };
+    if (tiles * groups(8) <= CUS) return {8, 64};
+    const int rows = R <= 8 ? 8 : 16;
+    const long g = groups(rows);
+    long k = one_round(g);
+    if (k > 2 && tiles * g <= 2 * CUS) k = 1;
+    const long rounds = (g + CUS - 1) / CUS;   // (more than one with more KV heads and rows than CUs)
+    if (k * rounds <= (R <= 8 ? 16 : R <= 16 ? 12 : 5)) return {rows, 64 * (int)k};
+    return {BM, 64 * (int)one_round(groups(BM))};
 }
 int attn_tree_chunk(int pos0, int nt, int nh, int nkv) { return plan(pos0, nt, nh, nkv).chunk; }
 
@@ -532,13 +546,14 @@ hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const u
     if (pos0 > 0) {
         smax = idx::split_count(pos0, chunk);
         hipError_t e;
-        if (plan(pos0, nt, nh, nkv).blocks) {
+        const int rows = plan(pos0, nt, nh, nkv).rows;
+        if (rows == BM) {
             const int nrb = (nt * (nh / nkv) + BM - 1) / BM;
             const unsigned grid = (unsigned)((smax * nkv + 7) / 8 * 8 * nrb);
             attn_tree_ctx_kernel<<<grid, 256, 0, st>>>(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, smax, nrb);
             e = hipGetLastError();
         } else {
-            e = launch_attn_all_partials(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, st);
+            e = launch_attn_all_partials(q, qts, kc, vc, kvd, pos0, nh, nkv, nt, scale, part, chunk, rows, st);
         }
         if (e != hipSuccess) return e;
     }

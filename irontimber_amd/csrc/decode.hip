@@ -884,33 +884,23 @@ hipError_t launch_attn_partials(const float* q, int qts, const uint16_t* kc, con
     return hipGetLastError();
 }
 
-// 260-word records of all nt tokens over keys 0 .. n-1, in splits of `chunk` keys (n > 0).
+// 260-word records of all nt tokens over keys 0 .. n-1, in splits of `chunk` keys (n > 0), 8 or 16 rows a workgroup.
 hipError_t launch_attn_all_partials(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int n,
-                                    int nh, int nkv, int nt, float scale, float* part, int chunk, hipStream_t st) {
+                                    int nh, int nkv, int nt, float scale, float* part, int chunk, int rows, hipStream_t st) {
     const int R = nt * (nh / nkv), smax = idx::split_count(n, chunk);
     const bool multi = chunk > TK;
-    // blocks of rows as in launch_attn_partials
-    const int rows = multi ? (R <= 8 ? 8 : R <= 16 ? 16 : R <= 24 ? 24 : 32) : (R <= 16 ? 8 : R <= 32 ? 16 : 32);
     const dim3 grid(smax, nkv, (R + rows - 1) / rows);
 #define IT_ALL(NB_, M_, VR_)                                                                                       \
     attn_decode_kernel<NB_, M_, VR_, false, true><<<grid, 256, 0, st>>>(q, qts, kc, vc, kvd, n, nh, nkv, nt, scale, part, \
                                                                        chunk, smax)
-    const bool vr = !multi && rows == 8 && (long)grid.x * grid.y * grid.z >= 64;
-    switch (rows / 8) {
-        case 1:
-            if (multi) IT_ALL(1, true, false);
-            else if (vr) IT_ALL(1, false, true);
-            else IT_ALL(1, false, false);
-            break;
-        case 2:
-            if (multi) IT_ALL(2, true, false);
-            else IT_ALL(2, false, false);
-            break;
-        case 3: IT_ALL(3, true, false); break;
-        default:
-            if (multi) IT_ALL(4, true, false);
-            else IT_ALL(4, false, false);
-            break;
+    const bool vr = (long)grid.x * grid.y * grid.z >= 64;   // as in launch_attn_partials
+    if (rows == 8) {
+        if (multi) IT_ALL(1, true, false);
+        else if (vr) IT_ALL(1, false, true);
+        else IT_ALL(1, false, false);
+    } else {
+        if (multi) IT_ALL(2, true, false);
+        else IT_ALL(2, false, false);
     }
 #undef IT_ALL
     return hipGetLastError();

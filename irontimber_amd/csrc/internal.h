@@ -110,9 +110,9 @@ hipError_t launch_tree_plan(const int* parent, int nt, int p0, uint64_t* anc, in
 hipError_t launch_kv_tree_commit(void* kc, void* vc, size_t row_bytes, int pos0, const uint64_t* anc, int leaf,
                                  hipStream_t st);
 // part: the 260-word records of the pos0 context keys in splits of chunk keys (attn_tree_chunk's or any other
-// multiple of 64), unused where pos0 is 0
+// multiple of 64), unused where pos0 is 0; rows: 8 or 16 a workgroup
 hipError_t launch_attn_all_partials(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int n,
-                                    int nh, int nkv, int nt, float scale, float* part, int chunk, hipStream_t st);
+                                    int nh, int nkv, int nt, float scale, float* part, int chunk, int rows, hipStream_t st);
 int attn_tree_chunk(int pos0, int nt, int nh, int nkv);
 hipError_t launch_attn_f32kv_all_partials(const float* q, int qts, const float* kc, const float* vc, int kvd, int n,
                                           int nh, int nkv, int nt, float scale, float* part, int chunk,
@@ -124,7 +124,7 @@ hipError_t launch_attn_tree(const float* q, int qts, const uint16_t* kc, const u
 hipError_t launch_attn_tree_f32kv(const float* q, int qts, const float* kc, const float* vc, int kvd, int pos0,
                                   int nh, int nkv, int nt, int nr, const uint64_t* anc, float scale, float* out, int ots,
                                   float* part, int chunk, hipStream_t st);
-// trace: U [nt][nv*S], k [nt][nk*S] (f32), G [nt][nv] (f64), written by launch_gdn_tree, read by the commit
+// trace: U [nt][nv*S], k [nt][nk*S] (f32), G [nt][nv] (f64, log2 units), written by launch_gdn_tree, read by the commit
 size_t gdn_tree_trace_bytes(int nt, int nv, int nk);
 hipError_t launch_gdn_tree(const float* x, int xts, const float* cw, int K, const float* cst, const float* br,
                            const float* ar, int bts, const float* dt, const float* a, const float* state,
