@@ -31,26 +31,19 @@ __device__ __forceinline__ uint64_t node_mask(const uint64_t* anc, int t) {
     return m >> t & 1 ? m : 0;
 }
 
-// The addresses of a node's conv inputs 1 .. K-1 tokens back: its ancestors' rows of x, and beyond the path's start
-// rows of the conv state (K - 1 rows, the newest last). m: the mask of its strict ancestors, taken bit by bit from the
-// top. Held as integers so that a lane can hand them to its wave.
+// The rows of a node's conv inputs 1 .. K-1 tokens back, among n nodes' and behind them the conv state's K - 1 (the newest
+// last): its ancestors, and beyond the path's start the state. m: the mask of its strict ancestors, taken bit by bit from
+// the top.
 template <int K>
-__device__ __forceinline__ void taps(uint64_t m, const float* x, int xts, const float* cst, int cd, uint64_t (&row)[K - 1]) {
-    int beyond = K - 2;
+__device__ __forceinline__ void taps(uint64_t m, int n, int (&row)[K - 1]) {
+    int beyond = n + K - 2;
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
         const int a = 63 - (int)__builtin_clzll(m | 1);
-        row[j] = (uint64_t)(uintptr_t)(m ? x + (size_t)a * xts : cst + (size_t)beyond * cd);
+        row[j] = m ? a : beyond;
         if (!m) --beyond;
         m &= ~((uint64_t)1 << a);
     }
-}
-typedef __attribute__((address_space(1))) const float gfloat;
-typedef __attribute__((address_space(1))) const f4 gf4;
-typedef __attribute__((address_space(1))) const char gchar;
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
-           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32;
 }
 __device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
     return (uint64_t)(uint32_t)__shfl((int)(uint32_t)v, lane) | (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane) << 32;
@@ -66,6 +59,10 @@ __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466
 // the products out by blocks of rows; the inverses of I + A's diagonal blocks go one to a wave, and then each of the first
 // NB waves solves for all of U in registers with f32 products (a few more than its share, but no exchange) and writes
 // the output rows of its block.
+// Measured: 3 nodes, 32 V heads 7.3 us; 26 nodes, 48 heads 13.5; 64 nodes, 32 heads 15.4. The floor is the state's bytes
+// (2 MB: 0.4 us) and a launch; what is left is a chain of phases on one workgroup a CU. In cycles for 64 nodes: conv and
+// norm of the q and k rows ~9,000 (each row by all eight workgroups of its head, bound by the vector units at two
+// waves a SIMD), products 5,000, inverses 2,100, solve 1,400, output 1,900.
 // NW: four waves for one block (three nodes: two workgroups a CU and little to share out), eight for more: with one
 // workgroup a CU they hide each other's loads.
 template <int K, int NB, int NW>
@@ -75,14 +72,18 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     const float* __restrict__ A, const float* __restrict__ state, const uint64_t* __restrict__ anc,
     float* __restrict__ out, int ots, int nt, int nv, int nk, float eps, float* __restrict__ trace) {
     constexpr int N = 16 * NB, AST = N + 4;
-    __shared__ __align__(16) _Float16 qk[2][2][N][HST];   // [q, k][hi, lo] rows, zeros for padding
+    constexpr int QKB = 4 * N * HST * 2, RAWB = (N + K - 1) * 2 * S * 4;
+    __shared__ __align__(16) char rows_[QKB > RAWB ? QKB : RAWB];
+    auto raw = (float (*)[2 * S])rows_;                   // q and k inputs of the nodes, then those of the conv state
+    auto qk = (_Float16 (*)[2][N][HST])rows_;             // after them: [q, k][hi, lo] rows
     __shared__ __align__(16) _Float16 sp[2][CW][HST];     // [hi, lo] the state slice, column by column, scaled
     __shared__ __align__(16) float mxs[NW][CW];           // column maxima of the waves' rows
     __shared__ float inv[CW];                             // what a column was divided by
     __shared__ __align__(16) float na[N][AST];            // -A
     __shared__ __align__(16) float pm[N][AST];            // (q_i . k_j) e^(G_i - G_j)
     __shared__ __align__(16) float tin[NB][16][20];       // inverses of the diagonal blocks of I + A
-    __shared__ float vs[N][RST], rs[N][RST], os[N][RST];  // conv'd V, right-hand sides, e^G q S0
+    __shared__ float vs[N][RST], os[N][RST];              // conv'd V, e^G q S0
+    __shared__ float rs[N + K - 1][RST];                  // V inputs, then right-hand sides
     __shared__ double gs[N];                              // G in log2 units
     __shared__ float bs[N];
     __shared__ uint64_t ms[N];
@@ -90,23 +91,24 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, c = l & 15, g = l >> 4;
     const int cb = blockIdx.x & 7, h = blockIdx.x >> 3, kh = h % nk, cd = (2 * nk + nv) * S;
 
-    // ---- everything that hangs on no other load: the masks (a node a lane, in every wave), the wave's own rows of x
-    // (a node's own input, whatever its path, and on its way the ancestors' rows into the caches), the state slice, conv
-    // weights, gates
-    const uint64_t m = l < nt ? node_mask(anc, l) : 0;
-    constexpr int PER = N / NW, BATCH = PER % 4 == 0 ? 4 : 3, VN = (N + 4 * NW - 1) / (4 * NW);
-    static_assert(PER % BATCH == 0 && PER * NW == N, "every node once, none past the LDS rows");
+    // ---- all loads but none that hangs on another: gates, the masks (a node a lane, in every wave), the wave's rows of x,
+    // the conv state, conv weights, the state slice
+    constexpr int PER = N / NW, VN = (N + 4 * NW - 1) / (4 * NW);
+    static_assert(PER * NW == N && NW >= K - 1, "every node once, none past the LDS rows");
     const int ch = (l < 32 ? kh : nk + kh) * S + 4 * (l & 31);         // lanes 0-31 four q channels each, 32-63 k
     const int chv = 2 * nk * S + h * S + cb * CW + (tid & 15);         // V channel; 16 lanes a node
-    // gates, a node a lane (by every wave, used by the last: under a branch the loads would be waited for at its end)
+    // gates, a node a lane (by every wave, used by the first: under a branch the loads would be waited for at its end)
     const size_t gate = (size_t)min(l, nt - 1) * bts + h;
     const float brv = br[gate], arv = ar[gate], dtv = dt[h], av = A[h];
+    const uint64_t m = l < nt ? node_mask(anc, l) : 0;
     f4 own[PER], wt[K];
     float ownv[VN], wv[K];
 #pragma unroll
     for (int i = 0; i < PER; ++i) own[i] = ld_f4(x + uniform_off((size_t)min(w + NW * i, nt - 1) * xts) + ch);
+    const f4 old = ld_f4(cst + (size_t)min(w, K - 2) * cd + ch);
 #pragma unroll
     for (int b = 0; b < VN; ++b) ownv[b] = x[(size_t)min(4 * NW * b + (tid >> 4), nt - 1) * xts + chv];
+    const float oldv = cst[(size_t)min(tid >> 4, K - 2) * cd + chv];
 #pragma unroll
     for (int i = 0; i < K; ++i) {
 #pragma unroll
@@ -121,64 +123,91 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
         sl[i] = ld_f4(state + ((size_t)h * S + (p >> 2)) * S + cb * CW + 4 * (p & 3));
     }
     const uint64_t above = m & ~((uint64_t)1 << l);   // strict ancestors
-    uint64_t row[K - 1];   // lane = node
-    taps<K>(above, x, xts, cst, cd, row);
+    int row[K - 1];   // lane = node
+    taps<K>(above, N, row);
     bool bad = false;
-    const float neg1 = in_register(-1.0f), ieps = eps > 0.f ? 1.0f / eps : INFINITY;
+    const float neg1 = in_register(-1.0f), ieps = eps > 0.f ? 1.0f / (eps * (float)LOG2E_D) : INFINITY;
+    if (w == 0) {
+        // gates and path sums, a node a lane of the first wave (its loads went out first), while they are on their way
+        double G = 0.0;
+        float beta = 0.f;
+        if (m) {
+            beta = sigmoid_hw(brv);
+            const float lg = softplus_hw(arv + dtv) * av;
+            G = lg < -200.f ? -200.0 : (double)lg;   // e^-200 is 0 in f32 already; sums stay finite
+        }
+        int up = above ? 63 - (int)__builtin_clzll(above) : -1;
+        while (__any(up >= 0)) {   // each round a node's sum covers twice as many nodes of its path
+            const int a = up < 0 ? l : up;
+            const double more = __builtin_bit_cast(double, shfl_u64(__builtin_bit_cast(uint64_t, G), a));
+            const int next = __shfl(up, a);
+            if (up >= 0) { G += more; up = next; }
+        }
+        if (l < N) { ms[l] = m; gs[l] = G * LOG2E_D; bs[l] = beta; }
+        if (l == 0) spoilt = 0;
+    }
 
-    // ---- conv + SiLU + L2 norm of the q and k heads, three or four nodes at a time (padding nodes read the conv state)
+    // ---- the inputs of the convs into LDS, where a node finds its ancestors' (from memory they would be a second round
+    // trip, and four rows a node through the CU's load path instead of one)
 #pragma unroll
-    for (int i0 = 0; i0 < PER; i0 += BATCH) {
-        f4 in[BATCH][K - 1];
+    for (int i = 0; i < PER; ++i) *(f4*)&raw[w + NW * i][4 * l] = own[i];
+    if (w < K - 1) *(f4*)&raw[N + w][4 * l] = old;
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i)
+    for (int b = 0; b < VN; ++b) {
+        const int t = 4 * NW * b + (tid >> 4);
+        if (t < N) rs[t][tid & 15] = ownv[b];
+    }
+    if ((tid >> 4) < K - 1) rs[N + (tid >> 4)][tid & 15] = oldv;
+    __syncthreads();
+    f4 in[PER][K - 1];
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j) in[i][j] = *(gf4*)((gchar*)lane_u64(row[j], w + NW * (i0 + i)) + 4u * (unsigned)ch);
-        if (i0 == 0 && w == NW - 1) {
-            // gates and path sums, a node a lane of the last wave, while its loads are out
-            double G = 0.0;
-            float beta = 0.f;
-            if (m) {
-                beta = sigmoid_hw(brv);
-                const float lg = softplus_hw(arv + dtv) * av;
-                G = lg < -200.f ? -200.0 : (double)lg;   // e^-200 is 0 in f32 already; sums stay finite
-            }
-            int up = above ? 63 - (int)__builtin_clzll(above) : -1;
-            while (__any(up >= 0)) {   // each round a node's sum covers twice as many nodes of its path
-                const int a = up < 0 ? l : up;
-                const double more = __builtin_bit_cast(double, shfl_u64(__builtin_bit_cast(uint64_t, G), a));
-                const int next = __shfl(up, a);
-                if (up >= 0) { G += more; up = next; }
-            }
-            if (l < N) { ms[l] = m; gs[l] = G * LOG2E_D; bs[l] = beta; }
-            if (l == 0) spoilt = 0;
-        }
+    for (int i = 0; i < PER; ++i)
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int t = w + NW * (i0 + i);
-            f4 y = in[i][K - 2] * wt[0];
+        for (int j = 0; j < K - 1; ++j) in[i][j] = ld_f4(&raw[__builtin_amdgcn_readlane(row[j], w + NW * i)][4 * l]);
+    float inp[VN][K - 1];
 #pragma unroll
-            for (int j = K - 3; j >= 0; --j) y += in[i][j] * wt[K - 2 - j];
-            y += own[i0 + i] * wt[K - 1];
+    for (int b = 0; b < VN; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = silu_hw(y[e]);
-            float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
-            ss += dppc<0xB1>(ss);
-            ss += dppc<0x4E>(ss);
-            ss += dppc<0x141>(ss);
-            ss += dppc<0x140>(ss);
-            ss = sum_xor16(ss);
-            const float f = fminf(__builtin_amdgcn_rsqf(ss), ieps);   // 1 / max(|y|, eps)
-            const bool live = lane_u64(m, t) != 0;
-            bad |= live && !finite(ss);
+        for (int j = 0; j < K - 1; ++j) inp[b][j] = rs[__shfl(row[j], min(4 * NW * b + (tid >> 4), N - 1))][tid & 15];
+    __syncthreads();   // the q and k rows take their inputs' place
+    // ---- conv + SiLU + L2 norm of the q and k heads (padding nodes take the conv state for ancestors; what their rows hold
+    // is not used). The weights carry a factor log2 e, so that the conv's result is the exponent of the SiLU; the norm takes
+    // the factor out again.
+    const uint64_t alive = __ballot(m != 0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = live ? y[e] * f : 0.f;
-            h2 h0, h1, l0, l1;
-            split2(f2{y[0], y[1]}, neg1, h0, l0);
-            split2(f2{y[2], y[3]}, neg1, h1, l1);
-            *(h4*)&qk[l >> 5][0][t][4 * (l & 31)] = h4{h0[0], h0[1], h1[0], h1[1]};
-            *(h4*)&qk[l >> 5][1][t][4 * (l & 31)] = h4{l0[0], l0[1], l1[0], l1[1]};
-        }
+    for (int i = 0; i < K; ++i) wt[i] *= (float)LOG2E_D;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int t = w + NW * i;
+        f4 y = in[i][K - 2] * wt[0];
+#pragma unroll
+        for (int j = K - 3; j >= 0; --j) y += in[i][j] * wt[K - 2 - j];
+        y += own[i] * wt[K - 1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-y[e]));
+        float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
+        ss += dppc<0xB1>(ss);
+        ss += dppc<0x4E>(ss);
+        ss += dppc<0x141>(ss);
+        ss += dppc<0x140>(ss);
+        ss = sum_xor16(ss);
+        const float f = fminf(__builtin_amdgcn_rsqf(ss), ieps);   // 1 / max(|y|, eps)
+        bad |= (alive >> t & 1) && !finite(ss);
+        y *= f;
+        h2 h0, h1, l0, l1;
+        split2(f2{y[0], y[1]}, neg1, h0, l0);
+        split2(f2{y[2], y[3]}, neg1, h1, l1);
+        *(h4*)&qk[l >> 5][0][t][4 * (l & 31)] = h4{h0[0], h0[1], h1[0], h1[1]};
+        *(h4*)&qk[l >> 5][1][t][4 * (l & 31)] = h4{l0[0], l0[1], l1[0], l1[1]};
+    }
+    // ---- conv + SiLU of the workgroup's V columns
+#pragma unroll
+    for (int b = 0; b < VN; ++b) {
+        const int t = 4 * NW * b + (tid >> 4);
+        float y = ownv[b] * wv[K - 1];
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) y += inp[b][j] * wv[K - 2 - j];
+        if (t < N) vs[t][tid & 15] = silu_hw(y);
     }
     // ---- column maxima of the slice: over the thread's pieces, the lanes of its column quad, the waves
     {
@@ -194,23 +223,6 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             mx[e] = max_xor32(max_xor16(mx[e]));
         }
         if (l < 4) *(f4*)&mxs[w][4 * l] = mx;
-    }
-    // ---- conv + SiLU of the workgroup's V columns
-    {
-        float in[VN][K - 1];
-#pragma unroll
-        for (int b = 0; b < VN; ++b)
-#pragma unroll
-            for (int j = 0; j < K - 1; ++j)
-                in[b][j] = ((gfloat*)shfl_u64(row[j], min(4 * NW * b + (tid >> 4), N - 1)))[chv];
-#pragma unroll
-        for (int b = 0; b < VN; ++b) {
-            const int t = 4 * NW * b + (tid >> 4);
-            float y = ownv[b] * wv[K - 1];
-#pragma unroll
-            for (int j = 0; j < K - 1; ++j) y += in[b][j] * wv[K - 2 - j];
-            if (t < N) vs[t][tid & 15] = silu_hw(y);
-        }
     }
     __syncthreads();
     // ---- the slice as f16 pairs: each column times the power of two that takes its largest value to 2^13 .. 2^14, so that
@@ -440,7 +452,8 @@ hipError_t launch_gdn_tree(const float* x, int xts, const float* cw, int K, cons
 
 // Workgroups 0 .. 8 nv - 1: 16 state rows of a head, thread = (row, 8 columns), the path's rank-one updates on top
 // of the decayed state. The others: 256 channels of the conv state, whose rows are the last K - 1 inputs of
-// {old state, the path's rows of x}; a thread reads its channel's old rows before it writes any.
+// {old state, the path's rows of x}; a thread reads its channel's old rows before it writes any. A launch and two dependent
+// round trips (mask, then k and U): 3.8 us for one node of 32 heads, 4.1 for a path of two, 5.4 for 48 heads and a path of 9.
 __global__ __launch_bounds__(256) void gdn_tree_commit_kernel(const float* __restrict__ x, int xts, int K, float* cst,
                                                               float* __restrict__ state,
                                                               const uint64_t* __restrict__ anc, int leaf, int nt,

@@ -211,7 +211,8 @@ hipError_t launch_attn_prep_f32kv(float* q, int qts, const float* k, const float
 // The same pass with the rotation given from outside: token t at position pos[t] (or pos0 + t), pair i
 // turning by position * freq[i], cos and sin times mscale, the pairs in halves or interleaved; K and V to
 // cache row row0 + t. The angle is the f64 product of an integer and an f32, so exact before it is reduced.
-// Workgroups and rows as in attn_prep_kernel. Bound by the bytes from some hundred tokens on.
+// Workgroups and rows as in attn_prep_kernel. Bound by the bytes from some hundred tokens on: 8192 tokens, 16/2 heads 62 us
+// = 5.14 TB/s, the rate of a large copy; one token 3.2 us, 37 tokens 24/4 heads 3.1.
 template <int E, class KVT, bool PAIRS>
 __global__ __launch_bounds__(64 * PREP_WAVES) void attn_prep_pos_kernel(
     float* __restrict__ q, int qts, const float* __restrict__ k, const float* __restrict__ v, int kts,

@@ -10,7 +10,7 @@ namespace it {
 
 // One wave, lane = node. The masks grow by pointer doubling: after round r a node's mask holds its
 // nearest 2^r - 1 ancestors and itself, and `up` the ancestor 2^r levels above (64 levels in 6 rounds). A
-// parent outside -1 .. t-1 makes a padding node, and so does a padding ancestor.
+// parent outside -1 .. t-1 makes a padding node, and so does a padding ancestor. PLAN_US for 64 nodes: one launch.
 __global__ __launch_bounds__(64) void tree_plan_kernel(const int* __restrict__ parent, int nt, int p0,
                                                        uint64_t* __restrict__ anc, int* __restrict__ pos) {
     const int t = threadIdx.x, p = t < nt ? parent[t] : -2;
@@ -38,6 +38,7 @@ hipError_t launch_tree_plan(const int* parent, int nt, int p0, uint64_t* anc, in
 // Rows pos0 + path[i] -> pos0 + i of both caches, path = the set bits of anc[leaf] up to leaf. A workgroup
 // owns 64 bytes of every row: one 16-byte piece of one path row a thread, all loaded before any is stored,
 // so the rows may overlap and one memory round trip serves the whole path. grid (row pieces / 4, 2 caches).
+// A launch and that round trip: 2.2 us for 7 rows of 512 values, 2.6 for 64 rows of 1024.
 __global__ __launch_bounds__(256) void kv_tree_commit_kernel(u4* kc, u4* vc, int pieces, int pos0,
                                                              const uint64_t* __restrict__ anc, int leaf) {
     __shared__ int path[64];
