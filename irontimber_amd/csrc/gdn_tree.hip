@@ -169,6 +169,21 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     for (int b = 0; b < VN; ++b)
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) inp[b][j] = rs[__shfl(row[j], min(4 * NW * b + (tid >> 4), N - 1))][tid & 15];
+    // ---- column maxima of the slice: over the thread's pieces, the lanes of its column quad, the waves
+    {
+        f4 mx = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < SL; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fabsf(sl[i][e]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            mx[e] = fmaxf(mx[e], dppc<0x124>(mx[e]));   // row_ror:4
+            mx[e] = fmaxf(mx[e], dppc<0x128>(mx[e]));   // row_ror:8
+            mx[e] = max_xor32(max_xor16(mx[e]));
+        }
+        if (l < 4) *(f4*)&mxs[w][4 * l] = mx;
+    }
     __syncthreads();   // the q and k rows take their inputs' place
     // ---- conv + SiLU + L2 norm of the q and k heads (padding nodes take the conv state for ancestors; what their rows hold
     // is not used). The weights carry a factor log2 e, so that the conv's result is the exponent of the SiLU; the norm takes
@@ -209,22 +224,6 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
         for (int j = 0; j < K - 1; ++j) y += inp[b][j] * wv[K - 2 - j];
         if (t < N) vs[t][tid & 15] = silu_hw(y);
     }
-    // ---- column maxima of the slice: over the thread's pieces, the lanes of its column quad, the waves
-    {
-        f4 mx = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < SL; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fabsf(sl[i][e]));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            mx[e] = fmaxf(mx[e], dppc<0x124>(mx[e]));   // row_ror:4
-            mx[e] = fmaxf(mx[e], dppc<0x128>(mx[e]));   // row_ror:8
-            mx[e] = max_xor32(max_xor16(mx[e]));
-        }
-        if (l < 4) *(f4*)&mxs[w][4 * l] = mx;
-    }
-    __syncthreads();
     // ---- the slice as f16 pairs: each column times the power of two that takes its largest value to 2^13 .. 2^14, so that
     // the pairs hold every value to 2^-22 of itself or 2^-39 of the column's largest
     {
