@@ -62,7 +62,8 @@ constexpr int F32KV_ROW = F32KV_HD + 4;                 // padded LDS row (float
 // src/vk/mod.rs:740).
 // CR: the same values in the piece layout of common.h (decode and short verify calls whose merge is
 // the wave merge).
-// ALL: every row sees all of the pos0 keys and no others (a drafted tree's nodes and their context).
+// ALL: every row sees all of the pos0 keys and no others (a drafted tree's nodes and their context). As fast as the causal
+// form, 8128 slots, 16/2 heads: 1 node 11.5 us (causal token 11.0), 8 nodes 21.4 (21.2), 16 nodes 31.9 (31.2).
 template <int RB, bool DIRECT, bool CR = false, bool ALL = false>
 __global__ __launch_bounds__(256 * RB) void attn_f32kv_kernel(const float* __restrict__ q, int qts,
                                                          const float* __restrict__ kc, const float* __restrict__ vc,

@@ -69,6 +69,13 @@ def test_conv_sizes(dev, K, nt):
     check(dev, 4, nt, 4, 2, "random", K=K)
 
 
+@pytest.mark.parametrize("K", [2, 3])
+@pytest.mark.parametrize("nt", [1, 16, 20, 41, 64])
+def test_conv_sizes_of_many_heads(dev, K, nt):
+    """48 heads: workgroups of 32 state columns."""
+    check(dev, 5, nt, 48, 16, "random", K=K)
+
+
 @pytest.mark.parametrize("decay", [0.0, 1e-3, 30.0, 1e4])
 @pytest.mark.parametrize("shape", ["chain", "padded"])
 def test_decays(dev, decay, shape):
@@ -116,6 +123,22 @@ def test_other_branches_do_not_matter(dev, bad, name):
     keep = [t for t in range(nt) if anc[t] and not int(anc[t]) >> spoilt & 1]
     assert (np.abs(got - want)[keep] <= tol[keep]).all()
     assert (np.abs(again[leaf][1] - states[leaf]) <= errs[leaf][:, None, None]).all()
+
+
+@pytest.mark.parametrize("nt", [14, 30, 60])
+def test_other_branches_do_not_matter_to_many_heads(dev, nt):
+    """The same with 32 state columns a workgroup: one branch's infinities reach no other node."""
+    nv, nk = 48, 16
+    d = inputs(12, nt, nv, nk)
+    par = ref.parents("random", nt, 12)
+    anc = ref.masks(par)
+    spoilt = nt - 1
+    d["x"][spoilt, ::3] = np.inf
+    got, _ = run(dev, d, anc, nv, nk)
+    d["x"][spoilt] = 0
+    want, tol, *_ = ref.gdn(d["x"], d["w"], d["conv"], d["beta"], d["alpha"], d["dt"], d["a"], d["state"], par, nv, nk, EPS)
+    assert (np.abs(got - want)[:spoilt] <= tol[:spoilt]).all()
+    assert not np.isfinite(got[spoilt]).all()
 
 
 def test_bits_that_are_no_ancestors(dev):
