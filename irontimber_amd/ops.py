@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._lib import call, lib
+from ._lib import ItError, call, last_error, lib
 
 KERNEL_AUTO, KERNEL_SPLITK, KERNEL_FLASH, KERNEL_FLASH_F32 = 0, 1, 2, 3
 
@@ -443,20 +443,20 @@ TREE_MAX = 64
 
 
 def _call_on(dev: int, name: str, *args) -> None:
-    """call(name, *args, stream) with device dev current and its current stream (asked for as a number: the stream
+    """call(name, *args, stream) with device dev current and its current stream (asked for as numbers: the stream
     object of torch.cuda.current_stream takes 1 us to make, a third of a short launch)."""
-    if dev == torch.cuda.current_device():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    elif getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev)):
+        raise ItError(f"{name}: {last_error()}")
 
 
 def _need_all(dtype: torch.dtype, dev: int, tensors, names: str) -> None:
-    """Every tensor contiguous, of dtype and on device dev; names in the tensors' order, for the message. One pass over
-    cheap queries: these checks are most of what a short call costs the host."""
+    """Every tensor (None: absent) contiguous, of dtype and on device dev; names in the tensors' order, for the message.
+    One pass over cheap queries: these checks are most of what a short call costs the host."""
     for t in tensors:
-        if t.dtype is not dtype or t.get_device() != dev or dev < 0 or not t.is_contiguous():
+        if t is not None and (t.dtype is not dtype or t.get_device() != dev or dev < 0 or not t.is_contiguous()):
             name = names.split()[[u is t for u in tensors].index(True)]
             _need(t, dtype, name)
             raise ValueError(f"{name} must be on the same device as the other tensors")
@@ -490,8 +490,7 @@ def rope_freqs(n_rot: int, base: float = 1e7, kind: str = "plain", factor: float
 
 def _prep_pos(name, kinds, q, k, v, kc, vc, pos, row0, nh, nkv, freq, mscale, layout, q_norm, k_norm, eps, pos0, *more):
     dev = q.get_device()
-    _need_all(torch.float32, dev, [t for t in (q, k, v, freq, q_norm, k_norm) if t is not None],
-              "q k v freq " + ("q_norm " if q_norm is not None else "") + "k_norm")
+    _need_all(torch.float32, dev, (q, k, v, freq, q_norm, k_norm), "q k v freq q_norm k_norm")
     if k.dim() != 2 or k.shape[1] % nkv != 0:
         raise ValueError("k must be [nt, nkv*hd]")
     nt, kvd = k.shape
