@@ -56,6 +56,14 @@ def test_long_context(dev, nt, shape):
     check(dev, 9, nt, 8100, 16, 2, shape)
 
 
+@pytest.mark.parametrize("nt,pos0,shape", [(1, 20000, "chain"), (2, 9001, "forest"), (3, 300, "star"), (5, 5003, "random"),
+                                           (8, 10007, "random"), (26, 1200, "padded"), (40, 2000, "random")])
+def test_forms_of_the_context(dev, nt, pos0, shape):
+    """8 rows a workgroup with one tile and with several, 16 rows with one (one and two workgroups a CU), two and five, and
+    64 rows."""
+    check(dev, 21, nt, pos0, 16, 2, shape)
+
+
 def test_sharp_and_flat_scores(dev):
     """One key takes nearly all the weight (scores up to about 100), and all keys the same (scores of zero)."""
     check(dev, 3, 9, 700, 16, 2, "random", kscale=25.0)
