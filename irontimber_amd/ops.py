@@ -464,12 +464,13 @@ def _need_all(dtype: torch.dtype, dev: int, tensors, names: str) -> None:
 
 def _need_caches(dtypes, dev: int, kvd: int, rows: int, kc: torch.Tensor, vc: torch.Tensor) -> None:
     for c in (kc, vc):
-        if c.dtype not in dtypes or not c.is_contiguous() or c.dim() != 2 or c.shape[1] != kvd:
+        shape = c.shape
+        if c.dtype not in dtypes or len(shape) != 2 or shape[1] != kvd or not c.is_contiguous():
             raise ValueError(f"kc and vc must be contiguous [rows, {kvd}] of {dtypes[0]}")
         if c.get_device() != dev or dev < 0:
             raise ValueError("kc and vc must be device tensors, on the same device as the other tensors")
-        if c.shape[0] < rows:
-            raise ValueError(f"cache too short: {c.shape[0]} rows, {rows} needed")
+        if shape[0] < rows:
+            raise ValueError(f"cache too short: {shape[0]} rows, {rows} needed")
 
 
 _F16 = (torch.float16, torch.int16)
@@ -491,19 +492,20 @@ def rope_freqs(n_rot: int, base: float = 1e7, kind: str = "plain", factor: float
 def _prep_pos(name, kinds, q, k, v, kc, vc, pos, row0, nh, nkv, freq, mscale, layout, q_norm, k_norm, eps, pos0, *more):
     dev = q.get_device()
     _need_all(torch.float32, dev, (q, k, v, freq, q_norm, k_norm), "q k v freq q_norm k_norm")
-    if k.dim() != 2 or k.shape[1] % nkv != 0:
+    shape = k.shape
+    if len(shape) != 2 or shape[1] % nkv != 0:
         raise ValueError("k must be [nt, nkv*hd]")
-    nt, kvd = k.shape
+    nt, kvd = shape
     hd = kvd // nkv
-    if q.shape != (nt, nh * 2 * hd) or v.shape != k.shape:
+    if q.shape != (nt, nh * 2 * hd) or v.shape != shape:
         raise ValueError("q must be [nt, nh*2*hd] and v the shape of k [nt, nkv*hd]")
     if row0 < 0:
         raise ValueError("row0 must not be negative")
     _need_caches(kinds, dev, kvd, row0 + nt, kc, vc)
-    if pos is not None:
+    if pos is not None and (pos.shape != (nt,) or pos.dtype is not torch.int32 or pos.get_device() != dev or
+                            not pos.is_contiguous()):
         _need_all(torch.int32, dev, (pos,), "pos")
-        if pos.shape != (nt,):
-            raise ValueError("pos must be [nt]")
+        raise ValueError("pos must be [nt]")
     if (q_norm is not None and q_norm.numel() != hd) or (k_norm is not None and k_norm.numel() != hd):
         raise ValueError("q_norm and k_norm must hold head_dim floats")
     if layout not in ROPE_LAYOUTS:
@@ -534,8 +536,8 @@ def attn_prep_pos_f32kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc: t
 
 
 def _need_anc(anc: torch.Tensor, dev: int, nt: int) -> None:
-    _need_all(torch.int64, dev, (anc,), "anc")
-    if anc.shape != (nt,):
+    if anc.shape != (nt,) or anc.dtype is not torch.int64 or anc.get_device() != dev or not anc.is_contiguous():
+        _need_all(torch.int64, dev, (anc,), "anc")
         raise ValueError(f"anc must be [{nt}]")
 
 
@@ -559,10 +561,10 @@ def attn_tree_f32kv_scratch_bytes(pos0: int, nt: int, nh: int, nkv: int, hd: int
 
 
 def _attn_tree(name, kinds, scratch_bytes, q, kc, vc, pos0, nh, nkv, anc, scale, out, scratch, rows):
-    dev = q.get_device()
-    if q.dim() != 2 or q.shape[1] % (2 * nh) != 0:
+    dev, shape = q.get_device(), q.shape
+    if len(shape) != 2 or shape[1] % (2 * nh) != 0:
         raise ValueError("q must be [nt, nh*2*hd]")
-    nt, hd = q.shape[0], q.shape[1] // (2 * nh)
+    nt, hd = shape[0], shape[1] // (2 * nh)
     kvd = nkv * hd
     if rows is None:
         rows = nt
@@ -580,7 +582,7 @@ def _attn_tree(name, kinds, scratch_bytes, q, kc, vc, pos0, nh, nkv, anc, scale,
         scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
     elif scratch.get_device() != dev or not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous, on the same device as the other tensors")
-    nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    nbytes = 0 if scratch is None else scratch.nbytes
     _call_on(dev, name, q.data_ptr(), nh * 2 * hd, kc.data_ptr(), vc.data_ptr(), kvd, pos0, hd, nh, nkv, nt, rows,
              anc.data_ptr(), scale, out.data_ptr(), nh * hd, _ptr(scratch), nbytes)
     return out
