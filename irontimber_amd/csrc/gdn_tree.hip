@@ -82,12 +82,11 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     __shared__ __align__(16) float na[N][AST];            // -A
     __shared__ __align__(16) float pm[N][AST];            // (q_i . k_j) e^(G_i - G_j)
     __shared__ __align__(16) float tin[NB][16][20];       // inverses of the diagonal blocks of I + A
-    __shared__ float vs[N][RST], os[N][RST];              // conv'd V, e^G q S0
+    __shared__ float vs[N][RST], os[N][RST];              // conv'd V, then U where it is summed node by node; e^G q S0
     __shared__ float rs[N + K - 1][RST];                  // V inputs, then right-hand sides
     __shared__ double gs[N];                              // G in log2 units
     __shared__ float bs[N];
     __shared__ uint64_t ms[N];
-    __shared__ int spoilt;                                // a value that is not finite went into the products
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, c = l & 15, g = l >> 4;
     const int cb = blockIdx.x % (S / CW), h = blockIdx.x / (S / CW), kh = h % nk, cd = (2 * nk + nv) * S;
 
@@ -125,7 +124,6 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     const uint64_t above = m & ~((uint64_t)1 << l);   // strict ancestors
     int row[K - 1];   // lane = node
     taps<K>(above, N, row);
-    bool bad = false;
     const float neg1 = in_register(-1.0f), ieps = eps > 0.f ? 1.0f / (eps * (float)LOG2E_D) : INFINITY;
     if (w == 0) {
         // gates and path sums, a node a lane of the first wave (its loads went out first), while they are on their way
@@ -144,7 +142,6 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             if (up >= 0) { G += more; up = next; }
         }
         if (l < N) { ms[l] = m; gs[l] = G * LOG2E_D; bs[l] = beta; }
-        if (l == 0) spoilt = 0;
     }
 
     // ---- the inputs of the convs into LDS, where a node finds its ancestors' (from memory they would be a second round
@@ -188,7 +185,6 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     // ---- conv + SiLU + L2 norm of the q and k heads (padding nodes take the conv state for ancestors; what their rows hold
     // is not used). The weights carry a factor log2 e, so that the conv's result is the exponent of the SiLU; the norm takes
     // the factor out again.
-    const uint64_t alive = __ballot(m != 0);
 #pragma unroll
     for (int i = 0; i < K; ++i) wt[i] *= (float)LOG2E_D;
 #pragma unroll
@@ -207,7 +203,6 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
         ss += dppc<0x140>(ss);
         ss = sum_xor16(ss);
         const float f = fminf(__builtin_amdgcn_rsqf(ss), ieps);   // 1 / max(|y|, eps)
-        bad |= (alive >> t & 1) && !finite(ss);
         y *= f;
         h2 h0, h1, l0, l1;
         split2(f2{y[0], y[1]}, neg1, h0, l0);
@@ -307,12 +302,10 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
                     const float d = acc[i] * inv[cc] * __builtin_amdgcn_exp2f((float)gt[i]);
                     const float v = which ? bt[i] * (d - vs[t][cc]) : d;
                     (which ? rs : os)[t][cc] = mt[i] ? v : 0.f;
-                    bad |= mt[i] && !finite(v);
                 }
             }
         }
         if (!SHARE || (w & 1)) {
-            // (finite where the rows are, which the conv has looked at, and the decays, which the state's products do)
             for (int bj = 0; bj <= bi; ++bj) {
                 const int j = 16 * bj + c;
                 const f4 acc = product(&qk[1][0][j][8 * g], &qk[1][1][j][8 * g]);
@@ -327,70 +320,75 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             }
         }
     }
-    if (bad) spoilt = 1;
     __syncthreads();
     const float scale = 1.0f / sqrtf((float)S);
     float* tu = trace + (size_t)h * S + cb * CW;   // U rows, then k rows, then G
     const size_t ustride = (size_t)nv * S;
-    if (spoilt) {
-        // The block products would carry a NaN or an infinity of one branch to others as 0 * NaN: the same sums node by
-        // node over the ancestors alone.
-        if (tid < CW) {
-            for (int t = 0; t < nt; ++t) {
-                float u = rs[t][tid], o = os[t][tid];
-                for (int j = 0; j < t; ++j)
-                    if (ms[t] >> j & 1) u += na[t][j] * rs[j][tid];
-                rs[t][tid] = u;
-                for (int j = 0; j <= t; ++j)
-                    if (ms[t] >> j & 1) o += pm[t][j] * rs[j][tid];
-                out[(size_t)t * ots + (size_t)h * S + cb * CW + tid] = o * scale;
-                tu[t * ustride + tid] = u;
-            }
+    // ---- (I + A_bb)^-1, lane column c: a column of the identity, each row's value taken to the rows below as soon as
+    // it is known (the four lane groups alike)
+    if (w < NB) {
+        f4 a[16][4];
+        float z[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            z[i] = i == c ? 1.f : 0.f;
+#pragma unroll
+            for (int j = 0; j < (i + 3) / 4; ++j) a[i][j] = ld_f4(&na[16 * w + i][16 * w + 4 * j]);
         }
-    } else {
-        // ---- (I + A_bb)^-1, lane column c: a column of the identity, each row's value taken to the rows below as soon as
-        // it is known (the four lane groups alike)
-        if (w < NB) {
-            f4 a[16][4];
-            float z[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                z[i] = i == c ? 1.f : 0.f;
+        for (int j = 0; j < 15; ++j)
 #pragma unroll
-                for (int j = 0; j < (i + 3) / 4; ++j) a[i][j] = ld_f4(&na[16 * w + i][16 * w + 4 * j]);
-            }
+            for (int i = j + 1; i < 16; ++i) z[i] += a[i][j / 4][j % 4] * z[j];
+        if (g == 0) {
 #pragma unroll
-            for (int j = 0; j < 15; ++j)
-#pragma unroll
-                for (int i = j + 1; i < 16; ++i) z[i] += a[i][j / 4][j % 4] * z[j];
-            if (g == 0) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) tin[w][i][c] = z[i];
-            }
+            for (int i = 0; i < 16; ++i) tin[w][i][c] = z[i];
         }
-        __syncthreads();
-        if (w < NB * CB) {
-            const int cc = 16 * (w / NB) + c;   // column
-            // ---- U block by block: u[b] holds rows 4 g + e of column cc, both a product's result and, in the order of
-            // the A operand's 16-byte reads, the next one's B operand
-            f4 u[NB];
+    }
+    __syncthreads();
+    if (w < NB * CB) {
+        const int cc = 16 * (w / NB) + c;   // column
+        // ---- U block by block: u[b] holds rows 4 g + e of column cc, both a product's result and, in the order of
+        // the A operand's 16-byte reads, the next one's B operand
+        f4 u[NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                f4 r;
+        for (int b = 0; b < NB; ++b) {
+            f4 r;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = rs[16 * b + 4 * g + i][cc];
+            for (int i = 0; i < 4; ++i) r[i] = rs[16 * b + 4 * g + i][cc];
 #pragma unroll
-                for (int j = 0; j < b; ++j) {
-                    const f4 a = ld_f4(&na[16 * b + c][16 * j + 4 * g]);
+            for (int j = 0; j < b; ++j) {
+                const f4 a = ld_f4(&na[16 * b + c][16 * j + 4 * g]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) r = mfma4(a[e], u[j][e], r);
+                for (int e = 0; e < 4; ++e) r = mfma4(a[e], u[j][e], r);
+            }
+            const f4 a = ld_f4(&tin[b][c][4 * g]);
+            u[b] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[b] = mfma4(a[e], r[e], u[b]);
+        }
+        bool fine = true;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) fine &= finite(u[b][e]);
+        // ---- output and trace rows of block w % NB
+        if (__any(!fine)) {
+            // What is not finite in one branch has gone to others as 0 * inf (wherever it came from, the conv, a gate, the
+            // state or the solve itself, U shows it): the same sums node by node over the ancestors alone. All waves of
+            // these columns found the same U, and leave them to the first.
+            if (w % NB == 0 && g == 0) {
+                for (int t = 0; t < nt; ++t) {
+                    float v = rs[t][cc], o = os[t][cc];
+                    for (int j = 0; j < t; ++j)
+                        if (ms[t] >> j & 1) v += na[t][j] * vs[j][cc];
+                    vs[t][cc] = v;
+                    for (int j = 0; j <= t; ++j)
+                        if (ms[t] >> j & 1) o += pm[t][j] * vs[j][cc];
+                    out[(size_t)t * ots + (size_t)h * S + cb * CW + cc] = o * scale;
+                    tu[t * ustride + cc] = v;
                 }
-                const f4 a = ld_f4(&tin[b][c][4 * g]);
-                u[b] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) u[b] = mfma4(a[e], r[e], u[b]);
             }
-            // ---- output and trace rows of block w % NB
+        } else {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (b != w % NB) continue;   // (static register indexes)
