@@ -86,6 +86,8 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     __shared__ float rs[N + K - 1][RST];                  // V inputs, then right-hand sides
     __shared__ double gs[N];                              // G in log2 units
     __shared__ float bs[N];
+    __shared__ float len[2][N];                           // lengths of the q and k rows: 1, or less below the norm's floor
+    __shared__ int below;                                 // some row is
     __shared__ uint64_t ms[N];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, c = l & 15, g = l >> 4;
     const int cb = blockIdx.x % (S / CW), h = blockIdx.x / (S / CW), kh = h % nk, cd = (2 * nk + nv) * S;
@@ -125,6 +127,7 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     int row[K - 1];   // lane = node
     taps<K>(above, N, row);
     const float neg1 = in_register(-1.0f), ieps = eps > 0.f ? 1.0f / (eps * (float)LOG2E_D) : INFINITY;
+    const float most = fmaxf(ieps, 9e18f);   // 1 / |y| where the sum of squares is the least normal number
     if (w == 0) {
         // gates and path sums, a node a lane of the first wave (its loads went out first), while they are on their way
         double G = 0.0;
@@ -141,7 +144,8 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
             const int next = __shfl(up, a);
             if (up >= 0) { G += more; up = next; }
         }
-        if (l < N) { ms[l] = m; gs[l] = G * LOG2E_D; bs[l] = beta; }
+        if (l < N) { ms[l] = m; gs[l] = G * LOG2E_D; bs[l] = beta; len[0][l] = len[1][l] = 1.0f; }
+        if (l == 0) below = 0;
     }
 
     // ---- the inputs of the convs into LDS, where a node finds its ancestors' (from memory they would be a second round
@@ -184,9 +188,11 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
     __syncthreads();   // the q and k rows take their inputs' place
     // ---- conv + SiLU + L2 norm of the q and k heads (padding nodes take the conv state for ancestors; what their rows hold
     // is not used). The weights carry a factor log2 e, so that the conv's result is the exponent of the SiLU; the norm takes
-    // the factor out again.
+    // the factor out again. A row below the norm's floor, y / eps, is brought to length 1 like the others, which the pairs
+    // (their step is 2^-25) hold to 2^-22, and its length goes into the products' results.
 #pragma unroll
     for (int i = 0; i < K; ++i) wt[i] *= (float)LOG2E_D;
+    float f[PER], fm = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int t = w + NW * i;
@@ -202,13 +208,21 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
         ss += dppc<0x141>(ss);
         ss += dppc<0x140>(ss);
         ss = sum_xor16(ss);
-        const float f = fminf(__builtin_amdgcn_rsqf(ss), ieps);   // 1 / max(|y|, eps)
-        y *= f;
+        f[i] = fminf(__builtin_amdgcn_rsqf(ss), most);   // 1 / |y|
+        y *= f[i];
         h2 h0, h1, l0, l1;
         split2(f2{y[0], y[1]}, neg1, h0, l0);
         split2(f2{y[2], y[3]}, neg1, h1, l1);
         *(h4*)&qk[l >> 5][0][t][4 * (l & 31)] = h4{h0[0], h0[1], h1[0], h1[1]};
         *(h4*)&qk[l >> 5][1][t][4 * (l & 31)] = h4{l0[0], l0[1], l1[0], l1[1]};
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) fm = fmaxf(fm, f[i]);
+    if (__any(fm > ieps)) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if ((l & 31) == 0 && f[i] > ieps) len[l >> 5][w + NW * i] = ieps / f[i];
+        below = 1;
     }
     // ---- conv + SiLU of the workgroup's V columns
 #pragma unroll
@@ -321,6 +335,21 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
         }
     }
     __syncthreads();
+    if (below) {   // the lengths of short rows into the products (the right-hand sides are beta (V - e^G k S0))
+        for (int i = tid; i < N * N; i += 64 * NW) {
+            const int t = i / N, j = i % N;
+            if (j > t) continue;
+            na[t][j] *= len[1][t] * len[1][j];
+            pm[t][j] *= len[0][t] * len[1][j];
+        }
+        for (int i = tid; i < N * CW; i += 64 * NW) {
+            const int t = i / CW, cc = i % CW;
+            const float bv = bs[t] * vs[t][cc], k = len[1][t];
+            os[t][cc] *= len[0][t];
+            if (ms[t] && k != 1.0f) rs[t][cc] = (rs[t][cc] - bv) * k + bv;
+        }
+        __syncthreads();
+    }
     const float scale = 1.0f / sqrtf((float)S);
     float* tu = trace + (size_t)h * S + cb * CW;   // U rows, then k rows, then G
     const size_t ustride = (size_t)nv * S;
@@ -417,7 +446,7 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(
         float* tk = trace + (size_t)nt * nv * S + (size_t)h * S + cb * CW;
         for (int i = tid; i < nt * CW; i += 64 * NW) {
             const int t = i / CW, d = cb * CW + i % CW;
-            tk[(size_t)t * nk * S + i % CW] = (float)qk[1][0][t][d] + (float)qk[1][1][t][d];
+            tk[(size_t)t * nk * S + i % CW] = ((float)qk[1][0][t][d] + (float)qk[1][1][t][d]) * len[1][t];
         }
     }
     if (cb == 0 && tid < nt) ((double*)(trace + (size_t)nt * (nv + nk) * S))[(size_t)tid * nv + h] = gs[tid];   // in log2 units

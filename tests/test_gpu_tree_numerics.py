@@ -35,3 +35,58 @@ def test_updates_that_overflow_stay_on_their_path(dev, nt, nv, nk):
     assert (np.abs(got - want)[keep] <= tol[keep]).all()
     for t in keep[1:]:
         assert (np.abs(done[t][1] - states[t]) <= errs[t][:, None, None]).all(), t
+
+
+def silu(x):
+    return x / (1 + np.exp(-x))
+
+
+@pytest.mark.parametrize("nv,nk", [(4, 2), (48, 16)])
+@pytest.mark.parametrize("nt,size", [(1, 0.3), (3, 1e-3), (20, 1e-3), (5, 1e-6), (40, 1e-9)])
+def test_rows_below_the_norms_floor(dev, nt, size, nv, nk):
+    """q rows of norm `size` * eps come out at length `size`, to the accuracy that full rows have: the output is `size` times
+    that of the same rows without a floor, and so is its bound. (k rows are full ones, so the states are too.)"""
+    announce(f"gdn_tree nt={nt} {nv}/{nk} q rows of {size} eps")
+    d = gdn_inputs(nt, nt, nv, nk)
+    par = ref.parents("random", nt, nt)
+    d["w"][:, :-1], d["w"][:, -1] = 0, 1
+    q = slice(0, nk * 128)
+    d["x"][:, q] *= size * EPS / 5.66               # |silu(z)| = |z| / 2 of 128 small normal values: 5.66 times their size
+    args = [d[k] for k in ("x", "w", "conv", "beta", "alpha", "dt", "a", "state")]
+    want, _, states, errs, _ = ref.gdn(*args, par, nv, nk, EPS)
+    _, tol, *_ = ref.gdn(*args, par, nv, nk, 1e-30)
+    row = np.linalg.norm(silu(d["x"][:, q].astype(np.float64)).reshape(nt, nk, 128), axis=-1) / EPS
+    assert (row < 1).all()
+    tol = tol * row[:, np.arange(nv) % nk, None]
+    got, done = gdn_run(dev, d, ref.masks(par), nv, nk, [nt - 1])
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+    assert (np.abs(done[nt - 1][1] - states[nt - 1]) <= errs[nt - 1][:, None, None]).all()
+
+
+@pytest.mark.parametrize("nv,nk", [(4, 2), (48, 16)])
+@pytest.mark.parametrize("nt,size", [(1, 0.3), (3, 1e-3), (20, 1e-3), (5, 1e-6), (40, 1e-9)])
+def test_updates_of_rows_below_the_norms_floor(dev, nt, size, nv, nk):
+    """k rows of norm `size` * eps on an empty state: what a chain leaves is `size` times a sum of updates, and as accurate."""
+    announce(f"gdn_tree nt={nt} {nv}/{nk} k rows of {size} eps")
+    d = gdn_inputs(nt, nt, nv, nk)
+    par = ref.parents("chain", nt)
+    d["w"][:, :-1], d["w"][:, -1] = 0, 1
+    d["state"][:] = 0
+    k = slice(nk * 128, 2 * nk * 128)
+    d["x"][:, k] *= size * EPS / 5.66
+    _, _, states, _, _ = ref.gdn(*(d[n] for n in ("x", "w", "conv", "beta", "alpha", "dt", "a", "state")), par, nv, nk, EPS)
+    x = d["x"].astype(np.float64)
+    row = np.linalg.norm(silu(x[:, k]).reshape(nt, nk, 128), axis=-1) / EPS
+    assert (row < 1).all()
+    # Each update k u^T: k relative to its row as in the layer's statement (the conv's sums here are one product: 6 steps of
+    # the largest element over the row's mean one, 12 of the norm, 4 of the pair), u = beta (v - what `size`^2 leaves): v and
+    # beta 20 steps, the decays 16 and the sum over the path 64.
+    z = np.abs(x[:, k]).reshape(nt, nk, 128)
+    rel = 6 * z.max(-1) * np.sqrt(128) / (row * EPS) + 16 + 20 + 16 + 64
+    u = np.abs(silu(x[:, 2 * nk * 128:])).reshape(nt, nv, 128).max(-1)
+    head = np.arange(nv) % nk
+    tol = (2.0 ** -24 * rel * row)[:, head] * u * (1 + size)
+    _, done = gdn_run(dev, d, ref.masks(par), nv, nk, [0, nt - 1])
+    for t in (0, nt - 1):
+        bound = tol[:t + 1].sum(0)[:, None, None]
+        assert (np.abs(done[t][1] - states[t]) <= bound).all(), float((np.abs(done[t][1] - states[t]) / bound).max())
