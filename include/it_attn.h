@@ -477,7 +477,8 @@ int it_tree_plan(const int32_t* parent, int nt, int p0, uint64_t* anc, int32_t* 
  * level asks for the newest ones, with anc pointing at their masks and rows counting all nodes so far. Rows that a node
  * does not see are not read for it, whatever they hold. A row without any bit is zeros. pos0 may be 0. Other arguments
  * and the result as for it_attn_f16 (f32 accumulation, q and the probabilities carried as f16 pairs: about 2e-6
- * relative). rows in 1 .. IT_TREE_MAX; nt as well.
+ * relative; a q row is scaled by a power of two of its own, so its size and that of `scale` do not matter). rows in
+ * 1 .. IT_TREE_MAX; nt as well.
  * scratch: the context's records; it_attn_tree_scratch_bytes(...) bytes give the library's split, with fewer the
  * splits get longer, and nt * nh * 1040 bytes are always enough (0 for pos0 = 0). Calls that overlap need one each. */
 size_t it_attn_tree_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv);

@@ -28,7 +28,7 @@ constexpr float LN2_F = 0.6931471805599453f;
 // of one KV head x one key split, four waves of 32 rows x half of each 64-key tile's keys: wave w takes rows
 // 32 (w & 1) .. +31 and keys 32 (w >> 1) .. +31, with a running maximum, sum and O of its own that are joined at the
 // end. The transposed products of the flash form (S^T = K q^T, O^T += V^T P^T, 32x32x16, one query row a lane
-// pair), twice each: q and P go in as f16 pairs hi + lo, so K and V, exact in f16, meet f32 operands to 2^-22 and the
+// pair), twice each: q (scaled) and P go in as f16 pairs hi + lo, so K and V, exact in f16, meet f32 operands to 2^-22 and the
 // f32 records keep f32's accuracy. A tile takes a wave 64 matrix ops of 32 cycles.
 // Splitting rows and keys between the waves halves what a wave reads from LDS against four waves of 16 rows: 1024
 // cycles of LDS a tile and workgroup beside 2048 of the matrix cores.
@@ -46,6 +46,7 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     __shared__ __align__(16) _Float16 V1[BN * HD];
     __shared__ float ms[2][BM], ls[2][BM];   // per key half
     __shared__ f2 rowml[BM];
+    __shared__ int rowex[BM];   // power of two that a q row was multiplied with
 
     // Row blocks of one (split, KV head) read the same keys: their ids differ by multiples of 8, which puts
     // them on one XCD and its L2.
@@ -81,13 +82,36 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
         }
         tile_to_lds32(kc, kvd, kb0, kend, cj, K0, w, l);
         tile_to_lds32(vc, kvd, kb0, kend, cj, V0, w, l);
-        const float sc = scale * LOG2E;
+        // Each row times the power of two that takes its largest value to 2^13 .. 2^14, so that the pairs hold every value to
+        // 2^-22 of itself or 2^-39 of the row's largest, whatever q's size. The maxima: rows i and i + 8 in the half-waves, i and
+        // i + 4 in their 16-lane rows, then over those 16 lanes.
+        float mx[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            mx[i] = fmaxf(fmaxf(fabsf(qx[i][0]), fabsf(qx[i][1])), fmaxf(fabsf(qx[i][2]), fabsf(qx[i][3])));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            swap32(mx[i], mx[i + 8]);
+            mx[i] = fmaxf(mx[i], mx[i + 8]);
+        }
+        int ex[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            swap16(mx[i], mx[i + 4]);
+            float m = fmaxf(mx[i], mx[i + 4]);
+            m = fmaxf(m, dppc<0xB1>(m));
+            m = fmaxf(m, dppc<0x4E>(m));
+            m = fmaxf(m, dppc<0x141>(m));
+            m = fmaxf(m, dppc<0x140>(m));
+            ex[i] = 14 - __builtin_amdgcn_frexp_expf(m);   // of row i + 4 (16-lane row & 1) + 8 (half-wave)
+            if ((l & 15) == 0) rowex[16 * w + i + 4 * ((l >> 4) & 1) + 8 * (l >> 5)] = ex[i];
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int row = 16 * w + i;
+            const int row = 16 * w + i, e = __builtin_amdgcn_readlane(ex[i & 3], 16 * ((i >> 2) & 1) + 32 * (i >> 3));
             h2 h0, h1, l0, l1;
-            split2(f2{qx[i][0] * sc, qx[i][1] * sc}, neg1, h0, l0);
-            split2(f2{qx[i][2] * sc, qx[i][3] * sc}, neg1, h1, l1);
+            split2(f2{__builtin_amdgcn_ldexpf(qx[i][0], e), __builtin_amdgcn_ldexpf(qx[i][1], e)}, neg1, h0, l0);
+            split2(f2{__builtin_amdgcn_ldexpf(qx[i][2], e), __builtin_amdgcn_ldexpf(qx[i][3], e)}, neg1, h1, l1);
             const h4 hi = {h0[0], h0[1], h1[0], h1[1]}, lo = {l0[0], l0[1], l1[0], l1[1]};
             const int to = row * HD + 8 * ((l >> 1) ^ (row & 31)) + 4 * (l & 1);
             *(h4*)(K1 + to) = hi;
@@ -101,6 +125,7 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
             ql[ks] = ld_h8(V1 + at);
         }
     }
+    const float back = __builtin_amdgcn_ldexpf(scale * LOG2E, -rowex[32 * wr + c]);   // from products to log2 units
     f16v o[8];
 #pragma unroll
     for (int db = 0; db < 8; ++db) o[db] = f16v{};
@@ -130,9 +155,8 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
     };
     // Online softmax in log2 units. The weights are 2^(s - m_run) with m_run 7 below the maximum seen when it was last
     // raised, and it is raised when a row's maximum passes m_run + 15: weights stay below 2^15, inside f16, and the pair
-    // hi + lo resolves 2^-24 of them, 2^-31 of a fresh maximum, so that many small weights still count. The score products
-    // start from -m_run instead of zero, so they come out as exponents; m_run is 0 while a row has seen no key.
-    f16v minit = f16v{};   // -m_run
+    // hi + lo resolves 2^-24 of them, 2^-31 of a fresh maximum, so that many small weights still count.
+    float minus = 0.f;     // -m_run, 0 while a row has seen no key
     f16v sc;               // the tile's exponents
     h8 ph[2], pl[2];       // its weights, hi and lo
     auto settle = [&](float mx) __attribute__((always_inline)) {   // mx: the largest exponent
@@ -149,10 +173,8 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
             for (int db = 0; db < 8; ++db) scale_acc(o[db], alpha);
             if (grow) m_run = mnew;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                sc[i] -= up;
-                minit[i] = m_run == -INFINITY ? 0.0f : -m_run;
-            }
+            for (int i = 0; i < 16; ++i) sc[i] -= up;
+            minus = m_run == -INFINITY ? 0.0f : -m_run;
         }
     };
     // keys at or past kend: exponent -inf; returns the largest of the rest
@@ -203,7 +225,7 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
         if (kb + 3 * BN > kend) offsets(offk, kb + 2 * BN);   // (a tile past the end: its last row again, unused)
         if (kb + 2 * BN > kend) offsets(offv, kb + BN);
         const char *kbase = row_base(kc, kb + 2 * BN), *vbase = row_base(vc, kb + BN);
-        f16v sa = minit;
+        f16v sa = f16v{};
         h8 k[16], v[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) k[i] = k_op(Kn, i);
@@ -226,8 +248,8 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
             if (j < 12) v[j + 4] = v_op(V, j + 4);
             o[j & 7] = mfma32x32x16(v[j], ph[j >> 3], o[j & 7]);
             if (j >= 4 && j < 12) {   // (the last score op's result takes the first steps)
-                sc[2 * j - 8] = sa[2 * j - 8];
-                sc[2 * j - 7] = sa[2 * j - 7];
+                sc[2 * j - 8] = __builtin_fmaf(sa[2 * j - 8], back, minus);
+                sc[2 * j - 7] = __builtin_fmaf(sa[2 * j - 7], back, minus);
                 mx = fmaxf(fmaxf(mx, sc[2 * j - 8]), sc[2 * j - 7]);
             }
             IT_FENCE;
@@ -260,14 +282,14 @@ __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restr
             sc = mfma32x32x16(k[i], ql[i], sc);
             IT_FENCE;
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] *= back;
         const float mx = max_xor32(mask(kb0));
         if (mx > -INFINITY) m_run = mx - P_BITS;   // (O and l are zero: nothing to rescale)
         const float up = mx > -INFINITY ? m_run : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            sc[i] -= up;
-            minit[i] = -up;
-        }
+        for (int i = 0; i < 16; ++i) sc[i] -= up;
+        minus = -up;
     }
     int kb = kb0;
     for (; kb + 2 * BN < kend; kb += 2 * BN) {   // two tiles whose successors exist

@@ -202,6 +202,24 @@ __device__ __forceinline__ void decode_partial(const float* __restrict__ q, int 
         const int idx = tid + 256 * it, row = idx >> 5, d0 = 8 * (idx & 31);
         h8 hi, lo;
         if (r0 + row >= R) qx[it][0] = qx[it][1] = f4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (ALL) {
+            // each row (32 lanes) times the power of two that takes its largest value to 2^13 .. 2^14, so that the pairs hold
+            // it to 2^-22 whatever its size; the scores' factor takes it back (Al is free until the first tile)
+            float m = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(fabsf(qx[it][0][j]), fabsf(qx[it][1][j])));
+            m = fmaxf(m, dppc<0xB1>(m));
+            m = fmaxf(m, dppc<0x4E>(m));
+            m = fmaxf(m, dppc<0x141>(m));
+            m = max_xor16(fmaxf(m, dppc<0x140>(m)));
+            const int e = 14 - __builtin_amdgcn_frexp_expf(m);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                qx[it][0][j] = __builtin_amdgcn_ldexpf(qx[it][0][j], e);
+                qx[it][1][j] = __builtin_amdgcn_ldexpf(qx[it][1][j], e);
+            }
+            if ((tid & 31) == 0) Al[row] = __builtin_amdgcn_ldexpf(sc2, -e);
+        }
         split_hi_lo(qx[it][0], qx[it][1], hi, lo);
         *(h8*)&Qs[0][row][d0] = hi;
         *(h8*)&Qs[1][row][d0] = lo;
@@ -246,6 +264,11 @@ __device__ __forceinline__ void decode_partial(const float* __restrict__ q, int 
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) qb[b][ks] = ld_h8(&Qs[c >> 3][8 * b + (c & 7)][32 * ks + 8 * g]);
+    float rsc[ALL ? NB : 1];   // from products to log2 units
+    if constexpr (ALL) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) rsc[b] = Al[8 * b + (c & 7)];
+    }
     // V goes out only now: the q planes were built while the K rows were in flight, and the scores
     // and softmax below run while V lands (the memory system is kept busy by the other waves' K)
     if constexpr (!VR) v_tile_to_lds(vc, kvd, head_off, p0, pend, V0, w, l);
@@ -274,7 +297,7 @@ __device__ __forceinline__ void decode_partial(const float* __restrict__ q, int 
             for (int i = 0; i < 4; ++i) {
                 const float v = sacc[b][i] + dpp_f<0x128>(sacc[b][i]);   // row_ror:8 -> column c ^ 8
                 const int key = kb + 16 * w + 4 * g + i;
-                x[b][i] = key < lb ? v * sc2 : -INFINITY;
+                x[b][i] = key < lb ? v * (ALL ? rsc[ALL ? b : 0] : sc2) : -INFINITY;
                 mx[b] = fmaxf(mx[b], x[b][i]);
             }
         }

@@ -4,6 +4,7 @@ import pytest
 
 from tests import tree_ref as ref
 from tests.gpu_util import announce
+from tests.test_gpu_attn_tree import inputs as attn_inputs, run as attn_run
 from tests.test_gpu_gdn_tree import EPS, inputs as gdn_inputs, run as gdn_run
 
 pytestmark = pytest.mark.gpu
@@ -90,3 +91,20 @@ def test_updates_of_rows_below_the_norms_floor(dev, nt, size, nv, nk):
     for t in (0, nt - 1):
         bound = tol[:t + 1].sum(0)[:, None, None]
         assert (np.abs(done[t][1] - states[t]) <= bound).all(), float((np.abs(done[t][1] - states[t]) / bound).max())
+
+
+@pytest.mark.parametrize("qscale,scale,kscale", [(1.0, 1 / 16, 6.0), (1.0, 1e-3, 375.0), (1.0, 1e-4, 3750.0), (0.02, 1 / 16, 300.0),
+                                                 (1.0, -1e-4, 3750.0), (1.0, 0.0, 1.0), (3e4, 1 / 16, 2e-4)])
+@pytest.mark.parametrize("nt,pos0", [(3, 700), (16, 1100), (64, 700), (64, 2100), (64, 4200)])
+def test_sizes_of_queries_keys_and_scale(dev, nt, pos0, qscale, scale, kscale):
+    """Scores of the same spread (6, so that few keys carry a row) from queries, keys and scales of other sizes, in every form of
+    the context."""
+    announce(f"attn_tree nt={nt} pos0={pos0} q {qscale} scale {scale} k {kscale}")
+    q, k, v = attn_inputs(nt, nt, pos0, 16, 2, kscale)
+    q[..., :256] *= qscale
+    anc = ref.masks(ref.parents("random", nt, nt))
+    # (the statement's bound takes a size from the scale: a negative one is given as the queries' sign)
+    sign = np.where(np.arange(512) < 256, np.float32(np.sign(scale)), np.float32(1))
+    want, tol = ref.attn(q * sign, k, v, pos0, 16, 2, anc, abs(scale))
+    got = attn_run(dev, q, k, v, pos0, 16, 2, anc, scale=scale)
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
