@@ -133,8 +133,7 @@ struct F32kvPlan { int chunk; size_t bytes; };
 // of 4 tiles); 320 / 384 / 512 keys gave 81 / 91 / 114 us (2 rounds of 5 / 6 / 8 tiles), all with four waves
 // a workgroup; with eight, 576 keys (one round of 9 tiles) take 59.6 against 68.5 us.
 constexpr int F32KV_CUS = 256;   // MI355X compute units
-int f32kv_rounds_chunk(long total, int nt, int nh, int nkv) {   // over `total` keys
-    const long blocks = ((long)nt * (nh / nkv) + 31) / 32;   // 32-row blocks of the multi-block kernel
+int f32kv_rounds_chunk(long total, int nkv, long blocks) {   // `blocks` workgroups a split and KV head, `total` keys
     int best = 64;
     long best_cost = -1;
     for (long c = 64; best_cost < 0 || c / 64 + 1 <= best_cost; c += 64) {   // (one round of longer splits costs more)
@@ -149,8 +148,11 @@ int f32kv_rounds_chunk(long total, int nt, int nh, int nkv) {   // over `total` 
     return best;
 }
 int f32kv_pref_chunk(int pos0, int nt, int nh, int nkv) {
-    if ((long)nt * (nh / nkv) <= 32) return auto_chunk(pos0, nt, nh, nkv, false);
-    return f32kv_rounds_chunk((long)pos0 + nt, nt, nh, nkv);
+    const long rows = (long)nt * (nh / nkv);
+    if (rows <= 32) return auto_chunk(pos0, nt, nh, nkv, false);
+    // (blocks of 32 rows, which 16/2 heads fill; 24/4 heads take 30 of 32 and launch up to one in 16 more. The split is
+    // part of the rounding of this call's results, so it stays.)
+    return f32kv_rounds_chunk((long)pos0 + nt, nkv, (rows + 31) / 32);
 }
 F32kvPlan plan_f32kv(int pos0, int nt, int nh, int nkv, size_t budget) {
     const long total = (long)pos0 + nt;
@@ -422,7 +424,12 @@ static int fit_tree(int pos0, int nt, int nh, int c, size_t budget) {
     return tree_scratch(pos0, nt, nh, c) <= budget ? c : 0;
 }
 static int tree_pref_chunk(bool f32kv, int pos0, int nt, int nh, int nkv) {
-    return f32kv ? f32kv_rounds_chunk(pos0, nt, nh, nkv) : it::attn_tree_chunk(pos0, nt, nh, nkv);
+    if (!f32kv) return it::attn_tree_chunk(pos0, nt, nh, nkv);
+    // By the workgroups that the launch makes, of whole nodes: 24/4 heads put five in 32 rows. Planned by 32-row blocks instead,
+    // 64 nodes at 4096 slots were 260 workgroups in place of 240, a second round: 148 us the call against 99; 36 nodes at 8128
+    // 169 against 98, 64 at 8128 270 against 178.
+    const int tokens = std::max(1, it::f32kv_rows(nt, nh / nkv).tokens);   // (0 with more heads a KV head than the call takes)
+    return f32kv_rounds_chunk(pos0, nkv, (nt + tokens - 1) / tokens);
 }
 static size_t tree_scratch_bytes(bool f32kv, int pos0, int nt, int nh, int nkv) {
     if (nt < 1 || nt > IT_TREE_MAX || pos0 < 0 || nh <= 0 || nkv <= 0 || nh % nkv) return 0;

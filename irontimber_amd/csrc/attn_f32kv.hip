@@ -236,8 +236,7 @@ hipError_t launch_attn_f32kv(const float* q, int qts, const float* kc, const flo
     const int smax = idx::split_count((long)pos0 + nt, chunk);
     const float qs = scale * 1.44269504088896340736f;
     // two 16-row blocks per workgroup once a call has more rows than one block holds
-    const int rb = nt * G > 16 ? 2 : 1;
-    const int tpw = 16 * rb / G;
+    const auto [rb, tpw] = f32kv_rows(nt, G);
     // the piece layout for the wave merge (one 16-row block: decode and short verify calls)
     const bool pieces = !direct && rb == 1 && piece_records(pos0, nt, nh, chunk);
     const dim3 grid((unsigned)smax, (unsigned)nkv, (unsigned)((nt + tpw - 1) / tpw));
@@ -267,7 +266,7 @@ hipError_t launch_attn_f32kv_all_partials(const float* q, int qts, const float* 
                                           hipStream_t st) {
     const int G = nh / nkv, smax = idx::split_count(n, chunk);
     const float qs = scale * 1.44269504088896340736f;
-    const int rb = nt * G > 16 ? 2 : 1, tpw = 16 * rb / G;
+    const auto [rb, tpw] = f32kv_rows(nt, G);
     const dim3 grid((unsigned)smax, (unsigned)nkv, (unsigned)((nt + tpw - 1) / tpw));
     if (rb == 2)
         attn_f32kv_kernel<2, false, false, true><<<grid, 512, 0, st>>>(q, qts, kc, vc, kvd, n, nh, nkv, nt, tpw, qs, part,

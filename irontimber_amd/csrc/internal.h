@@ -114,6 +114,12 @@ hipError_t launch_kv_tree_commit(void* kc, void* vc, size_t row_bytes, int pos0,
 hipError_t launch_attn_all_partials(const float* q, int qts, const uint16_t* kc, const uint16_t* vc, int kvd, int n,
                                     int nh, int nkv, int nt, float scale, float* part, int chunk, int rows, hipStream_t st);
 int attn_tree_chunk(int pos0, int nt, int nh, int nkv);
+// Row blocks of 16 (1 or 2) and whole tokens of a workgroup of the f32-KV partials, with G query heads per KV head
+struct F32kvRows { int blocks, tokens; };
+inline F32kvRows f32kv_rows(int nt, int G) {
+    const int rb = nt * G > 16 ? 2 : 1;
+    return {rb, 16 * rb / G};
+}
 hipError_t launch_attn_f32kv_all_partials(const float* q, int qts, const float* kc, const float* vc, int kvd, int n,
                                           int nh, int nkv, int nt, float scale, float* part, int chunk,
                                           hipStream_t st);

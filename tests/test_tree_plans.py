@@ -1,0 +1,25 @@
+"""The splits of the tree attentions' contexts: host code only."""
+import pytest
+
+from irontimber_amd import _lib
+
+CUS = 256
+RECORD = 1040
+
+
+@pytest.mark.parametrize("G", range(1, 17))
+@pytest.mark.parametrize("nkv", [1, 2, 4])
+def test_f32kv_splits_are_planned_by_the_workgroups_launched(G, nkv):
+    """A split's cost is the rounds of its workgroups over the CUs times the tiles each takes and one. The workgroups are
+    those of the launch: whole nodes, as many as fit 32 rows. No other split costs less than the chosen one."""
+    f = _lib.lib().it_attn_tree_f32kv_scratch_bytes
+    nh = G * nkv
+    for nt in range(1, 65):
+        per = (32 if nt * G > 16 else 16) // G
+        groups = nkv * -(-nt // per)
+        for pos0 in (600, 1000, 2048, 4096, 8128, 12000, 20000, 32768):
+            tiles = -(-pos0 // 64)
+            smax = f(pos0, nt, 256, nh, nkv) // (nt * nh * RECORD)
+            cost = lambda s: -(-s * groups // CUS) * (-(-tiles // s) + 1)
+            best = min(cost(-(-tiles // k)) for k in range(1, tiles + 1))
+            assert cost(smax) == best, (nt, pos0, smax)
