@@ -533,7 +533,7 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const float* __res
 constexpr int CUS = 256;   // MI355X compute units
 struct TreePlan { int rows, chunk; };   // rows: 8 or 16 (decode partials), or 64
 static TreePlan plan(int pos0, int nt, int nh, int nkv) {
-    const long tiles = (pos0 + 63) / 64, R = (long)nt * (nh / nkv);
+    const long tiles = ((long)pos0 + 63) / 64, R = (long)nt * (nh / nkv);
     const auto groups = [&](long rows) { return nkv * ((R + rows - 1) / rows); };
     const auto one_round = [&](long g) {   // tiles a split
         const long splits = std::max(1L, CUS / g);
