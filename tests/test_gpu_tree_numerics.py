@@ -1,11 +1,14 @@
 """Values at the ends of their range in the tree-verification calls, against the f64 statements."""
 import numpy as np
 import pytest
+import torch
 
+from irontimber_amd import ops
 from tests import tree_ref as ref
-from tests.gpu_util import announce
+from tests.gpu_util import announce, dev_f32, host
 from tests.test_gpu_attn_tree import inputs as attn_inputs, run as attn_run
 from tests.test_gpu_gdn_tree import EPS, inputs as gdn_inputs, run as gdn_run
+from tests.test_tree_plans import MERGES
 
 pytestmark = pytest.mark.gpu
 
@@ -107,4 +110,23 @@ def test_sizes_of_queries_keys_and_scale(dev, nt, pos0, qscale, scale, kscale):
     sign = np.where(np.arange(512) < 256, np.float32(np.sign(scale)), np.float32(1))
     want, tol = ref.attn(q * sign, k, v, pos0, 16, 2, anc, abs(scale))
     got = attn_run(dev, q, k, v, pos0, 16, 2, anc, scale=scale)
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("ramp", ["up", "down"])
+@pytest.mark.parametrize("f32,nt,pos0,nh,nkv", MERGES)
+def test_merges_of_every_form(dev, f32, nt, pos0, nh, nkv, ramp):
+    """Records joined by every form of the merge, with scores that grow or fall along the context: the largest are in the last
+    records, or in the first."""
+    announce(f"attn_tree merge f32={f32} nt={nt} pos0={pos0} {nh}/{nkv} {ramp}")
+    q, k, v = attn_inputs(pos0 + nt, nt, pos0, nh, nkv)
+    size = np.linspace(0.2, 6, pos0)[:, None].astype(np.float32)
+    k[:pos0] = (k[:pos0] * (size if ramp == "up" else size[::-1])).astype(np.float16)
+    kind = np.float32 if f32 else np.float16
+    k, v = k.astype(kind), v.astype(kind)
+    anc = ref.masks(ref.parents("random", nt, nt))
+    want, tol = ref.attn(q, k, v, pos0, nh, nkv, anc, 1 / 16)
+    call = ops.attn_tree_f32kv if f32 else ops.attn_tree_f16
+    got = host(call(dev_f32(q.reshape(nt, -1), dev), torch.from_numpy(k).to(dev), torch.from_numpy(v).to(dev), pos0, nh, nkv,
+                    torch.from_numpy(anc).to(dev))).reshape(nt, nh, 256)
     assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())

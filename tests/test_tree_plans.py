@@ -35,3 +35,22 @@ def test_sizes_of_any_context(nh, nkv, nt):
     for pos0 in (1 << 24, (1 << 31) - 65, (1 << 31) - 64, (1 << 31) - 63, (1 << 31) - 2, (1 << 31) - 1):
         got = f(pos0, nt, 256, nh, nkv)
         assert got % (nt * nh * RECORD) == 0 and got <= 2 * longest, pos0
+
+
+# (f32 cache, nodes, context, q heads, KV heads) whose merges take each form: 4 or 16 split lanes, one batch of records or more
+MERGES = [(False, 3, 700, 16, 2), (False, 16, 8128, 16, 2), (False, 9, 8100, 24, 4), (False, 20, 20000, 16, 2),
+          (False, 4, 16000, 16, 2), (False, 1, 20000, 16, 1), (True, 16, 4000, 16, 2), (True, 13, 16000, 16, 1),
+          (True, 1, 8128, 16, 2), (True, 8, 8128, 16, 2), (True, 1, 20000, 16, 1)]
+
+
+def merge_form(f32, nt, pos0, nh, nkv):
+    """(split lanes, whether there is more than one batch of records), as the launch chooses them."""
+    f = _lib.lib().it_attn_tree_f32kv_scratch_bytes if f32 else _lib.lib().it_attn_tree_scratch_bytes
+    smax = f(pos0, nt, 256, nh, nkv) // (nt * nh * RECORD)
+    lanes = 16 if smax > 32 and nt * nh <= 192 else 4
+    return lanes, smax > 8 * lanes
+
+
+def test_merge_cases_take_every_form():
+    for f32 in (False, True):
+        assert {merge_form(*c) for c in MERGES if c[0] == f32} == {(4, False), (4, True), (16, False), (16, True)}
