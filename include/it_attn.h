@@ -476,9 +476,13 @@ int it_tree_plan(const int32_t* parent, int nt, int p0, uint64_t* anc, int32_t* 
  * bit is set in anc[t] (higher bits are ignored). Verification asks for all nodes at once, nt = rows; drafting level by
  * level asks for the newest ones, with anc pointing at their masks and rows counting all nodes so far. Rows that a node
  * does not see are not read for it, whatever they hold. A row without any bit is zeros. pos0 may be 0. Other arguments
- * and the result as for it_attn_f16 (f32 accumulation, q and the probabilities carried as f16 pairs: about 2e-6
- * relative; a q row is scaled by a power of two of its own, so its size and that of `scale` do not matter). rows in
- * 1 .. IT_TREE_MAX; nt as well.
+ * and the result as for it_attn_f16. rows in 1 .. IT_TREE_MAX; nt as well.
+ * Accuracy: sums in f32. q is carried as f16 pairs of 22 bits (each row scaled by a power of two of its own, so its size and
+ * that of `scale` do not matter), which moves an output by about 2e-6 of the largest value where scores are of ordinary size
+ * (some tens at most). The context's probabilities are carried as f16 pairs with a step of their own: 2^-31 of a row's largest
+ * in calls of many rows or long contexts, but 2^-25 of the largest in a split in the others, where what is smaller is lost. So one
+ * key that outweighs n others of its split by 2^25 loses them, n * 2^-25 of the result: up to 3e-5 with the library's splits
+ * (1024 keys at most), and as much as the whole context makes of n with the smallest scratch.
  * scratch: the context's records; it_attn_tree_scratch_bytes(...) bytes give the library's split, with fewer the
  * splits get longer, and nt * nh * 1040 bytes are always enough (0 for pos0 = 0). Calls that overlap need one each. */
 size_t it_attn_tree_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv);
