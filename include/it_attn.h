@@ -513,8 +513,12 @@ int it_kv_tree_commit_f32(float* kc, float* vc, int kvd, int pos0, int nt, const
  *   anc: bits after t and a node whose own bit is clear (padding: zeros out) are ignored
  *   out [t*out_tok_stride + h*S + j], as it_gdn_step's
  *   trace: it_gdn_tree_trace_bytes(...) bytes, 16-byte aligned, one per layer: what it_gdn_tree_commit needs
- * f32 throughout (the decays of a path are summed in f64). A node's result does not depend on nodes that are not its
- * ancestors, whatever their inputs hold. */
+ * Accuracy: the normalised q and k rows (each at length 1) and the state's columns (each scaled by a power of two) go into the
+ * products as pairs of f16, 22 bits of a value that is not far below its row's or column's largest; sums, solve and
+ * updates are f32, the decays of a path summed in f64; SiLU, norms and gates take the hardware's exponential, logarithm, root and
+ * reciprocal (about 2^-23 each). The k rows that the trace keeps for the commit are the 22-bit ones. Outputs and committed states
+ * are about 3e-7 off relative to their size (normal inputs), 2 to 2.5 times an f32 computation's error. A node's result does
+ * not depend on nodes that are not its ancestors, whatever their inputs hold. */
 size_t it_gdn_tree_trace_bytes(int nt, int nv, int nk, int S);
 int it_gdn_tree(const float* x, int x_tok_stride, const float* w, int K, const float* conv_state,
                 const float* beta_raw, const float* alpha_raw, int ba_tok_stride, const float* dt, const float* a,
