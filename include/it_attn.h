@@ -80,7 +80,8 @@ int it_attn_prep_f16_q16(float* q, int q_tok_stride, const float* k, const float
  *   n_rot  : rotated dims per head, even, <= hd. layout IT_ROPE_HALVES: dims (i, i + n_rot/2) turn together, n_rot a
  *            multiple of hd/32; IT_ROPE_PAIRS: dims (2i, 2i + 1).
  *   freq   : device f32 [n_rot/2], the angle of pair i per position (it_rope_freqs makes the usual ones; 0 leaves a
- *            pair as it is). The angle pos * freq[i] is exact in f64 before it is reduced.
+ *            pair as it is). The angle pos * freq[i] is formed and reduced in f64: exact up to |pos| = 2^29, rounded to
+ *            53 bits beyond (2^-22 of a radian at 2^31 for frequencies up to 1).
  *   mscale : factor of cos and sin (1 but for stretched contexts).
  * The rest as for it_attn_prep_f16 / it_attn_prep_f32kv (q rewritten in place, the gates left as they are). No
  * counterpart in the reference, whose positions are pos0 + t and whose rotation is the model's. */
@@ -101,7 +102,8 @@ int it_attn_prep_pos_f32kv(float* q, int q_tok_stride, const float* k, const flo
  *   IT_ROPE_NTK    : the base times factor^(n_rot/(n_rot-2)), so the slowest pair is stretched by factor and the
  *                    fastest kept.
  *   IT_ROPE_YARN   : pairs of more than 32 turns over orig_ctx positions kept, those of less than one stretched by
- *                    factor, a linear blend between; *mscale = 0.1 ln(factor) + 1.
+ *                    factor, a linear blend between (its ends rounded outwards to whole pairs, the first pair at
+ *                    least); *mscale = 0.1 ln(factor) + 1.
  * *mscale is 1 for the others. */
 #define IT_ROPE_PLAIN 0
 #define IT_ROPE_LINEAR 1

@@ -210,7 +210,8 @@ hipError_t launch_attn_prep_f32kv(float* q, int qts, const float* k, const float
 
 // The same pass with the rotation given from outside: token t at position pos[t] (or pos0 + t), pair i
 // turning by position * freq[i], cos and sin times mscale, the pairs in halves or interleaved; K and V to
-// cache row row0 + t. The angle is the f64 product of an integer and an f32, so exact before it is reduced.
+// cache row row0 + t. The angle is the f64 product of an integer and an f32: exact before it is reduced up to
+// |pos| = 2^29 (53 bits); product and reduction are within 2^-22 of a radian up to 2^31 for frequencies up to 1.
 // Workgroups and rows as in attn_prep_kernel. Bound by the bytes from some hundred tokens on: 8192 tokens, 16/2 heads 62 us
 // = 5.14 TB/s, the rate of a large copy; one token 3.2 us, 37 tokens 24/4 heads 3.1.
 template <int E, class KVT, bool PAIRS>
