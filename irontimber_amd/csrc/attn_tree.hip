@@ -32,9 +32,13 @@ constexpr float LN2_F = 0.6931471805599453f;
 // f32 records keep f32's accuracy. A tile takes a wave 64 matrix ops of 32 cycles.
 // Splitting rows and keys between the waves halves what a wave reads from LDS against four waves of 16 rows: 1024
 // cycles of LDS a tile and workgroup beside 2048 of the matrix cores.
-// Measured, 64 nodes, 16/2 heads: 131072 keys 237-266 us = 1.04-1.16 PFLOP/s of matrix work (the pairs double the 137.5
-// GFLOP of the call; a large f16 product runs at 1.15 here: the card's power bounds both), 8128 keys 25.7 us: eight tiles of
-// 1.6 us, and 10 us at the ends (q 2 us, its conversion 1, the first tile 2, the join of the key halves 2.4, the records 2).
+// Measured, 64 nodes, 16/2 heads: 131072 keys 236-272 us = 1.01-1.17 PFLOP/s of matrix work (the pairs double the 137.5
+// GFLOP of the call; a large f16 product runs at 1.15 here). 2 / 4 / 8 / 16 / 32 / 128 tiles a workgroup take 17.3 / 20.0 / 26.4 /
+// 38.7 / 67.7 / 245 us at best: 1.5 us a tile in short runs, 1.85 in long ones, and 14 us beside the tiles (in the workgroup q 2,
+// its conversion 1.2, the first tile 2, the join of the key halves 2.4, the records 2; the rest outside it). For its 2,048 cycles
+// of matrix ops a tile takes 2,700 cycles in short runs and 3,240 in long ones, where the clock falls to 1.75 GHz; what the
+// cycles without a matrix op are is not known (without its loads, exponentials, operand reads or rescaling a tile is 3 %
+// shorter each).
 __global__ __launch_bounds__(256) void attn_tree_ctx_kernel(const float* __restrict__ q, int qts,
                                                             const uint16_t* __restrict__ kc,
                                                             const uint16_t* __restrict__ vc, int kvd, int n, int nh,
