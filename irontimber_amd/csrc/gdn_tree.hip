@@ -53,7 +53,7 @@ __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466
 // Workgroup = (V head h, CW = 16 or 32 state columns), NW waves; NB blocks of 16 nodes. A head's q and k rows are
 // convolved and normalised by each of its eight or four workgroups (into LDS), so no launch or barrier of the whole GPU
 // stands between the conv and the products. The inputs of the convs go into LDS first, where each node takes its
-// ancestors' rows, and the results take their place. The normalised rows, at most 1, and the state's columns, scaled, are
+// ancestors' rows, and the results take their place. The normalised rows, at length 1, and the state's columns, scaled, are
 // kept as f16 pairs hi + lo (2^-22), and their products take three f16 matrix ops of 16 cycles for 32 dims (hi hi, hi lo,
 // lo hi) where f32 ones would take eight of 32. The waves share the products out by blocks of rows; the inverses of I + A's
 // diagonal blocks go one to a wave, and then each of the first NB waves (a block of columns: NB) solves for all of U in
