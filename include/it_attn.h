@@ -501,7 +501,8 @@ int it_attn_tree_f32kv(const float* q, int q_tok_stride, const float* kc, const 
 
 /* Keeps the path of node `leaf` in a cache whose rows pos0 + t hold the nodes: row pos0 + i <- row pos0 + path[i], path
  * the nodes of anc[leaf] in order (in place; the rows after the path keep what they hold). leaf = -1, or a padding
- * node (its own bit is clear): nothing is kept and nothing moves. kvd a multiple of 8, kc and vc 16-byte aligned. */
+ * node (its own bit is clear): nothing is kept and nothing moves. kvd a multiple of 8, kc and vc 16-byte aligned and not the
+ * same rows (both are moved at once). */
 int it_kv_tree_commit_f16(uint16_t* kc, uint16_t* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,
                           void* stream);
 int it_kv_tree_commit_f32(float* kc, float* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,

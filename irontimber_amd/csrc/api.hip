@@ -500,6 +500,7 @@ static int kv_tree_commit(const char* who, void* kc, void* vc, int kvd, size_t s
     if (!kc || !vc || !anc) return fail("%s: null buffer", who);
     if (!aligned16(kc) || !aligned16(vc)) return fail("%s: kc/vc must be 16-byte aligned", who);
     if (leaf < 0) { g_err.clear(); return 0; }
+    if (kc == vc) return fail("%s: kc and vc must be two caches", who);   // (both are moved at once)
     return check(it::launch_kv_tree_commit(kc, vc, (size_t)kvd * size, pos0, anc, leaf, (hipStream_t)stream), who);
 }
 int it_kv_tree_commit_f16(uint16_t* kc, uint16_t* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,
