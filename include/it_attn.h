@@ -535,6 +535,80 @@ int it_gdn_tree_commit(const float* x, int x_tok_stride, int K, float* conv_stat
                        int leaf, int nt, int nv, int nk, int S, const void* trace, size_t trace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * A paged K/V cache in 8 bits, for several sequences or one with a long context, in half the bytes of the f16 cache. No
+ * counterpart in the reference, whose cache is one f16 array for one sequence (src/vk/mod.rs:551-554). A step:
+ *   it_attn_prep_pos_f16   K and V of the new tokens into f16 rows (a staging buffer as its cache, row0 = 0)
+ *   it_kv8_append          those rows into the cache                    (it_kv_append_f16)
+ *   it_attn_kv8            attention of the new tokens                  (it_attn_f16)
+ * The lengths and page tables are on the device, so that a captured step is replayed as they advance: the calls read len,
+ * the caller adds the tokens that it keeps.
+ *
+ * Rows: a page holds IT_KV8_PAGE rows of all KV heads. Row r of a sequence is in page table[seq][r / 64]. While a sequence
+ * holds `total` rows, the pages that are full, those before total / 64, are 8-bit codes, and the rows after them (at most
+ * 63) are f16 in the sequence's open buffer, which keeps the rows of the last two pages: so up to 64 rows can be taken
+ * back by a smaller length alone (drafts that a check rejects), rows before that only to a page's end, or by reading the page's
+ * rows (it_kv8_read) and appending them anew.
+ * Codes: each IT_KV8_BLOCK rows of a KV head have a scale s for K and one for V: the largest size / 127, rounded up to four
+ * significant bits or to a multiple of 2^-24 (at least that). A value x is kept as code = 128 + x / s, rounded to the nearest, ties to
+ * even, and at most 127 from 128 (113 where s is above 512); it stands for (code - 128) * s, which is an f16 number. Appending makes
+ * values finite: an infinity becomes the largest f16, a NaN 0.
+ * Sharing: a table may name a page that another one names. The calls write only to pages that a sequence fills, those from
+ * len / 64 on, so pages before that can be shared (a common beginning, a fork); a fork takes the open rows with it
+ * (it_kv8_copy) and needs pages of its own from len / 64 on. A page that no table names is free; nothing in it needs to be cleared.
+ *
+ * Device arrays of a call, int32, for the cache's nseq sequences: start [nseq + 1], len [nseq], table [nseq][max_pages]. The
+ * call's tokens start[i] .. start[i+1]-1 are the next rows of sequence i after its len[i] rows; start[i] = start[i+1]: none.
+ * ntok: rows of the token arrays; max_nt: a bound of the tokens of one sequence (tokens beyond it are left out; it chooses the kernel, so
+ * give the true one). Tokens of no sequence (after start[nseq]) are left alone. A sequence whose bounds are not in 0 .. ntok has no
+ * tokens. One whose length is negative, or whose rows its table cannot name, is not appended to, and its
+ * outputs are NaN. A page number outside the pool is not written, and what reads it is NaN.
+ * ---------------------------------------------------------------------------------------------- */
+#define IT_KV8_PAGE 64
+#define IT_KV8_BLOCK 16
+
+/* The buffers (16-byte aligned) and sizes of a layer's cache; the struct itself is host memory, read during the call.
+ * Element of a page and KV head that holds (row, dim), in kp / vp (bytes) and tk / tv (f16) alike:
+ *   K: (((row/16 * hd/64 + dim/64) * 64 + dim/8 % 4 * 16 + row % 16) * 16 + dim/32 % 2 * 8 + dim % 8
+ *   V: (dim/16 * 64 + row/4 % 4 * 16 + dim % 16) * 16 + row/16 * 4 + row % 4 */
+typedef struct {
+    uint8_t *kp, *vp;     /* codes [npages][nkv][64*hd] */
+    uint16_t* sc;         /* f16 scales [npages][nkv][8]: K's four blocks, then V's */
+    uint16_t *tk, *tv;    /* open rows, f16 [nseq][2][nkv][64*hd], page p in half p % 2 */
+    int npages, nseq, nkv, hd;   /* hd 128 or 256 */
+} it_kv8_cache;
+
+/* Appends f16 rows: token t is k[t*tok_stride + kh*hd + d] (tok_stride a multiple of 8, 16-byte aligned), as the pre-pass leaves it.
+ * Sequences must not share a page that the call fills. */
+int it_kv8_append(const it_kv8_cache* cache, const uint16_t* k, const uint16_t* v, int tok_stride, int ntok,
+                  const int32_t* start, const int32_t* len, const int32_t* table, int max_pages, int max_nt,
+                  void* stream);
+
+/* Rows first[i] .. of each sequence, start[i+1] - start[i] of them (at most max_rows), as f16 into rows start[i] .. of k and
+ * v; total[i]: the rows that the sequence holds (rows at or after total are not written). */
+int it_kv8_read(const it_kv8_cache* cache, uint16_t* k, uint16_t* v, int tok_stride, int ntok, const int32_t* start,
+                const int32_t* first, const int32_t* total, const int32_t* table, int max_pages, int max_rows,
+                void* stream);
+
+/* Copies pages src[i] to dst[i], i < n, and the open rows of sequences seq_src[i] to seq_dst[i], i < nseq, in one launch (either count
+ * may be 0): for forks, and to make a pool dense (the caller renames the pages in its tables). All copies run at
+ * once: destinations differ from each other and from every source. A number outside the cache is skipped. */
+int it_kv8_copy(const it_kv8_cache* cache, const int32_t* src, const int32_t* dst, int n, const int32_t* seq_src,
+                const int32_t* seq_dst, int nseq, void* stream);
+
+/* Causal GQA attention with sigmoid gate over the cache, of tokens whose rows have been appended: token t of sequence i sees
+ * its rows 0 .. len[i] + t. q as for it_attn_f16 (query | gate per head), out [t*out_tok_stride + h*hd + d] in f32, or f16 where
+ * out_f16 is nonzero. One token a sequence, a few (drafts), or prompts of any lengths, mixed.
+ * Accuracy: the softmax's sums and the products' sums are f32, K and V exact as stored. For an f32 output q and the probabilities go
+ * into the products as f16 pairs: q to 2^-22 of a value or 2^-39 of its row's largest, a probability to 2^-22 of itself or, where
+ * it is small, 2^-31 of its row's largest up to there (2^-25 once, if a later key outweighs all before it by less than 2^8). For an f16
+ * output both are one f16 (2^-12), about 3e-4 of the result beside the output's own rounding.
+ * scratch: it_attn_kv8_scratch_bytes bytes, 16-byte aligned (one per call that may overlap another). */
+size_t it_attn_kv8_scratch_bytes(int max_nt, int hd, int nh, int nkv);
+int it_attn_kv8(const it_kv8_cache* cache, const float* q, int q_tok_stride, int ntok, const int32_t* start,
+                const int32_t* len, const int32_t* table, int max_pages, int max_nt, int nh, float scale, void* out,
+                int out_tok_stride, int out_f16, void* scratch, size_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Reference-shaped dispatch policy (pure host functions, no device access).
  * ---------------------------------------------------------------------------------------------- */
 

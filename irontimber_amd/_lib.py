@@ -90,8 +90,19 @@ SIGNATURES = {
     "it_gdn_tree_commit": (c_int, [P, c_int, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_size_t, P]),
     "it_kv_tree_commit_f16": (c_int, [P, P, c_int, c_int, c_int, P, c_int, P]),
     "it_kv_tree_commit_f32": (c_int, [P, P, c_int, c_int, c_int, P, c_int, P]),
+    "it_kv8_append": (c_int, [P, P, P, c_int, c_int, P, P, P, c_int, c_int, P]),
+    "it_kv8_read": (c_int, [P, P, P, c_int, c_int, P, P, P, P, c_int, c_int, P]),
+    "it_kv8_copy": (c_int, [P, P, P, c_int, P, P, c_int, P]),
+    "it_attn_kv8_scratch_bytes": (c_size_t, [c_int] * 4),
+    "it_attn_kv8": (c_int, [P, P, c_int, c_int, P, P, P, c_int, c_int, c_int, c_float, P, c_int, c_int, P, c_size_t, P]),
     "it_prefill_chunks": (ctypes.c_long, [c_size_t, c_size_t, P, P, c_size_t]),
 }
+
+
+class Kv8CacheArgs(ctypes.Structure):
+    """it_kv8_cache"""
+    _fields_ = [("kp", P), ("vp", P), ("sc", P), ("tk", P), ("tv", P), ("npages", c_int), ("nseq", c_int),
+                ("nkv", c_int), ("hd", c_int)]
 
 
 class ItError(RuntimeError):

@@ -12,6 +12,7 @@
 #include <cstdarg>
 #include "../../include/it_attn.h"
 #include "internal.h"
+#include "kv8.h"
 
 namespace {
 
@@ -510,6 +511,92 @@ int it_kv_tree_commit_f16(uint16_t* kc, uint16_t* vc, int kvd, int pos0, int nt,
 int it_kv_tree_commit_f32(float* kc, float* vc, int kvd, int pos0, int nt, const uint64_t* anc, int leaf,
                           void* stream) {
     return kv_tree_commit("it_kv_tree_commit_f32", kc, vc, kvd, 4, pos0, nt, anc, leaf, stream);
+}
+
+// ---- the paged 8-bit cache
+static int validate_kv8(const char* who, const it_kv8_cache* c, it::Kv8* to) {
+    if (!c) return fail("%s: null cache", who);
+    if (c->hd != 128 && c->hd != 256) return fail("%s: head_dim %d unsupported (128 or 256)", who, c->hd);
+    if (c->nkv < 1 || c->nkv > 1024) return fail("%s: n_head_kv %d must be in [1, 1024]", who, c->nkv);
+    if (c->npages < 1) return fail("%s: %d pages", who, c->npages);
+    if (c->nseq < 1 || c->nseq > 65535) return fail("%s: nseq %d must be in [1, 65535]", who, c->nseq);
+    if (!c->kp || !c->vp || !c->sc || !c->tk || !c->tv) return fail("%s: null buffer in the cache", who);
+    if (!aligned16(c->kp) || !aligned16(c->vp) || !aligned16(c->sc) || !aligned16(c->tk) || !aligned16(c->tv))
+        return fail("%s: the cache's buffers must be 16-byte aligned", who);
+    *to = {c->kp, c->vp, (_Float16*)c->sc, (_Float16*)c->tk, (_Float16*)c->tv, c->npages, c->nseq, c->nkv, c->hd};
+    return 0;
+}
+static int validate_kv8_batch(const char* who, const it_kv8_cache* c, int ntok, const int32_t* start, const int32_t* len,
+                              const int32_t* table, int max_pages, int max_nt, it::Kv8Batch* to) {
+    if (ntok < 1) return fail("%s: ntok %d must be positive", who, ntok);
+    if (max_nt < 1) return fail("%s: a bound of %d tokens a sequence", who, max_nt);
+    if (max_pages < 1 || max_pages >= (1 << 25)) return fail("%s: max_pages %d must be in [1, 2^25)", who, max_pages);
+    if (!start || !len || !table) return fail("%s: null buffer", who);
+    *to = {start, len, table, c->nseq, ntok, max_pages, std::min(max_nt, ntok)};
+    return 0;
+}
+// f16 rows of K and V on the caller's side
+static int validate_kv8_rows(const char* who, const it_kv8_cache* c, const uint16_t* k, const uint16_t* v, int kts, int ntok) {
+    if (!k || !v) return fail("%s: null buffer", who);
+    if (!aligned16(k) || !aligned16(v) || kts % 8 != 0) return fail("%s: k/v must be 16-byte aligned, their stride a multiple of 8", who);
+    if (kts < 0 || (ntok > 1 && kts < c->nkv * c->hd)) return fail("%s: token strides overlap rows", who);
+    return 0;
+}
+int it_kv8_append(const it_kv8_cache* cache, const uint16_t* k, const uint16_t* v, int kts, int ntok, const int32_t* start,
+                  const int32_t* len, const int32_t* table, int max_pages, int max_nt, void* stream) {
+    const char* who = "it_kv8_append";
+    it::Kv8 c;
+    it::Kv8Batch b;
+    if (validate_kv8(who, cache, &c) || validate_kv8_batch(who, cache, ntok, start, len, table, max_pages, max_nt, &b) ||
+        validate_kv8_rows(who, cache, k, v, kts, ntok))
+        return -1;
+    return check(it::launch_kv8_append(c, b, k, v, kts, (hipStream_t)stream), who);
+}
+int it_kv8_read(const it_kv8_cache* cache, uint16_t* k, uint16_t* v, int kts, int ntok, const int32_t* start,
+                const int32_t* first, const int32_t* total, const int32_t* table, int max_pages, int max_rows,
+                void* stream) {
+    const char* who = "it_kv8_read";
+    it::Kv8 c;
+    it::Kv8Batch b;
+    if (validate_kv8(who, cache, &c) || validate_kv8_batch(who, cache, ntok, start, total, table, max_pages, max_rows, &b) ||
+        validate_kv8_rows(who, cache, k, v, kts, ntok))
+        return -1;
+    if (!first) return fail("%s: null buffer", who);
+    if (k == v) return fail("%s: k and v must be two buffers", who);
+    return check(it::launch_kv8_read(c, b, first, k, v, kts, (hipStream_t)stream), who);
+}
+int it_kv8_copy(const it_kv8_cache* cache, const int32_t* src, const int32_t* dst, int n, const int32_t* seq_src,
+                const int32_t* seq_dst, int nseq, void* stream) {
+    const char* who = "it_kv8_copy";
+    it::Kv8 c;
+    if (validate_kv8(who, cache, &c)) return -1;
+    if (n < 0 || n > c.npages) return fail("%s: %d page copies must be in [0, %d]", who, n, c.npages);
+    if (nseq < 0 || nseq > c.nseq) return fail("%s: %d sequence copies must be in [0, %d]", who, nseq, c.nseq);
+    if ((n && (!src || !dst)) || (nseq && (!seq_src || !seq_dst))) return fail("%s: null buffer", who);
+    if (((long)n * 2 + (long)nseq * 4) * c.nkv > INT32_MAX) return fail("%s: more copies than a launch holds", who);
+    return check(it::launch_kv8_copy(c, src, dst, n, seq_src, seq_dst, nseq, (hipStream_t)stream), who);
+}
+size_t it_attn_kv8_scratch_bytes(int max_nt, int hd, int nh, int nkv) {
+    if (max_nt < 1 || (hd != 128 && hd != 256) || nh < 1 || nkv < 1 || nh % nkv) return 0;
+    return it::attn_kv8_scratch_bytes(max_nt, hd, nh, nkv);
+}
+int it_attn_kv8(const it_kv8_cache* cache, const float* q, int qts, int ntok, const int32_t* start, const int32_t* len,
+                const int32_t* table, int max_pages, int max_nt, int nh, float scale, void* out, int ots, int out_f16,
+                void* scratch, size_t scratch_bytes, void* stream) {
+    const char* who = "it_attn_kv8";
+    it::Kv8 c;
+    it::Kv8Batch b;
+    if (validate_kv8(who, cache, &c) || validate_kv8_batch(who, cache, ntok, start, len, table, max_pages, max_nt, &b)) return -1;
+    if (nh < 1 || nh % c.nkv != 0) return fail("%s: n_head %d / n_head_kv %d invalid", who, nh, c.nkv);
+    if ((long)ntok * nh > (1L << 26)) return fail("%s: %d tokens of %d heads are more than 2^26 rows", who, ntok, nh);
+    if (!q || !out) return fail("%s: null buffer", who);
+    if (!aligned16(q) || !aligned16(out)) return fail("%s: q/out must be 16-byte aligned", who);
+    if (qts % 4 != 0 || ots % (out_f16 ? 8 : 4) != 0) return fail("%s: token strides must be multiples of 16 bytes", who);
+    if (qts < 0 || ots < 0 || (ntok > 1 && (qts < 2 * nh * c.hd || ots < nh * c.hd))) return fail("%s: token strides overlap rows", who);
+    const size_t need = it::attn_kv8_scratch_bytes(b.max_nt, c.hd, nh, c.nkv);
+    if (!scratch || !aligned16(scratch) || scratch_bytes < need)
+        return fail("%s: scratch of %zu bytes, %zu needed (16-byte aligned)", who, scratch ? scratch_bytes : 0, need);
+    return check(it::launch_attn_kv8(c, b, q, qts, nh, scale, out, ots, out_f16 != 0, (float*)scratch, (hipStream_t)stream), who);
 }
 
 size_t it_attn_f32kv_scratch_bytes(int pos0, int nt, int hd, int nh, int nkv) {

@@ -1,0 +1,604 @@
+// Causal GQA attention with sigmoid gate over the paged 8-bit cache, for one token a sequence up to whole prompts:
+//   out = sigmoid(gate) * sum_j p_j v_j / sum_j p_j,  p_j = e^(scale q.k_j), j <= len + t.
+//
+// A unit of work is (sequence, KV head, block of ROWS query rows r = t*G + g, split of the pages). Its workgroup takes a
+// page a step, the four waves sharing it:
+//   S^T = K q^T    wave w has the page's block w: 16 keys, all query rows
+//   softmax        running reference per row, common to the waves (their maxima meet in LDS)
+//   O^T += V^T P^T wave w has a quarter of the dims, all 64 keys and rows; P^T comes through LDS
+// K and V never pass through LDS: the page's element order is that of the matrix operands, so each code goes from memory into
+// the registers of the one wave that needs it and is converted there, once a workgroup. The products use f16 operands:
+// K and V are f16 numbers exactly (kv8.hip); q and P go in as f16 pairs hi + lo, 22 bits, for an f32 output, and as
+// one f16 each for an f16 output.
+// One barrier a page: P of page j and the maxima of page j + 1 are written before it and read behind it.
+//
+// The lengths are on the device, so every workgroup finds its unit by itself: pages per split from the total work, a prefix sum over
+// the sequences' unit counts. Sequences of one split are finished in place, the others' records {m, l, o} are joined by
+// the second kernel.
+#include <algorithm>
+
+#include "internal.h"
+#include "kv8.h"
+
+namespace it {
+namespace {
+
+constexpr float P_BITS = 7.0f;   // weights up to 2^15 of the reference: see `settle`
+
+// The loads that copy a wave's share of a page from memory into LDS stay in flight over barriers and other loads' waits, so they and
+// their waits are written out (the compiler waits for all of them at every barrier). They have no result register; LDS is
+// read behind `landed`.
+//
+// A barrier that orders LDS traffic only.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// Waits until at most N loads are still in flight; they land in the order that they were issued in.
+template <int N> __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// N KiB from `from` (each lane 16 bytes at off + 1024 i) to LDS from `to` on (lane l at 16 l + 1024 i: the instruction's offset
+// counts on both sides). What stood there has been read when they go out. m0 holds the LDS address; nothing else here uses it.
+template <int N> __device__ __forceinline__ void kib_to_lds(const uint8_t* from, unsigned off, uint8_t* to) {
+    typedef __attribute__((address_space(3))) uint8_t lds_u8;
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_u8*)to);
+    static_assert(N == 2 || N == 4, "a quarter of a page");
+    if constexpr (N == 4)
+        asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\t"
+                     "global_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %1, %2 offset:2048\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072"
+                     ::"s"(at), "v"(off), "s"(from) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\t"
+                     "global_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                     ::"s"(at), "v"(off), "s"(from) : "memory");
+}
+__device__ __forceinline__ int prefix_sum(int v, int l) {   // inclusive, over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int u = __shfl_up(v, d);
+        v += l >= d ? u : 0;
+    }
+    return v;
+}
+
+// Pages per split of this call (the same in both kernels; sums in a fixed order)
+template <int ROWS>
+__device__ __forceinline__ int call_chunk(const Kv8Batch& b, const Kv8Seq& s0, int G, int nkv, int wgs, int l) {
+    float sum = 0.f;
+    for (int i0 = 0; i0 < b.nseq; i0 += 64) {
+        const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
+        sum += wave_sum((float)((s.n * G + ROWS - 1) / ROWS) * (float)s.pages);
+    }
+    return kv8::chunk_pages(__builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sum))) * (float)nkv, wgs);
+}
+
+// What is found for a workgroup, in scalar registers: its sequence, the index of its unit (main kernel) or of its group of
+// rows that were split (merge), and the first record of the sequence.
+struct Found {
+    int seq, t0, n, len, pages, nrb, ns, at, rec;
+    bool any, bad;
+};
+template <int ROWS, bool GROUPS>
+__device__ __forceinline__ Found find(const Kv8Batch& b, const Kv8Seq& s0, int G, int nkv, int chunk, int id, int l) {
+    Found f;
+    f.any = false;
+    int base = 0, rbase = 0;
+    for (int i0 = 0; i0 < b.nseq; i0 += 64) {
+        const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
+        const int nrb = (s.n * G + ROWS - 1) / ROWS, ns = kv8::splits(s.pages, chunk);
+        const int recs = ns > 1 ? nrb * ns * nkv : 0, units = GROUPS ? (ns > 1 ? nrb * nkv : 0) : nrb * ns * nkv;
+        const int pu = prefix_sum(units, l), pr = prefix_sum(recs, l);
+        const unsigned long long hit = __ballot(base + pu > id);
+        if (hit) {
+            const int src = __builtin_ctzll(hit);
+            f.seq = i0 + src;
+            f.t0 = __builtin_amdgcn_readlane(s.t0, src);
+            f.n = __builtin_amdgcn_readlane(s.n, src);
+            f.len = __builtin_amdgcn_readlane(s.len, src);
+            f.pages = __builtin_amdgcn_readlane(s.pages, src);
+            f.bad = __builtin_amdgcn_readlane((int)s.bad, src) != 0;
+            f.nrb = __builtin_amdgcn_readlane(nrb, src);
+            f.ns = __builtin_amdgcn_readlane(ns, src);
+            f.at = id - base - __builtin_amdgcn_readlane(pu - units, src);
+            f.rec = rbase + __builtin_amdgcn_readlane(pr - recs, src);
+            f.any = true;
+            return f;
+        }
+        base += __builtin_amdgcn_readlane(pu, 63);
+        rbase += __builtin_amdgcn_readlane(pr, 63);
+    }
+    return f;
+}
+
+__device__ __forceinline__ void store4(float* p, f4 v) { *(f4*)p = v; }
+__device__ __forceinline__ void store4(_Float16* p, f4 v) { st4(p, v); }
+
+typedef int i4 __attribute__((ext_vector_type(4)));
+// D = A(16x64) B(64x16) + C in 8-bit integers; lane l holds A row / B column l & 15 with 16 consecutive bytes of the group l >> 4,
+// D as mfma16x16x32's.
+__device__ __forceinline__ i4 mfma_i8(u4 a, u4 b, i4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, a), __builtin_bit_cast(i4, b), c, 0, 0, 0);
+}
+// Byte k of four words, as a word each.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int k) {
+    const uint32_t pair = 0x04000400u + 0x0101u * k * 0x10001u;   // per 16 bits: byte k of the second, byte k of the first
+    const uint32_t ab = __builtin_amdgcn_perm(b, a, pair), cd = __builtin_amdgcn_perm(d, c, pair);
+    return __builtin_amdgcn_perm(cd, ab, 0x05040100u);
+}
+
+// Records: {m, l} [record][ROWS] (m in log2 units), then o [record][ROWS][HD].
+template <int HD, int RB, bool PAIRS, class OutT>
+__global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q,
+                                                                        int qts, int nh, float scale,
+                                                                        OutT* __restrict__ out, int ots,
+                                                                        float* __restrict__ part, int wgs) {
+    constexpr int ROWS = 16 * RB, NP = PAIRS ? 2 : 1, NJ = HD / 64, NK = HD / 32, ND = HD / 64, DG = PAIRS ? 3 : 2;
+    constexpr int KIB = 1024, QUARTER = 16 * HD;   // a wave's share of a page's codes
+    __shared__ __align__(16) uint8_t kbuf[4 * QUARTER], vbuf0[4 * QUARTER], vbuf1[4 * QUARTER];
+    __shared__ __align__(16) _Float16 pbuf[2][RB][2][NP][64 * 8];   // P^T operands: [parity][rows][keys][hi, lo]
+    __shared__ __align__(16) float mbuf[2][ROWS][4];                // row maxima by wave
+    __shared__ __align__(16) float lbuf[ROWS][4];
+
+    const int nkv = c.nkv, G = nh / nkv;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, lr = l & 15;
+    const Kv8Seq s0 = kv8_seq(b, l);
+    const int chunk = call_chunk<ROWS>(b, s0, G, nkv, wgs, l);
+    const Found u = find<ROWS, false>(b, s0, G, nkv, chunk, (int)blockIdx.x, l);
+    if (!u.any) return;
+    // the heaviest row blocks first; row blocks and heads of a split side by side
+    const int kh = u.at % nkv, rest = u.at / nkv, rb = u.nrb - 1 - rest % u.nrb, split = rest / u.nrb;
+    const int R = u.n * G, r0 = rb * ROWS;
+
+    // ---- this lane's query rows (one per 16-row block) and the keys they see
+    int qlim[RB];
+    const float* qrow[RB];
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+        const int r = min(r0 + 16 * x + lr, R - 1), t = r / G;
+        qlim[x] = r0 + 16 * x + lr < R ? u.len + t : -1;
+        qrow[x] = q + (size_t)(u.t0 + t) * qts + (size_t)(kh * G + r - t * G) * 2 * HD;
+    }
+    if (u.bad) {   // a sequence whose length cannot be: NaN
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+            const int r = r0 + 16 * x + lr, t = r / G;
+            if (r < R)
+                for (int d = 4 * (l >> 4) + 16 * w; d < HD; d += 64)
+                    store4(out + (size_t)(u.t0 + t) * ots + (size_t)(kh * G + r - t * G) * HD + d, f4{NAN, NAN, NAN, NAN});
+        }
+        return;
+    }
+    const int tmin = r0 / G, tmax = (min(R, r0 + ROWS) - 1) / G;
+    const int total = u.len + u.n, closed = total / kv8::PAGE;          // full pages; the open rows are page `closed`
+    const int p0 = (int)min((long)split * chunk, (long)u.pages);
+    const int p1 = (int)min((long)p0 + chunk, (long)(u.len + tmax) / kv8::PAGE + 1);
+    const bool tail = p1 > closed && p1 > p0;                            // the last page of the range is the open one
+    const int np = max(min(p1, closed) - p0, 0);                         // full pages of the range
+    const int clear = u.len + tmin;                                      // keys up to here are seen by every row
+    if (u.ns > 1 && np == 0 && !tail) return;   // no row of the block sees the split: its record is not read
+
+    // ---- pages. Lane i of `ids` and `scl` has the number and the scales of full page 64 n + i of the range; each is read
+    // anew every 64 pages, with its wait in the branch (no other load then waits for it). A page that the pool has not: NaN scores.
+    const int* table = b.table + (size_t)u.seq * b.max_pages + p0;
+    int ids = 0;
+    u4 scl = {};
+    auto load_ids = [&](int j) __attribute__((always_inline)) {
+        ids = table[min(j + l, max(np - 1, 0))];
+        asm volatile("" : "+v"(ids));
+    };
+    auto load_scales = [&]() __attribute__((always_inline)) {
+        const bool known = (unsigned)ids < (unsigned)c.npages;
+        scl = *(const u4*)(c.sc + (known ? (size_t)ids * nkv + kh : 0) * 8);
+        if (!known) scl = u4{0x7E007E00u, 0x7E007E00u, 0u, 0u};
+        asm volatile("" : "+v"(scl));
+    };
+    // This wave's quarter of a page's codes, K by block or V by dims, to LDS in the order that it is read back by the
+    // same wave. Past the end (the loads go out without a branch, so that their count is known): one piece for all lanes.
+    auto fetch = [&](const uint8_t* from, uint8_t* to, int j) __attribute__((always_inline)) {
+        const unsigned one = __builtin_amdgcn_readlane(ids, j & 63), id = one < (unsigned)c.npages ? one : 0;
+        kib_to_lds<NJ>(from + uniform_off(((size_t)id * nkv + kh) * (kv8::PAGE * HD) + w * QUARTER), j < np ? 16 * l : 0,
+                       to + w * QUARTER);
+    };
+
+    if (np > 0) {
+        load_ids(0);
+        load_scales();
+        fetch(c.kp, kbuf, 0);
+        fetch(c.vp, vbuf0, 0);
+    }
+
+    f4 o[RB][ND], sc[RB];
+    float m_run[RB], l_run[RB], back[RB];   // back: from integer products to log2 units
+    u4 qd[RB][NJ][DG];                      // q's digits, the highest first
+    const float neg1 = in_register(-1.0f);
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[x][d] = f4{};
+        m_run[x] = -INFINITY;
+        l_run[x] = 0.f;
+    }
+
+    // Masks scores of page p (block w: this lane's keys are 16 w + 4 g + 0..3) and puts their maxima to LDS
+    auto finish = [&](int x, int p, int par, bool mask) __attribute__((always_inline)) {
+        if (mask) {
+            const int key = p * kv8::PAGE + 16 * w + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (key + i > qlim[x]) sc[x][i] = -INFINITY;
+        }
+        const float m = max_xor32(max_xor16(fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3]))));
+        if (l < 16) mbuf[par][16 * x + l][w] = m;
+    };
+
+    // ---- q. The open page's keys are f16, so its products take q as f16 pairs (each row times the power of two that takes its
+    // largest value to 2^13 .. 2^14). The codes' products are integer ones: q in units of its largest value / 2^(8 DG - 1),
+    // as DG signed digits of 8 bits.
+    const size_t open = ((size_t)(u.seq * 2 + (closed & 1)) * nkv + kh) * (kv8::PAGE * HD) + w * QUARTER + 16 * l;
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+        f4 y[NK][2];
+        uint32_t mb = 0;
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+            y[ks][0] = ld_f4(qrow[x] + 32 * ks + 8 * g);
+            y[ks][1] = ld_f4(qrow[x] + 32 * ks + 8 * g + 4);
+        }
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float e = y[ks][i >> 2][i & 3];   // (a bit cast of the vector's element itself takes the first)
+                mb = max(mb, __builtin_bit_cast(uint32_t, e) & 0x7FFFFFFFu);
+            }
+        float m = __builtin_bit_cast(float, min(mb, 0x7F800000u));   // (infinity for a NaN)
+        m = max_xor32(max_xor16(m));
+        const int ex = max(__builtin_amdgcn_frexp_expf(m), -100);   // (so that 2^-ex is finite)
+        const bool fine = m < INFINITY;
+        if (tail) {
+            const float f = fine ? __builtin_amdgcn_ldexpf(scale * LOG2E, ex - 14) : NAN;
+            f4 a = {}, a2 = {};
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                const h8 k = ld_h8(c.tk + open + KIB * (ks >> 1) + 8 * (ks & 1));
+                h8 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    h2 h, r;
+                    split2(f2{__builtin_amdgcn_ldexpf(y[ks][i >> 1][2 * (i & 1)], 14 - ex),
+                              __builtin_amdgcn_ldexpf(y[ks][i >> 1][2 * (i & 1) + 1], 14 - ex)}, neg1, h, r);
+                    hi[2 * i] = h[0];
+                    hi[2 * i + 1] = h[1];
+                    lo[2 * i] = r[0];
+                    lo[2 * i + 1] = r[1];
+                }
+                a = mfma16x16x32(k, hi, a);
+                a2 = mfma16x16x32(k, lo, a2);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[x][i] = (a[i] + a2[i]) * f;
+            finish(x, closed, 0, true);
+        }
+        // |q| / 2^ex < 1; the highest digit at most 127 for all digits' roundings
+        constexpr float TOP = PAIRS ? 127 * 65536.f : 127 * 256.f;
+        constexpr uint32_t BIAS = PAIRS ? 0x808080u : 0x8080u;
+        const float to = __builtin_amdgcn_ldexpf(TOP, -ex);
+        back[x] = fine ? __builtin_amdgcn_ldexpf(scale * LOG2E / TOP, ex) : NAN;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t n[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)   // the digits: bytes of n + BIAS, each less 128
+                    n[i] = ((uint32_t)(int)rintf(y[2 * j + (e >> 1)][e & 1][i] * to) + BIAS) ^ BIAS;
+#pragma unroll
+                for (int k = 0; k < DG; ++k) qd[x][j][k][e] = bytes_of(n[0], n[1], n[2], n[3], DG - 1 - k);
+            }
+    }
+
+    // Scores of the wave's 16 keys of full page j, all rows
+    auto scores = [&](int j, int par, bool mask) __attribute__((always_inline)) {
+        const h2 two = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(w & 2 ? scl[1] : scl[0], j & 63));
+        const float ksc = (float)two[w & 1];
+        landed<NJ>();   // (V of page j may be under way)
+        u4 k[NJ];
+#pragma unroll
+        for (int i = 0; i < NJ; ++i) k[i] = *(const u4*)(kbuf + w * QUARTER + KIB * i + 16 * l) ^ 0x80808080u;   // signed
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+            i4 a[DG];
+#pragma unroll
+            for (int d = 0; d < DG; ++d) a[d] = i4{};
+#pragma unroll
+            for (int i = 0; i < NJ; ++i)
+#pragma unroll
+                for (int d = 0; d < DG; ++d) a[d] = mfma_i8(k[i], qd[x][i][d], a[d]);
+            const float f = back[x] * ksc;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float t = (float)(a[0][i] * 256 + a[1][i]);   // (|sums| of a digit < 2^22)
+                sc[x][i] = (PAIRS ? __builtin_fmaf(t, 256.f, (float)a[DG - 1][i]) : t) * f;
+            }
+            finish(x, p0 + j, par, mask);
+        }
+    };
+    // Weights 2^(s - m_run), with m_run 7 below the maximum seen when it was last raised; it is raised when a row's
+    // maximum passes m_run + 15. So weights stay below 2^15, inside f16, and small ones keep their digits: hi + lo
+    // resolves 2^-24, 2^-31 of a fresh maximum, and one f16 2^-24 in subnormals.
+    auto settle = [&](int par) __attribute__((always_inline)) {
+        float mx[RB];
+        bool grow = false;
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+            const f4 m4 = *(const f4*)mbuf[par][16 * x + lr];
+            mx[x] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+            grow = grow || mx[x] > m_run[x] + 2 * P_BITS + 1;   // (from -inf at the first visible key)
+        }
+        if (__any(grow)) {
+#pragma unroll
+            for (int x = 0; x < RB; ++x) {
+                const float mnew = mx[x] > m_run[x] + 2 * P_BITS + 1 ? mx[x] - P_BITS : m_run[x];
+                const float alpha = m_run[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[x] - mnew);
+                l_run[x] *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[x][d][i] *= alpha;
+                m_run[x] = mnew;
+            }
+        }
+    };
+    auto weights = [&](int par) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+            const float minus = m_run[x] == -INFINITY ? 0.f : m_run[x];
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(sc[x][i] - minus);
+                l_run[x] += e[i];
+            }
+            _Float16* to = &pbuf[par][x][w >> 1][0][l * 8 + 4 * (w & 1)];
+            if constexpr (PAIRS) {
+                h2 h0, h1, l0, l1;
+                split2(f2{e[0], e[1]}, neg1, h0, l0);
+                split2(f2{e[2], e[3]}, neg1, h1, l1);
+                *(h4*)to = h4{h0[0], h0[1], h1[0], h1[1]};
+                *(h4*)(to + 64 * 8) = h4{l0[0], l0[1], l1[0], l1[1]};
+            } else {
+                *(h4*)to = h4{(_Float16)e[0], (_Float16)e[1], (_Float16)e[2], (_Float16)e[3]};
+            }
+        }
+    };
+    // O of the wave's dims (vf: the V operand of a dim block and half of the keys)
+    auto values = [&](int par, auto&& vf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            h8 ph[RB], pl[RB];
+#pragma unroll
+            for (int x = 0; x < RB; ++x) {
+                ph[x] = *(const h8*)&pbuf[par][x][s][0][l * 8];
+                if constexpr (PAIRS) pl[x] = *(const h8*)&pbuf[par][x][s][NP - 1][l * 8];
+            }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const h8 v = vf(d, s);
+#pragma unroll
+                for (int x = 0; x < RB; ++x) {
+                    o[x][d] = mfma16x16x32(v, ph[x], o[x][d]);
+                    if constexpr (PAIRS) o[x][d] = mfma16x16x32(v, pl[x], o[x][d]);
+                }
+            }
+        }
+    };
+    // Full page j: its weights and the next page's scores, then its values. K of the page after goes out when K's buffer has
+    // been read, V of it likewise: on arrival here, K of j + 1 and V of j and j + 1 are under way or there.
+    auto step = [&](int j, int par, const uint8_t* v, uint8_t* vto) __attribute__((always_inline)) {
+        const h2 s01 = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(scl[2], j & 63));
+        const h2 s23 = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(scl[3], j & 63));
+        if (((j + 1) & 63) == 0) load_scales();
+        if (((j + 2) & 63) == 0) load_ids(j + 2);
+        settle(par);
+        weights(par);
+        scores(j + 1, par ^ 1, (p0 + j + 1) * kv8::PAGE + kv8::PAGE - 1 > clear);   // (past the end: not used)
+        fetch(c.kp, kbuf, j + 2);
+        lds_barrier();
+        values(par, [&](int d, int s) __attribute__((always_inline)) {
+            const u2 r = *(const u2*)(v + w * QUARTER + KIB * d + 16 * l + 8 * s);
+            const h2 f = s ? s23 : s01;
+            const h4 f0 = {f[0], f[0], f[0], f[0]}, f1 = {f[1], f[1], f[1], f[1]};
+            return cat_h4(codes4(r[0]) * f0, codes4(r[1]) * f1);
+        });
+        fetch(c.vp, vto, j + 2);
+    };
+    // the open page comes first: its scores are there
+    if (np > 0 && !tail) {
+        scores(0, 0, p0 * kv8::PAGE + kv8::PAGE - 1 > clear);
+        fetch(c.kp, kbuf, 1);
+        fetch(c.vp, vbuf1, 1);
+    }
+    lds_barrier();
+    int par = 0;
+    if (tail) {
+        settle(0);
+        weights(0);
+        if (np > 0) {
+            scores(0, 1, p0 * kv8::PAGE + kv8::PAGE - 1 > clear);
+            fetch(c.kp, kbuf, 1);
+            fetch(c.vp, vbuf1, 1);
+        }
+        lds_barrier();
+        const int have = total - closed * kv8::PAGE;   // rows that are not there hold anything
+        values(0, [&](int d, int s) __attribute__((always_inline)) {
+            h8 v = ld_h8(c.tv + open + KIB * d + 8 * s);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (32 * s + 16 * (i >> 2) + 4 * g + (i & 3) >= have) v[i] = (_Float16)0.f;
+            return v;
+        });
+        par = 1;
+    }
+    for (int j = 0; j < np; j += 2) {
+        step(j, par, vbuf0, vbuf0);
+        if (j + 1 < np) step(j + 1, par ^ 1, vbuf1, vbuf1);
+    }
+    landed<0>();   // the fetches past the end
+
+    // ---- sums over the waves' keys, then the rows out
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+        const float sum = sum_xor32(sum_xor16(l_run[x]));
+        if (l < 16) lbuf[16 * x + l][w] = sum;
+    }
+    lds_barrier();
+    if (u.ns > 1) {
+        const int nrec = kv8::max_records(wgs), rec = u.rec + kv8::record(split, u.nrb, rb, nkv, kh);
+        if (rec >= nrec) return;   // (cannot be: see max_records)
+        f2* ml = (f2*)part + (size_t)rec * ROWS;
+        float* po = part + (size_t)nrec * ROWS * 2 + (size_t)rec * ROWS * HD;
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+            const int row = 16 * x + lr;
+            if (r0 + row >= R) continue;
+            const f4 s4 = *(const f4*)lbuf[row];
+            if (w == 0 && g == 0) ml[row] = f2{m_run[x], (s4[0] + s4[1]) + (s4[2] + s4[3])};
+#pragma unroll
+            for (int d = 0; d < ND; ++d) *(f4*)(po + (size_t)row * HD + w * (HD / 4) + 16 * d + 4 * g) = o[x][d];
+        }
+        return;
+    }
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+        const int r = r0 + 16 * x + lr;
+        if (r >= R) continue;
+        const f4 s4 = *(const f4*)lbuf[16 * x + lr];
+        const float inv = 1.0f / ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+        const int t = r / G;
+        OutT* to = out + (size_t)(u.t0 + t) * ots + (size_t)(kh * G + r - t * G) * HD;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const int dim = w * (HD / 4) + 16 * d + 4 * g;
+            const f4 gate = ld_f4(qrow[x] + HD + dim);
+            f4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = o[x][d][i] * inv * sigmoid_hw(gate[i]);
+            store4(to + dim, v);
+        }
+    }
+}
+
+// Joins the records of sequences with more than one split. An item is (group of rows, row, 64 dims); thread = (split lane of
+// 16, 4 dims). The launch is as many workgroups as there can be items, or fewer, each taking several.
+template <int HD, int ROWS, class OutT>
+__global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q, int qts,
+                                                             int nh, OutT* __restrict__ out, int ots,
+                                                             const float* __restrict__ part, int wgs) {
+    constexpr int SL = 16, DQ = HD / 64;
+    __shared__ float red_m[SL], red_l[SL];
+    __shared__ __align__(16) f4 red_o[SL][16];
+    const int nkv = c.nkv, G = nh / nkv, tid = threadIdx.x, l = tid & 63, sg = tid >> 4, dl = tid & 15;
+    const Kv8Seq s0 = kv8_seq(b, l);
+    const int chunk = call_chunk<ROWS>(b, s0, G, nkv, wgs, l);
+    const int nrec = kv8::max_records(wgs);
+    for (int item = blockIdx.x;; item += gridDim.x) {
+        const int dq = item % DQ, row = item / DQ % ROWS;
+        const Found u = find<ROWS, true>(b, s0, G, nkv, chunk, item / (DQ * ROWS), l);
+        if (!u.any) return;
+        const int kh = u.at % nkv, rb = u.at / nkv, r = rb * ROWS + row;
+        if (r >= u.n * G) continue;   // (whole workgroup)
+        const int t = r / G, h = kh * G + r - t * G, need = (u.len + t) / kv8::PAGE / chunk + 1;
+        float m = -INFINITY, sum = 0.f;
+        f4 o = f4{};
+        for (int s = sg; s < need; s += SL) {
+            const size_t at = (size_t)(u.rec + kv8::record(s, u.nrb, rb, nkv, kh)) * ROWS + row;
+            const f2 ml = *((const f2*)part + at);
+            const f4 v = ld_f4(part + (size_t)nrec * ROWS * 2 + at * HD + 64 * dq + 4 * dl);
+            const float mn = fmaxf(m, ml[0]);
+            const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            const float e = ml[0] == -INFINITY ? (ml[1] == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(ml[0] - mn);
+            sum = sum * a + ml[1] * e;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = o[i] * a + v[i] * e;
+            m = mn;
+        }
+        __syncthreads();   // the last item's partial results have been read
+        if (dl == 0) {
+            red_m[sg] = m;
+            red_l[sg] = sum;
+        }
+        red_o[sg][dl] = o;
+        __syncthreads();
+        if (sg == 0) {
+            const int live = min(need, SL);
+            float M = -INFINITY, L = 0.f;
+            for (int s = 0; s < live; ++s) M = fmaxf(M, red_m[s]);
+            f4 v = f4{};
+            for (int s = 0; s < live; ++s) {
+                const float e = red_m[s] == -INFINITY ? (red_l[s] == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(red_m[s] - M);
+                L += red_l[s] * e;
+                const f4 y = red_o[s][dl];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += y[i] * e;
+            }
+            const int dim = 64 * dq + 4 * dl;
+            const f4 gate = ld_f4(q + (size_t)(u.t0 + t) * qts + (size_t)h * 2 * HD + HD + dim);
+            const float inv = 1.0f / L;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = v[i] * inv * sigmoid_hw(gate[i]);
+            store4(out + (size_t)(u.t0 + t) * ots + (size_t)h * HD + dim, v);
+        }
+    }
+}
+
+// Row blocks of a workgroup and the workgroups a call is shared out to
+struct Form { int rb, wgs; };
+Form form(int max_nt, int G) {
+    const long rows = (long)max_nt * G;
+    return rows <= 16 ? Form{1, 512} : rows <= 32 ? Form{2, 512} : Form{4, 256};
+}
+// Row blocks, over all KV heads, that the sequences of a call can have
+long max_groups(const Form& f, int nseq, int ntok, int max_nt, int G, int nkv) {
+    const long rows = 16 * f.rb, each = ((long)max_nt * G + rows - 1) / rows;
+    return std::min((long)ntok * G / rows + nseq, each * nseq) * nkv;
+}
+
+template <int HD, int RB, class OutT>
+hipError_t launch(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, OutT* out, int ots,
+                  float* part, const Form& f, hipStream_t st) {
+    const long groups = max_groups(f, b.nseq, b.ntok, b.max_nt, nh / c.nkv, c.nkv);
+    attn_kv8_kernel<HD, RB, sizeof(OutT) == 4, OutT>
+        <<<dim3((unsigned)(groups + f.wgs)), 256, 0, st>>>(c, b, q, qts, nh, scale, out, ots, part, f.wgs);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    // split groups have two splits at least, so there are at most max_records / 2 of them
+    const long items = std::min(groups, (long)kv8::max_records(f.wgs) / 2) * 16 * RB * (HD / 64);
+    attn_kv8_merge_kernel<HD, 16 * RB, OutT>
+        <<<dim3((unsigned)std::min(items, 4096L)), 256, 0, st>>>(c, b, q, qts, nh, out, ots, part, f.wgs);
+    return hipGetLastError();
+}
+template <int HD, class OutT>
+hipError_t launch_rb(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, OutT* out, int ots,
+                     float* part, hipStream_t st) {
+    const Form f = form(b.max_nt, nh / c.nkv);
+    if (f.rb == 1) return launch<HD, 1, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
+    if (f.rb == 2) return launch<HD, 2, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
+    return launch<HD, 4, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
+}
+
+}  // namespace
+
+size_t attn_kv8_scratch_bytes(int max_nt, int hd, int nh, int nkv) {
+    const Form f = form(max_nt, nh / nkv);
+    return (size_t)kv8::max_records(f.wgs) * 16 * f.rb * (hd + 2) * sizeof(float);
+}
+hipError_t launch_attn_kv8(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, void* out,
+                           int ots, bool f16out, float* part, hipStream_t st) {
+    if (f16out) {
+        _Float16* o = (_Float16*)out;
+        return c.hd == 256 ? launch_rb<256>(c, b, q, qts, nh, scale, o, ots, part, st)
+                           : launch_rb<128>(c, b, q, qts, nh, scale, o, ots, part, st);
+    }
+    float* o = (float*)out;
+    return c.hd == 256 ? launch_rb<256>(c, b, q, qts, nh, scale, o, ots, part, st)
+                       : launch_rb<128>(c, b, q, qts, nh, scale, o, ots, part, st);
+}
+
+}  // namespace it

@@ -145,6 +145,19 @@ hipError_t launch_attn_prep_pos(float* q, int qts, const float* k, const float* 
                                 int hd, int nh, int nkv, int nt, int n_rot, const float* freq, float mscale,
                                 bool pairs, int rtz, hipStream_t st);
 
+// The paged 8-bit cache (kv8.hip, attn_kv8.hip; arguments in kv8.h). part: attn_kv8_scratch_bytes.
+struct Kv8;
+struct Kv8Batch;
+hipError_t launch_kv8_append(const Kv8& c, const Kv8Batch& b, const uint16_t* k, const uint16_t* v, int kts,
+                             hipStream_t st);
+hipError_t launch_kv8_read(const Kv8& c, const Kv8Batch& b, const int* first, uint16_t* k, uint16_t* v, int kts,
+                           hipStream_t st);
+hipError_t launch_kv8_copy(const Kv8& c, const int* src, const int* dst, int n, const int* seq_src, const int* seq_dst,
+                           int nseq, hipStream_t st);
+size_t attn_kv8_scratch_bytes(int max_nt, int hd, int nh, int nkv);
+hipError_t launch_attn_kv8(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, void* out,
+                           int ots, bool f16out, float* part, hipStream_t st);
+
 // conv <- ck_conv (nc floats) and ssm <- ck_ssm (ns floats) in one launch.
 hipError_t launch_gdn_rollback(const float* ck_conv, float* conv, size_t nc, const float* ck_ssm, float* ssm,
                                size_t ns, hipStream_t st);

@@ -1,0 +1,43 @@
+// Index and split arithmetic of the paged 8-bit cache, shared by its kernels and compiled for the host by the tests.
+#pragma once
+#include <stdint.h>
+
+#ifdef __HIP__
+#define IT_HD __host__ __device__ __forceinline__
+#else
+#define IT_HD inline
+#endif
+
+namespace it {
+namespace kv8 {
+
+constexpr int PAGE = 64, BLOCK = 16;   // rows of a page, rows that share a scale
+
+// Element of a page and KV head that holds (row, dim), for the codes (bytes) and the open rows (f16) alike. The order is that of
+// the matrix operands: a wave's lane l reads 16 codes at 16 l of each KiB.
+//   K: KiB (row / 16, dim / 64); lane = 16 (dim / 8 % 4) + row % 16; then two runs of 8 dims, 32 apart
+//   V: KiB (dim / 16); lane = 16 (row / 4 % 4) + dim % 16; then four rows of each of the four blocks
+IT_HD int k_elem(int hd, int row, int dim) {
+    return (((row >> 4) * (hd >> 6) + (dim >> 6)) * 64 + ((dim >> 3) & 3) * 16 + (row & 15)) * 16 + ((dim >> 5) & 1) * 8 +
+           (dim & 7);
+}
+IT_HD int v_elem(int row, int dim) {
+    return ((dim >> 4) * 64 + ((row >> 2) & 3) * 16 + (dim & 15)) * 16 + (row >> 4) * 4 + (row & 3);
+}
+
+// Pages per split of an attention call: `work` is the sum over sequences and KV heads of row blocks times pages, shared
+// out to about `wgs` workgroups. The same in the partial and the merge kernel.
+IT_HD int chunk_pages(float work, int wgs) {
+    const float c = work / (float)wgs;
+    if (!(c < 33554432.0f)) return 33554432;   // no sequence has more pages
+    const int i = (int)c;
+    return (float)i < c ? i + 1 : i < 1 ? 1 : i;
+}
+IT_HD int splits(int pages, int chunk) { return (int)(((long)pages + chunk - 1) / chunk); }
+// Record of (split, row block, KV head) among a sequence's, and how many blocks of records all split sequences can
+// need: splits(p, c) <= 2 p / c where p > c, so at most 2 wgs and what f32 sums round off.
+IT_HD int record(int split, int nrb, int rb, int nkv, int kh) { return (split * nrb + rb) * nkv + kh; }
+IT_HD int max_records(int wgs) { return 2 * wgs + 16; }
+
+}  // namespace kv8
+}  // namespace it

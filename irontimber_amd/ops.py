@@ -6,10 +6,11 @@ torch's current stream. Buffer layouts and semantics are those of include/it_att
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
-from ._lib import ItError, call, last_error, lib
+from ._lib import ItError, Kv8CacheArgs, call, last_error, lib
 
 KERNEL_AUTO, KERNEL_SPLITK, KERNEL_FLASH, KERNEL_FLASH_F32 = 0, 1, 2, 3
 
@@ -670,3 +671,141 @@ def gdn_tree_commit(x: torch.Tensor, conv_state: torch.Tensor, state: torch.Tens
     _need_all(torch.uint8, dev, (trace,), "trace")
     _call_on(dev, "it_gdn_tree_commit", x.data_ptr(), cd, K, conv_state.data_ptr(), state.data_ptr(), anc.data_ptr(), leaf,
              nt, nv, nk, 128, trace.data_ptr(), trace.numel())
+
+
+# ---- a paged K/V cache in 8 bits (include/it_attn.h has the whole contract)
+
+KV8_PAGE, KV8_BLOCK = 64, 16
+
+
+class Kv8Cache(NamedTuple):
+    """A layer's buffers: codes kp, vp [npages, nkv, 64*hd] uint8, scales sc [npages, nkv, 8] f16, open rows tk, tv
+    [nseq, 2, nkv, 64*hd] f16 (it_kv8_cache)."""
+    kp: torch.Tensor
+    vp: torch.Tensor
+    sc: torch.Tensor
+    tk: torch.Tensor
+    tv: torch.Tensor
+
+
+def kv8_cache(npages: int, nseq: int, nkv: int, hd: int = 256, device="cuda") -> Kv8Cache:
+    """A cache of npages pages of 64 rows, for nseq sequences. What it holds before the first append does not matter."""
+    def new(dtype, *shape):
+        return torch.zeros(*shape, dtype=dtype, device=device)
+    return Kv8Cache(new(torch.uint8, npages, nkv, KV8_PAGE * hd), new(torch.uint8, npages, nkv, KV8_PAGE * hd),
+                    new(torch.float16, npages, nkv, 8), new(torch.float16, nseq, 2, nkv, KV8_PAGE * hd),
+                    new(torch.float16, nseq, 2, nkv, KV8_PAGE * hd))
+
+
+def _kv8(c: Kv8Cache):
+    """(device, nkv, hd, nseq, it_kv8_cache) of a cache whose buffers fit each other."""
+    kp, vp, sc, tk, tv = c
+    dev, shape, tail = kp.get_device(), kp.shape, tk.shape
+    if len(shape) != 3 or len(tail) != 4 or shape[2] % KV8_PAGE:
+        raise ValueError("kp must be [npages, nkv, 64*hd] and tk [nseq, 2, nkv, 64*hd]")
+    npages, nkv, size = shape
+    if vp.shape != shape or sc.shape != (npages, nkv, 8) or tail[1:] != (2, nkv, size) or tv.shape != tail:
+        raise ValueError("vp must have kp's shape, sc [npages, nkv, 8], tk and tv [nseq, 2, nkv, 64*hd]")
+    _need_all(torch.uint8, dev, (kp, vp), "kp vp")
+    _need_all(torch.float16, dev, (sc, tk, tv), "sc tk tv")
+    args = Kv8CacheArgs(kp.data_ptr(), vp.data_ptr(), sc.data_ptr(), tk.data_ptr(), tv.data_ptr(), npages, tail[0], nkv,
+                        size // KV8_PAGE)
+    return dev, nkv, size // KV8_PAGE, tail[0], args
+
+
+def _kv8_batch(dev: int, nseq: int, start: torch.Tensor, length: torch.Tensor, table: torch.Tensor) -> int:
+    _need_all(torch.int32, dev, (start, length, table), "start length table")
+    if start.shape != (nseq + 1,) or length.shape != (nseq,) or len(table.shape) != 2 or table.shape[0] != nseq:
+        raise ValueError(f"start must be [{nseq + 1}], length [{nseq}] and table [{nseq}, max_pages]: one of each for the "
+                         "cache's sequences")
+    return table.shape[1]
+
+
+def _kv8_rows(dev: int, kvd: int, k: torch.Tensor, v: torch.Tensor) -> int:
+    """Token stride of f16 rows k, v [ntok, kvd]; rows may lie apart, as a slice of wider ones."""
+    for t in (k, v):
+        if t.dtype is not torch.float16 or t.get_device() != dev or len(t.shape) != 2 or t.shape[1] != kvd:
+            raise ValueError(f"k and v must be [ntok, {kvd}] f16 on the cache's device")
+        if t.stride(1) != 1 or t.shape != k.shape or t.stride(0) != k.stride(0):
+            raise ValueError("k and v must have one shape and one stride, with each row's values side by side")
+    return k.stride(0)
+
+
+def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, length: torch.Tensor,
+               table: torch.Tensor, max_nt: int) -> None:
+    """Appends f16 rows k, v [ntok, nkv*hd]: rows start[i] .. start[i+1]-1 follow the length[i] rows that sequence i holds
+    (start [nseq+1], length [nseq], table [nseq, max_pages] int32 on the device; at most max_nt a sequence). Pages that
+    get full are quantised; length stays as it is (it_kv8_append)."""
+    dev, nkv, hd, nseq, args = _kv8(cache)
+    pages = _kv8_batch(dev, nseq, start, length, table)
+    stride = _kv8_rows(dev, nkv * hd, k, v)
+    _call_on(dev, "it_kv8_append", ctypes.addressof(args), k.data_ptr(), v.data_ptr(), stride, k.shape[0],
+             start.data_ptr(), length.data_ptr(), table.data_ptr(), pages, max_nt)
+
+
+def kv8_read(cache: Kv8Cache, start: torch.Tensor, first: torch.Tensor, total: torch.Tensor, table: torch.Tensor,
+             max_rows: int, rows: int, out: tuple[torch.Tensor, torch.Tensor] | None = None
+             ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows first[i] .. of the sequences as f16 k, v [rows, nkv*hd], start[i+1] - start[i] (at most max_rows) of sequence
+    i at row start[i]; total [nseq] the rows that each one holds (it_kv8_read). Rows that no sequence has are left as they are
+    in out, the tensors to write to."""
+    dev, nkv, hd, nseq, args = _kv8(cache)
+    pages = _kv8_batch(dev, nseq, start, total, table)
+    if first.shape != (nseq,):
+        raise ValueError(f"first must be [{nseq}]")
+    _need_all(torch.int32, dev, (first,), "first")
+    if out is None:
+        out = tuple(torch.empty(rows, nkv * hd, dtype=torch.float16, device=cache.kp.device) for _ in range(2))
+    k, v = out
+    stride = _kv8_rows(dev, nkv * hd, k, v)
+    if k.shape[0] != rows:
+        raise ValueError(f"out must be two of [{rows}, {nkv * hd}]")
+    _call_on(dev, "it_kv8_read", ctypes.addressof(args), k.data_ptr(), v.data_ptr(), stride, rows, start.data_ptr(),
+             first.data_ptr(), total.data_ptr(), table.data_ptr(), pages, max_rows)
+    return k, v
+
+
+def kv8_copy(cache: Kv8Cache, src: torch.Tensor | None = None, dst: torch.Tensor | None = None,
+             seq_src: torch.Tensor | None = None, seq_dst: torch.Tensor | None = None) -> None:
+    """Copies pages src[i] to dst[i] and the open rows of sequences seq_src[i] to seq_dst[i] (int32 on the device; no
+    destination twice, and none that is a source) (it_kv8_copy)."""
+    dev, _, _, _, args = _kv8(cache)
+    for a, b in ((src, dst), (seq_src, seq_dst)):
+        if (a is None) != (b is None) or (a is not None and (len(a.shape) != 1 or a.shape != b.shape)):
+            raise ValueError("src and dst, seq_src and seq_dst must be pairs of one length")
+    _need_all(torch.int32, dev, (src, dst, seq_src, seq_dst), "src dst seq_src seq_dst")
+    _call_on(dev, "it_kv8_copy", ctypes.addressof(args), _ptr(src), _ptr(dst), 0 if src is None else len(src), _ptr(seq_src),
+             _ptr(seq_dst), 0 if seq_src is None else len(seq_src))
+
+
+def attn_kv8_scratch_bytes(max_nt: int, nh: int, nkv: int, hd: int = 256) -> int:
+    return lib().it_attn_kv8_scratch_bytes(max_nt, hd, nh, nkv)
+
+
+def attn_kv8(cache: Kv8Cache, q: torch.Tensor, start: torch.Tensor, length: torch.Tensor, table: torch.Tensor, nh: int,
+             max_nt: int, scale: float | None = None, out: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
+             out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Attention of appended tokens over the cache: q [ntok, nh*2*hd] f32 (q | gate per head), token t of sequence i sees its
+    rows 0 .. length[i] + t -> out [ntok, nh*hd], f32 or f16 (out's type, or out_dtype). start, length, table, max_nt as for
+    kv8_append, length still without the new tokens (it_attn_kv8)."""
+    dev, nkv, hd, nseq, args = _kv8(cache)
+    pages = _kv8_batch(dev, nseq, start, length, table)
+    ntok = q.shape[0]
+    if q.shape != (ntok, nh * 2 * hd):
+        raise ValueError(f"q must be [ntok, {nh * 2 * hd}]")
+    _need_all(torch.float32, dev, (q,), "q")
+    if out is None:
+        out = torch.empty(ntok, nh * hd, dtype=out_dtype, device=q.device)
+    if out.dtype not in (torch.float32, torch.float16) or out.shape != (ntok, nh * hd):
+        raise ValueError(f"out must be [{ntok}, {nh * hd}] of float32 or float16")
+    _need_all(out.dtype, dev, (out,), "out")
+    if scale is None:
+        scale = 1.0 / hd ** 0.5
+    if scratch is None:
+        scratch = torch.empty(attn_kv8_scratch_bytes(max_nt, nh, nkv, hd), dtype=torch.uint8, device=q.device)
+    elif scratch.get_device() != dev or not scratch.is_contiguous():
+        raise ValueError("scratch must be contiguous, on the same device as the other tensors")
+    _call_on(dev, "it_attn_kv8", ctypes.addressof(args), q.data_ptr(), nh * 2 * hd, ntok, start.data_ptr(),
+             length.data_ptr(), table.data_ptr(), pages, max_nt, nh, scale, out.data_ptr(), nh * hd,
+             int(out.dtype is torch.float16), scratch.data_ptr(), scratch.nbytes)
+    return out

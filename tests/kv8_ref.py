@@ -1,0 +1,114 @@
+"""Plain 64-bit statements of the paged 8-bit cache's calls, sequence by sequence and row by row."""
+import numpy as np
+
+PAGE, BLOCK = 64, 16
+
+
+def k_elem(hd):
+    """Element of a page and KV head that holds (row, dim) of K: [64, hd] indices."""
+    r, d = np.arange(PAGE)[:, None], np.arange(hd)[None]
+    return ((r // 16 * (hd // 64) + d // 64) * 64 + d // 8 % 4 * 16 + r % 16) * 16 + d // 32 % 2 * 8 + d % 8
+
+
+def v_elem(hd):
+    r, d = np.arange(PAGE)[:, None], np.arange(hd)[None]
+    return (d // 16 * 64 + r // 4 % 4 * 16 + d % 16) * 16 + r // 16 * 4 + r % 4
+
+
+def finite(x):
+    """f16 rows as the cache takes them."""
+    return np.nan_to_num(x, nan=0.0, posinf=65504.0, neginf=-65504.0).astype(np.float16)
+
+
+def scale_of(amax):
+    """amax / 127 up to the next number of four significant bits or multiple of 2^-24, at least 2^-24; exact in float64."""
+    t = float(amax) / 127.0
+    unit = 2.0 ** -24
+    while 16 * unit < t:          # four bits: 8 .. 16 units
+        unit *= 2
+    n = int(np.ceil(float(amax) / (127.0 * unit)))
+    return max(n, 1) * unit
+
+
+def codes_of(x, s):
+    """Codes (0 .. 255) of f16 values x at scale s: nearest, ties to even."""
+    most = 113.0 if s > 512 else 127.0
+    return (np.clip(np.rint(x.astype(np.float64) / s), -most, most) + 128).astype(np.uint8)
+
+
+class Sequence:
+    """What a sequence holds: its f16 rows, and the values that stand for them in the cache."""
+
+    def __init__(self, nkv, hd):
+        self.nkv, self.hd = nkv, hd
+        self.k = np.zeros((0, nkv, hd), np.float16)
+        self.v = np.zeros((0, nkv, hd), np.float16)
+
+    def append(self, k, v):
+        self.k = np.concatenate([self.k, finite(k).reshape(-1, self.nkv, self.hd)])
+        self.v = np.concatenate([self.v, finite(v).reshape(-1, self.nkv, self.hd)])
+
+    def cut(self, rows):
+        self.k, self.v = self.k[:rows], self.v[:rows]
+
+    @property
+    def rows(self):
+        return len(self.k)
+
+    def page(self, p):
+        """(K codes, V codes [nkv, 64*hd], scales [nkv, 8]) of full page p, in the page's order."""
+        out, sc = [], np.zeros((self.nkv, 8))
+        for i, (x, at) in enumerate(((self.k, k_elem(self.hd)), (self.v, v_elem(self.hd)))):
+            c = np.zeros((self.nkv, PAGE * self.hd), np.uint8)
+            for h in range(self.nkv):
+                for a in range(4):
+                    r = slice(p * PAGE + 16 * a, p * PAGE + 16 * a + 16)
+                    s = sc[h, 4 * i + a] = scale_of(np.abs(x[r, h].astype(np.float64)).max())
+                    c[h, at[16 * a:16 * a + 16]] = codes_of(x[r, h], s)
+            out.append(c)
+        return out[0], out[1], sc
+
+    def values(self):
+        """K, V [rows, nkv, hd] float64 as the calls see them."""
+        full = self.rows // PAGE * PAGE
+        out = []
+        for x in (self.k, self.v):
+            y = x.astype(np.float64)
+            for a in range(0, full, BLOCK):
+                for h in range(self.nkv):
+                    s = scale_of(np.abs(y[a:a + BLOCK, h]).max())
+                    y[a:a + BLOCK, h] = (codes_of(x[a:a + BLOCK, h], s).astype(np.float64) - 128) * s
+            out.append(y)
+        return out
+
+
+def attention(q, k, v, before, scale, f16=False):
+    """q [n, nh, 2*hd] (query | gate), k, v [rows, nkv, hd] float64, token t sees rows 0 .. before + t -> (out [n, nh, hd]
+    float64, bound of an f32 or f16 evaluation's error).
+
+    The bound, with u = 2^-24 (f32) and the products' operands off by e = 2^-21 for pairs (q to 2^-22 of a value or 2^-24 of
+    its row's largest, the scale's product and the sums' conversion within the rest) or 2^-11 for one f16 each:
+    a score is off by ds <= scale sum |q||k| (e + hd u) + 4 u |s| (e of the row's largest |q| where that is more); a weight by
+    2 ds + e + 4 u of itself; sums over n keys by n u; so the output by 2 (2 ds + e + n u + 8 u) max |v| sigmoid(gate) at
+    most, plus its own rounding. Weights below 2^-31 (2^-24 for one f16) of the largest may be lost: n of those times max |v|."""
+    n, nh, hd2 = q.shape
+    hd, nkv = hd2 // 2, k.shape[1]
+    out, tol = np.zeros((n, nh, hd)), np.zeros((n, nh, hd))
+    u, e, lost = 2.0 ** -24, (2.0 ** -11 if f16 else 2.0 ** -21), (2.0 ** -24 if f16 else 2.0 ** -31)
+    q = q.astype(np.float64)
+    for h in range(nh):
+        kh, vh = k[:, h // (nh // nkv)], v[:, h // (nh // nkv)]
+        for t in range(n):
+            m = before + t + 1
+            x = q[t, h, :hd]
+            s = scale * (kh[:m] @ x)
+            w = np.exp(s - s.max())
+            gate = 1 / (1 + np.exp(-q[t, h, hd:]))
+            out[t, h] = (w @ vh[:m]) / w.sum() * gate
+            size = np.maximum(np.abs(x), 0 if f16 else np.abs(x).max() / 8)
+            ds = (abs(scale) * (np.abs(kh[:m]) @ size).max() * (e + hd * u) + 4 * u * np.abs(s).max())
+            top = np.abs(vh[:m]).max(0)
+            tol[t, h] = 2 * (2 * ds + e + (m + 8) * u + m * lost) * top * gate + 4 * u * np.abs(out[t, h])
+            if f16:
+                tol[t, h] += 2.0 ** -11 * np.abs(out[t, h]) + 2.0 ** -25
+    return out, tol + 1e-30
