@@ -38,15 +38,18 @@ template <int N> __device__ __forceinline__ void landed() { asm volatile("s_wait
 template <int N> __device__ __forceinline__ void kib_to_lds(const uint8_t* from, unsigned off, uint8_t* to) {
     typedef __attribute__((address_space(3))) uint8_t lds_u8;
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_u8*)to);
-    static_assert(N == 2 || N == 4, "a quarter of a page");
+    static_assert(N == 1 || N == 2 || N == 4, "a wave's share of a page");
     if constexpr (N == 4)
         asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\t"
                      "global_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
                      "global_load_lds_dwordx4 %1, %2 offset:2048\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072"
                      ::"s"(at), "v"(off), "s"(from) : "memory");
-    else
+    else if constexpr (N == 2)
         asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\t"
                      "global_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                     ::"s"(at), "v"(off), "s"(from) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\tglobal_load_lds_dwordx4 %1, %2"
                      ::"s"(at), "v"(off), "s"(from) : "memory");
 }
 __device__ __forceinline__ int prefix_sum(int v, int l) {   // inclusive, over the wave
@@ -61,6 +64,10 @@ __device__ __forceinline__ int prefix_sum(int v, int l) {   // inclusive, over t
 // Pages per split of this call (the same in both kernels; sums in a fixed order)
 template <int ROWS>
 __device__ __forceinline__ int call_chunk(const Kv8Batch& b, const Kv8Seq& s0, int G, int nkv, int wgs, int l) {
+    if (b.nseq == 1) {   // (the sum of one, without the exchanges)
+        const float one = (float)((__builtin_amdgcn_readfirstlane(s0.n) * G + ROWS - 1) / ROWS) * (float)__builtin_amdgcn_readfirstlane(s0.pages);
+        return kv8::chunk_pages(one * (float)nkv, wgs);
+    }
     float sum = 0.f;
     for (int i0 = 0; i0 < b.nseq; i0 += 64) {
         const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
@@ -78,6 +85,18 @@ struct Found {
 template <int ROWS, bool GROUPS>
 __device__ __forceinline__ Found find(const Kv8Batch& b, const Kv8Seq& s0, int G, int nkv, int chunk, int id, int l) {
     Found f;
+    if (b.nseq == 1) {
+        f = {0, 0, 0, 0, 0, 0, 0, id, 0, false, false};
+        f.t0 = __builtin_amdgcn_readfirstlane(s0.t0);
+        f.n = __builtin_amdgcn_readfirstlane(s0.n);
+        f.len = __builtin_amdgcn_readfirstlane(s0.len);
+        f.pages = __builtin_amdgcn_readfirstlane(s0.pages);
+        f.bad = __builtin_amdgcn_readfirstlane((int)s0.bad) != 0;
+        f.nrb = (f.n * G + ROWS - 1) / ROWS;
+        f.ns = kv8::splits(f.pages, chunk);
+        f.any = id < f.nrb * nkv * (GROUPS ? (f.ns > 1 ? 1 : 0) : f.ns);
+        return f;
+    }
     f.any = false;
     int base = 0, rbase = 0;
     for (int i0 = 0; i0 < b.nseq; i0 += 64) {
@@ -124,17 +143,24 @@ __device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c,
 }
 
 // Records: {m, l} [record][ROWS] (m in log2 units), then o [record][ROWS][HD].
+//
+// Wave w takes key block w of a page for the scores and weights, and dim blocks ND * w .. + ND-1 for O.
 template <int HD, int RB, bool PAIRS, class OutT>
-__global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q,
-                                                                        int qts, int nh, float scale,
-                                                                        OutT* __restrict__ out, int ots,
-                                                                        float* __restrict__ part, int wgs) {
+__global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q, int qts, int nh,
+                                                          float scale, OutT* __restrict__ out, int ots,
+                                                          float* __restrict__ part, int wgs) {
     constexpr int ROWS = 16 * RB, NP = PAIRS ? 2 : 1, NJ = HD / 64, NK = HD / 32, ND = HD / 64, DG = PAIRS ? 3 : 2;
     constexpr int KIB = 1024, QUARTER = 16 * HD;   // a wave's share of a page's codes
-    __shared__ __align__(16) uint8_t kbuf[4 * QUARTER], vbuf0[4 * QUARTER], vbuf1[4 * QUARTER];
+    // Forms of many rows keep a part of q's digits in LDS, and one page of V in place of two: 256 registers and half of a
+    // CU's LDS, so that two workgroups share a CU.
+    constexpr int KB = RB == 1 ? 2 : 1, VB = RB >= 3 ? 1 : 2;            // pages of K and of V
+    constexpr int QL = HD < 256 || RB < 3 ? 0 : RB - 2, NR = NJ - QL;    // of q's NJ groups of 64 dims: in LDS, in registers
+    __shared__ __align__(16) uint8_t kbuf[KB][4 * QUARTER], vbuf[VB][4 * QUARTER];
+    __shared__ __align__(16) u4 qlast[QL ? RB : 1][QL ? QL : 1][DG][QL ? 64 : 1];
     __shared__ __align__(16) _Float16 pbuf[2][RB][2][NP][64 * 8];   // P^T operands: [parity][rows][keys][hi, lo]
-    __shared__ __align__(16) float mbuf[2][ROWS][4];                // row maxima by wave
-    __shared__ __align__(16) float lbuf[ROWS][4];
+    __shared__ __align__(16) float mbuf[2][ROWS][4];                // row maxima by key block
+    __shared__ __align__(16) float lbuf[ROWS][4];                   // row sums by key block; at first q's maxima by dims
+    __shared__ int qlim[ROWS];                                      // the last key that a row sees
 
     const int nkv = c.nkv, G = nh / nkv;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, lr = l & 15;
@@ -146,22 +172,11 @@ __global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, K
     const int kh = u.at % nkv, rest = u.at / nkv, rb = u.nrb - 1 - rest % u.nrb, split = rest / u.nrb;
     const int R = u.n * G, r0 = rb * ROWS;
 
-    // ---- this lane's query rows (one per 16-row block) and the keys they see
-    int qlim[RB];
-    const float* qrow[RB];
-#pragma unroll
-    for (int x = 0; x < RB; ++x) {
-        const int r = min(r0 + 16 * x + lr, R - 1), t = r / G;
-        qlim[x] = r0 + 16 * x + lr < R ? u.len + t : -1;
-        qrow[x] = q + (size_t)(u.t0 + t) * qts + (size_t)(kh * G + r - t * G) * 2 * HD;
-    }
     if (u.bad) {   // a sequence whose length cannot be: NaN
-#pragma unroll
-        for (int x = 0; x < RB; ++x) {
-            const int r = r0 + 16 * x + lr, t = r / G;
+        for (int i = tid; i < ROWS * (HD / 4); i += 256) {
+            const int r = r0 + i / (HD / 4), t = r / G;
             if (r < R)
-                for (int d = 4 * (l >> 4) + 16 * w; d < HD; d += 64)
-                    store4(out + (size_t)(u.t0 + t) * ots + (size_t)(kh * G + r - t * G) * HD + d, f4{NAN, NAN, NAN, NAN});
+                store4(out + (size_t)(u.t0 + t) * ots + (size_t)(kh * G + r - t * G) * HD + 4 * (i % (HD / 4)), f4{NAN, NAN, NAN, NAN});
         }
         return;
     }
@@ -187,175 +202,264 @@ __global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, K
         const bool known = (unsigned)ids < (unsigned)c.npages;
         scl = *(const u4*)(c.sc + (known ? (size_t)ids * nkv + kh : 0) * 8);
         if (!known) scl = u4{0x7E007E00u, 0x7E007E00u, 0u, 0u};
-        asm volatile("" : "+v"(scl));
+    };
+    auto page_of = [&](int j) __attribute__((always_inline)) {
+        const unsigned id = __builtin_amdgcn_readlane(ids, j & 63);
+        return id < (unsigned)c.npages ? id : 0u;
     };
     // This wave's quarter of a page's codes, K by block or V by dims, to LDS in the order that it is read back by the
     // same wave. Past the end (the loads go out without a branch, so that their count is known): one piece for all lanes.
-    auto fetch = [&](const uint8_t* from, uint8_t* to, int j) __attribute__((always_inline)) {
-        const unsigned one = __builtin_amdgcn_readlane(ids, j & 63), id = one < (unsigned)c.npages ? one : 0;
+    auto fetch = [&](const uint8_t* from, uint8_t* to, int j, unsigned id) __attribute__((always_inline)) {
         kib_to_lds<NJ>(from + uniform_off(((size_t)id * nkv + kh) * (kv8::PAGE * HD) + w * QUARTER), j < np ? 16 * l : 0,
                        to + w * QUARTER);
     };
+    auto qrow = [&](int x) __attribute__((always_inline)) {
+        const int r = min(r0 + 16 * x + lr, R - 1), t = r / G;
+        return q + (size_t)(u.t0 + t) * qts + (size_t)(kh * G + r - t * G) * 2 * HD;
+    };
 
+    // What the first wait is not for goes out before it: q, and with one row block what the open page takes
+    const size_t open = ((size_t)(u.seq * 2 + (closed & 1)) * nkv + kh) * (kv8::PAGE * HD) + w * QUARTER + 16 * l;
+    f4 y[RB][4];
+    if (w < NJ) {
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+            const float* at = qrow(x) + 64 * w + 8 * g;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[x][e] = ld_f4(at + 32 * (e >> 1) + 4 * (e & 1));
+        }
+    }
+    constexpr bool AHEAD = RB == 1;
+    h8 ahead_k[AHEAD ? NK : 1], ahead_v[AHEAD ? ND : 1][2];
+    f4 ahead_q[AHEAD ? NK : 1][2];
+    if (AHEAD && tail) {
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+            ahead_k[ks] = ld_h8(c.tk + open + KIB * (ks >> 1) + 8 * (ks & 1));
+            ahead_q[ks][0] = ld_f4(qrow(0) + 32 * ks + 8 * g);
+            ahead_q[ks][1] = ld_f4(qrow(0) + 32 * ks + 8 * g + 4);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) ahead_v[d][e] = ld_h8(c.tv + open + KIB * d + 8 * e);
+    }
     if (np > 0) {
         load_ids(0);
+        fetch(c.kp, kbuf[0], 0, page_of(0));
+        if constexpr (VB == 2) fetch(c.vp, vbuf[0], 0, page_of(0));
+        if constexpr (KB == 2) fetch(c.kp, kbuf[1], 1, page_of(1));
         load_scales();
-        fetch(c.kp, kbuf, 0);
-        fetch(c.vp, vbuf0, 0);
     }
 
-    f4 o[RB][ND], sc[RB];
-    float m_run[RB], l_run[RB], back[RB];   // back: from integer products to log2 units
-    u4 qd[RB][NJ][DG];                      // q's digits, the highest first
+    f4 o[RB][ND], sc[RB];                 // sc: products of a page, times back * ksc in log2 units
+    // top: a row's reference + 15, neg: minus the reference (0 while there is none); back: from integer products to log2 units but
+    // for K's scale ksc of the page that sc holds
+    float top[RB], neg[RB], l_run[RB], back[RB], ksc = 1.f;
+    u4 qd[RB][NR][DG];                    // q's digits, the highest first
     const float neg1 = in_register(-1.0f);
 #pragma unroll
     for (int x = 0; x < RB; ++x) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[x][d] = f4{};
-        m_run[x] = -INFINITY;
+        top[x] = -INFINITY;
+        neg[x] = 0.f;
         l_run[x] = 0.f;
     }
 
-    // Masks scores of page p (block w: this lane's keys are 16 w + 4 g + 0..3) and puts their maxima to LDS
-    auto finish = [&](int x, int p, int par, bool mask) __attribute__((always_inline)) {
-        if (mask) {
-            const int key = p * kv8::PAGE + 16 * w + 4 * g;
+    // The keys that rows do not see get -inf (this lane's keys of page p are 16 w + 4 g + 0..3)
+    auto mask_keys = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (key + i > qlim[x]) sc[x][i] = -INFINITY;
+        for (int x = 0; x < RB; ++x) {
+            const int lim = qlim[16 * x + lr] - (p * kv8::PAGE + 16 * w + 4 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[x][i] = i > lim ? -INFINITY : sc[x][i];
         }
-        const float m = max_xor32(max_xor16(fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3]))));
-        if (l < 16) mbuf[par][16 * x + l][w] = m;
     };
-
-    // ---- q. The open page's keys are f16, so its products take q as f16 pairs (each row times the power of two that takes its
-    // largest value to 2^13 .. 2^14). The codes' products are integer ones: q in units of its largest value / 2^(8 DG - 1),
-    // as DG signed digits of 8 bits.
-    const size_t open = ((size_t)(u.seq * 2 + (closed & 1)) * nkv + kh) * (kv8::PAGE * HD) + w * QUARTER + 16 * l;
+    // The rows' maxima over the wave's 16 keys, to LDS. Values of different row blocks share the lane exchanges: lane row g ends with
+    // row block g of four, a half-wave with a row block of two.
+    auto maxima = [&](int par) __attribute__((always_inline)) {
+        float m[RB];
 #pragma unroll
-    for (int x = 0; x < RB; ++x) {
-        f4 y[NK][2];
-        uint32_t mb = 0;
-#pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-            y[ks][0] = ld_f4(qrow[x] + 32 * ks + 8 * g);
-            y[ks][1] = ld_f4(qrow[x] + 32 * ks + 8 * g + 4);
+        for (int x = 0; x < RB; ++x) m[x] = fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3])) * (back[x] * ksc);
+        int x = 0;
+        float v;
+        if constexpr (RB == 1) {
+            v = max_xor32(max_xor16(m[0]));
+        } else if constexpr (RB == 2) {
+            swap32(m[0], m[1]);
+            v = max_xor16(fmaxf(m[0], m[1]));
+            x = g >> 1;
+        } else {
+            float m3 = m[RB - 1];
+            swap32(m[0], m[2]);
+            swap32(m[1], m3);
+            float a = fmaxf(m[0], m[2]), e = fmaxf(m[1], m3);
+            swap16(a, e);
+            v = fmaxf(a, e);
+            x = min(2 * (g >> 1) + (g & 1), RB - 1);
         }
+        mbuf[par][16 * x + lr][w] = v;
+    };
+    // ---- q in units of its row's largest value / 2^(8 DG - 1), as DG signed digits of 8 bits, for integer products with the
+    // codes. Wave w makes those of dims 64 w .. (hd 128: two waves); they meet in LDS that is not in use yet, a row block at a time.
+    // A negative scale turns q round, and no unit is zero, so that -inf times it stays.
+    const float size = fabsf(scale) * LOG2E, sign = scale < 0.f ? -1.f : 1.f;
+    if (tid < ROWS) qlim[tid] = r0 + tid < R ? u.len + (r0 + tid) / G : -1;
+    {
+        if (w < NJ) {
 #pragma unroll
-        for (int ks = 0; ks < NK; ++ks)
+            for (int x = 0; x < RB; ++x) {
+                uint32_t mb = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float e = y[ks][i >> 2][i & 3];   // (a bit cast of the vector's element itself takes the first)
-                mb = max(mb, __builtin_bit_cast(uint32_t, e) & 0x7FFFFFFFu);
+                for (int i = 0; i < 16; ++i) {
+                    const float e = y[x][i >> 2][i & 3];   // (a bit cast of the vector's element itself takes the first)
+                    mb = max(mb, __builtin_bit_cast(uint32_t, e) & 0x7FFFFFFFu);
+                }
+                float m = __builtin_bit_cast(float, min(mb, 0x7F800000u));   // (infinity for a NaN)
+                lbuf[16 * x + lr][w] = max_xor32(max_xor16(m));
             }
-        float m = __builtin_bit_cast(float, min(mb, 0x7F800000u));   // (infinity for a NaN)
-        m = max_xor32(max_xor16(m));
-        const int ex = max(__builtin_amdgcn_frexp_expf(m), -100);   // (so that 2^-ex is finite)
-        const bool fine = m < INFINITY;
-        if (tail) {
-            const float f = fine ? __builtin_amdgcn_ldexpf(scale * LOG2E, ex - 14) : NAN;
+        }
+        lds_barrier();
+        u4* meet = VB == 2 ? (u4*)vbuf[VB - 1] : (u4*)pbuf;
+        static_assert(VB == 2 || sizeof(pbuf) >= NJ * DG * KIB, "room for a row block's digits");
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+            const f4 m4 = *(const f4*)lbuf[16 * x + lr];
+            const float m = NJ == 4 ? fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) : fmaxf(m4[0], m4[1]);
+            const int ex = max(__builtin_amdgcn_frexp_expf(m), -100);   // (so that 2^-ex is finite)
+            // |q| / 2^ex < 1; the highest digit at most 127 for all digits' roundings
+            constexpr float TOP = PAIRS ? 127 * 65536.f : 127 * 256.f;
+            constexpr uint32_t BIAS = PAIRS ? 0x808080u : 0x8080u;
+            const float to = __builtin_amdgcn_ldexpf(TOP * sign, -ex);
+            back[x] = m < INFINITY ? fmaxf(__builtin_amdgcn_ldexpf(size / TOP, ex), 1e-30f) : NAN;
+            if (w < NJ) {
+                u4 dg[DG];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t n[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)   // the digits: bytes of n + BIAS, each less 128
+                        n[i] = ((uint32_t)(int)rintf(y[x][e][i] * to) + BIAS) ^ BIAS;
+#pragma unroll
+                    for (int k = 0; k < DG; ++k) dg[k][e] = bytes_of(n[0], n[1], n[2], n[3], DG - 1 - k);
+                }
+#pragma unroll
+                for (int k = 0; k < DG; ++k) meet[(w * DG + k) * 64 + l] = dg[k];
+            }
+            lds_barrier();
+#pragma unroll
+            for (int j = 0; j < NR; ++j)
+#pragma unroll
+                for (int k = 0; k < DG; ++k) qd[x][j][k] = meet[(j * DG + k) * 64 + l];
+            if constexpr (QL > 0) {
+                for (int i = w; i < QL * DG; i += 4) qlast[x][i / DG][i % DG][l] = meet[(NR * DG + i) * 64 + l];
+            }
+            lds_barrier();
+        }
+    }
+    // The open page comes first. Its keys are f16, so its products take q as f16 pairs (each row times the power of two that takes
+    // its largest value to 2^13 .. 2^14).
+    if (tail) {
+        constexpr float TOP = PAIRS ? 127 * 65536.f : 127 * 256.f;
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+            const f4 m4 = *(const f4*)lbuf[16 * x + lr];
+            const float m = NJ == 4 ? fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) : fmaxf(m4[0], m4[1]);
+            const int ex = 14 - max(__builtin_amdgcn_frexp_expf(m), -100);
+            const float* at = qrow(x) + 8 * g;
             f4 a = {}, a2 = {};
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
-                const h8 k = ld_h8(c.tk + open + KIB * (ks >> 1) + 8 * (ks & 1));
+                const h8 k = AHEAD ? ahead_k[AHEAD ? ks : 0] : ld_h8(c.tk + open + KIB * (ks >> 1) + 8 * (ks & 1));
+                const f4 y[2] = {AHEAD ? ahead_q[AHEAD ? ks : 0][0] : ld_f4(at + 32 * ks),
+                                 AHEAD ? ahead_q[AHEAD ? ks : 0][1] : ld_f4(at + 32 * ks + 4)};
                 h8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    h2 h, r;
-                    split2(f2{__builtin_amdgcn_ldexpf(y[ks][i >> 1][2 * (i & 1)], 14 - ex),
-                              __builtin_amdgcn_ldexpf(y[ks][i >> 1][2 * (i & 1) + 1], 14 - ex)}, neg1, h, r);
+                    h2 h, e;
+                    split2(f2{__builtin_amdgcn_ldexpf(y[i >> 1][2 * (i & 1)] * sign, ex),
+                              __builtin_amdgcn_ldexpf(y[i >> 1][2 * (i & 1) + 1] * sign, ex)}, neg1, h, e);
                     hi[2 * i] = h[0];
                     hi[2 * i + 1] = h[1];
-                    lo[2 * i] = r[0];
-                    lo[2 * i + 1] = r[1];
+                    lo[2 * i] = e[0];
+                    lo[2 * i + 1] = e[1];
                 }
                 a = mfma16x16x32(k, hi, a);
                 a2 = mfma16x16x32(k, lo, a2);
             }
+            const f4 both = a + a2;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[x][i] = (a[i] + a2[i]) * f;
-            finish(x, closed, 0, true);
+            for (int i = 0; i < 4; ++i) sc[x][i] = both[i] * (TOP * 0x1p-14f);   // in units of back
         }
-        // |q| / 2^ex < 1; the highest digit at most 127 for all digits' roundings
-        constexpr float TOP = PAIRS ? 127 * 65536.f : 127 * 256.f;
-        constexpr uint32_t BIAS = PAIRS ? 0x808080u : 0x8080u;
-        const float to = __builtin_amdgcn_ldexpf(TOP, -ex);
-        back[x] = fine ? __builtin_amdgcn_ldexpf(scale * LOG2E / TOP, ex) : NAN;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t n[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)   // the digits: bytes of n + BIAS, each less 128
-                    n[i] = ((uint32_t)(int)rintf(y[2 * j + (e >> 1)][e & 1][i] * to) + BIAS) ^ BIAS;
-#pragma unroll
-                for (int k = 0; k < DG; ++k) qd[x][j][k][e] = bytes_of(n[0], n[1], n[2], n[3], DG - 1 - k);
-            }
+        mask_keys(closed);
+        maxima(0);
     }
 
-    // Scores of the wave's 16 keys of full page j, all rows
-    auto scores = [&](int j, int par, bool mask) __attribute__((always_inline)) {
+    // Scores of the wave's 16 keys of full page j
+    auto scores = [&](int j, int par) __attribute__((always_inline)) {
         const h2 two = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(w & 2 ? scl[1] : scl[0], j & 63));
-        const float ksc = (float)two[w & 1];
-        landed<NJ>();   // (V of page j may be under way)
+        ksc = (float)two[w & 1];
+        landed<KB * NJ>();   // all but the V that went out last, and with two pages of K the K before it
+        const uint8_t* from = kbuf[KB == 2 ? j & 1 : 0] + w * QUARTER + 16 * l;
         u4 k[NJ];
 #pragma unroll
-        for (int i = 0; i < NJ; ++i) k[i] = *(const u4*)(kbuf + w * QUARTER + KIB * i + 16 * l) ^ 0x80808080u;   // signed
+        for (int i = 0; i < NJ; ++i) k[i] = *(const u4*)(from + KIB * i) ^ 0x80808080u;   // signed
 #pragma unroll
         for (int x = 0; x < RB; ++x) {
             i4 a[DG];
 #pragma unroll
             for (int d = 0; d < DG; ++d) a[d] = i4{};
 #pragma unroll
-            for (int i = 0; i < NJ; ++i)
+            for (int i = 0; i < NR; ++i)
 #pragma unroll
                 for (int d = 0; d < DG; ++d) a[d] = mfma_i8(k[i], qd[x][i][d], a[d]);
-            const float f = back[x] * ksc;
+#pragma unroll
+            for (int i = 0; i < QL; ++i)
+#pragma unroll
+                for (int d = 0; d < DG; ++d) a[d] = mfma_i8(k[NR + i], qlast[x][i][d][l], a[d]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float t = (float)(a[0][i] * 256 + a[1][i]);   // (|sums| of a digit < 2^22)
-                sc[x][i] = (PAIRS ? __builtin_fmaf(t, 256.f, (float)a[DG - 1][i]) : t) * f;
+                const float t = (float)(a[0][i] * 256 + a[1][i]);   // (|sums| of a digit < 2^23)
+                sc[x][i] = PAIRS ? __builtin_fmaf(t, 256.f, (float)a[DG - 1][i]) : t;
             }
-            finish(x, p0 + j, par, mask);
         }
+        if ((p0 + j) * kv8::PAGE + kv8::PAGE - 1 > clear) mask_keys(p0 + j);
+        maxima(par);
     };
-    // Weights 2^(s - m_run), with m_run 7 below the maximum seen when it was last raised; it is raised when a row's
+    // Weights 2^(s - m_run) to LDS, with m_run 7 below the maximum seen when it was last raised; it is raised when a row's
     // maximum passes m_run + 15. So weights stay below 2^15, inside f16, and small ones keep their digits: hi + lo
-    // resolves 2^-24, 2^-31 of a fresh maximum, and one f16 2^-24 in subnormals.
-    auto settle = [&](int par) __attribute__((always_inline)) {
+    // resolves 2^-24, 2^-31 of a fresh maximum, and one f16 2^-24 in subnormals. The sums are those of the weights as rounded.
+    auto weights = [&](int par) __attribute__((always_inline)) {
         float mx[RB];
         bool grow = false;
 #pragma unroll
         for (int x = 0; x < RB; ++x) {
             const f4 m4 = *(const f4*)mbuf[par][16 * x + lr];
             mx[x] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            grow = grow || mx[x] > m_run[x] + 2 * P_BITS + 1;   // (from -inf at the first visible key)
+            grow = grow || mx[x] > top[x];   // (from -inf at the first visible key)
         }
-        if (__any(grow)) {
+        if (__any(grow)) {   // (all waves find the same)
 #pragma unroll
             for (int x = 0; x < RB; ++x) {
-                const float mnew = mx[x] > m_run[x] + 2 * P_BITS + 1 ? mx[x] - P_BITS : m_run[x];
-                const float alpha = m_run[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[x] - mnew);
-                l_run[x] *= alpha;
+                if (mx[x] > top[x]) {
+                    const float to = P_BITS - mx[x];
+                    const float f = top[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(to - neg[x]);
+                    l_run[x] *= f;
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
+                    for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[x][d][i] *= alpha;
-                m_run[x] = mnew;
+                        for (int i = 0; i < 4; ++i) o[x][d][i] *= f;
+                    neg[x] = to;
+                    top[x] = 2 * P_BITS + 1 - to;
+                }
             }
         }
-    };
-    auto weights = [&](int par) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < RB; ++x) {
-            const float minus = m_run[x] == -INFINITY ? 0.f : m_run[x];
             float e[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(sc[x][i] - minus);
-                l_run[x] += e[i];
-            }
+            for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][i], back[x] * ksc, neg[x]));
             _Float16* to = &pbuf[par][x][w >> 1][0][l * 8 + 4 * (w & 1)];
             if constexpr (PAIRS) {
                 h2 h0, h1, l0, l1;
@@ -363,8 +467,13 @@ __global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, K
                 split2(f2{e[2], e[3]}, neg1, h1, l1);
                 *(h4*)to = h4{h0[0], h0[1], h1[0], h1[1]};
                 *(h4*)(to + 64 * 8) = h4{l0[0], l0[1], l1[0], l1[1]};
+                l_run[x] += (e[0] + e[1]) + (e[2] + e[3]);
             } else {
-                *(h4*)to = h4{(_Float16)e[0], (_Float16)e[1], (_Float16)e[2], (_Float16)e[3]};
+                const h2 h0 = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[0], e[1]));
+                const h2 h1 = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[2], e[3]));
+                const h2 ones = {(_Float16)1.f, (_Float16)1.f};
+                *(h4*)to = h4{h0[0], h0[1], h1[0], h1[1]};
+                l_run[x] = __builtin_amdgcn_fdot2(h1, ones, __builtin_amdgcn_fdot2(h0, ones, l_run[x], false), false);
             }
         }
     };
@@ -382,72 +491,73 @@ __global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, K
             for (int d = 0; d < ND; ++d) {
                 const h8 v = vf(d, s);
 #pragma unroll
-                for (int x = 0; x < RB; ++x) {
-                    o[x][d] = mfma16x16x32(v, ph[x], o[x][d]);
-                    if constexpr (PAIRS) o[x][d] = mfma16x16x32(v, pl[x], o[x][d]);
+                for (int x = 0; x < RB; ++x) o[x][d] = mfma16x16x32(v, ph[x], o[x][d]);
+                if constexpr (PAIRS) {
+#pragma unroll
+                    for (int x = 0; x < RB; ++x) o[x][d] = mfma16x16x32(v, pl[x], o[x][d]);
                 }
             }
         }
     };
-    // Full page j: its weights and the next page's scores, then its values. K of the page after goes out when K's buffer has
-    // been read, V of it likewise: on arrival here, K of j + 1 and V of j and j + 1 are under way or there.
-    auto step = [&](int j, int par, const uint8_t* v, uint8_t* vto) __attribute__((always_inline)) {
+    // Full page j: its weights and the next page's scores, then its values. K and V of a later page go out when their buffers
+    // have been read: on arrival here K of j + 1 .. j + KB and V of j .. j + VB - 1 are under way or there.
+    auto step = [&](int j, int par) __attribute__((always_inline)) {
         const h2 s01 = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(scl[2], j & 63));
         const h2 s23 = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(scl[3], j & 63));
-        if (((j + 1) & 63) == 0) load_scales();
-        if (((j + 2) & 63) == 0) load_ids(j + 2);
-        settle(par);
+        if (((j + 1) & 63) == 0) {
+            load_scales();
+            asm volatile("" : "+v"(scl));
+        }
+        const unsigned vid = page_of(j + VB);
+        if (((j + 1 + KB) & 63) == 0) load_ids(j + 1 + KB);
+        const unsigned kid = page_of(j + 1 + KB);
+        __builtin_amdgcn_s_setprio(0);
         weights(par);
-        scores(j + 1, par ^ 1, (p0 + j + 1) * kv8::PAGE + kv8::PAGE - 1 > clear);   // (past the end: not used)
-        fetch(c.kp, kbuf, j + 2);
+        __builtin_amdgcn_s_setprio(1);
+        scores(j + 1, par ^ 1);   // (past the end: not used)
+        fetch(c.kp, kbuf[KB == 2 ? (j + 1) & 1 : 0], j + 1 + KB, kid);
         lds_barrier();
+        uint8_t* vj = vbuf[VB == 2 ? j & 1 : 0];
+        const uint8_t* v = vj + w * QUARTER + 16 * l;
+        if constexpr (VB == 1) landed<NJ>();   // all but K of page j + 2
         values(par, [&](int d, int s) __attribute__((always_inline)) {
-            const u2 r = *(const u2*)(v + w * QUARTER + KIB * d + 16 * l + 8 * s);
+            const u2 r = *(const u2*)(v + KIB * d + 8 * s);
             const h2 f = s ? s23 : s01;
             const h4 f0 = {f[0], f[0], f[0], f[0]}, f1 = {f[1], f[1], f[1], f[1]};
             return cat_h4(codes4(r[0]) * f0, codes4(r[1]) * f1);
         });
-        fetch(c.vp, vto, j + 2);
+        fetch(c.vp, vj, j + VB, vid);
     };
-    // the open page comes first: its scores are there
-    if (np > 0 && !tail) {
-        scores(0, 0, p0 * kv8::PAGE + kv8::PAGE - 1 > clear);
-        fetch(c.kp, kbuf, 1);
-        fetch(c.vp, vbuf1, 1);
-    }
-    lds_barrier();
+    if (np > 0) asm volatile("" : "+v"(scl));
     int par = 0;
     if (tail) {
-        settle(0);
-        weights(0);
-        if (np > 0) {
-            scores(0, 1, p0 * kv8::PAGE + kv8::PAGE - 1 > clear);
-            fetch(c.kp, kbuf, 1);
-            fetch(c.vp, vbuf1, 1);
-        }
         lds_barrier();
+        weights(0);
+        par = 1;
+    }
+    if (np > 0) {
+        if constexpr (VB == 1) landed<0>();
+        scores(0, par);
+        fetch(c.kp, kbuf[0], KB, page_of(KB));
+        fetch(c.vp, vbuf[VB - 1], VB - 1, page_of(VB - 1));
+    }
+    lds_barrier();
+    if (tail) {
         const int have = total - closed * kv8::PAGE;   // rows that are not there hold anything
         values(0, [&](int d, int s) __attribute__((always_inline)) {
-            h8 v = ld_h8(c.tv + open + KIB * d + 8 * s);
+            h8 v = AHEAD ? ahead_v[AHEAD ? d : 0][s] : ld_h8(c.tv + open + KIB * d + 8 * s);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (32 * s + 16 * (i >> 2) + 4 * g + (i & 3) >= have) v[i] = (_Float16)0.f;
             return v;
         });
-        par = 1;
     }
-    for (int j = 0; j < np; j += 2) {
-        step(j, par, vbuf0, vbuf0);
-        if (j + 1 < np) step(j + 1, par ^ 1, vbuf1, vbuf1);
-    }
+    for (int j = 0; j < np; ++j) step(j, (j + par) & 1);
     landed<0>();   // the fetches past the end
 
-    // ---- sums over the waves' keys, then the rows out
+    // ---- sums over the key blocks, then the rows out
 #pragma unroll
-    for (int x = 0; x < RB; ++x) {
-        const float sum = sum_xor32(sum_xor16(l_run[x]));
-        if (l < 16) lbuf[16 * x + l][w] = sum;
-    }
+    for (int x = 0; x < RB; ++x) lbuf[16 * x + lr][w] = sum_xor32(sum_xor16(l_run[x]));
     lds_barrier();
     if (u.ns > 1) {
         const int nrec = kv8::max_records(wgs), rec = u.rec + kv8::record(split, u.nrb, rb, nkv, kh);
@@ -459,9 +569,9 @@ __global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, K
             const int row = 16 * x + lr;
             if (r0 + row >= R) continue;
             const f4 s4 = *(const f4*)lbuf[row];
-            if (w == 0 && g == 0) ml[row] = f2{m_run[x], (s4[0] + s4[1]) + (s4[2] + s4[3])};
+            if (w == 0 && g == 0) ml[row] = f2{top[x] == -INFINITY ? -INFINITY : -neg[x], (s4[0] + s4[1]) + (s4[2] + s4[3])};
 #pragma unroll
-            for (int d = 0; d < ND; ++d) *(f4*)(po + (size_t)row * HD + w * (HD / 4) + 16 * d + 4 * g) = o[x][d];
+            for (int d = 0; d < ND; ++d) *(f4*)(po + (size_t)row * HD + 16 * (ND * w + d) + 4 * g) = o[x][d];
         }
         return;
     }
@@ -471,12 +581,13 @@ __global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, K
         if (r >= R) continue;
         const f4 s4 = *(const f4*)lbuf[16 * x + lr];
         const float inv = 1.0f / ((s4[0] + s4[1]) + (s4[2] + s4[3]));
-        const int t = r / G;
-        OutT* to = out + (size_t)(u.t0 + t) * ots + (size_t)(kh * G + r - t * G) * HD;
+        const int t = r / G, h = kh * G + r - t * G;
+        const float* gates = q + (size_t)(u.t0 + t) * qts + (size_t)h * 2 * HD + HD;
+        OutT* to = out + (size_t)(u.t0 + t) * ots + (size_t)h * HD;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const int dim = w * (HD / 4) + 16 * d + 4 * g;
-            const f4 gate = ld_f4(qrow[x] + HD + dim);
+            const int dim = 16 * (ND * w + d) + 4 * g;
+            const f4 gate = ld_f4(gates + dim);
             f4 v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = o[x][d][i] * inv * sigmoid_hw(gate[i]);
@@ -485,60 +596,92 @@ __global__ __launch_bounds__(256, RB <= 2 ? 2 : 1) void attn_kv8_kernel(Kv8 c, K
     }
 }
 
-// Joins the records of sequences with more than one split. An item is (group of rows, row, 64 dims); thread = (split lane of
-// 16, 4 dims). The launch is as many workgroups as there can be items, or fewer, each taking several.
-template <int HD, int ROWS, class OutT>
+// Joins the records of sequences with more than one split. An item is (group of rows, row, 4 DL dims); thread = (split lane of
+// 256 / DL, 4 dims), NB records in flight a thread; rows: those that a group can have. The launch is as many workgroups as there
+// can be items, or fewer, each taking several.
+template <int HD, int ROWS, int DL, class OutT>
 __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q, int qts,
                                                              int nh, OutT* __restrict__ out, int ots,
-                                                             const float* __restrict__ part, int wgs) {
-    constexpr int SL = 16, DQ = HD / 64;
-    __shared__ float red_m[SL], red_l[SL];
-    __shared__ __align__(16) f4 red_o[SL][16];
-    const int nkv = c.nkv, G = nh / nkv, tid = threadIdx.x, l = tid & 63, sg = tid >> 4, dl = tid & 15;
+                                                             const float* __restrict__ part, int wgs, int rows) {
+    constexpr int SL = 256 / DL, DQ = HD / (4 * DL), NB = 4;
+    __shared__ float red_m[4], red_l[4][DL];
+    __shared__ __align__(16) f4 red_o[4][DL];
+    const int nkv = c.nkv, G = nh / nkv, tid = threadIdx.x, l = tid & 63, sg = tid / DL, dl = tid % DL;
     const Kv8Seq s0 = kv8_seq(b, l);
     const int chunk = call_chunk<ROWS>(b, s0, G, nkv, wgs, l);
     const int nrec = kv8::max_records(wgs);
+    // weight of a record or partial result whose maximum is m, against the largest M
+    auto share = [](float m, float sum, float M) { return m == -INFINITY ? (sum == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(m - M); };
     for (int item = blockIdx.x;; item += gridDim.x) {
-        const int dq = item % DQ, row = item / DQ % ROWS;
-        const Found u = find<ROWS, true>(b, s0, G, nkv, chunk, item / (DQ * ROWS), l);
+        const int dq = item % DQ, row = item / DQ % rows;
+        const Found u = find<ROWS, true>(b, s0, G, nkv, chunk, item / (DQ * rows), l);
         if (!u.any) return;
         const int kh = u.at % nkv, rb = u.at / nkv, r = rb * ROWS + row;
         if (r >= u.n * G) continue;   // (whole workgroup)
         const int t = r / G, h = kh * G + r - t * G, need = (u.len + t) / kv8::PAGE / chunk + 1;
+        const float* base = part + (size_t)nrec * ROWS * 2;
         float m = -INFINITY, sum = 0.f;
         f4 o = f4{};
-        for (int s = sg; s < need; s += SL) {
-            const size_t at = (size_t)(u.rec + kv8::record(s, u.nrb, rb, nkv, kh)) * ROWS + row;
-            const f2 ml = *((const f2*)part + at);
-            const f4 v = ld_f4(part + (size_t)nrec * ROWS * 2 + at * HD + 64 * dq + 4 * dl);
-            const float mn = fmaxf(m, ml[0]);
-            const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-            const float e = ml[0] == -INFINITY ? (ml[1] == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(ml[0] - mn);
-            sum = sum * a + ml[1] * e;
+        for (int s = sg; s < need; s += SL * NB) {   // (past the last record: the last again, uncounted)
+            f2 ml[NB];
+            f4 v[NB];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = o[i] * a + v[i] * e;
-            m = mn;
+            for (int i = 0; i < NB; ++i) {
+                const size_t at = (size_t)(u.rec + kv8::record(min(s + i * SL, need - 1), u.nrb, rb, nkv, kh)) * ROWS + row;
+                ml[i] = *((const f2*)part + at);
+                v[i] = ld_f4(base + at * HD + 4 * (DL * dq + dl));
+            }
+            float M = m;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                if (s + i * SL >= need) ml[i] = f2{-INFINITY, 0.f};
+                M = fmaxf(M, ml[i][0]);
+            }
+            const float a = share(m, sum, M);
+            sum *= a;
+            o *= a;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const float e = share(ml[i][0], ml[i][1], M);
+                sum += ml[i][1] * e;
+                if (s + i * SL < need) o += v[i] * e;
+            }
+            m = M;
+        }
+        // the split lanes of a wave, then the four waves
+        float M = max_xor32(m);
+        if constexpr (DL == 8) {
+            M = max_xor16(M);
+            M = fmaxf(M, dppc<0x128>(M));   // row_ror 8
+        }
+        const float e = share(m, sum, M);
+        float all[5] = {sum * e, o[0] * e, o[1] * e, o[2] * e, o[3] * e};
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            all[i] = sum_xor32(all[i]);
+            if constexpr (DL == 8) {
+                all[i] = sum_xor16(all[i]);
+                all[i] += dppc<0x128>(all[i]);
+            }
         }
         __syncthreads();   // the last item's partial results have been read
-        if (dl == 0) {
-            red_m[sg] = m;
-            red_l[sg] = sum;
+        if (l < DL) {
+            if (l == 0) red_m[tid >> 6] = M;
+            red_l[tid >> 6][l] = all[0];
+            red_o[tid >> 6][l] = f4{all[1], all[2], all[3], all[4]};
         }
-        red_o[sg][dl] = o;
         __syncthreads();
-        if (sg == 0) {
-            const int live = min(need, SL);
-            float M = -INFINITY, L = 0.f;
-            for (int s = 0; s < live; ++s) M = fmaxf(M, red_m[s]);
+        if (tid < DL) {
+            M = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+            float L = 0.f;
             f4 v = f4{};
-            for (int s = 0; s < live; ++s) {
-                const float e = red_m[s] == -INFINITY ? (red_l[s] == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(red_m[s] - M);
-                L += red_l[s] * e;
-                const f4 y = red_o[s][dl];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] += y[i] * e;
+            for (int i = 0; i < 4; ++i) {
+                const float f = share(red_m[i], red_l[i][tid], M);
+                L += red_l[i][tid] * f;
+                v += red_o[i][tid] * f;
             }
-            const int dim = 64 * dq + 4 * dl;
+            const int dim = 4 * (DL * dq + dl);
             const f4 gate = ld_f4(q + (size_t)(u.t0 + t) * qts + (size_t)h * 2 * HD + HD + dim);
             const float inv = 1.0f / L;
 #pragma unroll
@@ -550,9 +693,9 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
 
 // Row blocks of a workgroup and the workgroups a call is shared out to
 struct Form { int rb, wgs; };
-Form form(int max_nt, int G) {
+Form form(int max_nt, int G, bool f16out) {
     const long rows = (long)max_nt * G;
-    return rows <= 16 ? Form{1, 512} : rows <= 32 ? Form{2, 512} : Form{4, 256};
+    return rows <= 16 ? Form{1, 512} : rows <= 32 ? Form{2, 512} : f16out ? Form{4, 512} : Form{3, 512};
 }
 // Row blocks, over all KV heads, that the sequences of a call can have
 long max_groups(const Form& f, int nseq, int ntok, int max_nt, int G, int nkv) {
@@ -565,29 +708,39 @@ hipError_t launch(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int 
                   float* part, const Form& f, hipStream_t st) {
     const long groups = max_groups(f, b.nseq, b.ntok, b.max_nt, nh / c.nkv, c.nkv);
     attn_kv8_kernel<HD, RB, sizeof(OutT) == 4, OutT>
-        <<<dim3((unsigned)(groups + f.wgs)), 256, 0, st>>>(c, b, q, qts, nh, scale, out, ots, part, f.wgs);
+        <<<dim3((unsigned)(groups + f.wgs + 1)), 256, 0, st>>>(c, b, q, qts, nh, scale, out, ots, part, f.wgs);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // split groups have two splits at least, so there are at most max_records / 2 of them
-    const long items = std::min(groups, (long)kv8::max_records(f.wgs) / 2) * 16 * RB * (HD / 64);
-    attn_kv8_merge_kernel<HD, 16 * RB, OutT>
-        <<<dim3((unsigned)std::min(items, 4096L)), 256, 0, st>>>(c, b, q, qts, nh, out, ots, part, f.wgs);
+    // split groups have two splits at least, so there are at most max_records / 2 of them. Few rows: many splits, so many
+    // split lanes
+    const int rows = (int)std::min((long)16 * RB, (long)b.max_nt * (nh / c.nkv));
+    const long split_rows = std::min(groups, (long)kv8::max_records(f.wgs) / 2) * rows;
+    if (split_rows * (HD / 32) <= 1024)
+        attn_kv8_merge_kernel<HD, 16 * RB, 8, OutT><<<dim3((unsigned)(split_rows * (HD / 32))), 256, 0, st>>>(
+            c, b, q, qts, nh, out, ots, part, f.wgs, rows);
+    else
+        attn_kv8_merge_kernel<HD, 16 * RB, 32, OutT><<<dim3((unsigned)std::min(split_rows * (HD / 128), 2048L)), 256, 0, st>>>(
+            c, b, q, qts, nh, out, ots, part, f.wgs, rows);
     return hipGetLastError();
 }
 template <int HD, class OutT>
 hipError_t launch_rb(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, OutT* out, int ots,
                      float* part, hipStream_t st) {
-    const Form f = form(b.max_nt, nh / c.nkv);
+    const Form f = form(b.max_nt, nh / c.nkv, sizeof(OutT) == 2);
     if (f.rb == 1) return launch<HD, 1, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
     if (f.rb == 2) return launch<HD, 2, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
-    return launch<HD, 4, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
+    return launch<HD, sizeof(OutT) == 2 ? 4 : 3, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
 }
 
 }  // namespace
 
 size_t attn_kv8_scratch_bytes(int max_nt, int hd, int nh, int nkv) {
-    const Form f = form(max_nt, nh / nkv);
-    return (size_t)kv8::max_records(f.wgs) * 16 * f.rb * (hd + 2) * sizeof(float);
+    size_t most = 0;
+    for (bool f16out : {false, true}) {
+        const Form f = form(max_nt, nh / nkv, f16out);
+        most = std::max(most, (size_t)kv8::max_records(f.wgs) * 16 * f.rb * (hd + 2) * sizeof(float));
+    }
+    return most;
 }
 hipError_t launch_attn_kv8(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, void* out,
                            int ots, bool f16out, float* part, hipStream_t st) {
