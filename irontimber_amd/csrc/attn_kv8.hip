@@ -65,15 +65,17 @@ __device__ __forceinline__ int prefix_sum(int v, int l) {   // inclusive, over t
 template <int ROWS>
 __device__ __forceinline__ int call_chunk(const Kv8Batch& b, const Kv8Seq& s0, int G, int nkv, int wgs, int l) {
     if (b.nseq == 1) {   // (the sum of one, without the exchanges)
-        const float one = (float)((__builtin_amdgcn_readfirstlane(s0.n) * G + ROWS - 1) / ROWS) * (float)__builtin_amdgcn_readfirstlane(s0.pages);
-        return kv8::chunk_pages(one * (float)nkv, wgs);
+        const float blocks = (float)((__builtin_amdgcn_readfirstlane(s0.n) * G + ROWS - 1) / ROWS);
+        return kv8::chunk_pages(blocks * (float)__builtin_amdgcn_readfirstlane(s0.pages) * (float)nkv, blocks * (float)nkv, wgs);
     }
-    float sum = 0.f;
+    float sum = 0.f, blocks = 0.f;
     for (int i0 = 0; i0 < b.nseq; i0 += 64) {
         const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
-        sum += wave_sum((float)((s.n * G + ROWS - 1) / ROWS) * (float)s.pages);
+        const float nrb = (float)((s.n * G + ROWS - 1) / ROWS);
+        sum += wave_sum(nrb * (float)s.pages);
+        blocks += wave_sum(nrb);
     }
-    return kv8::chunk_pages(__builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sum))) * (float)nkv, wgs);
+    return kv8::chunk_pages(readlane_f(sum, 0) * (float)nkv, readlane_f(blocks, 0) * (float)nkv, wgs);
 }
 
 // What is found for a workgroup, in scalar registers: its sequence, the index of its unit (main kernel) or of its group of
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
         return q + (size_t)(u.t0 + t) * qts + (size_t)(kh * G + r - t * G) * 2 * HD;
     };
 
-    // What the first wait is not for goes out before it: q, and with one row block what the open page takes
+    // What the first wait is not for goes out before it: q, and the open page's keys
     const size_t open = ((size_t)(u.seq * 2 + (closed & 1)) * nkv + kh) * (kv8::PAGE * HD) + w * QUARTER + 16 * l;
     f4 y[RB][4];
     if (w < NJ) {
@@ -229,20 +231,10 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
             for (int e = 0; e < 4; ++e) y[x][e] = ld_f4(at + 32 * (e >> 1) + 4 * (e & 1));
         }
     }
-    constexpr bool AHEAD = RB == 1;
-    h8 ahead_k[AHEAD ? NK : 1], ahead_v[AHEAD ? ND : 1][2];
-    f4 ahead_q[AHEAD ? NK : 1][2];
-    if (AHEAD && tail) {
+    h8 ko[NK];
+    if (tail) {
 #pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-            ahead_k[ks] = ld_h8(c.tk + open + KIB * (ks >> 1) + 8 * (ks & 1));
-            ahead_q[ks][0] = ld_f4(qrow(0) + 32 * ks + 8 * g);
-            ahead_q[ks][1] = ld_f4(qrow(0) + 32 * ks + 8 * g + 4);
-        }
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) ahead_v[d][e] = ld_h8(c.tv + open + KIB * d + 8 * e);
+        for (int ks = 0; ks < NK; ++ks) ko[ks] = ld_h8(c.tk + open + KIB * (ks >> 1) + 8 * (ks & 1));
     }
     if (np > 0) {
         load_ids(0);
@@ -321,16 +313,59 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
             }
         }
         lds_barrier();
+        auto row_max = [&](int x) __attribute__((always_inline)) {
+            const f4 m4 = *(const f4*)lbuf[16 * x + lr];
+            return NJ == 4 ? fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) : fmaxf(m4[0], m4[1]);
+        };
+        auto row_exp = [&](int x) __attribute__((always_inline)) { return max(__builtin_amdgcn_frexp_expf(row_max(x)), -100); };   // (so that 2^-ex is finite)
+        // |q| / 2^ex < 1; the highest digit at most 127 for all digits' roundings
+        constexpr float TOP = PAIRS ? 127 * 65536.f : 127 * 256.f;
+        constexpr uint32_t BIAS = PAIRS ? 0x808080u : 0x8080u;
+        // The open page comes first. Its keys are f16, so its products take q as f16 pairs (each row times the power of two that
+        // takes its largest value to 2^13 .. 2^14). Wave w makes those of its dims too: all of the row in each wave is four times
+        // the code, and code that few workgroups run is as slow as its fetching (16 rows 2.4, 32 rows 6.5 us).
         u4* meet = VB == 2 ? (u4*)vbuf[VB - 1] : (u4*)pbuf;
-        static_assert(VB == 2 || sizeof(pbuf) >= NJ * DG * KIB, "room for a row block's digits");
+        static_assert(VB == 2 || sizeof(pbuf) >= 4 * NJ * KIB, "room for a row block's pairs");
+        if (tail) {
+#pragma unroll
+            for (int x = 0; x < RB; ++x) {
+                const int ex = 14 - row_exp(x);
+                if (w < NJ) {
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks) {
+                        const f4* z = &y[x][2 * ks];
+                        h8 hi, lo;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            h2 h, e;
+                            split2(f2{__builtin_amdgcn_ldexpf(z[i >> 1][2 * (i & 1)] * sign, ex),
+                                      __builtin_amdgcn_ldexpf(z[i >> 1][2 * (i & 1) + 1] * sign, ex)}, neg1, h, e);
+                            hi[2 * i] = h[0];
+                            hi[2 * i + 1] = h[1];
+                            lo[2 * i] = e[0];
+                            lo[2 * i + 1] = e[1];
+                        }
+                        meet[(2 * w + ks) * 128 + l] = __builtin_bit_cast(u4, hi);
+                        meet[(2 * w + ks) * 128 + 64 + l] = __builtin_bit_cast(u4, lo);
+                    }
+                }
+                lds_barrier();
+                f4 a = {}, a2 = {};
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) {
+                    a = mfma16x16x32(ko[ks], ld_h8(meet + ks * 128 + l), a);
+                    a2 = mfma16x16x32(ko[ks], ld_h8(meet + ks * 128 + 64 + l), a2);
+                }
+                const f4 both = a + a2;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[x][i] = both[i] * (TOP * 0x1p-14f);   // in units of back
+                lds_barrier();
+            }
+        }
 #pragma unroll
         for (int x = 0; x < RB; ++x) {
-            const f4 m4 = *(const f4*)lbuf[16 * x + lr];
-            const float m = NJ == 4 ? fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) : fmaxf(m4[0], m4[1]);
-            const int ex = max(__builtin_amdgcn_frexp_expf(m), -100);   // (so that 2^-ex is finite)
-            // |q| / 2^ex < 1; the highest digit at most 127 for all digits' roundings
-            constexpr float TOP = PAIRS ? 127 * 65536.f : 127 * 256.f;
-            constexpr uint32_t BIAS = PAIRS ? 0x808080u : 0x8080u;
+            const float m = row_max(x);
+            const int ex = row_exp(x);
             const float to = __builtin_amdgcn_ldexpf(TOP * sign, -ex);
             back[x] = m < INFINITY ? fmaxf(__builtin_amdgcn_ldexpf(size / TOP, ex), 1e-30f) : NAN;
             if (w < NJ) {
@@ -358,44 +393,6 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
             lds_barrier();
         }
     }
-    // The open page comes first. Its keys are f16, so its products take q as f16 pairs (each row times the power of two that takes
-    // its largest value to 2^13 .. 2^14).
-    if (tail) {
-        constexpr float TOP = PAIRS ? 127 * 65536.f : 127 * 256.f;
-#pragma unroll
-        for (int x = 0; x < RB; ++x) {
-            const f4 m4 = *(const f4*)lbuf[16 * x + lr];
-            const float m = NJ == 4 ? fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) : fmaxf(m4[0], m4[1]);
-            const int ex = 14 - max(__builtin_amdgcn_frexp_expf(m), -100);
-            const float* at = qrow(x) + 8 * g;
-            f4 a = {}, a2 = {};
-#pragma unroll
-            for (int ks = 0; ks < NK; ++ks) {
-                const h8 k = AHEAD ? ahead_k[AHEAD ? ks : 0] : ld_h8(c.tk + open + KIB * (ks >> 1) + 8 * (ks & 1));
-                const f4 y[2] = {AHEAD ? ahead_q[AHEAD ? ks : 0][0] : ld_f4(at + 32 * ks),
-                                 AHEAD ? ahead_q[AHEAD ? ks : 0][1] : ld_f4(at + 32 * ks + 4)};
-                h8 hi, lo;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    h2 h, e;
-                    split2(f2{__builtin_amdgcn_ldexpf(y[i >> 1][2 * (i & 1)] * sign, ex),
-                              __builtin_amdgcn_ldexpf(y[i >> 1][2 * (i & 1) + 1] * sign, ex)}, neg1, h, e);
-                    hi[2 * i] = h[0];
-                    hi[2 * i + 1] = h[1];
-                    lo[2 * i] = e[0];
-                    lo[2 * i + 1] = e[1];
-                }
-                a = mfma16x16x32(k, hi, a);
-                a2 = mfma16x16x32(k, lo, a2);
-            }
-            const f4 both = a + a2;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[x][i] = both[i] * (TOP * 0x1p-14f);   // in units of back
-        }
-        mask_keys(closed);
-        maxima(0);
-    }
-
     // Scores of the wave's 16 keys of full page j
     auto scores = [&](int j, int par) __attribute__((always_inline)) {
         const h2 two = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(w & 2 ? scl[1] : scl[0], j & 63));
@@ -530,7 +527,14 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     };
     if (np > 0) asm volatile("" : "+v"(scl));
     int par = 0;
+    h8 vo[ND][2];
     if (tail) {
+        mask_keys(closed);
+        maxima(0);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) vo[d][e] = ld_h8(c.tv + open + KIB * d + 8 * e);
         lds_barrier();
         weights(0);
         par = 1;
@@ -545,7 +549,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     if (tail) {
         const int have = total - closed * kv8::PAGE;   // rows that are not there hold anything
         values(0, [&](int d, int s) __attribute__((always_inline)) {
-            h8 v = AHEAD ? ahead_v[AHEAD ? d : 0][s] : ld_h8(c.tv + open + KIB * d + 8 * s);
+            h8 v = vo[d][s];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (32 * s + 16 * (i >> 2) + 4 * g + (i & 3) >= have) v[i] = (_Float16)0.f;

@@ -26,9 +26,10 @@ IT_HD int v_elem(int row, int dim) {
 }
 
 // Pages per split of an attention call: `work` is the sum over sequences and KV heads of row blocks times pages, shared
-// out to about `wgs` workgroups. The same in the partial and the merge kernel.
-IT_HD int chunk_pages(float work, int wgs) {
-    const float c = work / (float)wgs;
+// out to about `wgs` workgroups; each of the `groups` row blocks may leave one split that is not full, which the count allows
+// for while they are few. The same in the partial and the merge kernel.
+IT_HD int chunk_pages(float work, float groups, int wgs) {
+    const float room = (float)wgs - groups, c = work / (room < 0.5f * (float)wgs ? 0.5f * (float)wgs : room);
     if (!(c < 33554432.0f)) return 33554432;   // no sequence has more pages
     const int i = (int)c;
     return (float)i < c ? i + 1 : i < 1 ? 1 : i;

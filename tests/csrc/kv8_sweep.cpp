@@ -31,17 +31,18 @@ int main() {
     for (int it = 0; it < 20000; ++it) {
         const int nseq = 1 + rnd(it % 3 ? 8 : 130), nkv = 1 + rnd(8), wgs = it % 2 ? 256 : 512, most = 1 << (1 + rnd(it % 7 ? 12 : 25));
         std::vector<int> nrb(nseq), pages(nseq);
-        float sum = 0.f;
+        float sum = 0.f, blocks = 0.f;
         for (int i0 = 0; i0 < nseq; i0 += 64) {
             float part = 0.f;
             for (int i = i0; i < nseq && i < i0 + 64; ++i) {
                 nrb[i] = rnd(4) ? 1 + rnd(it % 5 ? 3 : 500) : 0;
                 pages[i] = 1 + rnd(most);
                 part += (float)nrb[i] * (float)pages[i];
+                blocks += (float)nrb[i];
             }
             sum += part;
         }
-        const int chunk = kv8::chunk_pages(sum * (float)nkv, wgs);
+        const int chunk = kv8::chunk_pages(sum * (float)nkv, blocks * (float)nkv, wgs);
         if (chunk < 1) die("chunk", chunk, it);
         long units = 0, groups = 0, recs = 0, split_groups = 0;
         for (int i = 0; i < nseq; ++i) {
