@@ -13,20 +13,28 @@
 namespace it {
 namespace {
 
+// The largest size among 8 values, as f16 bits (of two halves: the packed maximum), which order as the sizes do; 0x7C00 and up:
+// one is not finite.
+__device__ __forceinline__ uint32_t sizes(h8 x) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    const u4 u = __builtin_bit_cast(u4, x) & 0x7FFF7FFFu;
+    const us2 a = __builtin_elementwise_max(__builtin_bit_cast(us2, (uint32_t)u[0]), __builtin_bit_cast(us2, (uint32_t)u[1]));
+    const us2 b = __builtin_elementwise_max(__builtin_bit_cast(us2, (uint32_t)u[2]), __builtin_bit_cast(us2, (uint32_t)u[3]));
+    const us2 m = __builtin_elementwise_max(a, b);
+    return m[0] > m[1] ? m[0] : m[1];
+}
+__device__ __forceinline__ float size_of(uint32_t bits) { return (float)__builtin_bit_cast(_Float16, (unsigned short)bits); }
 // An infinity is stored as the largest f16, a NaN as 0: a value that no query may see must not reach its products.
-__device__ __forceinline__ _Float16 finite(_Float16 x) {
-    const _Float16 top = (_Float16)65504.f;
-    return x != x ? (_Float16)0.f : x > top ? top : x < -top ? -top : x;
-}
 __device__ __forceinline__ h8 finite8(h8 x) {
+    if (__any(sizes(x) >= 0x7C00u)) {
+        const _Float16 top = (_Float16)65504.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = finite(x[i]);
+        for (int i = 0; i < 8; ++i) {
+            const _Float16 v = x[i];
+            x[i] = v != v ? (_Float16)0.f : v > top ? top : v < -top ? -top : v;
+        }
+    }
     return x;
-}
-__device__ __forceinline__ float largest(h8 x, float m) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf((float)x[i]));
-    return m;
 }
 // A block's scale from its largest size. amax has 11 bits and 127 * s 11, so they differ by 2^-15 or not at all, and the
 // rounded quotient falls on the same side of s as the exact one.
@@ -35,121 +43,174 @@ __device__ __forceinline__ float block_scale(float amax) {
     if (t < 0x1p-21f) return fmaxf(ceilf(t * 0x1p24f), 1.0f) * 0x1p-24f;
     return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, t) + 0xFFFFFu) & ~0xFFFFFu);
 }
-// x / s to the nearest step, ties to even; likewise no quotient is nearer to a tie than f32 tells. s is above 512 only
-// as 576, of which 113 steps still are f16.
-__device__ __forceinline__ uint32_t code(_Float16 x, float s) {
-    const float top = s > 512.f ? 113.f : 127.f;
-    return (uint32_t)(int)(fminf(fmaxf(rintf((float)x / s), -top), top) + 128.f);
+// Steps of a block: x / s to the nearest, ties to even, at most 127 (113 at s = 576, the one scale above 512: more is no f16).
+// The quotient is x * (1 / s) with one correction by the residual, which is exact: a tie comes out as one, and no other
+// quotient is nearer to a tie than 2^-13. 
+struct Steps {
+    float s, inv, top;
+    __device__ __forceinline__ explicit Steps(float scale) : Steps(scale, 1.0f / scale) {}
+    __device__ __forceinline__ Steps(float scale, float inverse) : s(scale), inv(inverse), top(scale > 512.f ? 113.f : 127.f) {}
+    __device__ __forceinline__ float of(_Float16 v) const {
+        const float x = (float)v, q = x * inv;
+        return __builtin_amdgcn_fmed3f(rintf(__builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q)), -top, top) + 128.f;
+    }
+};
+// Codes of four values, the first lowest
+__device__ __forceinline__ uint32_t codes_of(const Steps& t, _Float16 a, _Float16 b, _Float16 c, _Float16 d) {
+    uint32_t u = __builtin_amdgcn_cvt_pk_u8_f32(t.of(a), 0, 0);
+    u = __builtin_amdgcn_cvt_pk_u8_f32(t.of(b), 1, u);
+    u = __builtin_amdgcn_cvt_pk_u8_f32(t.of(c), 2, u);
+    return __builtin_amdgcn_cvt_pk_u8_f32(t.of(d), 3, u);
 }
 
-// Workgroup = (sequence, touched page, KV head, K or V). Quantises the page if the call fills it; the workgroups of the
-// first two pages also write the new rows of the last two pages to the open buffer, each those of its own half of it,
-// after its page's old open rows have been read (a half is read and written by one workgroup only).
-// Bound by bytes: two read and one written a value (two where a page stays open).
+// Workgroup = (sequence, touched page or half of the open buffer, KV head, K or V). A page is quantised if the call fills it;
+// a half takes the new rows of its page among the last two. Where it still holds old rows that the first page needs and that
+// another page's rows replace, the first page's workgroup writes it, after it has read them.
+// Both kinds work in the page's order, which the old open rows have already. New rows of V get there through LDS.
+// A wave a KiB of codes, 16 values a lane: with 4 waves of 64 values each the call was as slow as the fetching of the code that
+// each CU then runs once or twice (8192 rows 23.5 us, so 12.4).
+// Bound by bytes, two read and one written a value, and in short calls by three dependent round trips (bounds, rows, stores).
 template <int HD>
-__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8 c, Kv8Batch b, const _Float16* __restrict__ k,
-                                                         const _Float16* __restrict__ v, int kts) {
-    constexpr int CH = HD / 8, PITCH = HD + 8;   // (rows four apart in LDS: 16 banks apart)
+__global__ __launch_bounds__(4 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, const _Float16* __restrict__ k,
+                                                            const _Float16* __restrict__ v, int kts) {
+    constexpr int NT = 4 * HD, CH = HD / 8, PITCH = HD + 8;   // (rows four apart in LDS: 16 banks apart)
     __shared__ __align__(16) _Float16 tile[kv8::PAGE * PITCH];
-    __shared__ float vs[4];
-    const int i = blockIdx.z, kh = blockIdx.y >> 1, which = blockIdx.y & 1, j = blockIdx.x;
+    __shared__ float most[HD / 16][4];
+    const int i = blockIdx.z, kh = blockIdx.y >> 1, which = blockIdx.y & 1, j = (int)blockIdx.x - 2;   // -2, -1: halves
     const Kv8Seq s = kv8_seq(b, i);
-    const int p = s.len / kv8::PAGE + j, total = s.len + s.n;
-    if (s.n == 0 || s.bad || (long)p * kv8::PAGE >= total) return;
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
-    const int row0 = p * kv8::PAGE;
+    if (s.n == 0 || s.bad) return;
+    const int first = s.len / kv8::PAGE, p = first + j, total = s.len + s.n, last = (total - 1) / kv8::PAGE;
+    if (p > last) return;
+    const bool behind = s.len % kv8::PAGE != 0 && last >= first + 2;   // half first % 2 is written behind page `first`
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, lr = l & 15;
     const _Float16* src = (which ? v : k) + (size_t)s.t0 * kts + (size_t)kh * HD;   // token t at t * kts
     _Float16* open = (which ? c.tv : c.tk) + ((size_t)i * 2 * c.nkv + kh) * (kv8::PAGE * HD);
     const size_t half = (size_t)c.nkv * kv8::PAGE * HD;
-    if (row0 + kv8::PAGE <= total) {
+    // Rows from .. to - 1 of V, from row0 on, into the tile, a row of 8 dims a thread and turn
+    auto stage = [&](int row0, int from, int to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int row = row0 + (n * NT + tid) / CH, ch = tid % CH;
+            if (row >= from && row < to)
+                *(h8*)(tile + (row - row0) * PITCH + 8 * ch) = finite8(ld_h8(src + (size_t)(row - s.len) * kts + 8 * ch));
+        }
+    };
+    // This lane's four rows of each block and one dim of dim block w, from the tile where they are from .. to - 1, else x
+    auto pick = [&](int row0, int from, int to, h8 (&x)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int r = 16 * (e >> 2) + 4 * g + (e & 3);
+            const _Float16 z = tile[r * PITCH + 16 * w + lr];
+            x[e >> 3][e & 7] = row0 + r >= from && row0 + r < to ? z : x[e >> 3][e & 7];
+        }
+    };
+    const int row0 = p * kv8::PAGE;
+    if (j >= 0 && row0 + kv8::PAGE <= total) {
         const int id = b.table[(size_t)i * b.max_pages + p];
         const bool known = (unsigned)id < (unsigned)c.npages;
         const size_t unit = known ? (size_t)id * c.nkv + kh : 0;
-        const _Float16* old = open + (p & 1) * half;
+        const _Float16* old = open + (p & 1) * half + (w * 64 + l) * 16;
+        h8 x[2] = {};
         if (!which) {
-            // wave = block: each lane holds a row's runs of 8 dims as the page orders them
-            const int row = 16 * w + (l & 15), t = row0 + row - s.len;
-            h8 x[CH / 4];
-            float m = 0.f;
+            // wave = (block, 64 dims): each lane holds two runs of 8 dims of a row
+            const int a = w / (HD / 64), row = row0 + 16 * a + lr, dim = 64 * (w % (HD / 64)) + 8 * g;
 #pragma unroll
-            for (int ks = 0; ks < CH / 4; ++ks) {
-                const _Float16* at = t >= 0 ? src + (size_t)t * kts + 32 * ks + 8 * (l >> 4)
-                                            : old + ((w * (HD / 64) + (ks >> 1)) * 64 + l) * 16 + 8 * (ks & 1);
-                x[ks] = ld_h8(at);
-            }
-#pragma unroll
-            for (int ks = 0; ks < CH / 4; ++ks) {
-                x[ks] = finite8(x[ks]);
-                m = largest(x[ks], m);
-            }
-            const float sc = block_scale(wave_max(m));
-            if (known) {
-#pragma unroll
-                for (int jj = 0; jj < HD / 64; ++jj) {
-                    u4 y;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const h8 z = x[2 * jj + (e >> 1)];
-                        const int o = 4 * (e & 1);
-                        y[e] = code(z[o], sc) | code(z[o + 1], sc) << 8 | code(z[o + 2], sc) << 16 | code(z[o + 3], sc) << 24;
-                    }
-                    *(u4*)(c.kp + unit * (kv8::PAGE * HD) + ((w * (HD / 64) + jj) * 64 + l) * 16) = y;
-                }
-                if (l == 0) c.sc[unit * 8 + w] = (_Float16)sc;
-            }
-        } else {
-            // wave = block for the rows in; through LDS to four rows of each block and one dim a lane
-            float m = 0.f;
-#pragma unroll
-            for (int n = 0; n < CH / 4; ++n) {
-                const int row = 16 * w + (n * 64 + l) / CH, ch = (n * 64 + l) % CH, t = row0 + row - s.len;
-                h8 x;
-                if (t >= 0) {
-                    x = finite8(ld_h8(src + (size_t)t * kts + 8 * ch));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = old[kv8::v_elem(row, 8 * ch + e)];
-                }
-                m = largest(x, m);
-                *(h8*)(tile + row * PITCH + 8 * ch) = x;
-            }
-            const float sc = block_scale(wave_max(m));
-            if (l == 0) {
-                vs[w] = sc;
-                if (known) c.sc[unit * 8 + 4 + w] = (_Float16)sc;
-            }
+            for (int h = 0; h < 2; ++h)
+                x[h] = finite8(ld_h8(row >= s.len ? src + (size_t)(row - s.len) * kts + dim + 32 * h : old + 8 * h));
+            const float m = wave_max(size_of(max(sizes(x[0]), sizes(x[1]))));
+            if (l == 0) most[w][0] = m;
             __syncthreads();
+            float top = 0.f;
+#pragma unroll
+            for (int n = 0; n < HD / 64; ++n) top = fmaxf(top, most[a * (HD / 64) + n][0]);
+            const Steps t(block_scale(top));
             if (known) {
+                u4 y;
 #pragma unroll
-                for (int db = w; db < HD / 16; db += 4) {
-                    u4 y;
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        const _Float16* z = tile + (16 * a + 4 * (l >> 4)) * PITCH + 16 * db + (l & 15);
-                        y[a] = code(z[0], vs[a]) | code(z[PITCH], vs[a]) << 8 | code(z[2 * PITCH], vs[a]) << 16 |
-                               code(z[3 * PITCH], vs[a]) << 24;
-                    }
-                    *(u4*)(c.vp + unit * (kv8::PAGE * HD) + (db * 64 + l) * 16) = y;
+                for (int e = 0; e < 4; ++e) {
+                    const h8 z = x[e >> 1];
+                    const int o = 4 * (e & 1);
+                    y[e] = codes_of(t, z[o], z[o + 1], z[o + 2], z[o + 3]);
                 }
+                *(u4*)(c.kp + unit * (kv8::PAGE * HD) + (w * 64 + l) * 16) = y;
+                if (l == 0 && w % (HD / 64) == 0) c.sc[unit * 8 + a] = (_Float16)t.s;
+            }
+        } else {
+            if (row0 < s.len) {
+                x[0] = ld_h8(old);
+                x[1] = ld_h8(old + 8);
+            }
+            stage(row0, s.len, total);
+            __syncthreads();
+            pick(row0, s.len, total, x);
+            // largest sizes of the four blocks, lane row g ending with block g, then one lane in four with each wave's
+            float m[4];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                h8 z = {};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] = x[a >> 1][4 * (a & 1) + e];
+                m[a] = size_of(sizes(z));
+            }
+            swap32(m[0], m[2]);
+            swap32(m[1], m[3]);
+            float m0 = fmaxf(m[0], m[2]), m1 = fmaxf(m[1], m[3]);
+            swap16(m0, m1);
+            m0 = fmaxf(m0, m1);
+            m0 = fmaxf(m0, dppc<0xB1>(m0));
+            m0 = fmaxf(m0, dppc<0x4E>(m0));
+            m0 = fmaxf(m0, dppc<0x141>(m0));
+            m0 = fmaxf(m0, dppc<0x140>(m0));
+            if (lr == 0) most[w][2 * (g >> 1) + (g & 1)] = m0;
+            __syncthreads();
+            m0 = most[min(l >> 2, HD / 16 - 1)][l & 3];
+            m0 = fmaxf(m0, dppc<0x124>(m0));   // row_ror 4, 8
+            m0 = fmaxf(m0, dppc<0x128>(m0));
+            const Steps mine(block_scale(max_xor32(max_xor16(m0))));   // of block l % 4
+            if (known && tid < 4) c.sc[unit * 8 + 4 + tid] = (_Float16)mine.s;
+            u4 y;
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const Steps t(readlane_f(mine.s, a), readlane_f(mine.inv, a));
+                const h8 z = x[a >> 1];
+                const int o = 4 * (a & 1);
+                y[a] = codes_of(t, z[o], z[o + 1], z[o + 2], z[o + 3]);
+            }
+            if (known) *(u4*)(c.vp + unit * (kv8::PAGE * HD) + (w * 64 + l) * 16) = y;
+        }
+        __syncthreads();   // old open rows read before the half is written below, and the tile before it is filled anew
+    }
+    if (j > 0 || (j == 0 && !behind)) return;
+    const int parity = j < 0 ? j + 2 : first & 1, pt = last - ((last ^ parity) & 1);   // the half's page among the last two
+    if (pt < first || (j < 0 && behind && parity == (first & 1))) return;
+    const int r0 = pt * kv8::PAGE, from = max(s.len, r0), to = (int)min((long)total, (long)r0 + kv8::PAGE);
+    _Float16* dst = open + (pt & 1) * half;
+    if (!which || to - from <= 4) {
+        for (int n = tid; n < (to - from) * CH; n += NT) {
+            const int row = from + n / CH, ch = n % CH;
+            const h8 x = finite8(ld_h8(src + (size_t)(row - s.len) * kts + 8 * ch));
+            if (!which) {
+                *(h8*)(dst + kv8::k_elem(HD, row - r0, 8 * ch)) = x;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dst[kv8::v_elem(row - r0, 8 * ch + e)] = x[e];
             }
         }
-        __syncthreads();   // old open rows read before the half is written below
+        return;
     }
-    if (j >= 2) return;
-    const int last = (total - 1) / kv8::PAGE, pt = last - ((last ^ p) & 1);   // the page of this half among the last two
-    const int lo = max(s.len, pt * kv8::PAGE), hi = min(total, (pt + 1) * kv8::PAGE);
-    _Float16* to = open + (pt & 1) * half;
-    for (int n = tid; n < (hi - lo) * CH; n += 256) {
-        const int row = lo + n / CH, ch = n % CH;
-        const h8 x = finite8(ld_h8(src + (size_t)(row - s.len) * kts + 8 * ch));
-        const int r = row - pt * kv8::PAGE;
-        if (!which) {
-            *(h8*)(to + kv8::k_elem(HD, r, 8 * ch)) = x;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) to[kv8::v_elem(r, 8 * ch + e)] = x[e];
-        }
+    // many rows of V: through LDS, in whole pieces of the page's order that keep the rows before `from`; the rows from `to` on
+    // hold anything
+    h8* piece = (h8*)(dst + (w * 64 + l) * 16);
+    h8 x[2] = {};
+    if (from > r0) {
+        x[0] = piece[0];
+        x[1] = piece[1];
     }
+    stage(r0, from, to);
+    __syncthreads();
+    pick(r0, from, to, x);
+    piece[0] = x[0];
+    piece[1] = x[1];
 }
 
 // Workgroup = (sequence, page, KV head, K or V): rows first[i] .. of a sequence that holds len[i] rows, as f16.
@@ -258,10 +319,10 @@ static int touched(int rows) { return (int)(((long)rows + 2 * (kv8::PAGE - 1)) /
 
 hipError_t launch_kv8_append(const Kv8& c, const Kv8Batch& b, const uint16_t* k, const uint16_t* v, int kts,
                              hipStream_t st) {
-    const dim3 grid(touched(b.max_nt), 2 * c.nkv, b.nseq);
+    const dim3 grid(2 + touched(b.max_nt), 2 * c.nkv, b.nseq);
     const auto *kk = (const _Float16*)k, *vv = (const _Float16*)v;
-    if (c.hd == 256) kv8_append_kernel<256><<<grid, 256, 0, st>>>(c, b, kk, vv, kts);
-    else kv8_append_kernel<128><<<grid, 256, 0, st>>>(c, b, kk, vv, kts);
+    if (c.hd == 256) kv8_append_kernel<256><<<grid, 1024, 0, st>>>(c, b, kk, vv, kts);
+    else kv8_append_kernel<128><<<grid, 512, 0, st>>>(c, b, kk, vv, kts);
     return hipGetLastError();
 }
 hipError_t launch_kv8_read(const Kv8& c, const Kv8Batch& b, const int* first, uint16_t* k, uint16_t* v, int kts,

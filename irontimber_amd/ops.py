@@ -6,6 +6,7 @@ torch's current stream. Buffer layouts and semantics are those of include/it_att
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -698,7 +699,8 @@ def kv8_cache(npages: int, nseq: int, nkv: int, hd: int = 256, device="cuda") ->
 
 
 def _kv8(c: Kv8Cache):
-    """(device, nkv, hd, nseq, it_kv8_cache) of a cache whose buffers fit each other."""
+    """(device, nkv, hd, nseq, it_kv8_cache) of a cache whose buffers fit each other. (The checks of these calls are most of
+    what a short one costs the host: one expression over cheap queries, and messages only once it fails.)"""
     kp, vp, sc, tk, tv = c
     dev, shape, tail = kp.get_device(), kp.shape, tk.shape
     if len(shape) != 3 or len(tail) != 4 or shape[2] % KV8_PAGE:
@@ -706,19 +708,27 @@ def _kv8(c: Kv8Cache):
     npages, nkv, size = shape
     if vp.shape != shape or sc.shape != (npages, nkv, 8) or tail[1:] != (2, nkv, size) or tv.shape != tail:
         raise ValueError("vp must have kp's shape, sc [npages, nkv, 8], tk and tv [nseq, 2, nkv, 64*hd]")
-    _need_all(torch.uint8, dev, (kp, vp), "kp vp")
-    _need_all(torch.float16, dev, (sc, tk, tv), "sc tk tv")
-    args = Kv8CacheArgs(kp.data_ptr(), vp.data_ptr(), sc.data_ptr(), tk.data_ptr(), tv.data_ptr(), npages, tail[0], nkv,
-                        size // KV8_PAGE)
-    return dev, nkv, size // KV8_PAGE, tail[0], args
+    if not (dev >= 0 and kp.dtype is torch.uint8 and vp.dtype is torch.uint8 and sc.dtype is torch.float16 and
+            tk.dtype is torch.float16 and tv.dtype is torch.float16 and vp.get_device() == dev and sc.get_device() == dev and
+            tk.get_device() == dev and tv.get_device() == dev and kp.is_contiguous() and vp.is_contiguous() and
+            sc.is_contiguous() and tk.is_contiguous() and tv.is_contiguous()):
+        _need_all(torch.uint8, dev, (kp, vp), "kp vp")
+        _need_all(torch.float16, dev, (sc, tk, tv), "sc tk tv")
+    hd = size // KV8_PAGE
+    return dev, nkv, hd, tail[0], Kv8CacheArgs(kp.data_ptr(), vp.data_ptr(), sc.data_ptr(), tk.data_ptr(), tv.data_ptr(),
+                                               npages, tail[0], nkv, hd)
 
 
 def _kv8_batch(dev: int, nseq: int, start: torch.Tensor, length: torch.Tensor, table: torch.Tensor) -> int:
-    _need_all(torch.int32, dev, (start, length, table), "start length table")
-    if start.shape != (nseq + 1,) or length.shape != (nseq,) or len(table.shape) != 2 or table.shape[0] != nseq:
+    shape = table.shape
+    if not (start.dtype is torch.int32 and length.dtype is torch.int32 and table.dtype is torch.int32 and
+            start.get_device() == dev and length.get_device() == dev and table.get_device() == dev and
+            start.is_contiguous() and length.is_contiguous() and table.is_contiguous()):
+        _need_all(torch.int32, dev, (start, length, table), "start length table")
+    if start.shape != (nseq + 1,) or length.shape != (nseq,) or len(shape) != 2 or shape[0] != nseq:
         raise ValueError(f"start must be [{nseq + 1}], length [{nseq}] and table [{nseq}, max_pages]: one of each for the "
                          "cache's sequences")
-    return table.shape[1]
+    return shape[1]
 
 
 def _kv8_rows(dev: int, kvd: int, k: torch.Tensor, v: torch.Tensor) -> int:
@@ -726,7 +736,7 @@ def _kv8_rows(dev: int, kvd: int, k: torch.Tensor, v: torch.Tensor) -> int:
     for t in (k, v):
         if t.dtype is not torch.float16 or t.get_device() != dev or len(t.shape) != 2 or t.shape[1] != kvd:
             raise ValueError(f"k and v must be [ntok, {kvd}] f16 on the cache's device")
-        if t.stride(1) != 1 or t.shape != k.shape or t.stride(0) != k.stride(0):
+        if t.shape != k.shape or t.stride() != k.stride() or t.stride(1) != 1:
             raise ValueError("k and v must have one shape and one stride, with each row's values side by side")
     return k.stride(0)
 
@@ -778,6 +788,7 @@ def kv8_copy(cache: Kv8Cache, src: torch.Tensor | None = None, dst: torch.Tensor
              _ptr(seq_dst), 0 if seq_src is None else len(seq_src))
 
 
+@functools.lru_cache(maxsize=256)
 def attn_kv8_scratch_bytes(max_nt: int, nh: int, nkv: int, hd: int = 256) -> int:
     return lib().it_attn_kv8_scratch_bytes(max_nt, hd, nh, nkv)
 
@@ -790,22 +801,26 @@ def attn_kv8(cache: Kv8Cache, q: torch.Tensor, start: torch.Tensor, length: torc
     kv8_append, length still without the new tokens (it_attn_kv8)."""
     dev, nkv, hd, nseq, args = _kv8(cache)
     pages = _kv8_batch(dev, nseq, start, length, table)
-    ntok = q.shape[0]
-    if q.shape != (ntok, nh * 2 * hd):
-        raise ValueError(f"q must be [ntok, {nh * 2 * hd}]")
-    _need_all(torch.float32, dev, (q,), "q")
+    shape, width = q.shape, nh * hd
+    ntok = shape[0]
+    if len(shape) != 2 or shape[1] != 2 * width:
+        raise ValueError(f"q must be [ntok, {2 * width}]")
+    if q.dtype is not torch.float32 or q.get_device() != dev or not q.is_contiguous():
+        _need_all(torch.float32, dev, (q,), "q")
     if out is None:
-        out = torch.empty(ntok, nh * hd, dtype=out_dtype, device=q.device)
-    if out.dtype not in (torch.float32, torch.float16) or out.shape != (ntok, nh * hd):
-        raise ValueError(f"out must be [{ntok}, {nh * hd}] of float32 or float16")
-    _need_all(out.dtype, dev, (out,), "out")
+        out = torch.empty(ntok, width, dtype=out_dtype, device=q.device)
+    kind = out.dtype
+    if (kind is not torch.float32 and kind is not torch.float16) or out.shape != (ntok, width):
+        raise ValueError(f"out must be [{ntok}, {width}] of float32 or float16")
+    if out.get_device() != dev or not out.is_contiguous():
+        _need_all(kind, dev, (out,), "out")
     if scale is None:
         scale = 1.0 / hd ** 0.5
     if scratch is None:
         scratch = torch.empty(attn_kv8_scratch_bytes(max_nt, nh, nkv, hd), dtype=torch.uint8, device=q.device)
     elif scratch.get_device() != dev or not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous, on the same device as the other tensors")
-    _call_on(dev, "it_attn_kv8", ctypes.addressof(args), q.data_ptr(), nh * 2 * hd, ntok, start.data_ptr(),
-             length.data_ptr(), table.data_ptr(), pages, max_nt, nh, scale, out.data_ptr(), nh * hd,
-             int(out.dtype is torch.float16), scratch.data_ptr(), scratch.nbytes)
+    _call_on(dev, "it_attn_kv8", ctypes.addressof(args), q.data_ptr(), 2 * width, ntok, start.data_ptr(), length.data_ptr(),
+             table.data_ptr(), pages, max_nt, nh, scale, out.data_ptr(), width, kind is torch.float16, scratch.data_ptr(),
+             scratch.nbytes)
     return out
