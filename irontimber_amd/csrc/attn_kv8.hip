@@ -160,7 +160,8 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     __shared__ __align__(16) uint8_t kbuf[KB][4 * QUARTER], vbuf[VB][4 * QUARTER];
     __shared__ __align__(16) u4 qlast[QL ? RB : 1][QL ? QL : 1][DG][QL ? 64 : 1];
     __shared__ __align__(16) _Float16 pbuf[2][RB][2][NP][64 * 8];   // P^T operands: [parity][rows][keys][hi, lo]
-    __shared__ __align__(16) float mbuf[2][ROWS][4];                // row maxima by key block
+    __shared__ __align__(16) float mbuf[ROWS][4];                   // row maxima by key block
+    __shared__ __align__(16) int over[2][4];                        // whether a wave's weights are too large
     __shared__ __align__(16) float lbuf[ROWS][4];                   // row sums by key block; at first q's maxima by dims
     __shared__ int qlim[ROWS];                                      // the last key that a row sees
 
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     };
     // The rows' maxima over the wave's 16 keys, to LDS. Values of different row blocks share the lane exchanges: lane row g ends with
     // row block g of four, a half-wave with a row block of two.
-    auto maxima = [&](int par) __attribute__((always_inline)) {
+    auto maxima = [&]() __attribute__((always_inline)) {
         float m[RB];
 #pragma unroll
         for (int x = 0; x < RB; ++x) m[x] = fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3])) * (back[x] * ksc);
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
             v = fmaxf(a, e);
             x = min(2 * (g >> 1) + (g & 1), RB - 1);
         }
-        mbuf[par][16 * x + lr][w] = v;
+        mbuf[16 * x + lr][w] = v;
     };
     // ---- q in units of its row's largest value / 2^(8 DG - 1), as DG signed digits of 8 bits, for integer products with the
     // codes. Wave w makes those of dims 64 w .. (hd 128: two waves); they meet in LDS that is not in use yet, a row block at a time.
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
         }
     }
     // Scores of the wave's 16 keys of full page j
-    auto scores = [&](int j, int par) __attribute__((always_inline)) {
+    auto scores = [&](int j) __attribute__((always_inline)) {
         const h2 two = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(w & 2 ? scl[1] : scl[0], j & 63));
         ksc = (float)two[w & 1];
         landed<KB * NJ>();   // all but the V that went out last, and with two pages of K the K before it
@@ -421,42 +422,41 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
                 sc[x][i] = PAIRS ? __builtin_fmaf(t, 256.f, (float)a[DG - 1][i]) : t;
             }
         }
-        if ((p0 + j) * kv8::PAGE + kv8::PAGE - 1 > clear) mask_keys(p0 + j);
-        maxima(par);
     };
-    // Weights 2^(s - m_run) to LDS, with m_run 7 below the maximum seen when it was last raised; it is raised when a row's
-    // maximum passes m_run + 15. So weights stay below 2^15, inside f16, and small ones keep their digits: hi + lo
-    // resolves 2^-24, 2^-31 of a fresh maximum, and one f16 2^-24 in subnormals. The sums are those of the weights as rounded.
-    auto weights = [&](int par) __attribute__((always_inline)) {
-        float mx[RB];
-        bool grow = false;
+    // Weights are 2^(s - m), with a reference m that is 7 below the row's maximum when it is set, and set anew when a weight passes
+    // 2^15. So weights stay inside f16, and small ones keep their digits: hi + lo resolves 2^-24, 2^-31 of a fresh
+    // maximum, and one f16 2^-24 in subnormals. `reference` takes the maxima of the page that sc holds to all waves.
+    auto reference = [&]() __attribute__((always_inline)) {
+        maxima();
+        lds_barrier();
 #pragma unroll
         for (int x = 0; x < RB; ++x) {
-            const f4 m4 = *(const f4*)mbuf[par][16 * x + lr];
-            mx[x] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            grow = grow || mx[x] > top[x];   // (from -inf at the first visible key)
-        }
-        if (__any(grow)) {   // (all waves find the same)
+            const f4 m4 = *(const f4*)mbuf[16 * x + lr];
+            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+            if (mx > top[x]) {   // (from -inf at the first visible key; all waves find the same)
+                const float to = P_BITS - mx;
+                const float f = top[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(to - neg[x]);
+                l_run[x] *= f;
 #pragma unroll
-            for (int x = 0; x < RB; ++x) {
-                if (mx[x] > top[x]) {
-                    const float to = P_BITS - mx[x];
-                    const float f = top[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(to - neg[x]);
-                    l_run[x] *= f;
+                for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[x][d][i] *= f;
-                    neg[x] = to;
-                    top[x] = 2 * P_BITS + 1 - to;
-                }
+                    for (int i = 0; i < 4; ++i) o[x][d][i] *= f;
+                neg[x] = to;
+                top[x] = 2 * P_BITS + 1 - to;
             }
         }
+    };
+    // The weights of the page that sc holds to LDS; returns their sums, of the weights as rounded, and whether one is too large
+    struct Sums { float s[RB]; bool over; };
+    auto weights = [&](int par) __attribute__((always_inline)) {
+        Sums r;
+        float most = 0.f;
 #pragma unroll
         for (int x = 0; x < RB; ++x) {
             float e[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][i], back[x] * ksc, neg[x]));
+            most = fmaxf(fmaxf(most, fmaxf(e[0], e[1])), fmaxf(e[2], e[3]));
             _Float16* to = &pbuf[par][x][w >> 1][0][l * 8 + 4 * (w & 1)];
             if constexpr (PAIRS) {
                 h2 h0, h1, l0, l1;
@@ -464,15 +464,31 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
                 split2(f2{e[2], e[3]}, neg1, h1, l1);
                 *(h4*)to = h4{h0[0], h0[1], h1[0], h1[1]};
                 *(h4*)(to + 64 * 8) = h4{l0[0], l0[1], l1[0], l1[1]};
-                l_run[x] += (e[0] + e[1]) + (e[2] + e[3]);
+                r.s[x] = (e[0] + e[1]) + (e[2] + e[3]);
             } else {
                 const h2 h0 = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[0], e[1]));
                 const h2 h1 = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[2], e[3]));
                 const h2 ones = {(_Float16)1.f, (_Float16)1.f};
                 *(h4*)to = h4{h0[0], h0[1], h1[0], h1[1]};
-                l_run[x] = __builtin_amdgcn_fdot2(h1, ones, __builtin_amdgcn_fdot2(h0, ones, l_run[x], false), false);
+                r.s[x] = __builtin_amdgcn_fdot2(h1, ones, __builtin_amdgcn_fdot2(h0, ones, 0.f, false), false);
             }
         }
+        r.over = __any(most > 32768.f);
+        return r;
+    };
+    // The page's weights behind a barrier, under a reference that holds them (nearly always the one that there is)
+    auto settle = [&](int par) __attribute__((always_inline)) {
+        Sums r = weights(par);
+        if (l == 0) over[par][w] = r.over;
+        lds_barrier();
+        const i4 any = *(const i4*)over[par];
+        if (__builtin_amdgcn_readfirstlane(any[0] | any[1] | any[2] | any[3])) {
+            reference();
+            r = weights(par);
+            lds_barrier();
+        }
+#pragma unroll
+        for (int x = 0; x < RB; ++x) l_run[x] += r.s[x];
     };
     // O of the wave's dims (vf: the V operand of a dim block and half of the keys)
     auto values = [&](int par, auto&& vf) __attribute__((always_inline)) {
@@ -496,7 +512,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
             }
         }
     };
-    // Full page j: its weights and the next page's scores, then its values. K and V of a later page go out when their buffers
+    // Full page j: its weights, then the next page's scores and its values. K and V of a later page go out when their buffers
     // have been read: on arrival here K of j + 1 .. j + KB and V of j .. j + VB - 1 are under way or there.
     auto step = [&](int j, int par) __attribute__((always_inline)) {
         const h2 s01 = __builtin_bit_cast(h2, (uint32_t)__builtin_amdgcn_readlane(scl[2], j & 63));
@@ -508,12 +524,12 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
         const unsigned vid = page_of(j + VB);
         if (((j + 1 + KB) & 63) == 0) load_ids(j + 1 + KB);
         const unsigned kid = page_of(j + 1 + KB);
+        if ((p0 + j) * kv8::PAGE + kv8::PAGE - 1 > clear) mask_keys(p0 + j);
         __builtin_amdgcn_s_setprio(0);
-        weights(par);
+        settle(par);
         __builtin_amdgcn_s_setprio(1);
-        scores(j + 1, par ^ 1);   // (past the end: not used)
+        scores(j + 1);   // (past the end: not used)
         fetch(c.kp, kbuf[KB == 2 ? (j + 1) & 1 : 0], j + 1 + KB, kid);
-        lds_barrier();
         uint8_t* vj = vbuf[VB == 2 ? j & 1 : 0];
         const uint8_t* v = vj + w * QUARTER + 16 * l;
         if constexpr (VB == 1) landed<NJ>();   // all but K of page j + 2
@@ -529,23 +545,25 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     int par = 0;
     h8 vo[ND][2];
     if (tail) {
-        mask_keys(closed);
-        maxima(0);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 2; ++e) vo[d][e] = ld_h8(c.tv + open + KIB * d + 8 * e);
-        lds_barrier();
-        weights(0);
+        mask_keys(closed);
+        reference();
+        settle(0);
         par = 1;
     }
     if (np > 0) {
         if constexpr (VB == 1) landed<0>();
-        scores(0, par);
+        scores(0);
         fetch(c.kp, kbuf[0], KB, page_of(KB));
         fetch(c.vp, vbuf[VB - 1], VB - 1, page_of(VB - 1));
+        if (!tail || closed * kv8::PAGE > clear) {   // rows without a reference: all, or those that see no open row
+            if (p0 * kv8::PAGE + kv8::PAGE - 1 > clear) mask_keys(p0);
+            reference();
+        }
     }
-    lds_barrier();
     if (tail) {
         const int have = total - closed * kv8::PAGE;   // rows that are not there hold anything
         values(0, [&](int d, int s) __attribute__((always_inline)) {
