@@ -4,13 +4,20 @@
 // A unit of work is (sequence, KV head, block of ROWS query rows r = t*G + g, split of the pages). Its workgroup takes a
 // page a step, the four waves sharing it:
 //   S^T = K q^T    wave w has the page's block w: 16 keys, all query rows
-//   softmax        running reference per row, common to the waves (their maxima meet in LDS)
-//   O^T += V^T P^T wave w has a quarter of the dims, all 64 keys and rows; P^T comes through LDS
-// K and V never pass through LDS: the page's element order is that of the matrix operands, so each code goes from memory into
-// the registers of the one wave that needs it and is converted there, once a workgroup. The products use f16 operands:
-// K and V are f16 numbers exactly (kv8.hip); q and P go in as f16 pairs hi + lo, 22 bits, for an f32 output, and as
-// one f16 each for an f16 output.
-// One barrier a page: P of page j and the maxima of page j + 1 are written before it and read behind it.
+//   softmax        a running reference per row, common to the waves; P^T goes through LDS
+//   O^T += V^T P^T wave w has a quarter of the dims, all 64 keys and rows
+// K's codes are integers already, so K q^T is integer products with q in signed 8-bit digits, fixed point in its row's largest
+// value: three digits (2^-23 of it) for an f32 output, two (2^-15) for an f16 one. A digit more costs a product of 16 x 16 x 64
+// a key block, where converting K would cost the vector units 6 operations for 4 codes, and they are what is short here. V's
+// codes become f16 times their scale, exactly; P goes in as an f16 pair for an f32 output, as one f16 for an f16 one.
+// The open page (f16 rows) comes first, with q as f16 pairs.
+//
+// The page's element order is that of the matrix operands. Each wave copies the 4 hd bytes that it alone needs straight into its
+// part of LDS, a page or two ahead, and reads them back without a barrier; one barrier a page, for P.
+//
+// What bounds it (MI355X, hd 256): few tokens, the bytes of the codes: 7.0 - 7.6 TB/s of them in a long context, behind 7 us for a
+// launch's first page and 4 for the join of the splits. Whole prompts, the vector units beside the matrix ones: the
+// softmax, 96 operations for a page's V and 16 for its K are 360 of a step's 464 in a wave, matrix units 41 % busy, 0.87 PFLOP/s.
 //
 // The lengths are on the device, so every workgroup finds its unit by itself: pages per split from the total work, a prefix sum over
 // the sequences' unit counts. Sequences of one split are finished in place, the others' records {m, l, o} are joined by
@@ -618,66 +625,107 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     }
 }
 
-// Joins the records of sequences with more than one split. An item is (group of rows, row, 4 DL dims); thread = (split lane of
-// 256 / DL, 4 dims), NB records in flight a thread; rows: those that a group can have. The launch is as many workgroups as there
-// can be items, or fewer, each taking several.
+// Joins the records of sequences with more than one split. A workgroup takes (group of rows, row, 4 DL dims), with 256 / DL split
+// lanes; where DL is 32 and a sequence has few splits, each of its waves takes a row alone, and fewer workgroups do. NB records are
+// in flight a thread. rows: those that a group can have. The launch is as many workgroups as there can be items, or fewer,
+// each taking several; groups come side by side, so that those with work are spread.
 template <int HD, int ROWS, int DL, class OutT>
 __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q, int qts,
                                                              int nh, OutT* __restrict__ out, int ots,
                                                              const float* __restrict__ part, int wgs, int rows) {
-    constexpr int SL = 256 / DL, DQ = HD / (4 * DL), NB = 4;
+    constexpr int SL = 256 / DL, DQ = HD / (4 * DL), NB = 4, FEW = DL == 32 ? 16 : 0, WL = HD / 4;   // WL: lanes of a wave's row
     __shared__ float red_m[4], red_l[4][DL];
     __shared__ __align__(16) f4 red_o[4][DL];
-    const int nkv = c.nkv, G = nh / nkv, tid = threadIdx.x, l = tid & 63, sg = tid / DL, dl = tid % DL;
+    const int nkv = c.nkv, G = nh / nkv, tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
     const Kv8Seq s0 = kv8_seq(b, l);
     const int chunk = call_chunk<ROWS>(b, s0, G, nkv, wgs, l);
     const int nrec = kv8::max_records(wgs);
     // weight of a record or partial result whose maximum is m, against the largest M
     auto share = [](float m, float sum, float M) { return m == -INFINITY ? (sum == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(m - M); };
-    for (int item = blockIdx.x;; item += gridDim.x) {
-        const int dq = item % DQ, row = item / DQ % rows;
-        const Found u = find<ROWS, true>(b, s0, G, nkv, chunk, item / (DQ * rows), l);
-        if (!u.any) return;
-        const int kh = u.at % nkv, rb = u.at / nkv, r = rb * ROWS + row;
-        if (r >= u.n * G) continue;   // (whole workgroup)
+    struct Part { float m, sum; f4 o; };
+    int groups = 0;        // row blocks that were split
+    bool alone_all = true;   // and all into few
+    for (int i0 = 0; i0 < b.nseq; i0 += 64) {
+        const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
+        const int ns = kv8::splits(s.pages, chunk), n = ns > 1 ? (s.n * G + ROWS - 1) / ROWS * nkv : 0;
+        groups += b.nseq == 1 ? __builtin_amdgcn_readfirstlane(n) : __builtin_amdgcn_readlane(prefix_sum(n, l), 63);
+        if (__any(n > 0 && ns > FEW)) alone_all = false;
+    }
+    const int each = alone_all ? (rows + 3) / 4 : DQ * rows;
+    for (int item = blockIdx.x; item < groups * each; item += gridDim.x) {
+        const int sub = item / groups;
+        const Found u = find<ROWS, true>(b, s0, G, nkv, chunk, item - sub * groups, l);
+        if (!u.any) return;   // (cannot be)
+        const bool alone = u.ns <= FEW;
+        const int kh = u.at % nkv, rb = u.at / nkv, row = alone ? 4 * sub + w : sub / DQ, r = rb * ROWS + row;
+        if (row >= rows || r >= u.n * G) continue;   // (all threads that join the row)
         const int t = r / G, h = kh * G + r - t * G, need = (u.len + t) / kv8::PAGE / chunk + 1;
         const float* base = part + (size_t)nrec * ROWS * 2;
-        float m = -INFINITY, sum = 0.f;
-        f4 o = f4{};
-        for (int s = sg; s < need; s += SL * NB) {   // (past the last record: the last again, uncounted)
-            f2 ml[NB];
-            f4 v[NB];
+        auto gather = [&](int first, int lanes, int dim) __attribute__((always_inline)) {
+            Part p = {-INFINITY, 0.f, f4{}};
+            for (int s = first; s < need; s += lanes * NB) {   // (past the last record: the last again, uncounted)
+                f2 ml[NB];
+                f4 v[NB];
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                const size_t at = (size_t)(u.rec + kv8::record(min(s + i * SL, need - 1), u.nrb, rb, nkv, kh)) * ROWS + row;
-                ml[i] = *((const f2*)part + at);
-                v[i] = ld_f4(base + at * HD + 4 * (DL * dq + dl));
-            }
-            float M = m;
+                for (int i = 0; i < NB; ++i) {
+                    const size_t at = (size_t)(u.rec + kv8::record(min(s + i * lanes, need - 1), u.nrb, rb, nkv, kh)) * ROWS + row;
+                    ml[i] = *((const f2*)part + at);
+                    v[i] = ld_f4(base + at * HD + dim);
+                }
+                float M = p.m;
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                if (s + i * SL >= need) ml[i] = f2{-INFINITY, 0.f};
-                M = fmaxf(M, ml[i][0]);
-            }
-            const float a = share(m, sum, M);
-            sum *= a;
-            o *= a;
+                for (int i = 0; i < NB; ++i) {
+                    if (s + i * lanes >= need) ml[i] = f2{-INFINITY, 0.f};
+                    M = fmaxf(M, ml[i][0]);
+                }
+                const float a = share(p.m, p.sum, M);
+                p.sum *= a;
+                p.o *= a;
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                const float e = share(ml[i][0], ml[i][1], M);
-                sum += ml[i][1] * e;
-                if (s + i * SL < need) o += v[i] * e;
+                for (int i = 0; i < NB; ++i) {
+                    const float e = share(ml[i][0], ml[i][1], M);
+                    p.sum += ml[i][1] * e;
+                    if (s + i * lanes < need) p.o += v[i] * e;
+                }
+                p.m = M;
             }
-            m = M;
+            return p;
+        };
+        auto finish = [&](const Part& p, int dim) __attribute__((always_inline)) {
+            const f4 gate = ld_f4(q + (size_t)(u.t0 + t) * qts + (size_t)h * 2 * HD + HD + dim);
+            const float inv = 1.0f / p.sum;
+            f4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = p.o[i] * inv * sigmoid_hw(gate[i]);
+            store4(out + (size_t)(u.t0 + t) * ots + (size_t)h * HD + dim, v);
+        };
+        // p against the largest M of the lanes it is joined with
+        auto scaled = [&](Part p, float M) __attribute__((always_inline)) {
+            const float e = share(p.m, p.sum, M);
+            return Part{M, p.sum * e, p.o * e};
+        };
+        if (alone) {
+            const int dim = 4 * (l % WL);
+            Part p = gather(l / WL, 64 / WL, dim);
+            if constexpr (WL == 32) {
+                p = scaled(p, max_xor32(p.m));
+                p.sum = sum_xor32(p.sum);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p.o[i] = sum_xor32(p.o[i]);
+            }
+            if (l < WL) finish(p, dim);
+            continue;
         }
         // the split lanes of a wave, then the four waves
-        float M = max_xor32(m);
+        const int dim = 4 * (DL * (sub % DQ) + tid % DL);
+        Part p = gather(tid / DL, SL, dim);
+        float M = max_xor32(p.m);
         if constexpr (DL == 8) {
             M = max_xor16(M);
             M = fmaxf(M, dppc<0x128>(M));   // row_ror 8
         }
-        const float e = share(m, sum, M);
-        float all[5] = {sum * e, o[0] * e, o[1] * e, o[2] * e, o[3] * e};
+        p = scaled(p, M);
+        float all[5] = {p.sum, p.o[0], p.o[1], p.o[2], p.o[3]};
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
             all[i] = sum_xor32(all[i]);
@@ -688,81 +736,83 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
         }
         __syncthreads();   // the last item's partial results have been read
         if (l < DL) {
-            if (l == 0) red_m[tid >> 6] = M;
-            red_l[tid >> 6][l] = all[0];
-            red_o[tid >> 6][l] = f4{all[1], all[2], all[3], all[4]};
+            if (l == 0) red_m[w] = M;
+            red_l[w][l] = all[0];
+            red_o[w][l] = f4{all[1], all[2], all[3], all[4]};
         }
         __syncthreads();
         if (tid < DL) {
             M = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
-            float L = 0.f;
-            f4 v = f4{};
+            p = Part{M, 0.f, f4{}};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float f = share(red_m[i], red_l[i][tid], M);
-                L += red_l[i][tid] * f;
-                v += red_o[i][tid] * f;
+                p.sum += red_l[i][tid] * f;
+                p.o += red_o[i][tid] * f;
             }
-            const int dim = 4 * (DL * dq + dl);
-            const f4 gate = ld_f4(q + (size_t)(u.t0 + t) * qts + (size_t)h * 2 * HD + HD + dim);
-            const float inv = 1.0f / L;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = v[i] * inv * sigmoid_hw(gate[i]);
-            store4(out + (size_t)(u.t0 + t) * ots + (size_t)h * HD + dim, v);
+            finish(p, dim);
         }
     }
 }
 
-// Row blocks of a workgroup and the workgroups a call is shared out to
-struct Form { int rb, wgs; };
-Form form(int max_nt, int G, bool f16out) {
-    const long rows = (long)max_nt * G;
-    return rows <= 16 ? Form{1, 512} : rows <= 32 ? Form{2, 512} : f16out ? Form{4, 512} : Form{3, 512};
+constexpr int WGS = 512;   // workgroups that a call's pages are shared out to: two a CU, as many as fit side by side
+
+// Row blocks of 16 rb rows, over all KV heads, that the sequences of a call can have
+long max_groups(int rb, int nseq, int ntok, int max_nt, int G, int nkv) {
+    const long rows = 16 * rb, each = ((long)max_nt * G + rows - 1) / rows;
+    return std::min((long)ntok * G / rows + std::min(nseq, ntok), each * nseq) * nkv;
 }
-// Row blocks, over all KV heads, that the sequences of a call can have
-long max_groups(const Form& f, int nseq, int ntok, int max_nt, int G, int nkv) {
-    const long rows = 16 * f.rb, each = ((long)max_nt * G + rows - 1) / rows;
-    return std::min((long)ntok * G / rows + nseq, each * nseq) * nkv;
+// Groups of 16 rows that share a workgroup's pages. All rows of a sequence if they are 32 or fewer. Of more rows, blocks of 32 have
+// the shorter steps and the sooner first page, blocks of 64 (48 for an f32 output: more do not fit the registers) half
+// the conversions of V. So the large ones where there are enough of them to fill the card, by the most that the
+// call's shapes allow. us with 32 / with the large ones (16 heads, 2 KV heads, hd 256; tokens after rows):
+//   f16, one sequence 64 after 4032   30 / 37    256 after 3840   47 / 50    256 after 32512   233 / 189    8192 after 0   734 / 627
+//        32 sequences of 5 after 8187   94 / 73    8 of 8 after 8184   39 / 41    32 of 64 after 1984   118 / 99
+//   f32, one sequence 64 after 4032   32 / 36    512 after 3584   86 / 88    4096 after 0   265 / 262    32 of 5 after 8187   106 / 83
+//        seven prompts of 24 heads   461 / 435
+int row_groups(const Kv8Batch& b, int G, int nkv, bool f16out) {
+    const long rows = (long)b.max_nt * G;
+    if (rows <= 32) return rows <= 16 ? 1 : 2;
+    const int most = f16out ? 4 : 3;
+    const long groups = max_groups(most, b.nseq, b.ntok, b.max_nt, G, nkv);
+    return (f16out ? groups >= 64 : groups >= 2048 || (rows <= 48 && groups >= 32)) ? most : 2;
 }
 
 template <int HD, int RB, class OutT>
 hipError_t launch(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, OutT* out, int ots,
-                  float* part, const Form& f, hipStream_t st) {
-    const long groups = max_groups(f, b.nseq, b.ntok, b.max_nt, nh / c.nkv, c.nkv);
+                  float* part, hipStream_t st) {
+    const long groups = max_groups(RB, b.nseq, b.ntok, b.max_nt, nh / c.nkv, c.nkv);
     attn_kv8_kernel<HD, RB, sizeof(OutT) == 4, OutT>
-        <<<dim3((unsigned)(groups + f.wgs + 1)), 256, 0, st>>>(c, b, q, qts, nh, scale, out, ots, part, f.wgs);
+        <<<dim3((unsigned)(groups + WGS + 1)), 256, 0, st>>>(c, b, q, qts, nh, scale, out, ots, part, WGS);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // split groups have two splits at least, so there are at most max_records / 2 of them. Few rows: many splits, so many
     // split lanes
     const int rows = (int)std::min((long)16 * RB, (long)b.max_nt * (nh / c.nkv));
-    const long split_rows = std::min(groups, (long)kv8::max_records(f.wgs) / 2) * rows;
+    const long split_rows = std::min(groups, (long)kv8::max_records(WGS) / 2) * rows;
     if (split_rows * (HD / 32) <= 1024)
         attn_kv8_merge_kernel<HD, 16 * RB, 8, OutT><<<dim3((unsigned)(split_rows * (HD / 32))), 256, 0, st>>>(
-            c, b, q, qts, nh, out, ots, part, f.wgs, rows);
+            c, b, q, qts, nh, out, ots, part, WGS, rows);
     else
         attn_kv8_merge_kernel<HD, 16 * RB, 32, OutT><<<dim3((unsigned)std::min(split_rows * (HD / 128), 2048L)), 256, 0, st>>>(
-            c, b, q, qts, nh, out, ots, part, f.wgs, rows);
+            c, b, q, qts, nh, out, ots, part, WGS, rows);
     return hipGetLastError();
 }
 template <int HD, class OutT>
 hipError_t launch_rb(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, OutT* out, int ots,
                      float* part, hipStream_t st) {
-    const Form f = form(b.max_nt, nh / c.nkv, sizeof(OutT) == 2);
-    if (f.rb == 1) return launch<HD, 1, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
-    if (f.rb == 2) return launch<HD, 2, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
-    return launch<HD, sizeof(OutT) == 2 ? 4 : 3, OutT>(c, b, q, qts, nh, scale, out, ots, part, f, st);
+    const int rb = row_groups(b, nh / c.nkv, c.nkv, sizeof(OutT) == 2);
+    if (rb == 1) return launch<HD, 1, OutT>(c, b, q, qts, nh, scale, out, ots, part, st);
+    if (rb == 2) return launch<HD, 2, OutT>(c, b, q, qts, nh, scale, out, ots, part, st);
+    return launch<HD, sizeof(OutT) == 2 ? 4 : 3, OutT>(c, b, q, qts, nh, scale, out, ots, part, st);
 }
 
 }  // namespace
 
 size_t attn_kv8_scratch_bytes(int max_nt, int hd, int nh, int nkv) {
-    size_t most = 0;
-    for (bool f16out : {false, true}) {
-        const Form f = form(max_nt, nh / nkv, f16out);
-        most = std::max(most, (size_t)kv8::max_records(f.wgs) * 16 * f.rb * (hd + 2) * sizeof(float));
-    }
-    return most;
+    const long rows = (long)max_nt * (nh / nkv);
+    const int rb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;   // (the most that `row_groups` takes, for any number of sequences)
+    return (size_t)kv8::max_records(WGS) * 16 * rb * (hd + 2) * sizeof(float);
 }
 hipError_t launch_attn_kv8(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, void* out,
                            int ots, bool f16out, float* part, hipStream_t st) {

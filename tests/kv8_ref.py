@@ -86,11 +86,13 @@ def attention(q, k, v, before, scale, f16=False):
     """q [n, nh, 2*hd] (query | gate), k, v [rows, nkv, hd] float64, token t sees rows 0 .. before + t -> (out [n, nh, hd]
     float64, bound of an f32 or f16 evaluation's error).
 
-    The bound, with u = 2^-24 (f32) and the products' operands off by e = 2^-21 for pairs (q to 2^-22 of a value or 2^-24 of
-    its row's largest, the scale's product and the sums' conversion within the rest) or 2^-11 for one f16 each:
-    a score is off by ds <= scale sum |q||k| (e + hd u) + 4 u |s| (e of the row's largest |q| where that is more); a weight by
-    2 ds + e + 4 u of itself; sums over n keys by n u; so the output by 2 (2 ds + e + n u + 8 u) max |v| sigmoid(gate) at
-    most, plus its own rounding. Weights below 2^-31 (2^-24 for one f16) of the largest may be lost: n of those times max |v|."""
+    The bound, with u = 2^-24 (f32), for q in fixed point of its row's largest (three 8-bit digits: half a step is at most 2^-23
+    of it; two, for an f16 output: 2^-15) or as an f16 pair (open rows: 2^-22 of the value), and weights as f16 pairs (2^-22)
+    or one f16 rounded toward zero, which leaves a weight 2^-11 about its middle (their sums take them as rounded):
+    with e = 2^-21 or 2^-11, a score is off by ds <= scale sum |q||k| (e + hd u) + 4 u |s|, |q| counted as a quarter or
+    a sixteenth of the row's largest at least; a weight by 2 ds + e + 4 u of itself; sums over n keys by n u; so the output
+    by 2 (2 ds + e + n u + 8 u) max |v| sigmoid(gate) at most, plus its own rounding. Weights below 2^-31 (2^-24 for one f16) of
+    the largest may be lost: n of those times max |v|."""
     n, nh, hd2 = q.shape
     hd, nkv = hd2 // 2, k.shape[1]
     out, tol = np.zeros((n, nh, hd)), np.zeros((n, nh, hd))
@@ -105,7 +107,7 @@ def attention(q, k, v, before, scale, f16=False):
             w = np.exp(s - s.max())
             gate = 1 / (1 + np.exp(-q[t, h, hd:]))
             out[t, h] = (w @ vh[:m]) / w.sum() * gate
-            size = np.maximum(np.abs(x), 0 if f16 else np.abs(x).max() / 8)
+            size = np.maximum(np.abs(x), np.abs(x).max() / (16 if f16 else 4))
             ds = (abs(scale) * (np.abs(kh[:m]) @ size).max() * (e + hd * u) + 4 * u * np.abs(s).max())
             top = np.abs(vh[:m]).max(0)
             tol[t, h] = 2 * (2 * ds + e + (m + 8) * u + m * lost) * top * gate + 4 * u * np.abs(out[t, h])

@@ -266,6 +266,45 @@ def test_whole_prompts(dev):
         e.attend(e.queries(sum(counts), 32), start, length, counts, 32, f16=f16)
 
 
+@pytest.mark.parametrize("before,counts,nh,nkv,hd,f16", [
+    ([9000, 700, 200, 130], [20, 20, 20, 20], 16, 2, 256, False),       # one of many splits, others of few and of one
+    ([9000, 700, 200, 130], [20, 20, 20, 20], 8, 1, 128, False),
+    ([61 + 37 * i for i in range(16)], [5] * 16, 16, 2, 256, False),    # 40 rows each, many sequences
+    ([61 + 37 * i for i in range(16)], [5] * 16, 8, 1, 128, True),
+    ([0, 300], [600, 200], 128, 16, 128, False),                        # enough row blocks for the largest of each type
+    ([0, 300, 63, 0, 128], [1, 203, 97, 0, 5], 24, 4, 256, True),
+    ([1000, 0, 63], [129, 64, 65], 16, 2, 256, True),
+])
+def test_forms(dev, before, counts, nh, nkv, hd, f16):
+    """Batches whose sizes call for each number of row blocks and each way of joining splits."""
+    announce(f"kv8 forms {len(counts)} {sum(counts)} {nh}/{nkv} {hd} f16={f16}")
+    e = Engine(dev, len(counts), nkv, hd, max(b + c for b, c in zip(before, counts)) // 64 + 1)
+    e.append(before)
+    start, length = e.append(counts)
+    e.attend(e.queries(sum(counts), nh), start, length, counts, nh, f16=f16)
+
+
+@pytest.mark.parametrize("before,n", [(60, 10), (0, 70), (128, 3), (190, 4), (1000, 90), (0, 1)])
+@pytest.mark.parametrize("nh", [2, 16, 64])
+def test_scores_far_below_zero(dev, before, n, nh):
+    """Every score is some -150 in log2 units, so that weights under no reference would vanish: also for the rows of a block that
+    see none of the open page, which comes first, and where the full pages' scores are far above the open page's."""
+    e = Engine(dev, 1, 2, 256, 20)
+    base = np.random.default_rng(11).standard_normal(512)
+    base /= np.sqrt((base * base).mean())
+    k, v = e.rows(before + n)
+    low = 1.0 if nh > 2 else 2.0 - (np.arange(before + n) < (before + n) // 64 * 64)[:, None]     # (twice as low in the open page)
+    k = (k.astype(np.float32) * 0.1 - base * low).astype(np.float16)
+    if before:
+        e.append([before], rows=(k[:before], v[:before]))
+    start, length = e.append([n], rows=(k[before:], v[before:]))
+    q = e.queries(n, nh)
+    for h in range(nh):
+        q[:, h, :256] = q[:, h, :256] * 0.1 + 6.5 * base[:256] * (1 if h < nh // 2 else 0) + 6.5 * base[256:] * (0 if h < nh // 2 else 1)
+    for f16 in (False, True):
+        e.attend(q, start, length, [n], nh, f16=f16)
+
+
 def test_sharp_flat_and_odd_scores(dev):
     """One key takes nearly all the weight, in the last or the first page; all keys the same; scales of any sign and size."""
     for kscale, qscale, scale in ((20.0, 1.0, None), (0.0, 1.0, None), (1.0, 1.0, -0.07), (1.0, 1e-30, None), (1.0, 1e4, 1e-5),
