@@ -473,8 +473,8 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
                 *(h4*)(to + 64 * 8) = h4{l0[0], l0[1], l1[0], l1[1]};
                 r.s[x] = (e[0] + e[1]) + (e[2] + e[3]);
             } else {
-                const h2 h0 = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[0], e[1]));
-                const h2 h1 = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[2], e[3]));
+                const h2 h0 = __builtin_convertvector((f2{e[0], e[1]}), h2);
+                const h2 h1 = __builtin_convertvector((f2{e[2], e[3]}), h2);
                 const h2 ones = {(_Float16)1.f, (_Float16)1.f};
                 *(h4*)to = h4{h0[0], h0[1], h1[0], h1[1]};
                 r.s[x] = __builtin_amdgcn_fdot2(h1, ones, __builtin_amdgcn_fdot2(h0, ones, 0.f, false), false);

@@ -88,8 +88,7 @@ def attention(q, k, v, before, scale, f16=False):
 
     The bound, with u = 2^-24 (f32), for q in fixed point of its row's largest (three 8-bit digits: half a step is at most 2^-23
     of it; two, for an f16 output: 2^-15) or as an f16 pair (open rows: 2^-22 of the value), and weights as f16 pairs (2^-22)
-    or one f16 rounded toward zero, which leaves a weight 2^-11 about its middle (their sums take them as rounded):
-    with e = 2^-21 or 2^-11, a score is off by ds <= scale sum |q||k| (e + hd u) + 4 u |s|, |q| counted as a quarter or
+    or one f16 (2^-11; their sums take them as rounded): with e = 2^-21 or 2^-11, a score is off by ds <= scale sum |q||k| (e + hd u) + 4 u |s|, |q| counted as a quarter or
     a sixteenth of the row's largest at least; a weight by 2 ds + e + 4 u of itself; sums over n keys by n u; so the output
     by 2 (2 ds + e + n u + 8 u) max |v| sigmoid(gate) at most, plus its own rounding. Weights below 2^-31 (2^-24 for one f16) of
     the largest may be lost: n of those times max |v|."""
