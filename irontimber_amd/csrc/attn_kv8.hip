@@ -566,10 +566,6 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
         scores(0);
         fetch(c.kp, kbuf[0], KB, page_of(KB));
         fetch(c.vp, vbuf[VB - 1], VB - 1, page_of(VB - 1));
-        if (!tail || closed * kv8::PAGE > clear) {   // rows without a reference: all, or those that see no open row
-            if (p0 * kv8::PAGE + kv8::PAGE - 1 > clear) mask_keys(p0);
-            reference();
-        }
     }
     if (tail) {
         const int have = total - closed * kv8::PAGE;   // rows that are not there hold anything
@@ -580,6 +576,10 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
                 if (32 * s + 16 * (i >> 2) + 4 * g + (i & 3) >= have) v[i] = (_Float16)0.f;
             return v;
         });
+    }
+    if (np > 0 && (!tail || closed * kv8::PAGE > clear)) {   // rows without a reference: all, or those that see no open row
+        if (p0 * kv8::PAGE + kv8::PAGE - 1 > clear) mask_keys(p0);
+        reference();   // (behind the open page's values: it rescales O)
     }
     for (int j = 0; j < np; ++j) step(j, (j + par) & 1);
     landed<0>();   // the fetches past the end

@@ -305,6 +305,30 @@ def test_scores_far_below_zero(dev, before, n, nh):
         e.attend(q, start, length, [n], nh, f16=f16)
 
 
+@pytest.mark.parametrize("nkv,hd", [(4, 128), (2, 256)])
+def test_full_pages_far_above_the_open_page(dev, nkv, hd):
+    """Enough sequences that a workgroup has the open page and full ones; rows that see both, whose reference is raised between
+    them, beside rows that see the full pages alone."""
+    nseq, G = 48, 8
+    e = Engine(dev, nseq, nkv, hd, 4)
+    base = np.random.default_rng(13).standard_normal(hd)
+    base /= np.sqrt((base * base).mean())
+    def append(counts):
+        k, v = e.rows(sum(counts))
+        rows = np.concatenate([s.rows + np.arange(c) for s, c in zip(e.seqs, counts)])
+        last = np.concatenate([np.full(c, (s.rows + c) // 64 * 64 if s.rows else 128) for s, c in zip(e.seqs, counts)])
+        low = np.where(rows < last, 0.5, 2.0)[:, None, None]
+        k = (k.reshape(-1, nkv, hd).astype(np.float32) * 0.2 - base * low).astype(np.float16).reshape(len(k), -1)
+        return e.append(counts, rows=(k, v))
+    append([40 + i % 31 if i % 2 else 100 + i for i in range(nseq)])
+    counts = [30 + i % 7 for i in range(nseq)]
+    start, length = append(counts)
+    q = e.queries(sum(counts), nkv * G)
+    q[:, :, :hd] = q[:, :, :hd] * 0.1 + 1.5 * base
+    for f16 in (False, True):
+        e.attend(q, start, length, counts, nkv * G, f16=f16)
+
+
 def test_sharp_flat_and_odd_scores(dev):
     """One key takes nearly all the weight, in the last or the first page; all keys the same; scales of any sign and size."""
     for kscale, qscale, scale in ((20.0, 1.0, None), (0.0, 1.0, None), (1.0, 1.0, -0.07), (1.0, 1e-30, None), (1.0, 1e4, 1e-5),
