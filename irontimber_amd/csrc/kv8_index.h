@@ -27,12 +27,20 @@ IT_HD int v_elem(int row, int dim) {
 
 // Pages per split of an attention call: `work` is the sum over sequences and KV heads of row blocks times pages, shared
 // out to about `wgs` workgroups; each of the `groups` row blocks may leave one split that is not full, which the count allows
-// for while they are few. The same in the partial and the merge kernel.
-IT_HD int chunk_pages(float work, float groups, int wgs) {
-    const float room = (float)wgs - groups, c = work / (room < 0.5f * (float)wgs ? 0.5f * (float)wgs : room);
+// for while they are few. Half of the workgroups if there is more than a FEW row blocks and they need take no more than SHORT
+// pages: those pages are then quicker than the records of twice the splits (us, 16 heads, 2 KV heads, hd 256: 64 tokens after
+// 4032 28.4 / 30.0, 12 after 8180 21.2 / 23.1, but the 18 pages of 64 after 8128 36.7 / 33.8, and the four row blocks of 4
+// tokens after 8190, 24 heads, 20.0 / 19.4). The same in the partial and the merge kernel.
+constexpr int FEW = 4, SHORT = 10;
+IT_HD int pages_each(float work, float groups, float wgs) {
+    const float room = wgs - groups, c = work / (room < 0.5f * wgs ? 0.5f * wgs : room);
     if (!(c < 33554432.0f)) return 33554432;   // no sequence has more pages
     const int i = (int)c;
     return (float)i < c ? i + 1 : i < 1 ? 1 : i;
+}
+IT_HD int chunk_pages(float work, float groups, int wgs) {
+    const int half = pages_each(work, groups, 0.5f * (float)wgs);
+    return groups > (float)FEW && half <= SHORT ? half : pages_each(work, groups, (float)wgs);
 }
 IT_HD int splits(int pages, int chunk) { return (int)(((long)pages + chunk - 1) / chunk); }
 // Record of (split, row block, KV head) among a sequence's, and how many blocks of records all split sequences can
