@@ -584,7 +584,7 @@ int it_kv8_append(const it_kv8_cache* cache, const uint16_t* k, const uint16_t* 
                   void* stream);
 
 /* Rows first[i] .. of each sequence, start[i+1] - start[i] of them (at most max_rows), as f16 into rows start[i] .. of k and
- * v; total[i]: the rows that the sequence holds (rows at or after total are not written). */
+ * v; total[i]: the rows that the sequence holds (rows at or after total are not written), all of them or at most 64 fewer. */
 int it_kv8_read(const it_kv8_cache* cache, uint16_t* k, uint16_t* v, int tok_stride, int ntok, const int32_t* start,
                 const int32_t* first, const int32_t* total, const int32_t* table, int max_pages, int max_rows,
                 void* stream);
@@ -598,10 +598,12 @@ int it_kv8_copy(const it_kv8_cache* cache, const int32_t* src, const int32_t* ds
 /* Causal GQA attention with sigmoid gate over the cache, of tokens whose rows have been appended: token t of sequence i sees
  * its rows 0 .. len[i] + t. q as for it_attn_f16 (query | gate per head), out [t*out_tok_stride + h*hd + d] in f32, or f16 where
  * out_f16 is nonzero. One token a sequence, a few (drafts), or prompts of any lengths, mixed.
- * Accuracy: the softmax's sums and the products' sums are f32, K and V exact as stored. For an f32 output q and the probabilities go
- * into the products as f16 pairs: q to 2^-22 of a value or 2^-39 of its row's largest, a probability to 2^-22 of itself or, where
- * it is small, 2^-31 of its row's largest up to there (2^-25 once, if a later key outweighs all before it by less than 2^8). For an f16
- * output both are one f16 (2^-12), about 3e-4 of the result beside the output's own rounding.
+ * len[i] and its tokens together are the rows appended so far, or at most 64 fewer: of the rows after the last full page that they
+ * make, only the last two pages' stand in the open buffer. (So after one long append, call it for all of its tokens.)
+ * Accuracy: the softmax's sums and the products' sums are f32, K and V exact as stored. For an f32 output q goes into the products
+ * in fixed point, to 2^-23 of its head's largest value (2^-22 of itself against the open rows), a probability as an f16 pair, to
+ * 2^-22 of itself or, where it is small, 2^-31 of its row's largest up to there. For an f16 output q to 2^-15, a probability as
+ * one f16 (2^-12): about 1.5e-4 of the result beside the output's own rounding.
  * scratch: it_attn_kv8_scratch_bytes bytes, 16-byte aligned (one per call that may overlap another). */
 size_t it_attn_kv8_scratch_bytes(int max_nt, int hd, int nh, int nkv);
 int it_attn_kv8(const it_kv8_cache* cache, const float* q, int q_tok_stride, int ntok, const int32_t* start,

@@ -329,6 +329,57 @@ def test_full_pages_far_above_the_open_page(dev, nkv, hd):
         e.attend(q, start, length, counts, nkv * G, f16=f16)
 
 
+def test_a_pool_past_32_bits(dev):
+    """Pages whose bytes lie past 2^32 in a pool, through every call."""
+    nkv, hd, far = 8, 256, 36000                     # 128 KiB a page: 4.7e9 bytes of K and of V
+    e = Engine(dev, 2, nkv, hd, 6, spare=far)
+    order = np.random.default_rng(1).permutation(12)
+    e.table_np = (far + order).reshape(2, 6).astype(np.int32)
+    e.table_np[0, 1] = 3
+    e.table.copy_(torch.from_numpy(e.table_np))
+    e.append([200, 130])
+    start, length = e.append([3, 70])
+    e.attend(e.queries(73, 16), start, length, [3, 70], 16)
+    def check():
+        k, v = ops.kv8_read(e.cache, e.ints([0, 203, 403]), e.ints([0, 0]), e.ints([203, 200]), e.table, 203, 403)
+        at = 0
+        for s in e.seqs:
+            wk, wv = (x.reshape(len(x), -1).astype(np.float16) for x in s.values())
+            assert np.array_equal(host(k[at:at + s.rows]), wk) and np.array_equal(host(v[at:at + s.rows]), wv)
+            at += s.rows
+    check()
+    ops.kv8_copy(e.cache, src=e.ints([int(e.table_np[0, 1]), int(e.table_np[1, 0])]), dst=e.ints([far - 1, 5]))
+    e.table_np[0, 1], e.table_np[1, 0] = far - 1, 5
+    e.table.copy_(torch.from_numpy(e.table_np))
+    check()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_idle_slots_and_padding(dev, f16):
+    """A captured engine's shapes: more slots than sequences, token arrays longer than the batch, a bound above what comes."""
+    e = Engine(dev, 70, 2, 256, 40)
+    lens = [0] * 70
+    lens[3], lens[68] = 2300, 77
+    e.append(lens)
+    counts = [0] * 70
+    counts[3], counts[68] = 5, 1
+    k, v = e.rows(6)
+    pad = np.full((34, 512), np.nan, np.float16)
+    start, length = e.batch(counts)
+    ops.kv8_append(e.cache, *(torch.from_numpy(np.concatenate([x, pad])).to(dev) for x in (k, v)), start, length, e.table, 8)
+    e.seqs[3].append(k[:5], v[:5])
+    e.seqs[68].append(k[5:], v[5:])
+    e.check_buffers()
+    q = e.queries(40, 16)
+    q[6:] = np.nan
+    out = torch.full((40, 4096), 7.0, device=dev, dtype=torch.float16 if f16 else torch.float32)
+    ops.attn_kv8(e.cache, dev_f32(q.reshape(40, -1), dev), start, length, e.table, 16, 8, out=out)
+    assert (host(out)[6:] == 7.0).all()
+    for i, at, n in ((3, 0, 5), (68, 5, 1)):
+        want, tol = ref.attention(q[at:at + n], *e.seqs[i].values(), e.seqs[i].rows - n, 1 / 16, f16)
+        assert (np.abs(host(out)[at:at + n].reshape(want.shape) - want) <= tol).all()
+
+
 def test_sharp_flat_and_odd_scores(dev):
     """One key takes nearly all the weight, in the last or the first page; all keys the same; scales of any sign and size."""
     for kscale, qscale, scale in ((20.0, 1.0, None), (0.0, 1.0, None), (1.0, 1.0, -0.07), (1.0, 1e-30, None), (1.0, 1e4, 1e-5),

@@ -117,6 +117,17 @@ def test_attention_refusals(kw, text):
     refused("it_attn_kv8", addr(cache()), *a.values(), None, text=text)
 
 
+@pytest.mark.parametrize("kw,text", [(dict(nh=1 << 24, ntok=2, qts=1 << 30), "overlap"), (dict(nh=1 << 24, ntok=2, ots=1 << 20, qts=0x7ffffff0), "overlap"),
+                                     (dict(nh=1024, ntok=65535, qts=1 << 20, ots=1 << 19), "sequences")])
+def test_attention_refusals_of_sizes_past_32_bits(kw, text):
+    """Widths of a token's row that pass an int, and more row blocks than a launch has room for."""
+    many = cache(nkv=1024, nseq=65535) if text == "sequences" else cache()
+    a = dict(q=F, qts=16384, ntok=8, start=F, len=F, table=F, pages=4, max_nt=8, nh=16, scale=0.1, out=F, ots=8192, f16=0,
+             scratch=F, nbytes=1 << 62)
+    a.update(kw)
+    refused("it_attn_kv8", addr(many), *a.values(), None, text=text)
+
+
 def test_scratch_sizes():
     f = _lib.lib().it_attn_kv8_scratch_bytes
     for args in ((0, 256, 16, 2), (1, 64, 16, 2), (1, 256, 16, 3), (1, 256, 0, 2), (1, 256, 16, 0), (-1, 256, 16, 2)):
