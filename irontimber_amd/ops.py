@@ -798,7 +798,7 @@ def attn_kv8(cache: Kv8Cache, q: torch.Tensor, start: torch.Tensor, length: torc
              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Attention of appended tokens over the cache: q [ntok, nh*2*hd] f32 (q | gate per head), token t of sequence i sees its
     rows 0 .. length[i] + t -> out [ntok, nh*hd], f32 or f16 (out's type, or out_dtype). start, length, table, max_nt as for
-    kv8_append, length still without the new tokens (it_attn_kv8)."""
+    kv8_append, length still without the new tokens: all rows that were appended, or at most 64 fewer (it_attn_kv8)."""
     dev, nkv, hd, nseq, args = _kv8(cache)
     pages = _kv8_batch(dev, nseq, start, length, table)
     shape, width = q.shape, nh * hd

@@ -6,6 +6,7 @@ import torch
 from irontimber_amd import _lib, ops
 from tests import kv8_ref as ref
 from tests.gpu_util import announce, dev_f32, host
+from tests.test_gpu_guard_bands import assert_bands, banded
 
 pytestmark = pytest.mark.gpu
 
@@ -548,6 +549,29 @@ def test_strides_through_the_c_abi(dev):
     want, tol = ref.attention(q, *e.seqs[0].values(), 0, 1 / 16)
     assert (np.abs(got[:, :1024].reshape(want.shape) - want) <= tol).all()
     assert (got[:, 1024:] == 4.0).all()
+
+
+@pytest.mark.parametrize("before,counts,nh,nkv,hd,f16", [
+    ([8200], [1], 16, 2, 256, False), ([3, 0, 4000], [3, 4, 2], 24, 4, 256, False), ([500, 2100], [60, 9], 16, 2, 256, False),
+    ([700], [300], 16, 2, 256, True), ([300] * 40, [5] * 40, 8, 1, 128, True), ([9000], [16], 8, 1, 128, False)])
+def test_scratch_and_cache_bands(dev, before, counts, nh, nkv, hd, f16):
+    """Scratch of exactly the bytes asked for, and a cache whose buffers are exactly as long as its sizes say, between bands of a
+    sentinel byte: nothing is written outside them."""
+    announce(f"kv8 bands {sum(counts)} {nh}/{nkv} {hd} f16={f16}")
+    e = Engine(dev, len(counts), nkv, hd, max(b + c for b, c in zip(before, counts)) // 64 + 1, spare=0)
+    held = [banded(t.nbytes, dev) for t in e.cache]
+    e.cache = ops.Kv8Cache(*(view.view(t.dtype).view(t.shape) for (_, view), t in zip(held, e.cache)))
+    for t in e.cache[2:]:
+        t.fill_(float("nan"))
+    e.append(before)
+    start, length = e.append(counts)
+    n = ops.attn_kv8_scratch_bytes(max(counts), nh, nkv, hd)
+    buf, scratch = banded(n, dev)
+    e.attend(e.queries(sum(counts), nh), start, length, counts, nh, f16=f16, scratch=scratch)
+    assert_bands(buf, n)
+    ops.kv8_copy(e.cache, e.ints([0]), e.ints([int(e.cache.kp.shape[0]) - 1]), e.ints([0]), e.ints([len(counts) - 1]))
+    for (whole, _), t in zip(held, e.cache):
+        assert_bands(whole, t.nbytes)
 
 
 def test_the_same_call_gives_the_same_bits(dev):
