@@ -589,12 +589,13 @@ int it_attn_kv8(const it_kv8_cache* cache, const float* q, int qts, int ntok, co
     if (validate_kv8(who, cache, &c) || validate_kv8_batch(who, cache, ntok, start, len, table, max_pages, max_nt, &b)) return -1;
     if (nh < 1 || nh % c.nkv != 0) return fail("%s: n_head %d / n_head_kv %d invalid", who, nh, c.nkv);
     if ((long)ntok * nh > (1L << 26)) return fail("%s: %d tokens of %d heads are more than 2^26 rows", who, ntok, nh);
-    // (a launch has less than 2^32 threads, 256 for every row block)
+    // (row blocks and workgroups are counted in 32 bits)
     if ((long)std::min(ntok, c.nseq) * c.nkv > (1L << 23)) return fail("%s: %d sequences of %d KV heads are more than 2^23", who, std::min(ntok, c.nseq), c.nkv);
     if (!q || !out) return fail("%s: null buffer", who);
     if (!aligned16(q) || !aligned16(out)) return fail("%s: q/out must be 16-byte aligned", who);
     if (qts % 4 != 0 || ots % (out_f16 ? 8 : 4) != 0) return fail("%s: token strides must be multiples of 16 bytes", who);
     if (qts < 0 || ots < 0 || (ntok > 1 && (qts < 2L * nh * c.hd || ots < (long)nh * c.hd))) return fail("%s: token strides overlap rows", who);
+    if (nh / c.nkv > (1 << 16)) return fail("%s: %d query heads share a KV head, more than 2^16", who, nh / c.nkv);
     const size_t need = it::attn_kv8_scratch_bytes(b.max_nt, c.hd, nh, c.nkv);
     if (!scratch || !aligned16(scratch) || scratch_bytes < need)
         return fail("%s: scratch of %zu bytes, %zu needed (16-byte aligned)", who, scratch ? scratch_bytes : 0, need);

@@ -68,6 +68,10 @@ __device__ __forceinline__ int prefix_sum(int v, int l) {   // inclusive, over t
     return v;
 }
 
+// x / d for 0 <= x < 2^21, inv = rcp(d): (x + 1/2) / d is off by less than 1/2d. (Indices by full divisions were 1,700 of
+// the 12,800 cycles of a one-page workgroup.)
+__device__ __forceinline__ int div_small(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
+
 // Pages per split of this call (the same in both kernels; sums in a fixed order)
 template <int ROWS>
 __device__ __forceinline__ int call_chunk(const Kv8Batch& b, const Kv8Seq& s0, int G, int nkv, int wgs, int l) {
@@ -85,8 +89,8 @@ __device__ __forceinline__ int call_chunk(const Kv8Batch& b, const Kv8Seq& s0, i
     return kv8::chunk_pages(readlane_f(sum, 0) * (float)nkv, readlane_f(blocks, 0) * (float)nkv, wgs);
 }
 
-// What is found for a workgroup, in scalar registers: its sequence, the index of its unit (main kernel) or of its group of
-// rows that were split (merge), and the first record of the sequence.
+// What is found for a workgroup, in scalar registers: its sequence, the index of its unit (main kernel) or of its row block that
+// was split (merge) among the sequence's, a KV head's alone, and the first record of the sequence.
 struct Found {
     int seq, t0, n, len, pages, nrb, ns, at, rec;
     bool any, bad;
@@ -103,7 +107,7 @@ __device__ __forceinline__ Found find(const Kv8Batch& b, const Kv8Seq& s0, int G
         f.bad = __builtin_amdgcn_readfirstlane((int)s0.bad) != 0;
         f.nrb = (f.n * G + ROWS - 1) / ROWS;
         f.ns = kv8::splits(f.pages, chunk);
-        f.any = id < f.nrb * nkv * (GROUPS ? (f.ns > 1 ? 1 : 0) : f.ns);
+        f.any = id < f.nrb * (GROUPS ? (f.ns > 1 ? 1 : 0) : f.ns);
         return f;
     }
     f.any = false;
@@ -111,7 +115,7 @@ __device__ __forceinline__ Found find(const Kv8Batch& b, const Kv8Seq& s0, int G
     for (int i0 = 0; i0 < b.nseq; i0 += 64) {
         const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
         const int nrb = (s.n * G + ROWS - 1) / ROWS, ns = kv8::splits(s.pages, chunk);
-        const int recs = ns > 1 ? nrb * ns * nkv : 0, units = GROUPS ? (ns > 1 ? nrb * nkv : 0) : nrb * ns * nkv;
+        const int recs = ns > 1 ? nrb * ns * nkv : 0, units = GROUPS ? (ns > 1 ? nrb : 0) : nrb * ns;
         const int pu = prefix_sum(units, l), pr = prefix_sum(recs, l);
         const unsigned long long hit = __ballot(base + pu > id);
         if (hit) {
@@ -155,7 +159,7 @@ __device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c,
 //
 // Wave w takes key block w of a page for the scores and weights, and dim blocks ND * w .. + ND-1 for O.
 template <int HD, int RB, bool PAIRS, class OutT>
-__global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q, int qts, int nh,
+__global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q, int qts, int G,
                                                           float scale, OutT* __restrict__ out, int ots,
                                                           float* __restrict__ part, int wgs) {
     constexpr int ROWS = 16 * RB, NP = PAIRS ? 2 : 1, NJ = HD / 64, NK = HD / 32, ND = HD / 64, DG = PAIRS ? 3 : 2;
@@ -172,25 +176,35 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     __shared__ __align__(16) float lbuf[ROWS][4];                   // row sums by key block; at first q's maxima by dims
     __shared__ int qlim[ROWS];                                      // the last key that a row sees
 
-    const int nkv = c.nkv, G = nh / nkv;
+    const int nkv = c.nkv;   // G: query heads of a KV head
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, lr = l & 15;
     const Kv8Seq s0 = kv8_seq(b, l);
     const int chunk = call_chunk<ROWS>(b, s0, G, nkv, wgs, l);
-    const Found u = find<ROWS, false>(b, s0, G, nkv, chunk, (int)blockIdx.x, l);
+    const Found u = find<ROWS, false>(b, s0, G, nkv, chunk, (int)(blockIdx.z * gridDim.y + blockIdx.y), l);
     if (!u.any) return;
-    // the heaviest row blocks first; row blocks and heads of a split side by side
-    const int kh = u.at % nkv, rest = u.at / nkv, rb = u.nrb - 1 - rest % u.nrb, split = rest / u.nrb;
-    const int R = u.n * G, r0 = rb * ROWS;
+    // the heaviest row blocks first; heads and row blocks of a split side by side
+    const int kh = blockIdx.x;
+    int rb = 0, split = u.at, tmin = 0, tmax = u.n - 1;
+    const int R = u.n * G;
+    if (u.nrb > 1) {
+        split = (unsigned)u.at / (unsigned)u.nrb;
+        rb = u.nrb - 1 - (u.at - split * u.nrb);
+        tmin = (unsigned)(rb * ROWS) / (unsigned)G;
+        tmax = (unsigned)(min(R, rb * ROWS + ROWS) - 1) / (unsigned)G;
+    }
+    // row r0 + i of the block: its token, and by that its query head
+    const int r0 = rb * ROWS, over0 = r0 - tmin * G;
+    const float rcp_G = __builtin_amdgcn_rcpf((float)G);
+    auto token = [&](int i) __attribute__((always_inline)) { return tmin + div_small(over0 + i, rcp_G); };
 
     if (u.bad) {   // a sequence whose length cannot be: NaN
         for (int i = tid; i < ROWS * (HD / 4); i += 256) {
-            const int r = r0 + i / (HD / 4), t = r / G;
+            const int r = r0 + i / (HD / 4), t = token(i / (HD / 4));
             if (r < R)
                 store4(out + (size_t)(u.t0 + t) * ots + (size_t)(kh * G + r - t * G) * HD + 4 * (i % (HD / 4)), f4{NAN, NAN, NAN, NAN});
         }
         return;
     }
-    const int tmin = r0 / G, tmax = (min(R, r0 + ROWS) - 1) / G;
     const int total = u.len + u.n, closed = total / kv8::PAGE;          // full pages; the open rows are page `closed`
     const int p0 = (int)min((long)split * chunk, (long)u.pages);
     const int p1 = (int)min((long)p0 + chunk, (long)(u.len + tmax) / kv8::PAGE + 1);
@@ -224,7 +238,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
                        to + w * QUARTER);
     };
     auto qrow = [&](int x) __attribute__((always_inline)) {
-        const int r = min(r0 + 16 * x + lr, R - 1), t = r / G;
+        const int i = min(16 * x + lr, R - 1 - r0), r = r0 + i, t = token(i);
         return q + (size_t)(u.t0 + t) * qts + (size_t)(kh * G + r - t * G) * 2 * HD;
     };
 
@@ -305,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     // codes. Wave w makes those of dims 64 w .. (hd 128: two waves); they meet in LDS that is not in use yet, a row block at a time.
     // A negative scale turns q round, and no unit is zero, so that -inf times it stays.
     const float size = fabsf(scale) * LOG2E, sign = scale < 0.f ? -1.f : 1.f;
-    if (tid < ROWS) qlim[tid] = r0 + tid < R ? u.len + (r0 + tid) / G : -1;
+    if (tid < ROWS) qlim[tid] = r0 + tid < R ? u.len + token(tid) : -1;
     {
         if (w < NJ) {
 #pragma unroll
@@ -610,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
         if (r >= R) continue;
         const f4 s4 = *(const f4*)lbuf[16 * x + lr];
         const float inv = 1.0f / ((s4[0] + s4[1]) + (s4[2] + s4[3]));
-        const int t = r / G, h = kh * G + r - t * G;
+        const int t = token(16 * x + lr), h = kh * G + r - t * G;
         const float* gates = q + (size_t)(u.t0 + t) * qts + (size_t)h * 2 * HD + HD;
         OutT* to = out + (size_t)(u.t0 + t) * ots + (size_t)h * HD;
 #pragma unroll
@@ -631,35 +645,37 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
 // each taking several; groups come side by side, so that those with work are spread.
 template <int HD, int ROWS, int DL, class OutT>
 __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q, int qts,
-                                                             int nh, OutT* __restrict__ out, int ots,
+                                                             int G, OutT* __restrict__ out, int ots,
                                                              const float* __restrict__ part, int wgs, int rows) {
     constexpr int SL = 256 / DL, DQ = HD / (4 * DL), NB = 4, FEW = DL == 32 ? 16 : 0, WL = HD / 4;   // WL: lanes of a wave's row
     __shared__ float red_m[4], red_l[4][DL];
     __shared__ __align__(16) f4 red_o[4][DL];
-    const int nkv = c.nkv, G = nh / nkv, tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
+    const int nkv = c.nkv, kh = blockIdx.x, tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
     const Kv8Seq s0 = kv8_seq(b, l);
     const int chunk = call_chunk<ROWS>(b, s0, G, nkv, wgs, l);
     const int nrec = kv8::max_records(wgs);
     // weight of a record or partial result whose maximum is m, against the largest M
     auto share = [](float m, float sum, float M) { return m == -INFINITY ? (sum == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(m - M); };
     struct Part { float m, sum; f4 o; };
-    int groups = 0;        // row blocks that were split
+    int groups = 0;          // row blocks that were split
     bool alone_all = true;   // and all into few
     for (int i0 = 0; i0 < b.nseq; i0 += 64) {
         const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
-        const int ns = kv8::splits(s.pages, chunk), n = ns > 1 ? (s.n * G + ROWS - 1) / ROWS * nkv : 0;
+        const int ns = kv8::splits(s.pages, chunk), n = ns > 1 ? (s.n * G + ROWS - 1) / ROWS : 0;
         groups += b.nseq == 1 ? __builtin_amdgcn_readfirstlane(n) : __builtin_amdgcn_readlane(prefix_sum(n, l), 63);
         if (__any(n > 0 && ns > FEW)) alone_all = false;
     }
     const int each = alone_all ? (rows + 3) / 4 : DQ * rows;
-    for (int item = blockIdx.x; item < groups * each; item += gridDim.x) {
-        const int sub = item / groups;
+    const float rcp_groups = __builtin_amdgcn_rcpf((float)groups), rcp_G = __builtin_amdgcn_rcpf((float)G);
+    for (int item = blockIdx.y; item < groups * each; item += gridDim.y) {   // (at most 520 groups of 128)
+        const int sub = div_small(item, rcp_groups);
         const Found u = find<ROWS, true>(b, s0, G, nkv, chunk, item - sub * groups, l);
         if (!u.any) return;   // (cannot be)
         const bool alone = u.ns <= FEW;
-        const int kh = u.at % nkv, rb = u.at / nkv, row = alone ? 4 * sub + w : sub / DQ, r = rb * ROWS + row;
+        const int rb = u.at, row = alone ? 4 * sub + w : sub / DQ, r = rb * ROWS + row;
         if (row >= rows || r >= u.n * G) continue;   // (all threads that join the row)
-        const int t = r / G, h = kh * G + r - t * G, need = (u.len + t) / kv8::PAGE / chunk + 1;
+        const int t = u.nrb == 1 ? div_small(row, rcp_G) : (int)((unsigned)r / (unsigned)G), h = kh * G + r - t * G;
+        const int last = (u.len + t) / kv8::PAGE, need = (chunk == 1 ? last : (int)((unsigned)last / (unsigned)chunk)) + 1;
         const float* base = part + (size_t)nrec * ROWS * 2;
         auto gather = [&](int first, int lanes, int dim) __attribute__((always_inline)) {
             Part p = {-INFINITY, 0.f, f4{}};
@@ -757,10 +773,10 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
 
 constexpr int WGS = 512;   // workgroups that a call's pages are shared out to: two a CU, as many as fit side by side
 
-// Row blocks of 16 rb rows, over all KV heads, that the sequences of a call can have
-long max_groups(int rb, int nseq, int ntok, int max_nt, int G, int nkv) {
+// Row blocks of 16 rb rows that the sequences of a call can have, of a KV head
+long max_groups(int rb, int nseq, int ntok, int max_nt, int G) {
     const long rows = 16 * rb, each = ((long)max_nt * G + rows - 1) / rows;
-    return std::min((long)ntok * G / rows + std::min(nseq, ntok), each * nseq) * nkv;
+    return std::min((long)ntok * G / rows + std::min(nseq, ntok), each * nseq);
 }
 // Groups of 16 rows that share a workgroup's pages. All rows of a sequence if they are 32 or fewer. Of more rows, blocks of 32 have
 // the shorter steps and the sooner first page, blocks of 64 (48 for an f32 output: more do not fit the registers) half
@@ -774,28 +790,30 @@ int row_groups(const Kv8Batch& b, int G, int nkv, bool f16out) {
     const long rows = (long)b.max_nt * G;
     if (rows <= 32) return rows <= 16 ? 1 : 2;
     const int most = f16out ? 4 : 3;
-    const long groups = max_groups(most, b.nseq, b.ntok, b.max_nt, G, nkv);
+    const long groups = max_groups(most, b.nseq, b.ntok, b.max_nt, G) * nkv;
     return (f16out ? groups >= 64 : groups >= 2048 || (rows <= 48 && groups >= 32)) ? most : 2;
 }
 
 template <int HD, int RB, class OutT>
 hipError_t launch(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int nh, float scale, OutT* out, int ots,
                   float* part, hipStream_t st) {
-    const long groups = max_groups(RB, b.nseq, b.ntok, b.max_nt, nh / c.nkv, c.nkv);
+    const int G = nh / c.nkv;
+    const long groups = max_groups(RB, b.nseq, b.ntok, b.max_nt, G), units = std::min(groups + (WGS + c.nkv - 1) / c.nkv + 1, groups * b.max_pages);
+    const long fold = (units + 65534) / 65535;
     attn_kv8_kernel<HD, RB, sizeof(OutT) == 4, OutT>
-        <<<dim3((unsigned)(groups + WGS + 1)), 256, 0, st>>>(c, b, q, qts, nh, scale, out, ots, part, WGS);
+        <<<dim3(c.nkv, (unsigned)((units + fold - 1) / fold), (unsigned)fold), 256, 0, st>>>(c, b, q, qts, G, scale, out, ots, part, WGS);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // split groups have two splits at least, so there are at most max_records / 2 of them. Few rows: many splits, so many
     // split lanes
-    const int rows = (int)std::min((long)16 * RB, (long)b.max_nt * (nh / c.nkv));
-    const long split_rows = std::min(groups, (long)kv8::max_records(WGS) / 2) * rows;
-    if (split_rows * (HD / 32) <= 1024)
-        attn_kv8_merge_kernel<HD, 16 * RB, 8, OutT><<<dim3((unsigned)(split_rows * (HD / 32))), 256, 0, st>>>(
-            c, b, q, qts, nh, out, ots, part, WGS, rows);
+    const int rows = (int)std::min((long)16 * RB, (long)b.max_nt * G);
+    const long split_rows = std::min(groups, (long)kv8::max_records(WGS) / 2 / c.nkv + 1) * rows, most = std::max(2048 / c.nkv, 1);
+    if (split_rows * c.nkv * (HD / 32) <= 1024)
+        attn_kv8_merge_kernel<HD, 16 * RB, 8, OutT><<<dim3(c.nkv, (unsigned)(split_rows * (HD / 32))), 256, 0, st>>>(
+            c, b, q, qts, G, out, ots, part, WGS, rows);
     else
-        attn_kv8_merge_kernel<HD, 16 * RB, 32, OutT><<<dim3((unsigned)std::min(split_rows * (HD / 128), 2048L)), 256, 0, st>>>(
-            c, b, q, qts, nh, out, ots, part, WGS, rows);
+        attn_kv8_merge_kernel<HD, 16 * RB, 32, OutT><<<dim3(c.nkv, (unsigned)std::min(split_rows * (HD / 128), most)), 256, 0, st>>>(
+            c, b, q, qts, G, out, ots, part, WGS, rows);
     return hipGetLastError();
 }
 template <int HD, class OutT>

@@ -32,17 +32,27 @@ IT_HD int v_elem(int row, int dim) {
 // 4032 28.4 / 30.0, 12 after 8180 21.2 / 23.1, but the 18 pages of 64 after 8128 36.7 / 33.8, and the four row blocks of 4
 // tokens after 8190, 24 heads, 20.0 / 19.4). The same in the partial and the merge kernel.
 constexpr int FEW = 4, SHORT = 10;
+IT_HD float reciprocal(float x) {   // (to a rounding or two; the splits need not be exact, only alike)
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_rcpf(x);
+#else
+    return 1.0f / x;
+#endif
+}
 IT_HD int pages_each(float work, float groups, float wgs) {
-    const float room = wgs - groups, c = work / (room < 0.5f * wgs ? 0.5f * wgs : room);
+    const float room = wgs - groups, c = work * reciprocal(room < 0.5f * wgs ? 0.5f * wgs : room);
     if (!(c < 33554432.0f)) return 33554432;   // no sequence has more pages
     const int i = (int)c;
     return (float)i < c ? i + 1 : i < 1 ? 1 : i;
 }
 IT_HD int chunk_pages(float work, float groups, int wgs) {
-    const int half = pages_each(work, groups, 0.5f * (float)wgs);
-    return groups > (float)FEW && half <= SHORT ? half : pages_each(work, groups, (float)wgs);
+    if (groups > (float)FEW) {
+        const int half = pages_each(work, groups, 0.5f * (float)wgs);
+        if (half <= SHORT) return half;
+    }
+    return pages_each(work, groups, (float)wgs);
 }
-IT_HD int splits(int pages, int chunk) { return (int)(((long)pages + chunk - 1) / chunk); }
+IT_HD int splits(int pages, int chunk) { return (int)(((unsigned)pages + (unsigned)chunk - 1u) / (unsigned)chunk); }   // (both at most 2^25)
 // Record of (split, row block, KV head) among a sequence's, and how many blocks of records all split sequences can
 // need: splits(p, c) <= 2 p / c where p > c, so at most 2 wgs and what f32 sums round off.
 IT_HD int record(int split, int nrb, int rb, int nkv, int kh) { return (split * nrb + rb) * nkv + kh; }

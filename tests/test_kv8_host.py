@@ -118,6 +118,7 @@ def test_attention_refusals(kw, text):
 
 
 @pytest.mark.parametrize("kw,text", [(dict(nh=1 << 24, ntok=2, qts=1 << 30), "overlap"), (dict(nh=1 << 24, ntok=2, ots=1 << 20, qts=0x7ffffff0), "overlap"),
+                                     (dict(nh=1 << 18, ntok=1, qts=0, ots=0), "share"),
                                      (dict(nh=1024, ntok=65535, qts=1 << 20, ots=1 << 19), "sequences")])
 def test_attention_refusals_of_sizes_past_32_bits(kw, text):
     """Widths of a token's row that pass an int, and more row blocks than a launch has room for."""
