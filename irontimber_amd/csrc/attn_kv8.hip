@@ -778,17 +778,20 @@ long max_groups(int rb, int nseq, int ntok, int max_nt, int G) {
     const long rows = 16 * rb, each = ((long)max_nt * G + rows - 1) / rows;
     return std::min((long)ntok * G / rows + std::min(nseq, ntok), each * nseq);
 }
-// Groups of 16 rows that share a workgroup's pages. All rows of a sequence if they are 32 or fewer. Of more rows, blocks of 32 have
-// the shorter steps and the sooner first page, blocks of 64 (48 for an f32 output: more do not fit the registers) half
-// the conversions of V. So the large ones where there are enough of them to fill the card, by the most that the
-// call's shapes allow. us with 32 / with the large ones (16 heads, 2 KV heads, hd 256; tokens after rows):
-//   f16, one sequence 64 after 4032   30 / 37    256 after 3840   47 / 50    256 after 32512   233 / 189    8192 after 0   734 / 627
-//        32 sequences of 5 after 8187   94 / 73    8 of 8 after 8184   39 / 41    32 of 64 after 1984   118 / 99
-//   f32, one sequence 64 after 4032   32 / 36    512 after 3584   86 / 88    4096 after 0   265 / 262    32 of 5 after 8187   106 / 83
-//        seven prompts of 24 heads   461 / 435
+// Groups of 16 rows that share a workgroup's pages. One, if there are no more rows, or up to four times as many over tables of
+// few pages: then several workgroups with a short way to their pages are sooner than one with a long way. Else all of a sequence's
+// rows up to 32; of more, blocks of 32 have the shorter steps and the sooner first page, blocks of 64 (48 for an f32 output: more do
+// not fit the registers) half the conversions of V, so the large ones where there are enough of them to fill the card, by the most
+// that the call's shapes allow. us (16 heads, 2 KV heads, hd 256; tokens after rows):
+//   16 / 32, f32, in a graph    4 after 508   10.8 / 12.4    4 after 8188   15.4 / 16.5    8 after 504   12.7 / 14.5    4 after 131068   51.7 / 43.5
+//   32 / 64, f16   64 after 4032   30 / 37    256 after 3840   47 / 50    256 after 32512   233 / 189    8192 after 0   734 / 627
+//                  32 sequences of 5 after 8187   94 / 73    8 of 8 after 8184   39 / 41    32 of 64 after 1984   118 / 99
+//   32 / 48, f32   64 after 4032   32 / 36    512 after 3584   86 / 88    4096 after 0   265 / 262    32 of 5 after 8187   106 / 83
+//                  seven prompts of 24 heads   461 / 435
 int row_groups(const Kv8Batch& b, int G, int nkv, bool f16out) {
     const long rows = (long)b.max_nt * G;
-    if (rows <= 32) return rows <= 16 ? 1 : 2;
+    if (rows <= 16 || (rows <= 64 && (long)std::min(b.nseq, b.ntok) * nkv * b.max_pages < WGS)) return 1;
+    if (rows <= 32) return 2;
     const int most = f16out ? 4 : 3;
     const long groups = max_groups(most, b.nseq, b.ntok, b.max_nt, G) * nkv;
     return (f16out ? groups >= 64 : groups >= 2048 || (rows <= 48 && groups >= 32)) ? most : 2;

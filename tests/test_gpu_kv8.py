@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 class Engine:
     """A cache with its tables on the device, and the same sequences in the reference. Pages come from a shuffled list."""
 
-    def __init__(self, dev, nseq, nkv, hd, max_pages, seed=0, spare=2):
+    def __init__(self, dev, nseq, nkv, hd, max_pages, seed=0, spare=2, wide=0):
         self.dev, self.nkv, self.hd, self.nseq = dev, nkv, hd, nseq
         npages = nseq * max_pages + spare
         self.cache = ops.kv8_cache(npages, nseq, nkv, hd, dev)
@@ -24,7 +24,7 @@ class Engine:
             t.fill_(float("nan"))
         order = np.random.default_rng(seed).permutation(npages)
         self.table_np = order[:nseq * max_pages].reshape(nseq, max_pages).astype(np.int32)
-        self.table = torch.from_numpy(self.table_np.copy()).to(dev)
+        self.table = torch.from_numpy(np.pad(self.table_np, ((0, 0), (0, wide)), constant_values=-1)).to(dev)
         self.seqs = [ref.Sequence(nkv, hd) for _ in range(nseq)]
         self.rng = np.random.default_rng(seed + 1)
 
@@ -222,6 +222,27 @@ def test_attention_geometries(dev, nh, nkv, hd, f16):
     for counts in ([100, 64, 1, 0], [1, 1, 0, 1], [3, 4, 5, 1], [17, 2, 90, 128], [1, 1, 1, 1]):
         start, length = e.append(counts)
         e.attend(e.queries(sum(counts), nh), start, length, counts, nh, f16=f16)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 256), (24, 4, 256), (8, 8, 128), (7, 1, 256), (32, 2, 128), (34, 1, 128)])
+@pytest.mark.parametrize("f16", [False, True])
+def test_geometries_over_wide_tables(dev, nh, nkv, hd, f16):
+    """Tables that could name long contexts call for row blocks of more rows."""
+    announce(f"kv8 wide {nh}/{nkv} {hd} f16={f16}")
+    e = Engine(dev, 4, nkv, hd, 8, wide=600)
+    for counts in ([100, 64, 1, 0], [3, 4, 5, 1], [17, 2, 90, 128], [2, 1, 2, 3], [8, 8, 8, 8]):
+        start, length = e.append(counts)
+        e.attend(e.queries(sum(counts), nh), start, length, counts, nh, f16=f16)
+
+
+@pytest.mark.parametrize("before,n", [(0, 2), (63, 4), (64, 3), (4103, 4), (9000, 8), (200, 8)])
+def test_lengths_over_wide_tables(dev, before, n):
+    e = Engine(dev, 1, 2, 256, before // 64 + 2, wide=600)
+    if before:
+        e.append([before])
+    start, length = e.append([n])
+    for f16 in (False, True):
+        e.attend(e.queries(n, 16), start, length, [n], 16, f16=f16)
 
 
 @pytest.mark.parametrize("before", [0, 1, 15, 62, 63, 64, 65, 127, 128, 191, 319, 640])
