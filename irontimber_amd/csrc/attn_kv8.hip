@@ -677,7 +677,9 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
         const int t = u.nrb == 1 ? div_small(row, rcp_G) : (int)((unsigned)r / (unsigned)G), h = kh * G + r - t * G;
         const int last = (u.len + t) / kv8::PAGE, need = (chunk == 1 ? last : (int)((unsigned)last / (unsigned)chunk)) + 1;
         const float* base = part + (size_t)nrec * ROWS * 2;
-        auto gather = [&](int first, int lanes, int dim) __attribute__((always_inline)) {
+        const int dim = 4 * (alone ? l % WL : DL * (sub % DQ) + tid % DL);
+        const f4 gate = ld_f4(q + (size_t)(u.t0 + t) * qts + (size_t)h * 2 * HD + HD + dim);   // (beside the records)
+        auto gather = [&](int first, int lanes) __attribute__((always_inline)) {
             Part p = {-INFINITY, 0.f, f4{}};
             for (int s = first; s < need; s += lanes * NB) {   // (past the last record: the last again, uncounted)
                 f2 ml[NB];
@@ -707,8 +709,7 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
             }
             return p;
         };
-        auto finish = [&](const Part& p, int dim) __attribute__((always_inline)) {
-            const f4 gate = ld_f4(q + (size_t)(u.t0 + t) * qts + (size_t)h * 2 * HD + HD + dim);
+        auto finish = [&](const Part& p) __attribute__((always_inline)) {
             const float inv = 1.0f / p.sum;
             f4 v;
 #pragma unroll
@@ -721,20 +722,18 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
             return Part{M, p.sum * e, p.o * e};
         };
         if (alone) {
-            const int dim = 4 * (l % WL);
-            Part p = gather(l / WL, 64 / WL, dim);
+            Part p = gather(l / WL, 64 / WL);
             if constexpr (WL == 32) {
                 p = scaled(p, max_xor32(p.m));
                 p.sum = sum_xor32(p.sum);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p.o[i] = sum_xor32(p.o[i]);
             }
-            if (l < WL) finish(p, dim);
+            if (l < WL) finish(p);
             continue;
         }
         // the split lanes of a wave, then the four waves
-        const int dim = 4 * (DL * (sub % DQ) + tid % DL);
-        Part p = gather(tid / DL, SL, dim);
+        Part p = gather(tid / DL, SL);
         float M = max_xor32(p.m);
         if constexpr (DL == 8) {
             M = max_xor16(M);
@@ -766,7 +765,7 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
                 p.sum += red_l[i][tid] * f;
                 p.o += red_o[i][tid] * f;
             }
-            finish(p, dim);
+            finish(p);
         }
     }
 }
