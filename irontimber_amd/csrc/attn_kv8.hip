@@ -59,12 +59,15 @@ template <int N> __device__ __forceinline__ void kib_to_lds(const uint8_t* from,
         asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\tglobal_load_lds_dwordx4 %1, %2"
                      ::"s"(at), "v"(off), "s"(from) : "memory");
 }
-__device__ __forceinline__ int prefix_sum(int v, int l) {   // inclusive, over the wave
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int u = __shfl_up(v, d);
-        v += l >= d ? u : 0;
-    }
+// Inclusive, over the wave: within rows of 16 lanes, then the rows before (by lane moves; through LDS the batch's 32 lengths
+// were 1,500 cycles of the way to a page)
+__device__ __forceinline__ int prefix_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15 to the next row: rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31 to rows 2 and 3
     return v;
 }
 
@@ -116,7 +119,7 @@ __device__ __forceinline__ Found find(const Kv8Batch& b, const Kv8Seq& s0, int G
         const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
         const int nrb = (s.n * G + ROWS - 1) / ROWS, ns = kv8::splits(s.pages, chunk);
         const int recs = ns > 1 ? nrb * ns * nkv : 0, units = GROUPS ? (ns > 1 ? nrb : 0) : nrb * ns;
-        const int pu = prefix_sum(units, l), pr = prefix_sum(recs, l);
+        const int pu = prefix_sum(units), pr = prefix_sum(recs);
         const unsigned long long hit = __ballot(base + pu > id);
         if (hit) {
             const int src = __builtin_ctzll(hit);
@@ -665,7 +668,7 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
     for (int i0 = 0; i0 < b.nseq; i0 += 64) {
         const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
         const int ns = kv8::splits(s.pages, chunk), n = ns > 1 ? (s.n * G + ROWS - 1) / ROWS : 0;
-        groups += b.nseq == 1 ? __builtin_amdgcn_readfirstlane(n) : __builtin_amdgcn_readlane(prefix_sum(n, l), 63);
+        groups += b.nseq == 1 ? __builtin_amdgcn_readfirstlane(n) : __builtin_amdgcn_readlane(prefix_sum(n), 63);
         if (__any(n > 0 && ns > FEW)) alone_all = false;
     }
     const int each = alone_all ? (rows + 3) / 4 : DQ * rows;
