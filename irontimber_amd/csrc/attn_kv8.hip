@@ -89,7 +89,23 @@ __device__ __forceinline__ int call_chunk(const Kv8Batch& b, const Kv8Seq& s0, i
         sum += wave_sum(nrb * (float)s.pages);
         blocks += wave_sum(nrb);
     }
-    return kv8::chunk_pages(readlane_f(sum, 0) * (float)nkv, readlane_f(blocks, 0) * (float)nkv, wgs);
+    const float work = readlane_f(sum, 0) * (float)nkv, groups = readlane_f(blocks, 0) * (float)nkv;
+    int chunk = kv8::chunk_pages(work, groups, wgs);
+    if (chunk > (ROWS == 16 ? 12 : 18) && groups <= (float)wgs) {   // (of fewer, the count costs more than it gives)
+        float rcp[kv8::TRIES], units[kv8::TRIES] = {};
+#pragma unroll
+        for (int k = 0; k < kv8::TRIES; ++k) rcp[k] = __builtin_amdgcn_rcpf((float)kv8::fewer_pages(work, groups, wgs, k));
+        for (int i0 = 0; i0 < b.nseq; i0 += 64) {
+            const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
+            const float nrb = (float)((s.n * G + ROWS - 1) / ROWS);
+#pragma unroll
+            for (int k = 0; k < kv8::TRIES; ++k) units[k] += wave_sum(nrb * kv8::about_splits(s.pages, rcp[k]));
+        }
+#pragma unroll
+        for (int k = kv8::TRIES - 1; k >= 0; --k)
+            if (readlane_f(units[k], 0) * (float)nkv <= (float)wgs) chunk = kv8::fewer_pages(work, groups, wgs, k);
+    }
+    return chunk;
 }
 
 // What is found for a workgroup, in scalar registers: its sequence, the index of its unit (main kernel) or of its row block that

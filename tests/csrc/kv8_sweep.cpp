@@ -68,6 +68,37 @@ int main() {
         if (recs > kv8::max_records(wgs)) die("records", recs, wgs);
         if (2 * split_groups > kv8::max_records(wgs)) die("groups", split_groups, wgs);
     }
+    // Fewer pages per split where the count allows: the records still fit, whatever the count is off by
+    for (int it = 0; it < 20000; ++it) {
+        const int nseq = 1 + rnd(130), nkv = 1 + rnd(8), wgs = 512, most = 1 << (1 + rnd(it % 7 ? 12 : 25));
+        std::vector<int> nrb(nseq), pages(nseq);
+        float sum = 0.f, blocks = 0.f;
+        for (int i = 0; i < nseq; ++i) {
+            nrb[i] = rnd(4) ? 1 + rnd(3) : 0;
+            pages[i] = it % 3 ? 1 + rnd(most) : most;
+            sum += (float)nrb[i] * (float)pages[i];
+            blocks += (float)nrb[i];
+        }
+        for (int k = 0; k < kv8::TRIES; ++k) {
+            const int chunk = kv8::fewer_pages(sum * (float)nkv, blocks * (float)nkv, wgs, k);
+            if (chunk < 1 || (k && chunk < kv8::fewer_pages(sum * (float)nkv, blocks * (float)nkv, wgs, k - 1))) die("fewer", chunk, k);
+            if (chunk == 33554432) continue;
+            float units = 0.f;
+            long exact = 0, recs = 0;
+            for (int i = 0; i < nseq; ++i) {
+                const int ns = kv8::splits(pages[i], chunk);
+                const float about = kv8::about_splits(pages[i], 1.0f / (float)chunk);
+                if (about > (float)ns || about < (float)ns - 1) die("about", pages[i], chunk);
+                units += (float)nrb[i] * about;
+                exact += (long)nrb[i] * ns * nkv;
+                if (ns > 1) recs += (long)nrb[i] * ns * nkv;
+            }
+            if (units * (float)nkv > (float)wgs) continue;
+            if (exact > (long)(blocks * (float)nkv) + wgs + 1) die("fewer units", exact, it);
+            if (recs > kv8::max_records(wgs)) die("fewer records", recs, it);
+            ++checks;
+        }
+    }
     std::printf("ok %ld\n", checks);
     return 0;
 }
