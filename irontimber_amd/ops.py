@@ -733,12 +733,13 @@ def _kv8_batch(dev: int, nseq: int, start: torch.Tensor, length: torch.Tensor, t
 
 def _kv8_rows(dev: int, kvd: int, k: torch.Tensor, v: torch.Tensor) -> int:
     """Token stride of f16 rows k, v [ntok, kvd]; rows may lie apart, as a slice of wider ones."""
-    for t in (k, v):
-        if t.dtype is not torch.float16 or t.get_device() != dev or len(t.shape) != 2 or t.shape[1] != kvd:
-            raise ValueError(f"k and v must be [ntok, {kvd}] f16 on the cache's device")
-        if t.shape != k.shape or t.stride() != k.stride() or t.stride(1) != 1:
-            raise ValueError("k and v must have one shape and one stride, with each row's values side by side")
-    return k.stride(0)
+    shape, step = k.shape, k.stride()
+    if not (k.dtype is torch.float16 and v.dtype is torch.float16 and k.get_device() == dev and v.get_device() == dev and
+            len(shape) == 2 and shape[1] == kvd):
+        raise ValueError(f"k and v must be [ntok, {kvd}] f16 on the cache's device")
+    if v.shape != shape or v.stride() != step or step[1] != 1:
+        raise ValueError("k and v must have one shape and one stride, with each row's values side by side")
+    return step[0]
 
 
 def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, length: torch.Tensor,
@@ -763,9 +764,11 @@ def kv8_read(cache: Kv8Cache, start: torch.Tensor, first: torch.Tensor, total: t
     pages = _kv8_batch(dev, nseq, start, total, table)
     if first.shape != (nseq,):
         raise ValueError(f"first must be [{nseq}]")
-    _need_all(torch.int32, dev, (first,), "first")
+    if first.dtype is not torch.int32 or first.get_device() != dev or not first.is_contiguous():
+        _need_all(torch.int32, dev, (first,), "first")
     if out is None:
-        out = tuple(torch.empty(rows, nkv * hd, dtype=torch.float16, device=cache.kp.device) for _ in range(2))
+        at = cache.kp.device
+        out = (torch.empty(rows, nkv * hd, dtype=torch.float16, device=at), torch.empty(rows, nkv * hd, dtype=torch.float16, device=at))
     k, v = out
     stride = _kv8_rows(dev, nkv * hd, k, v)
     if k.shape[0] != rows:
