@@ -15,7 +15,7 @@
 // The page's element order is that of the matrix operands. Each wave copies the 4 hd bytes that it alone needs straight into its
 // part of LDS, a page or two ahead, and reads them back without a barrier; one barrier a page, for P.
 //
-// What bounds it (MI355X, hd 256): few tokens, the bytes of the codes: 7.0 - 7.6 TB/s of them in a long context, behind 7 us for a
+// What bounds it (MI355X, hd 256): few tokens, the bytes of the codes: 7.0 - 7.6 TB/s of them in a long context, behind 6 us for a
 // launch's first page and 4 for the join of the splits. Whole prompts, the vector units beside the matrix ones: the
 // softmax, 96 operations for a page's V and 16 for its K are 360 of a step's 464 in a wave, matrix units 41 % busy, 0.87 PFLOP/s.
 //

@@ -279,6 +279,19 @@ def test_one_split_of_many_pages(dev):
     e.attend(e.queries(sum(counts), 8), start, length, counts, 8, f16=True)
 
 
+@pytest.mark.parametrize("alike", [True, False])
+def test_many_sequences_of_many_pages(dev, alike):
+    """A batch past one wave's 64 sequences, whose splits are chosen by counting them."""
+    nseq, nkv, hd = 68, 2, 128
+    e = Engine(dev, nseq, nkv, hd, 48)
+    lens = [2900 if alike else 2000 + (i * 379) % 1000 for i in range(nseq)]
+    e.append(lens)
+    counts = [0 if i in (5, 64) else 1 + i % 2 for i in range(nseq)]
+    start, length = e.append(counts)
+    for f16 in (False, True):
+        e.attend(e.queries(sum(counts), 16), start, length, counts, 16, f16=f16)
+
+
 def test_whole_prompts(dev):
     """Prompts long enough that no row block is split."""
     for f16 in (False, True):
