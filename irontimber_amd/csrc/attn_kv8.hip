@@ -48,12 +48,12 @@ template <int N> __device__ __forceinline__ void kib_to_lds(const uint8_t* from,
     static_assert(N == 1 || N == 2 || N == 4, "a wave's share of a page");
     if constexpr (N == 4)
         asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\t"
-                     "global_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
-                     "global_load_lds_dwordx4 %1, %2 offset:2048\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072"
+                     "global_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:0x400\n\t"
+                     "global_load_lds_dwordx4 %1, %2 offset:0x800\n\tglobal_load_lds_dwordx4 %1, %2 offset:0xC00"
                      ::"s"(at), "v"(off), "s"(from) : "memory");
     else if constexpr (N == 2)
         asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\t"
-                     "global_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                     "global_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:0x400"
                      ::"s"(at), "v"(off), "s"(from) : "memory");
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\tglobal_load_lds_dwordx4 %1, %2"
