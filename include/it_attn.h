@@ -604,6 +604,8 @@ int it_kv8_copy(const it_kv8_cache* cache, const int32_t* src, const int32_t* ds
  * in fixed point, to 2^-23 of its head's largest value (2^-22 of itself against the open rows), a probability as an f16 pair, to
  * 2^-22 of itself or, where it is small, 2^-31 of its row's largest up to there. For an f16 output q to 2^-15, a probability as
  * one f16 (2^-12): about 1.5e-4 of the result beside the output's own rounding.
+ * At most 2^26 tokens times heads, 2^23 sequences times KV heads, 2^16 query heads of a KV head. Which sequences share a call
+ * decides how the pages are split, so it moves results by roundings; the same call gives the same bits.
  * scratch: it_attn_kv8_scratch_bytes bytes, 16-byte aligned (one per call that may overlap another). */
 size_t it_attn_kv8_scratch_bytes(int max_nt, int hd, int nh, int nkv);
 int it_attn_kv8(const it_kv8_cache* cache, const float* q, int q_tok_stride, int ntok, const int32_t* start,
