@@ -67,13 +67,13 @@ __device__ __forceinline__ uint32_t codes_of(const Steps& t, _Float16 a, _Float1
 // a half takes the new rows of its page among the last two. Where it still holds old rows that the first page needs and that
 // another page's rows replace, the first page's workgroup writes it, after it has read them.
 // Both kinds work in the page's order, which the old open rows have already. New rows of V get there through LDS.
-// A wave a KiB of codes, 16 values a lane: with 4 waves of 64 values each the call was as slow as the fetching of the code that
-// each CU then runs once or twice (8192 rows 23.5 us, so 12.4).
+// A wave U = 2 KiB of codes, 32 values a lane: with more to a wave the call is as slow as the fetching of the code that each CU then
+// runs once or twice, with less as the starting of its waves (U 1, 2, 4: 8192 rows 12.1, 10.8, 11.3 us, one page 5.3, 5.0, 5.8).
 // Bound by bytes, two read and one written a value, and in short calls by three dependent round trips (bounds, rows, stores).
 template <int HD>
-__global__ __launch_bounds__(4 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, const _Float16* __restrict__ k,
+__global__ __launch_bounds__(2 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, const _Float16* __restrict__ k,
                                                             const _Float16* __restrict__ v, int kts) {
-    constexpr int NT = 4 * HD, CH = HD / 8, PITCH = HD + 8;   // (rows four apart in LDS: 16 banks apart)
+    constexpr int NT = 2 * HD, NW = NT / 64, U = 2, CH = HD / 8, PITCH = HD + 8;   // (rows four apart in LDS: 16 banks apart)
     __shared__ __align__(16) _Float16 tile[kv8::PAGE * PITCH];
     __shared__ float most[HD / 16][4];
     const int i = blockIdx.z, kh = blockIdx.y >> 1, which = blockIdx.y & 1, j = (int)blockIdx.x - 2;   // -2, -1: halves
@@ -89,18 +89,18 @@ __global__ __launch_bounds__(4 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, c
     // Rows from .. to - 1 of V, from row0 on, into the tile, a row of 8 dims a thread and turn
     auto stage = [&](int row0, int from, int to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < 2 * U; ++n) {
             const int row = row0 + (n * NT + tid) / CH, ch = tid % CH;
             if (row >= from && row < to)
                 *(h8*)(tile + (row - row0) * PITCH + 8 * ch) = finite8(ld_h8(src + (size_t)(row - s.len) * kts + 8 * ch));
         }
     };
-    // This lane's four rows of each block and one dim of dim block w, from the tile where they are from .. to - 1, else x
-    auto pick = [&](int row0, int from, int to, h8 (&x)[2]) __attribute__((always_inline)) {
+    // This lane's four rows of each block and one dim of dim block kib, from the tile where they are from .. to - 1, else x
+    auto pick = [&](int kib, int row0, int from, int to, h8 (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int r = 16 * (e >> 2) + 4 * g + (e & 3);
-            const _Float16 z = tile[r * PITCH + 16 * w + lr];
+            const _Float16 z = tile[r * PITCH + 16 * kib + lr];
             x[e >> 3][e & 7] = row0 + r >= from && row0 + r < to ? z : x[e >> 3][e & 7];
         }
     };
@@ -109,48 +109,67 @@ __global__ __launch_bounds__(4 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, c
         const int id = b.table[(size_t)i * b.max_pages + p];
         const bool known = (unsigned)id < (unsigned)c.npages;
         const size_t unit = known ? (size_t)id * c.nkv + kh : 0;
-        const _Float16* old = open + (p & 1) * half + (w * 64 + l) * 16;
-        h8 x[2] = {};
+        const _Float16* old = open + (p & 1) * half + (w * 64 + l) * 16;   // (KiB w + NW u: 1024 NW u on)
+        h8 x[U][2] = {};
         if (!which) {
-            // wave = (block, 64 dims): each lane holds two runs of 8 dims of a row
-            const int a = w / (HD / 64), row = row0 + 16 * a + lr, dim = 64 * (w % (HD / 64)) + 8 * g;
+            // KiB = (block, 64 dims): each lane holds two runs of 8 dims of a row
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                x[h] = finite8(ld_h8(row >= s.len ? src + (size_t)(row - s.len) * kts + dim + 32 * h : old + 8 * h));
-            const float m = wave_max(size_of(max(sizes(x[0]), sizes(x[1]))));
-            if (l == 0) most[w][0] = m;
+            for (int u = 0; u < U; ++u) {
+                const int kib = w + NW * u, row = row0 + 16 * (kib / (HD / 64)) + lr, dim = 64 * (kib % (HD / 64)) + 8 * g;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    x[u][h] = finite8(ld_h8(row >= s.len ? src + (size_t)(row - s.len) * kts + dim + 32 * h : old + NW * 1024 * u + 8 * h));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float m = wave_max(size_of(max(sizes(x[u][0]), sizes(x[u][1]))));
+                if (l == 0) most[w + NW * u][0] = m;
+            }
             __syncthreads();
-            float top = 0.f;
 #pragma unroll
-            for (int n = 0; n < HD / 64; ++n) top = fmaxf(top, most[a * (HD / 64) + n][0]);
-            const Steps t(block_scale(top));
-            if (known) {
-                u4 y;
+            for (int u = 0; u < U; ++u) {
+                const int kib = w + NW * u, a = kib / (HD / 64);
+                float top = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const h8 z = x[e >> 1];
-                    const int o = 4 * (e & 1);
-                    y[e] = codes_of(t, z[o], z[o + 1], z[o + 2], z[o + 3]);
+                for (int n = 0; n < HD / 64; ++n) top = fmaxf(top, most[a * (HD / 64) + n][0]);
+                const Steps t(block_scale(top));
+                if (known) {
+                    u4 y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const h8 z = x[u][e >> 1];
+                        const int o = 4 * (e & 1);
+                        y[e] = codes_of(t, z[o], z[o + 1], z[o + 2], z[o + 3]);
+                    }
+                    *(u4*)(c.kp + unit * (kv8::PAGE * HD) + (kib * 64 + l) * 16) = y;
+                    if (l == 0 && kib % (HD / 64) == 0) c.sc[unit * 8 + a] = (_Float16)t.s;
                 }
-                *(u4*)(c.kp + unit * (kv8::PAGE * HD) + (w * 64 + l) * 16) = y;
-                if (l == 0 && w % (HD / 64) == 0) c.sc[unit * 8 + a] = (_Float16)t.s;
             }
         } else {
             if (row0 < s.len) {
-                x[0] = ld_h8(old);
-                x[1] = ld_h8(old + 8);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    x[u][0] = ld_h8(old + NW * 1024 * u);
+                    x[u][1] = ld_h8(old + NW * 1024 * u + 8);
+                }
             }
             stage(row0, s.len, total);
             __syncthreads();
-            pick(row0, s.len, total, x);
+#pragma unroll
+            for (int u = 0; u < U; ++u) pick(w + NW * u, row0, s.len, total, x[u]);
             // largest sizes of the four blocks, lane row g ending with block g, then one lane in four with each wave's
             float m[4];
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-                h8 z = {};
+                uint32_t most_bits = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[e] = x[a >> 1][4 * (a & 1) + e];
-                m[a] = size_of(sizes(z));
+                for (int u = 0; u < U; ++u) {
+                    h8 z = {};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[e] = x[u][a >> 1][4 * (a & 1) + e];
+                    most_bits = max(most_bits, sizes(z));
+                }
+                m[a] = size_of(most_bits);
             }
             swap32(m[0], m[2]);
             swap32(m[1], m[3]);
@@ -163,20 +182,23 @@ __global__ __launch_bounds__(4 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, c
             m0 = fmaxf(m0, dppc<0x140>(m0));
             if (lr == 0) most[w][2 * (g >> 1) + (g & 1)] = m0;
             __syncthreads();
-            m0 = most[min(l >> 2, HD / 16 - 1)][l & 3];
+            m0 = most[min(l >> 2, NW - 1)][l & 3];
             m0 = fmaxf(m0, dppc<0x124>(m0));   // row_ror 4, 8
             m0 = fmaxf(m0, dppc<0x128>(m0));
             const Steps mine(block_scale(max_xor32(max_xor16(m0))));   // of block l % 4
             if (known && tid < 4) c.sc[unit * 8 + 4 + tid] = (_Float16)mine.s;
-            u4 y;
 #pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                const Steps t(readlane_f(mine.s, a), readlane_f(mine.inv, a));
-                const h8 z = x[a >> 1];
-                const int o = 4 * (a & 1);
-                y[a] = codes_of(t, z[o], z[o + 1], z[o + 2], z[o + 3]);
+            for (int u = 0; u < U; ++u) {
+                u4 y;
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const Steps t(readlane_f(mine.s, a), readlane_f(mine.inv, a));
+                    const h8 z = x[u][a >> 1];
+                    const int o = 4 * (a & 1);
+                    y[a] = codes_of(t, z[o], z[o + 1], z[o + 2], z[o + 3]);
+                }
+                if (known) *(u4*)(c.vp + unit * (kv8::PAGE * HD) + ((w + NW * u) * 64 + l) * 16) = y;
             }
-            if (known) *(u4*)(c.vp + unit * (kv8::PAGE * HD) + (w * 64 + l) * 16) = y;
         }
         __syncthreads();   // old open rows read before the half is written below, and the tile before it is filled anew
     }
@@ -200,17 +222,23 @@ __global__ __launch_bounds__(4 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, c
     }
     // many rows of V: through LDS, in whole pieces of the page's order that keep the rows before `from`; the rows from `to` on
     // hold anything
-    h8* piece = (h8*)(dst + (w * 64 + l) * 16);
-    h8 x[2] = {};
+    h8* piece = (h8*)(dst + (w * 64 + l) * 16);   // (KiB w + NW u: 128 NW u on)
+    h8 x[U][2] = {};
     if (from > r0) {
-        x[0] = piece[0];
-        x[1] = piece[1];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            x[u][0] = piece[NW * 128 * u];
+            x[u][1] = piece[NW * 128 * u + 1];
+        }
     }
     stage(r0, from, to);
     __syncthreads();
-    pick(r0, from, to, x);
-    piece[0] = x[0];
-    piece[1] = x[1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        pick(w + NW * u, r0, from, to, x[u]);
+        piece[NW * 128 * u] = x[u][0];
+        piece[NW * 128 * u + 1] = x[u][1];
+    }
 }
 
 // Workgroup = (sequence, page, KV head, K or V): rows first[i] .. of a sequence that holds len[i] rows, as f16.
@@ -321,8 +349,8 @@ hipError_t launch_kv8_append(const Kv8& c, const Kv8Batch& b, const uint16_t* k,
                              hipStream_t st) {
     const dim3 grid(2 + touched(b.max_nt), 2 * c.nkv, b.nseq);
     const auto *kk = (const _Float16*)k, *vv = (const _Float16*)v;
-    if (c.hd == 256) kv8_append_kernel<256><<<grid, 1024, 0, st>>>(c, b, kk, vv, kts);
-    else kv8_append_kernel<128><<<grid, 512, 0, st>>>(c, b, kk, vv, kts);
+    if (c.hd == 256) kv8_append_kernel<256><<<grid, 512, 0, st>>>(c, b, kk, vv, kts);
+    else kv8_append_kernel<128><<<grid, 256, 0, st>>>(c, b, kk, vv, kts);
     return hipGetLastError();
 }
 hipError_t launch_kv8_read(const Kv8& c, const Kv8Batch& b, const int* first, uint16_t* k, uint16_t* v, int kts,
