@@ -242,10 +242,11 @@ __global__ __launch_bounds__(2 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, c
 }
 
 // Workgroup = (sequence, page, KV head, K or V): rows first[i] .. of a sequence that holds len[i] rows, as f16.
+// A wave two KiB, as in appending (four waves of four KiB, one after the other: a page 4.2 us, so 3.4; 8192 rows 8.2, so 7.6).
 template <int HD>
-__global__ __launch_bounds__(256) void kv8_read_kernel(Kv8 c, Kv8Batch b, const int* __restrict__ first,
+__global__ __launch_bounds__(2 * HD) void kv8_read_kernel(Kv8 c, Kv8Batch b, const int* __restrict__ first,
                                                        _Float16* __restrict__ k, _Float16* __restrict__ v, int kts) {
-    constexpr int CH = HD / 8, PITCH = HD + 8;
+    constexpr int NT = 2 * HD, NW = NT / 64, U = 2, CH = HD / 8, PITCH = HD + 8;
     __shared__ __align__(16) _Float16 tile[kv8::PAGE * PITCH];
     const int i = blockIdx.z, kh = blockIdx.y >> 1, which = blockIdx.y & 1;
     const int t0 = b.start[i], t1 = b.start[i + 1], r0 = first[i], total = b.len[i];
@@ -264,38 +265,49 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8 c, Kv8Batch b, const 
     const uint8_t* page = (which ? c.vp : c.kp) + unit * (kv8::PAGE * HD);
     const _Float16 bad = __builtin_bit_cast(_Float16, (uint16_t)0x7E00);   // a page that the pool has not: NaN
     const _Float16* sc = c.sc + unit * 8 + 4 * which;
-    for (int n = w; n < HD / 16; n += 4) {   // KiB n of the page
-        h8 x[2];
-        if (is_open) {
-            x[0] = ld_h8(open + (n * 64 + l) * 16);
-            x[1] = ld_h8(open + (n * 64 + l) * 16 + 8);
-        } else {
-            const u4 y = *(const u4*)(page + (n * 64 + l) * 16);
+    // this wave's KiB w and w + NW of the page, both under way at once
+    h8 x[U][2];
+    if (is_open) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            x[u][0] = ld_h8(open + ((w + NW * u) * 64 + l) * 16);
+            x[u][1] = ld_h8(open + ((w + NW * u) * 64 + l) * 16 + 8);
+        }
+    } else {
+        u4 y[U];
+        const h4 four = *(const h4*)sc;
+#pragma unroll
+        for (int u = 0; u < U; ++u) y[u] = *(const u4*)(page + ((w + NW * u) * 64 + l) * 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-                const h4 z = codes4(y[a]);
-                const _Float16 f = known ? sc[which ? a : n / (HD / 64)] : bad;
+                const h4 z = codes4(y[u][a]);
+                const _Float16 f = known ? which ? four[a] : sc[(w + NW * u) / (HD / 64)] : bad;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[a >> 1][4 * (a & 1) + e] = z[e] * f;
+                for (int e = 0; e < 4; ++e) x[u][a >> 1][4 * (a & 1) + e] = z[e] * f;
             }
-        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int n = w + NW * u;
         if (!which) {
             const int row = 16 * (n / (HD / 64)) + (l & 15), dim = 64 * (n % (HD / 64)) + 8 * (l >> 4);
             if (row >= lo && row < hi) {
-                *(h8*)(dst + (long)row * kts + dim) = x[0];
-                *(h8*)(dst + (long)row * kts + dim + 32) = x[1];
+                *(h8*)(dst + (long)row * kts + dim) = x[u][0];
+                *(h8*)(dst + (long)row * kts + dim + 32) = x[u][1];
             }
         } else {
 #pragma unroll
             for (int a = 0; a < 4; ++a)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    tile[(16 * a + 4 * (l >> 4) + e) * PITCH + 16 * n + (l & 15)] = x[a >> 1][4 * (a & 1) + e];
+                    tile[(16 * a + 4 * (l >> 4) + e) * PITCH + 16 * n + (l & 15)] = x[u][a >> 1][4 * (a & 1) + e];
         }
     }
     if (!which) return;   // (whole workgroup)
     __syncthreads();
-    for (int n = tid; n < (hi - lo) * CH; n += 256) {
+    for (int n = tid; n < (hi - lo) * CH; n += NT) {
         const int row = lo + n / CH, ch = n % CH;
         *(h8*)(dst + (long)row * kts + 8 * ch) = *(const h8*)(tile + row * PITCH + 8 * ch);
     }
@@ -357,7 +369,7 @@ hipError_t launch_kv8_read(const Kv8& c, const Kv8Batch& b, const int* first, ui
                            hipStream_t st) {
     const dim3 grid(touched(b.max_nt), 2 * c.nkv, b.nseq);
     auto *kk = (_Float16*)k, *vv = (_Float16*)v;
-    if (c.hd == 256) kv8_read_kernel<256><<<grid, 256, 0, st>>>(c, b, first, kk, vv, kts);
+    if (c.hd == 256) kv8_read_kernel<256><<<grid, 512, 0, st>>>(c, b, first, kk, vv, kts);
     else kv8_read_kernel<128><<<grid, 256, 0, st>>>(c, b, first, kk, vv, kts);
     return hipGetLastError();
 }
