@@ -185,8 +185,8 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     constexpr int KIB = 1024, QUARTER = 16 * HD;   // a wave's share of a page's codes
     // Forms of many rows keep a part of q's digits in LDS, and one page of V in place of two: 256 registers and half of a
     // CU's LDS, so that two workgroups share a CU.
-    constexpr int KB = RB == 1 ? 2 : 1, VB = RB >= 3 ? 1 : 2;            // pages of K and of V
-    constexpr int QL = HD < 256 || RB < 3 ? 0 : RB - 2, NR = NJ - QL;    // of q's NJ groups of 64 dims: in LDS, in registers
+    constexpr int KB = RB == 1 ? 2 : 1, VB = RB == 4 || (RB == 3 && PAIRS) ? 1 : 2;   // pages of K and of V
+    constexpr int QL = HD < 256 || VB == 2 ? 0 : RB - 2, NR = NJ - QL;    // of q's NJ groups of 64 dims: in LDS, in registers
     __shared__ __align__(16) uint8_t kbuf[KB][4 * QUARTER], vbuf[VB][4 * QUARTER];
     __shared__ __align__(16) u4 qlast[QL ? RB : 1][QL ? QL : 1][DG][QL ? 64 : 1];
     __shared__ __align__(16) _Float16 pbuf[2][RB][2][NP][64 * 8];   // P^T operands: [parity][rows][keys][hi, lo]
@@ -801,21 +801,26 @@ long max_groups(int rb, int nseq, int ntok, int max_nt, int G) {
 }
 // Groups of 16 rows that share a workgroup's pages. One, if there are no more rows, or up to four times as many over tables of
 // few pages: then several workgroups with a short way to their pages are sooner than one with a long way. Else all of a sequence's
-// rows up to 32; of more, blocks of 32 have the shorter steps and the sooner first page, blocks of 64 (48 for an f32 output: more do
-// not fit the registers) half the conversions of V, so the large ones where there are enough of them to fill the card, by the most
-// that the call's shapes allow. us (16 heads, 2 KV heads, hd 256; tokens after rows):
+// rows up to 32; of more, blocks of 32 have the shorter steps and the sooner first page, blocks of 48 or 64 (f16 outputs: more do
+// not fit the registers) fewer conversions of V a row, so the large ones where there are enough of them to fill the card, by
+// the most that the call's shapes allow. 64 for full batches of few tokens that it divides better; 48 else, which leave more of
+// q in registers and share out the unlike blocks of a prompt more evenly.
+// us (16 heads, 2 KV heads, hd 256; tokens after rows):
 //   16 / 32, f32, in a graph    4 after 508   10.8 / 12.4    4 after 8188   15.4 / 16.5    8 after 504   12.7 / 14.5    4 after 131068   51.7 / 43.5
-//   32 / 64, f16   64 after 4032   30 / 37    256 after 3840   47 / 50    256 after 32512   233 / 189    8192 after 0   734 / 627
-//                  32 sequences of 5 after 8187   94 / 73    8 of 8 after 8184   39 / 41    32 of 64 after 1984   118 / 99
+//   32 / 48 / 64, f16   64 after 4032   30 / - / 37    256 after 3840   47 / 45 / 51    256 after 32512   233 / 192 / 192    2048 after 0   68 / 60 / 78
+//                       8192 after 0   734 / 619 / 626    512 after 32256   467 / 394 / 376    32 sequences of 5 after 8187   94 / 63 / 68
+//                       of 8 after 8184   95 / 98 / 75    of 64 after 1984   118 / 113 / 100    1000 after 3000, 24 heads   - / 112 / 139
 //   32 / 48, f32   64 after 4032   32 / 36    512 after 3584   86 / 88    4096 after 0   265 / 262    32 of 5 after 8187   106 / 83
 //                  seven prompts of 24 heads   461 / 435
 int row_groups(const Kv8Batch& b, int G, int nkv, bool f16out) {
     const long rows = (long)b.max_nt * G;
     if (rows <= 16 || (rows <= 64 && (long)std::min(b.nseq, b.ntok) * nkv * b.max_pages < WGS)) return 1;
     if (rows <= 32) return 2;
-    const int most = f16out ? 4 : 3;
-    const long groups = max_groups(most, b.nseq, b.ntok, b.max_nt, G) * nkv;
-    return (f16out ? groups >= 64 : groups >= 2048 || (rows <= 48 && groups >= 32)) ? most : 2;
+    const long groups = max_groups(f16out ? 4 : 3, b.nseq, b.ntok, b.max_nt, G) * nkv;
+    if (!f16out) return groups >= 2048 || (rows <= 48 && groups >= 32) ? 3 : 2;
+    if (groups < 64) return 2;
+    const bool full = b.nseq > 1 && (long)b.nseq * b.max_nt == b.ntok && rows <= 1024;
+    return full && (rows + 63) / 64 * 64 <= (rows + 47) / 48 * 48 ? 4 : 3;
 }
 
 template <int HD, int RB, class OutT>
@@ -846,7 +851,10 @@ hipError_t launch_rb(const Kv8& c, const Kv8Batch& b, const float* q, int qts, i
     const int rb = row_groups(b, nh / c.nkv, c.nkv, sizeof(OutT) == 2);
     if (rb == 1) return launch<HD, 1, OutT>(c, b, q, qts, nh, scale, out, ots, part, st);
     if (rb == 2) return launch<HD, 2, OutT>(c, b, q, qts, nh, scale, out, ots, part, st);
-    return launch<HD, sizeof(OutT) == 2 ? 4 : 3, OutT>(c, b, q, qts, nh, scale, out, ots, part, st);
+    if constexpr (sizeof(OutT) == 2) {
+        if (rb == 4) return launch<HD, 4, OutT>(c, b, q, qts, nh, scale, out, ots, part, st);
+    }
+    return launch<HD, 3, OutT>(c, b, q, qts, nh, scale, out, ots, part, st);
 }
 
 }  // namespace

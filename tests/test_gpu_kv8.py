@@ -309,6 +309,9 @@ def test_whole_prompts(dev):
     ([0, 300], [600, 200], 128, 16, 128, False),                        # enough row blocks for the largest of each type
     ([0, 300, 63, 0, 128], [1, 203, 97, 0, 5], 24, 4, 256, True),
     ([1000, 0, 63], [129, 64, 65], 16, 2, 256, True),
+    ([37 * i for i in range(9)], [16] * 9, 24, 4, 256, True),           # full batches: 96 rows in two blocks of 48, 128 in two of 64
+    ([37 * i for i in range(9)], [16] * 9, 32, 4, 256, True),
+    ([37 * i for i in range(17)], [8] * 17, 64, 8, 128, True),
 ])
 def test_forms(dev, before, counts, nh, nkv, hd, f16):
     """Batches whose sizes call for each number of row blocks and each way of joining splits."""
