@@ -16,8 +16,9 @@
 // part of LDS, a page or two ahead, and reads them back without a barrier; one barrier a page, for P.
 //
 // What bounds it (MI355X, hd 256): few tokens, the bytes of the codes: 7.0 - 7.6 TB/s of them in a long context, behind 6 us for a
-// launch's first page and 4 for the join of the splits. Whole prompts, the vector units beside the matrix ones: the
-// softmax, 96 operations for a page's V and 16 for its K are 360 of a step's 464 in a wave, matrix units 41 % busy, 0.87 PFLOP/s.
+// launch's first page and 4 for the join of the splits. Whole prompts, the vector units beside the matrix ones: of a wave's
+// instructions for 48 rows and a page 235 are vector ones (softmax, 96 for V, 16 for K's sign) and 48 matrix ones, vector issue is
+// busy 63 % of the cycles, matrix units 40 %: 0.89 PFLOP/s.
 //
 // The lengths are on the device, so every workgroup finds its unit by itself: pages per split from the total work, a prefix sum over
 // the sequences' unit counts. Sequences of one split are finished in place, the others' records {m, l, o} are joined by
