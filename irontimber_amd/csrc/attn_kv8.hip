@@ -562,9 +562,11 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
             load_scales();
             asm volatile("" : "+v"(scl));
         }
-        const unsigned vid = page_of(j + VB);
+        unsigned vid = page_of(j + VB);
         if (((j + 1 + KB) & 63) == 0) load_ids(j + 1 + KB);
         const unsigned kid = page_of(j + 1 + KB);
+        if constexpr (VB == 1 + KB) vid = kid;   // (the same page: its number may be among those just read)
+        static_assert(VB <= 1 + KB, "V's page numbers are read no later than K's");
         if ((p0 + j) * kv8::PAGE + kv8::PAGE - 1 > clear) mask_keys(p0 + j);
         __builtin_amdgcn_s_setprio(0);
         settle(par);

@@ -292,6 +292,34 @@ def test_many_sequences_of_many_pages(dev, alike):
         e.attend(e.queries(sum(counts), 16), start, length, counts, 16, f16=f16)
 
 
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("f16", [False, True])
+def test_forms_over_many_pages_of_one_split(dev, hd, f16):
+    """Every number of row blocks over more than twice 64 pages in one workgroup: 130 sequences that share a beginning."""
+    nseq, nkv, before = 130, 2, 64 * 131 + 3
+    e = Engine(dev, nseq, nkv, hd, 2, spare=140)
+    base = np.random.default_rng(2).permutation(140)[:132].astype(np.int32)
+    e.table_np = np.repeat(base[None], nseq, 0)
+    e.table = torch.from_numpy(e.table_np.copy()).to(dev)
+    k, v = e.rows(before)
+    for p in (64, 128):                              # the first pages of the second and third 64: a third of the weight
+        k.reshape(before, nkv, hd)[64 * p:64 * p + 64] = np.float16(1)
+    e.append([before] + [0] * (nseq - 1), rows=(k, v))
+    ops.kv8_copy(e.cache, seq_src=e.ints([0] * (nseq - 1)), seq_dst=e.ints(list(range(1, nseq))))
+    for s in e.seqs[1:]:
+        s.k, s.v = e.seqs[0].k, e.seqs[0].v
+    for n in (1, 4, 5, 8):                           # 8, 32, 40 and 64 rows; no page gets full
+        start, length = e.append([n] * nseq)
+        q = e.queries(n * nseq, 16)
+        q[:, :, :hd] += np.float32(4 / hd ** 0.5)
+        out = torch.empty(n * nseq, 16 * hd, device=dev, dtype=torch.float16 if f16 else torch.float32)
+        got = host(ops.attn_kv8(e.cache, dev_f32(q.reshape(n * nseq, -1), dev), start, length, e.table, 16, n, out=out))
+        for i in (0, 101):
+            want, tol = ref.attention(q[i * n:i * n + n], *e.seqs[i].values(), e.seqs[i].rows - n, 1 / hd ** 0.5, f16)
+            err = np.abs(got[i * n:i * n + n].reshape(want.shape).astype(np.float64) - want)
+            assert (err <= tol).all(), (n, i, float((err - tol).max()))
+
+
 def test_whole_prompts(dev):
     """Prompts long enough that no row block is split."""
     for f16 in (False, True):
