@@ -301,8 +301,14 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
         l_run[x] = 0.f;
     }
 
-    // The keys that rows do not see get -inf (this lane's keys of page p are 16 w + 4 g + 0..3)
+    // The keys that rows do not see get -inf (this lane's keys of page p are 16 w + 4 g + 0..3). An unknown page's scale is NaN, which
+    // would reach these rows as NaN * -inf: there the scores that are seen become NaN in its place.
     auto mask_keys = [&](int p) __attribute__((always_inline)) {
+        if (__any(ksc != ksc)) {
+#pragma unroll
+            for (int x = 0; x < RB; ++x) sc[x] = f4{NAN, NAN, NAN, NAN};
+            ksc = 1.f;
+        }
 #pragma unroll
         for (int x = 0; x < RB; ++x) {
             const int lim = qlim[16 * x + lr] - (p * kv8::PAGE + 16 * w + 4 * g);

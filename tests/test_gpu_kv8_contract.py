@@ -1,0 +1,50 @@
+"""What the 8-bit cache's calls promise at the edge of their contract."""
+import numpy as np
+import pytest
+import torch
+
+from irontimber_amd import ops
+from tests.gpu_util import announce, dev_f32, host
+from tests.test_gpu_kv8 import Engine
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("before,n,nh,nkv,hd,page", [
+    (50, 90, 16, 2, 256, 1), (60, 6, 16, 2, 256, 1), (62, 68, 4, 2, 128, 1), (120, 300, 16, 2, 256, 3), (4080, 100, 16, 2, 256, 64),
+    (0, 700, 24, 4, 256, 6), (4090, 8, 8, 1, 128, 64)])
+@pytest.mark.parametrize("f16", [torch.float32, torch.float16])
+def test_an_unknown_page_is_lost_to_what_reads_it_alone(dev, before, n, nh, nkv, hd, page, f16):
+    """A full page whose number is outside the pool: tokens before it, that share a block of rows with later ones, keep their
+    outputs bit by bit; those that see it are NaN."""
+    announce(f"kv8 unknown page {page} after {before} + {n} {nh}/{nkv} {hd}")
+    for bad in (-1, 10 ** 6):
+        e = Engine(dev, 1, nkv, hd, (before + n) // 64 + 3)
+        if before:
+            e.append([before])
+        start, length = e.append([n + (64 - (before + n) % 64)])          # the page is full for all of these tokens
+        m = int(start[1])
+        q = dev_f32(e.queries(m, nh).reshape(m, -1), dev)
+        run = lambda table: host(ops.attn_kv8(e.cache, q, start, length, table, nh, m, out_dtype=f16))
+        good = run(e.table)
+        table = e.table.clone()
+        table[0, page] = bad
+        got = run(table)
+        first = max(page * 64 - before, 0)
+        assert 0 < first < m and np.isfinite(good).all()
+        assert np.array_equal(got[:first], good[:first])
+        assert np.isnan(got[first:]).all()
+
+
+def test_an_unknown_page_beside_an_open_one(dev):
+    """Rows that see neither, the unknown page alone, and both."""
+    e = Engine(dev, 1, 2, 256, 4)
+    e.append([60])
+    start, length = e.append([80])                                        # page 1 full, 12 open rows
+    q = dev_f32(e.queries(80, 16).reshape(80, -1), dev)
+    table = e.table.clone()
+    table[0, 1] = -7
+    for f16 in (torch.float32, torch.float16):
+        good = host(ops.attn_kv8(e.cache, q, start, length, e.table, 16, 80, out_dtype=f16))
+        got = host(ops.attn_kv8(e.cache, q, start, length, table, 16, 80, out_dtype=f16))
+        assert np.array_equal(got[:4], good[:4]) and np.isnan(got[4:]).all()
