@@ -343,7 +343,8 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
     };
     // ---- q in units of its row's largest value / 2^(8 DG - 1), as DG signed digits of 8 bits, for integer products with the
     // codes. Wave w makes those of dims 64 w .. (hd 128: two waves); they meet in LDS that is not in use yet, a row block at a time.
-    // A negative scale turns q round, and no unit is zero, so that -inf times it stays.
+    // A negative scale turns q round, and no unit is zero, so that -inf times it stays; where q or the scale is not finite it is NaN (the
+    // maximum with the least unit would make one of a NaN).
     const float size = fabsf(scale) * LOG2E, sign = scale < 0.f ? -1.f : 1.f;
     if (tid < ROWS) qlim[tid] = r0 + tid < R ? u.len + token(tid) : -1;
     {
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(256, 2) void attn_kv8_kernel(Kv8 c, Kv8Batch b, con
             const float m = row_max(x);
             const int ex = row_exp(x);
             const float to = __builtin_amdgcn_ldexpf(TOP * sign, -ex);
-            back[x] = m < INFINITY ? fmaxf(__builtin_amdgcn_ldexpf(size / TOP, ex), 1e-30f) : NAN;
+            back[x] = m < INFINITY && size < INFINITY ? fmaxf(__builtin_amdgcn_ldexpf(size / TOP, ex), 1e-30f) : NAN;
             if (w < NJ) {
                 u4 dg[DG];
 #pragma unroll

@@ -48,3 +48,13 @@ def test_an_unknown_page_beside_an_open_one(dev):
         good = host(ops.attn_kv8(e.cache, q, start, length, e.table, 16, 80, out_dtype=f16))
         got = host(ops.attn_kv8(e.cache, q, start, length, table, 16, 80, out_dtype=f16))
         assert np.array_equal(got[:4], good[:4]) and np.isnan(got[4:]).all()
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_a_scale_that_is_no_number(dev, scale):
+    e = Engine(dev, 2, 2, 256, 3)
+    e.append([70, 0])
+    start, length = e.append([3, 30])
+    q = dev_f32(e.queries(33, 16).reshape(33, -1), dev)
+    for f16 in (torch.float32, torch.float16):
+        assert np.isnan(host(ops.attn_kv8(e.cache, q, start, length, e.table, 16, 30, scale=scale, out_dtype=f16))).all()
