@@ -584,7 +584,8 @@ int it_kv8_append(const it_kv8_cache* cache, const uint16_t* k, const uint16_t* 
                   void* stream);
 
 /* Rows first[i] .. of each sequence, start[i+1] - start[i] of them (at most max_rows), as f16 into rows start[i] .. of k and
- * v; total[i]: the rows that the sequence holds (rows at or after total are not written), all of them or at most 64 fewer. */
+ * v; total[i]: the rows that the sequence holds (rows at or after total are not written), all of them or at most 64 fewer. Where
+ * first[i] or total[i] is negative, or total[i] more than the table can name, the sequence's rows start[i] .. are NaN. */
 int it_kv8_read(const it_kv8_cache* cache, uint16_t* k, uint16_t* v, int tok_stride, int ntok, const int32_t* start,
                 const int32_t* first, const int32_t* total, const int32_t* table, int max_pages, int max_rows,
                 void* stream);

@@ -250,8 +250,18 @@ __global__ __launch_bounds__(2 * HD) void kv8_read_kernel(Kv8 c, Kv8Batch b, con
     __shared__ __align__(16) _Float16 tile[kv8::PAGE * PITCH];
     const int i = blockIdx.z, kh = blockIdx.y >> 1, which = blockIdx.y & 1;
     const int t0 = b.start[i], t1 = b.start[i + 1], r0 = first[i], total = b.len[i];
-    if (t0 < 0 || t1 > b.ntok || t1 <= t0 || r0 < 0 || total > (long)b.max_pages * kv8::PAGE) return;
-    const int r1 = (int)min((long)total, (long)r0 + min(t1 - t0, b.max_nt));   // one past the last row
+    if (t0 < 0 || t1 > b.ntok || t1 <= t0) return;
+    const int count = min(t1 - t0, b.max_nt);
+    if (r0 < 0 || total < 0 || total > (long)b.max_pages * kv8::PAGE) {   // rows that cannot be: NaN (grid.x * 64 >= count)
+        const uint32_t nans = 0x7E007E00u;
+        _Float16* lost = (which ? v : k) + (long)t0 * kts + (size_t)kh * HD;
+        for (int n = threadIdx.x; n < kv8::PAGE * CH; n += NT) {
+            const int row = (int)blockIdx.x * kv8::PAGE + n / CH;
+            if (row < count) *(u4*)(lost + (long)row * kts + 8 * (n % CH)) = u4{nans, nans, nans, nans};
+        }
+        return;
+    }
+    const int r1 = (int)min((long)total, (long)r0 + count);   // one past the last row
     const int p = r0 / kv8::PAGE + blockIdx.x, row0 = p * kv8::PAGE;
     if ((long)p * kv8::PAGE >= r1) return;
     const int lo = max(r0, row0) - row0, hi = min(r1 - row0, kv8::PAGE);       // rows of the page

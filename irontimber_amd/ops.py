@@ -759,7 +759,7 @@ def kv8_read(cache: Kv8Cache, start: torch.Tensor, first: torch.Tensor, total: t
              ) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows first[i] .. of the sequences as f16 k, v [rows, nkv*hd], start[i+1] - start[i] (at most max_rows) of sequence
     i at row start[i]; total [nseq] the rows that each one holds (it_kv8_read). Rows that no sequence has are left as they are
-    in out, the tensors to write to."""
+    in out, the tensors to write to; rows that cannot be (a negative first or total, more than the table can name) are NaN."""
     dev, nkv, hd, nseq, args = _kv8(cache)
     pages = _kv8_batch(dev, nseq, start, total, table)
     if first.shape != (nseq,):

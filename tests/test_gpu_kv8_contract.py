@@ -50,6 +50,39 @@ def test_an_unknown_page_beside_an_open_one(dev):
         assert np.array_equal(got[:4], good[:4]) and np.isnan(got[4:]).all()
 
 
+def test_reading_rows_that_cannot_be(dev):
+    """A sequence with more rows than its table can name, or with a negative length or first row, is read as NaN; a page outside
+    the pool too; the others as always, and rows of no sequence stay."""
+    e = Engine(dev, 6, 2, 256, 3)
+    e.append([100, 150, 70, 80, 192, 130])
+    first, counts = [0, 90, 3, -5, 128, 60], [100, 60, 30, 70, 64, 70]
+    total = e.ints([100, 193, -1, 80, 192, 130])
+    table = e.table.clone()
+    table[5, 1] = e.cache.kp.shape[0]
+    start = e.ints(np.concatenate([[0], np.cumsum(counts)]).tolist())
+    n = sum(counts)
+    out = tuple(torch.full((n + 5, 512), 9.0, device=dev, dtype=torch.float16) for _ in range(2))
+    ops.kv8_read(e.cache, start, e.ints(first), total, table, max(counts), n + 5, out)
+    for i in range(2):
+        got, at = host(out[i]), 0
+        for j, (s, f, c) in enumerate(zip(e.seqs, first, counts)):
+            here = got[at:at + c]
+            if j in (1, 2, 3):
+                assert np.isnan(here).all(), j
+            else:
+                want = s.values()[i].reshape(s.rows, 512)[f:f + c].astype(np.float16)
+                if j == 5:
+                    want[64 - f:128 - f] = np.nan
+                assert np.array_equal(here, want, equal_nan=True), j
+            at += c
+        assert (got[at:] == 9.0).all()
+    at = e.ints([0, 0, 50, 50, 50, 50, 50])               # at most 20 of its 50 rows
+    out = torch.full((50, 512), 9.0, device=dev, dtype=torch.float16), torch.full((50, 512), 9.0, device=dev, dtype=torch.float16)
+    ops.kv8_read(e.cache, at, e.ints(first), total, table, 20, 50, out)
+    for x in out:
+        assert np.isnan(host(x)[:20]).all() and (host(x)[20:] == 9.0).all()
+
+
 @pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
 def test_a_scale_that_is_no_number(dev, scale):
     e = Engine(dev, 2, 2, 256, 3)
