@@ -545,16 +545,22 @@ int it_gdn_tree_commit(const float* x, int x_tok_stride, int K, float* conv_stat
  *
  * Rows: a page holds IT_KV8_PAGE rows of all KV heads. Row r of a sequence is in page table[seq][r / 64]. While a sequence
  * holds `total` rows, the pages that are full, those before total / 64, are 8-bit codes, and the rows after them (at most
- * 63) are f16 in the sequence's open buffer, which keeps the rows of the last two pages: so up to 64 rows can be taken
- * back by a smaller length alone (drafts that a check rejects), rows before that only to a page's end, or by reading the page's
- * rows (it_kv8_read) and appending them anew.
+ * 63) are f16 in the sequence's open buffer, which has room for two pages: page p in half p % 2, until a row of page p + 2 is
+ * written there.
+ * Taking rows back (drafts that a check rejects): a smaller length alone does it, to any page's end, or into a page whose rows still
+ * stand in the open buffer, which is page `lowest` or a later one. The caller keeps that number for each sequence:
+ *   0 at first;  after an append to `total` rows  max(lowest, (total - 1) / 64 - 1);  after a cut to `to` rows  min(lowest, to / 64)
+ * So up to 64 of a call's own rows can always be taken back. Not always 64 rows after an earlier cut: 126 rows and four drafts are
+ * 130, so page 2 has the half of page 0, and has it still when three drafts are taken back and 127 rows are left. Into a page before
+ * `lowest`: to the page's start, with its rows read (it_kv8_read) before that and appended anew.
  * Codes: each IT_KV8_BLOCK rows of a KV head have a scale s for K and one for V: the largest size / 127, rounded up to four
  * significant bits or to a multiple of 2^-24 (at least that). A value x is kept as code = 128 + x / s, rounded to the nearest, ties to
  * even, and at most 127 from 128 (113 where s is above 512); it stands for (code - 128) * s, which is an f16 number. Appending makes
  * values finite: an infinity becomes the largest f16, a NaN 0.
  * Sharing: a table may name a page that another one names. The calls write only to pages that a sequence fills, those from
  * len / 64 on, so pages before that can be shared (a common beginning, a fork); a fork takes the open rows with it
- * (it_kv8_copy) and needs pages of its own from len / 64 on. A page that no table names is free; nothing in it needs to be cleared.
+ * (it_kv8_copy; `lowest` goes with them) and needs pages of its own from len / 64 on. A cut into a shared page needs another page
+ * named in its place first, as rows appended then fill it anew. A page that no table names is free; nothing in it needs to be cleared.
  *
  * Device arrays of a call, int32, for the cache's nseq sequences: start [nseq + 1], len [nseq], table [nseq][max_pages]. The
  * call's tokens start[i] .. start[i+1]-1 are the next rows of sequence i after its len[i] rows; start[i] = start[i+1]: none.
@@ -584,7 +590,7 @@ int it_kv8_append(const it_kv8_cache* cache, const uint16_t* k, const uint16_t* 
                   void* stream);
 
 /* Rows first[i] .. of each sequence, start[i+1] - start[i] of them (at most max_rows), as f16 into rows start[i] .. of k and
- * v; total[i]: the rows that the sequence holds (rows at or after total are not written), all of them or at most 64 fewer. Where
+ * v; total[i]: the rows that the sequence holds, or fewer that it may be cut to (rows at or after total are not written). Where
  * first[i] or total[i] is negative, or total[i] more than the table can name, the sequence's rows start[i] .. are NaN. */
 int it_kv8_read(const it_kv8_cache* cache, uint16_t* k, uint16_t* v, int tok_stride, int ntok, const int32_t* start,
                 const int32_t* first, const int32_t* total, const int32_t* table, int max_pages, int max_rows,
@@ -599,8 +605,8 @@ int it_kv8_copy(const it_kv8_cache* cache, const int32_t* src, const int32_t* ds
 /* Causal GQA attention with sigmoid gate over the cache, of tokens whose rows have been appended: token t of sequence i sees
  * its rows 0 .. len[i] + t. q as for it_attn_f16 (query | gate per head), out [t*out_tok_stride + h*hd + d] in f32, or f16 where
  * out_f16 is nonzero. One token a sequence, a few (drafts), or prompts of any lengths, mixed.
- * len[i] and its tokens together are the rows appended so far, or at most 64 fewer: of the rows after the last full page that they
- * make, only the last two pages' stand in the open buffer. (So after one long append, call it for all of its tokens.)
+ * len[i] and its tokens together are the rows that the sequence holds, or fewer that it may be cut to: the rows after the last full
+ * page that they make have to stand in the open buffer. (So after one long append, call it for all of its tokens.)
  * Accuracy: the softmax's sums and the products' sums are f32, K and V exact as stored. For an f32 output q goes into the products
  * in fixed point, to 2^-23 of its head's largest value (2^-22 of itself against the open rows), a probability as an f16 pair, to
  * 2^-22 of itself or, where it is small, 2^-31 of its row's largest up to there. For an f16 output q to 2^-15, a probability as

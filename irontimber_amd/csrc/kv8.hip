@@ -5,8 +5,8 @@
 // f16 number, and what reads the cache computes with exact operands. s is the block's largest size / 127 rounded up,
 // which costs 1/16 of a step on average (1/8 at most) against 127 steps exactly.
 // A scale belongs to whole blocks, so a page is quantised once, when its last row arrives; until then its rows stand in
-// the sequence's open buffer, in f16 and in the page's own element order. That buffer keeps the last two pages' rows, so
-// that rows taken back (drafts that a check rejects) need nothing but a smaller length.
+// the sequence's open buffer, in f16 and in the page's own element order. That buffer has room for two pages, so that a call's rows
+// that are taken back (drafts that a check rejects) need nothing but a smaller length.
 #include "internal.h"
 #include "kv8.h"
 

@@ -746,7 +746,8 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, start: torch.T
                table: torch.Tensor, max_nt: int) -> None:
     """Appends f16 rows k, v [ntok, nkv*hd]: rows start[i] .. start[i+1]-1 follow the length[i] rows that sequence i holds
     (start [nseq+1], length [nseq], table [nseq, max_pages] int32 on the device; at most max_nt a sequence). Pages that
-    get full are quantised; length stays as it is (it_kv8_append)."""
+    get full are quantised; length stays as it is (it_kv8_append). Up to 64 of a call's own rows are taken back by a smaller length;
+    further back by the rule of it_attn.h alone, or by kv8_read and appending anew."""
     dev, nkv, hd, nseq, args = _kv8(cache)
     pages = _kv8_batch(dev, nseq, start, length, table)
     stride = _kv8_rows(dev, nkv * hd, k, v)
@@ -801,7 +802,8 @@ def attn_kv8(cache: Kv8Cache, q: torch.Tensor, start: torch.Tensor, length: torc
              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Attention of appended tokens over the cache: q [ntok, nh*2*hd] f32 (q | gate per head), token t of sequence i sees its
     rows 0 .. length[i] + t -> out [ntok, nh*hd], f32 or f16 (out's type, or out_dtype). start, length, table, max_nt as for
-    kv8_append, length still without the new tokens: all rows that were appended, or at most 64 fewer (it_attn_kv8)."""
+    kv8_append, length still without the new tokens: with them all rows that the sequence holds, or fewer that it may be cut to
+    (it_attn_kv8)."""
     dev, nkv, hd, nseq, args = _kv8(cache)
     pages = _kv8_batch(dev, nseq, start, length, table)
     shape, width = q.shape, nh * hd

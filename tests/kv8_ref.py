@@ -113,3 +113,21 @@ def attention(q, k, v, before, scale, f16=False):
             if f16:
                 tol[t, h] += 2.0 ** -11 * np.abs(out[t, h]) + 2.0 ** -25
     return out, tol + 1e-30
+
+
+class Cuts:
+    """To which lengths a sequence may be cut by its length alone: to a page's end, or into page `lowest` or a later one."""
+
+    def __init__(self):
+        self.rows = self.lowest = 0
+
+    def append(self, n):
+        self.rows += n
+        self.lowest = max(self.lowest, (self.rows - 1) // PAGE - 1)
+
+    def may(self, to):
+        return 0 <= to <= self.rows and (to % PAGE == 0 or to // PAGE >= self.lowest)
+
+    def cut(self, to):
+        assert self.may(to)
+        self.rows, self.lowest = to, min(self.lowest, to // PAGE)

@@ -91,3 +91,44 @@ def test_a_scale_that_is_no_number(dev, scale):
     q = dev_f32(e.queries(33, 16).reshape(33, -1), dev)
     for f16 in (torch.float32, torch.float16):
         assert np.isnan(host(ops.attn_kv8(e.cache, q, start, length, e.table, 16, 30, scale=scale, out_dtype=f16))).all()
+
+
+def test_rows_taken_back_twice(dev):
+    """126 rows, four drafts that cross a page's end, three of them taken back: the drafts' page has taken the open rows of the
+    page two before it, so a cut into that page reads its rows and appends them anew."""
+    e = Engine(dev, 1, 2, 256, 4)
+    e.append([126])
+    e.append([4])
+    e.seqs[0].cut(127)
+    e.append([1])
+    e.seqs[0].cut(100)                                   # page 1 still stands in the open buffer
+    start, length = e.append([2])
+    e.check_buffers()
+    e.attend(e.queries(2, 16), start, length, [2], 16)
+    k, v = ops.kv8_read(e.cache, e.ints([0, 63]), e.ints([0]), e.ints([102]), e.table, 63, 63)
+    want = [x[:63].astype(np.float16).reshape(63, -1) for x in e.seqs[0].values()]
+    assert np.array_equal(host(k), want[0]) and np.array_equal(host(v), want[1])
+    e.seqs[0].cut(0)
+    e.append([63], rows=(host(k), host(v)))
+    start, length = e.append([4])
+    e.check_buffers()
+    e.attend(e.queries(4, 16), start, length, [4], 16)
+
+
+def test_cuts_by_the_rule(dev):
+    """Appends and cuts at random: a length may fall to a page's end, or into a page from the lowest that stands in the open buffer
+    on (kv8_ref.Cuts)."""
+    from tests.kv8_ref import Cuts
+    e, rng, cuts = Engine(dev, 1, 1, 128, 9), np.random.default_rng(8), Cuts()
+    for turn in range(40):
+        room = 9 * 64 - cuts.rows
+        n = int(min(rng.choice([1, 3, 30, 63, 64, 65, 130, 300]), room))
+        if n:
+            start, length = e.append([n])
+            cuts.append(n)
+            e.check_buffers()
+            if turn % 4 == 0:
+                e.attend(e.queries(n, 8), start, length, [n], 8)
+        to = int(rng.choice([x for x in range(cuts.rows + 1) if cuts.may(x)]))
+        cuts.cut(to)
+        e.seqs[0].cut(to)
