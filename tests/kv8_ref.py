@@ -115,6 +115,69 @@ def attention(q, k, v, before, scale, f16=False):
     return out, tol + 1e-30
 
 
+def attention_rms(q, k, v, before, scale, f16=False, full=None):
+    """As `attention`, with how far errors of the documented precisions carry in the mean: (out [n, nh, hd] float64, spread of an
+    element's error [n, nh, hd], its own roundings [n, nh, hd]). full: rows before this one stand in full pages (all rows, if none
+    is given). An output's error is at most SIGMAS spreads and the roundings.
+
+    out = sum_j p_j v_j. A relative error e_j of weight j moves it by p_j e_j (v_j - out), where the sum of the weights has the same
+    errors (one f16: its sum takes it as rounded), and by p_j e_j v_j else. The e_j of different keys are
+    independent as far as K and V are; so the spread is the root of the sum of p_j^2 e_j^2 (v_j - out)^2, with e_j^2 the sum of
+    - the score's error by q: half a step is h = 2^-15 (f16) or 2^-23 of the row's largest |q|, times 128/127 (the highest digit
+      ends at 127), even in +-h: scale |k_j| h / sqrt 3; against open rows 2^-22 of each q_d, where that is more
+    - the score's f32 roundings: 4 of |s_j - s_max| + |s_max| + 1 at 2^-24, and the open rows' sum of hd products in f32
+    - the weight's: 2^-11 (one f16) or 2^-22 (a pair) / sqrt 3 of itself, or 2^-31 of the largest.
+    The sum over m keys in f32 adds 2^-24 / sqrt 3 of a partial sum, in row order or of a split (so at most twice the largest in row
+    order), at each of m / 16 products of matrix instructions and 16 more; and inside those, over 8 values, three times the root of
+    the sum of (p_j v_j)^2.
+    The roundings: 6 * 2^-24 of the result for the division and the gate, and half a step of f16 for such an output."""
+    n, nh, hd2 = q.shape
+    hd, nkv = hd2 // 2, k.shape[1]
+    G = nh // nkv
+    out, spread = np.zeros((n, nh, hd)), np.zeros((n, nh, hd))
+    u, h0, ew = 2.0 ** -24, 2.0 ** (-15 if f16 else -23) * 128 / 127, 2.0 ** (-11 if f16 else -22)
+    full = k.shape[0] if full is None else full
+    q = q.astype(np.float64)
+    for kh in range(nkv):
+        for t in range(n):
+            m = before + t + 1
+            x, kk, vv = q[t, kh * G:kh * G + G, :hd], k[:m, kh], v[:m, kh]
+            s = scale * (x @ kk.T)                                    # [G, m]
+            most = s.max(1, keepdims=True)
+            w = np.exp(s - most)
+            p = w / w.sum(1, keepdims=True)
+            o = p @ vv
+            k2 = kk * kk
+            h = np.abs(x).max(1, keepdims=True) * h0
+            e2 = scale * scale * k2.sum(1) * h * h / 3
+            open_ = np.arange(m) >= full
+            if open_.any():
+                e2 = e2 + open_ * scale * scale * (2.0 ** -44 / 3 + hd * u * u) * ((x * x) @ k2.T)
+            e2 = e2 + (4 * u * (np.abs(s - most) + np.abs(most) + 1)) ** 2
+            a2 = p * p * (e2 + ew * ew / 3) + (2.0 ** -31 * p.max(1, keepdims=True)) ** 2 / 3
+            # sum_j a2_j (v_j - o)^2 or, for pairs, of v_j^2 + o^2 at most
+            var = a2 @ (vv * vv) + (0 if f16 else 1) * a2.sum(1, keepdims=True) * o * o
+            if f16:
+                var = var - 2 * o * (a2 @ vv) + a2.sum(1, keepdims=True) * o * o
+            part = np.stack([np.abs(np.cumsum(row[:, None] * vv, 0)).max(0) for row in p])
+            var = np.maximum(var, 0) + u * u * ((m / 16 + 16) / 3 * (2 * part) ** 2 + 9 * (p * p) @ (vv * vv))
+            gate = 1 / (1 + np.exp(-np.clip(q[t, kh * G:kh * G + G, hd:], -700, 700)))
+            out[t, kh * G:kh * G + G] = o * gate
+            spread[t, kh * G:kh * G + G] = np.sqrt(var) * gate
+    own = 6 * u * np.abs(out)
+    if f16:
+        own = own + 2.0 ** -11 * np.abs(out) + 2.0 ** -25
+    return out, spread, own
+
+
+SIGMAS = 6.0
+
+
+def too_far(got, want, spread, own):
+    """Whether a row [.., hd] of outputs has an element further off than `attention_rms` allows."""
+    return ~(np.abs(got - want) <= SIGMAS * spread + own + 1e-30).all(-1)
+
+
 class Cuts:
     """To which lengths a sequence may be cut by its length alone: to a page's end, or into page `lowest` or a later one."""
 
