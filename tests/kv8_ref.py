@@ -127,8 +127,8 @@ def attention_rms(q, k, v, before, scale, f16=False, full=None):
       ends at 127), even in +-h: scale |k_j| h / sqrt 3; against open rows 2^-22 of each q_d, where that is more
     - the score's f32 roundings: 4 of |s_j - s_max| + |s_max| + 1 at 2^-24, and the open rows' sum of hd products in f32
     - the weight's: 2^-11 (one f16) or 2^-22 (a pair) / sqrt 3 of itself, or 2^-31 of the largest.
-    The sum over m keys in f32 adds 2^-24 / sqrt 3 of a partial sum, in row order or of a split (so at most twice the largest in row
-    order), at each of m / 16 products of matrix instructions and 16 more; and inside those, over 8 values, three times the root of
+    The sum over m keys in f32 adds 2^-24 / sqrt 3 of a partial sum, page after page or of a split (so at most twice the largest page
+    after page), at each of m / 16 products of matrix instructions and 16 more; and inside those, over 8 values, three times the root of
     the sum of (p_j v_j)^2.
     The roundings: 6 * 2^-24 of the result for the division and the gate, and half a step of f16 for such an output."""
     n, nh, hd2 = q.shape
@@ -139,15 +139,16 @@ def attention_rms(q, k, v, before, scale, f16=False, full=None):
     full = k.shape[0] if full is None else full
     q = q.astype(np.float64)
     for kh in range(nkv):
+        key, val = np.ascontiguousarray(k[:, kh]), np.ascontiguousarray(v[:, kh])
+        key2, val2 = key * key, val * val
         for t in range(n):
             m = before + t + 1
-            x, kk, vv = q[t, kh * G:kh * G + G, :hd], k[:m, kh], v[:m, kh]
+            x, kk, vv, k2, v2 = q[t, kh * G:kh * G + G, :hd], key[:m], val[:m], key2[:m], val2[:m]
             s = scale * (x @ kk.T)                                    # [G, m]
             most = s.max(1, keepdims=True)
             w = np.exp(s - most)
             p = w / w.sum(1, keepdims=True)
             o = p @ vv
-            k2 = kk * kk
             h = np.abs(x).max(1, keepdims=True) * h0
             e2 = scale * scale * k2.sum(1) * h * h / 3
             open_ = np.arange(m) >= full
@@ -156,11 +157,12 @@ def attention_rms(q, k, v, before, scale, f16=False, full=None):
             e2 = e2 + (4 * u * (np.abs(s - most) + np.abs(most) + 1)) ** 2
             a2 = p * p * (e2 + ew * ew / 3) + (2.0 ** -31 * p.max(1, keepdims=True)) ** 2 / 3
             # sum_j a2_j (v_j - o)^2 or, for pairs, of v_j^2 + o^2 at most
-            var = a2 @ (vv * vv) + (0 if f16 else 1) * a2.sum(1, keepdims=True) * o * o
+            var = a2 @ v2 + (0 if f16 else 1) * a2.sum(1, keepdims=True) * o * o
             if f16:
                 var = var - 2 * o * (a2 @ vv) + a2.sum(1, keepdims=True) * o * o
-            part = np.stack([np.abs(np.cumsum(row[:, None] * vv, 0)).max(0) for row in p])
-            var = np.maximum(var, 0) + u * u * ((m / 16 + 16) / 3 * (2 * part) ** 2 + 9 * (p * p) @ (vv * vv))
+            ends = np.stack([p[:, a:a + PAGE] @ vv[a:a + PAGE] for a in range(0, m, PAGE)])
+            part = np.abs(np.cumsum(ends, 0)).max(0)
+            var = np.maximum(var, 0) + u * u * ((m / 16 + 16) / 3 * (2 * part) ** 2 + 9 * (p * p) @ v2)
             gate = 1 / (1 + np.exp(-np.clip(q[t, kh * G:kh * G + G, hd:], -700, 700)))
             out[t, kh * G:kh * G + G] = o * gate
             spread[t, kh * G:kh * G + G] = np.sqrt(var) * gate
