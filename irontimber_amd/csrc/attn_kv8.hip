@@ -7,9 +7,13 @@
 //   softmax        a running reference per row, common to the waves; P^T goes through LDS
 //   O^T += V^T P^T wave w has a quarter of the dims, all 64 keys and rows
 // K's codes are integers already, so K q^T is integer products with q in signed 8-bit digits, fixed point in its row's largest
-// value: three digits (2^-23 of it) for an f32 output, two (2^-15) for an f16 one. A digit more costs a product of 16 x 16 x 64
+// value: three digits (2^-23 of it) for an f32 output, two (2^-15) for most f16 ones. A digit more costs a product of 16 x 16 x 64
 // a key block, where converting K would cost the vector units 6 operations for 4 codes, and they are what is short here. V's
-// codes become f16 times their scale, exactly; P goes in as an f16 pair for an f32 output, as one f16 for an f16 one.
+// codes become f16 times their scale, exactly; P goes in as an f16 pair for an f32 output, as one f16 for an f16 one. What an f16
+// output, whose own rounding is 2.1e-4, loses by that and what it would cost (error against 64 bits, us; as said / with pairs / and
+// three digits): 8192-token prompt 2.7e-4 628, 2.1e-4 786, 2.1e-4 900; 512 tokens after 32256 383, 481, 573; in blocks of 16 rows, 32
+// ragged sequences of a token each, 2.3e-4 19.5, 2.1e-4 20.2, 2.1e-4 20.3. So blocks of 16 rows are as for an f32 output
+// (PAIRS), larger ones not.
 // The open page (f16 rows) comes first, with q as f16 pairs.
 //
 // The page's element order is that of the matrix operands. Each wave copies the 4 hd bytes that it alone needs straight into its
@@ -839,7 +843,8 @@ hipError_t launch(const Kv8& c, const Kv8Batch& b, const float* q, int qts, int 
     const int G = nh / c.nkv;
     const long groups = max_groups(RB, b.nseq, b.ntok, b.max_nt, G), units = std::min(groups + (WGS + c.nkv - 1) / c.nkv + 1, groups * b.max_pages);
     const long fold = (units + 65534) / 65535;
-    attn_kv8_kernel<HD, RB, sizeof(OutT) == 4, OutT>
+    constexpr bool pairs = sizeof(OutT) == 4 || RB == 1;   // (see the top: in blocks of 16 rows fewer bits save next to nothing)
+    attn_kv8_kernel<HD, RB, pairs, OutT>
         <<<dim3(c.nkv, (unsigned)((units + fold - 1) / fold), (unsigned)fold), 256, 0, st>>>(c, b, q, qts, G, scale, out, ots, part, WGS);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

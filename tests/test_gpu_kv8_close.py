@@ -93,3 +93,15 @@ def test_single_large_dims(dev, before, n, large):
     q[:, 3, 200] = large
     for f16 in (False, True):
         e.attend(q, start, length, [n], 16, f16=f16)
+
+
+@pytest.mark.parametrize("lens,counts,nh,nkv,hd", [
+    ([600], [1], 16, 2, 256), ([9000, 64, 131, 0], [1, 2, 0, 1], 16, 2, 256), ([5000], [4], 8, 2, 128), ([37 * i for i in range(70)], [1] * 70, 64, 4, 128)])
+def test_few_rows_are_as_exact_in_f16(dev, lens, counts, nh, nkv, hd):
+    """At most 16 query rows of a KV head: an f16 output is the f32 one, rounded to nearest."""
+    e = Engine(dev, len(lens), nkv, hd, max(a + b for a, b in zip(lens, counts)) // 64 + 1)
+    e.append(lens)
+    start, length = e.append(counts)
+    q = dev_f32(e.queries(sum(counts), nh).reshape(sum(counts), -1), dev)
+    run = lambda t: ops.attn_kv8(e.cache, q, start, length, e.table, nh, max(counts), out_dtype=t)
+    assert torch.equal(run(torch.float16), run(torch.float32).half())
