@@ -46,7 +46,8 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // Waits until at most N loads are still in flight; they land in the order that they were issued in.
 template <int N> __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // N KiB from `from` (each lane 16 bytes at off + 1024 i) to LDS from `to` on (lane l at 16 l + 1024 i: the instruction's offset
-// counts on both sides). What stood there has been read when they go out. m0 holds the LDS address; nothing else here uses it.
+// counts on both sides). What stood there has been read when they go out. m0 holds the LDS address: the compiler reserves it, and no
+// instruction of its own here uses it (tests/test_kv8_asm.py).
 template <int N> __device__ __forceinline__ void kib_to_lds(const uint8_t* from, unsigned off, uint8_t* to) {
     typedef __attribute__((address_space(3))) uint8_t lds_u8;
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_u8*)to);
