@@ -611,7 +611,7 @@ int it_kv8_copy(const it_kv8_cache* cache, const int32_t* src, const int32_t* ds
  * in fixed point, to 2^-23 of its head's largest value (2^-22 of itself against the open rows), a probability as an f16 pair, to
  * 2^-22 of itself or, where it is small, 2^-31 of its row's largest up to there. An f16 output is that rounded where max_nt times the
  * query heads of a KV head is at most 16; of more rows it may go by q to 2^-15, a probability as one f16, to 2^-11 of itself: root
- * mean square up to 2e-4 of the result over many keys, beside the 2.1e-4 of the output's own rounding (an 8192-token prompt 2.7e-4
+ * mean square up to 2.1e-4 of the result over many keys, beside the 2.1e-4 of the output's own rounding (an 8192-token prompt 2.7e-4
  * in all). A program that needs the f32 products there takes an f32 output.
  * At most 2^26 tokens times heads, 2^23 sequences times KV heads, 2^16 query heads of a KV head. Which sequences share a call
  * decides how the pages are split, so it moves results by roundings; the same call gives the same bits.

@@ -19,8 +19,9 @@
 // The page's element order is that of the matrix operands. Each wave copies the 4 hd bytes that it alone needs straight into its
 // part of LDS, a page or two ahead, and reads them back without a barrier; one barrier a page, for P.
 //
-// What bounds it (MI355X, hd 256): few tokens, the bytes of the codes: 7.0 - 7.6 TB/s of them in a long context, behind 6 us for a
-// launch's first page and 4 for the join of the splits. Whole prompts, the vector units beside the matrix ones: of a wave's
+// What bounds it (MI355X, hd 256): few tokens, the bytes of the codes: a token after 65535, 131071, 262143 and 524287 rows takes 25.3,
+// 35.6, 57.4 and 104 us in a graph over inputs that no cache holds, so 6.5, 6.1 and 5.7 TB/s from each to the next, behind 6 us to a
+// launch's first page, 1.4 for its records and 4 for the join of the splits. Whole prompts, the vector units beside the matrix ones: of a wave's
 // instructions for 48 rows and a page 235 are vector ones (softmax, 96 for V, 16 for K's sign) and 48 matrix ones, vector issue is
 // busy 63 % of the cycles, matrix units 40 %: 0.89 PFLOP/s.
 //
@@ -97,7 +98,9 @@ __device__ __forceinline__ int call_chunk(const Kv8Batch& b, const Kv8Seq& s0, i
     }
     const float work = readlane_f(sum, 0) * (float)nkv, groups = readlane_f(blocks, 0) * (float)nkv;
     int chunk = kv8::chunk_pages(work, groups, wgs);
-    if (chunk > (ROWS == 16 ? 12 : 18) && groups <= (float)wgs) {   // (of fewer, the count costs more than it gives)
+    // (of fewer, the count costs more than it gives: us, counted / not, ten pages, 16 sequences of 4096 rows 27.8 / 24.6, 32 of four
+    // tokens after 4096 47.7 / 45.5; of 22 pages, 64 sequences of 4096 rows 60.8 / 62.6, 8 of 32 tokens after 4096 54.2 / 58.5)
+    if (chunk > (ROWS == 16 ? 12 : 18) && groups <= (float)wgs) {
         float rcp[kv8::TRIES], units[kv8::TRIES] = {};
 #pragma unroll
         for (int k = 0; k < kv8::TRIES; ++k) rcp[k] = __builtin_amdgcn_rcpf((float)kv8::fewer_pages(work, groups, wgs, k));
@@ -684,7 +687,7 @@ template <int HD, int ROWS, int DL, class OutT>
 __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, const float* __restrict__ q, int qts,
                                                              int G, OutT* __restrict__ out, int ots,
                                                              const float* __restrict__ part, int wgs, int rows) {
-    constexpr int SL = 256 / DL, DQ = HD / (4 * DL), NB = 4, FEW = DL == 32 ? 16 : 0, WL = HD / 4;   // WL: lanes of a wave's row
+    constexpr int SL = 256 / DL, DQ = HD / (4 * DL), NB = 4, ALONE = DL == 32 ? 16 : 0, WL = HD / 4;   // WL: lanes of a wave's row
     __shared__ float red_m[4], red_l[4][DL];
     __shared__ __align__(16) f4 red_o[4][DL];
     const int nkv = c.nkv, kh = blockIdx.x, tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
@@ -700,7 +703,7 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
         const Kv8Seq s = i0 == 0 ? s0 : kv8_seq(b, i0 + l);
         const int ns = kv8::splits(s.pages, chunk), n = ns > 1 ? (s.n * G + ROWS - 1) / ROWS : 0;
         groups += b.nseq == 1 ? __builtin_amdgcn_readfirstlane(n) : __builtin_amdgcn_readlane(prefix_sum(n), 63);
-        if (__any(n > 0 && ns > FEW)) alone_all = false;
+        if (__any(n > 0 && ns > ALONE)) alone_all = false;
     }
     const int each = alone_all ? (rows + 3) / 4 : DQ * rows;
     const float rcp_groups = __builtin_amdgcn_rcpf((float)groups), rcp_G = __builtin_amdgcn_rcpf((float)G);
@@ -708,7 +711,7 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8 c, Kv8Batch b, 
         const int sub = div_small(item, rcp_groups);
         const Found u = find<ROWS, true>(b, s0, G, nkv, chunk, item - sub * groups, l);
         if (!u.any) return;   // (cannot be)
-        const bool alone = u.ns <= FEW;
+        const bool alone = u.ns <= ALONE;
         const int rb = u.at, row = alone ? 4 * sub + w : sub / DQ, r = rb * ROWS + row;
         if (row >= rows || r >= u.n * G) continue;   // (all threads that join the row)
         const int t = u.nrb == 1 ? div_small(row, rcp_G) : (int)((unsigned)r / (unsigned)G), h = kh * G + r - t * G;
@@ -827,6 +830,9 @@ long max_groups(int rb, int nseq, int ntok, int max_nt, int G) {
 //                       of 8 after 8184   95 / 98 / 75    of 64 after 1984   118 / 113 / 100    1000 after 3000, 24 heads   - / 112 / 139
 //   32 / 48, f32   64 after 4032   32 / 36    512 after 3584   86 / 88    4096 after 0   265 / 262    32 of 5 after 8187   106 / 83
 //                  seven prompts of 24 heads   461 / 435
+// (512 tokens after 32256 are the one size seen where 48 rows, f16, are behind 64, by 2 to 5 %; 256 after 32512 180 / 183, 1000 after
+// 16000 386 / 460.) The tables' widths count, not the lengths, which the host has not: 4 tokens after 508 rows 10.5 where the tables
+// have 10 pages, 12.1 where they have 2049.
 int row_groups(const Kv8Batch& b, int G, int nkv, bool f16out) {
     const long rows = (long)b.max_nt * G;
     if (rows <= 16 || (rows <= 64 && (long)std::min(b.nseq, b.ntok) * nkv * b.max_pages < WGS)) return 1;

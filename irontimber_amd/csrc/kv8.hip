@@ -68,7 +68,8 @@ __device__ __forceinline__ uint32_t codes_of(const Steps& t, _Float16 a, _Float1
 // another page's rows replace, the first page's workgroup writes it, after it has read them.
 // Both kinds work in the page's order, which the old open rows have already. New rows of V get there through LDS.
 // A wave U = 2 KiB of codes, 32 values a lane: with more to a wave the call is as slow as the fetching of the code that each CU then
-// runs once or twice, with less as the starting of its waves (U 1, 2, 4: 8192 rows 12.1, 10.8, 11.3 us, one page 5.3, 5.0, 5.8).
+// runs once or twice, with less as the starting of its waves (U 1, 2, 4: 8192 rows 12.1, 10.8, 11.3 us, one page 5.3, 5.0, 5.8,
+// in a graph of three inputs, which the last cache holds, on one card; U 2 over twelve inputs 12.1, by the profiler 11.6, a page 5.4).
 // Bound by bytes, two read and one written a value, and in short calls by three dependent round trips (bounds, rows, stores).
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, const _Float16* __restrict__ k,
@@ -242,7 +243,8 @@ __global__ __launch_bounds__(2 * HD) void kv8_append_kernel(Kv8 c, Kv8Batch b, c
 }
 
 // Workgroup = (sequence, page, KV head, K or V): rows first[i] .. of a sequence that holds len[i] rows, as f16.
-// A wave two KiB, as in appending (four waves of four KiB, one after the other: a page 4.2 us, so 3.4; 8192 rows 8.2, so 7.6).
+// A wave two KiB, as in appending (four waves of four KiB, one after the other: a page 4.2 us, so 3.4; 8192 rows 8.2, so 7.6, taken as
+// there; over twelve inputs 8.7, by the profiler 7.9, a page 3.9).
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void kv8_read_kernel(Kv8 c, Kv8Batch b, const int* __restrict__ first,
                                                        _Float16* __restrict__ k, _Float16* __restrict__ v, int kts) {

@@ -30,7 +30,8 @@ IT_HD int v_elem(int row, int dim) {
 // for while they are few. Half of the workgroups if there is more than a FEW row blocks and they need take no more than SHORT
 // pages: those pages are then quicker than the records of twice the splits (us, 16 heads, 2 KV heads, hd 256: 64 tokens after
 // 4032 28.4 / 30.0, 12 after 8180 21.2 / 23.1, but the 18 pages of 64 after 8128 36.7 / 33.8, and the four row blocks of 4
-// tokens after 8190, 24 heads, 20.0 / 19.4). The same in the partial and the merge kernel.
+// tokens after 8190, 24 heads, 20.0 / 19.4). Between: 11 pages 26.3 / 27.5, 14 29.8 / 30.3, 16 32.7 / 31.9; the two row blocks of a
+// token after 8191 12.8 / 12.2. The same in the partial and the merge kernel.
 constexpr int FEW = 4, SHORT = 10;
 IT_HD float reciprocal(float x) {   // (to a rounding or two; the splits need not be exact, only alike)
 #ifdef __HIP_DEVICE_COMPILE__

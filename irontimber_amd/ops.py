@@ -804,7 +804,7 @@ def attn_kv8(cache: Kv8Cache, q: torch.Tensor, start: torch.Tensor, length: torc
     rows 0 .. length[i] + t -> out [ntok, nh*hd], f32 or f16 (out's type, or out_dtype). start, length, table, max_nt as for
     kv8_append, length still without the new tokens: with them all rows that the sequence holds, or fewer that it may be cut to
     (it_attn_kv8). An f16 output of more than 16 query rows of a KV head (max_nt times its heads) is not the f32 one rounded:
-    probabilities go into its products as one f16 and q with two digits in place of three, which costs up to 2e-4 of the result in
+    probabilities go into its products as one f16 and q with two digits in place of three, which costs up to 2.1e-4 of the result in
     the mean beside the rounding's 2.1e-4."""
     dev, nkv, hd, nseq, args = _kv8(cache)
     pages = _kv8_batch(dev, nseq, start, length, table)
